@@ -12,7 +12,7 @@ from .delayarray import (DelayArray, NPArray, Scalar, NumpyEx, BinaryNumpyEx, Bi
                          sum, max, min, abs, mean, var, average, where, clip, WhereEx,
                          std, count_nonzero, isclose, allclose, norm)
 from .delayarray import any_ as any, all_ as all  # noqa: F401,A004
-from . import random  # noqa: F401
+from . import nn, random  # noqa: F401
 
 backend = _be.backend
 pi = _be.backend.np.pi

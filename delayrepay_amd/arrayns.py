@@ -8,7 +8,7 @@ them on the host and upload.
 import numpy
 
 from . import hiprt
-from .devarray import ndarray
+from .devarray import from_dlpack, ndarray
 from .hip import assign, materialise, run_reduce_product
 
 
@@ -78,6 +78,8 @@ class _Fallback:
 
     array = asarray
     asanyarray = asarray
+
+    from_dlpack = staticmethod(from_dlpack)
 
     @staticmethod
     def ascontiguousarray(obj, dtype=None):

@@ -7,6 +7,7 @@ environment variable and is never used by the HIP backend.
 """
 import numpy
 
+from . import cpu_nn as operators  # noqa: F401
 from .visitor import Visitor
 
 np = numpy

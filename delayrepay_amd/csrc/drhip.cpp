@@ -30,6 +30,13 @@ extern "C" void drhip_k_launch_matmul(int is_double, const void* A, const void* 
 extern "C" int drhip_k_cumsum(int kind, void* temp, size_t* temp_bytes, const void* in, void* out,
                               size_t n, hipStream_t s);
 
+extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad);
+extern "C" int drhip_k_attention(const drhip_attention_t* a, hipStream_t s);
+extern "C" int drhip_k_attention_grad(const drhip_attention_t* a, hipStream_t s);
+extern "C" uint64_t drhip_k_rotary_work(const drhip_rotary_t* p);
+extern "C" int drhip_k_rotary(const drhip_rotary_t* p, hipStream_t s);
+extern "C" int drhip_k_sample(const drhip_sample_t* p, hipStream_t s);
+
 extern "C" int drhip_k_scratch_init(int device);
 extern "C" void* drhip_k_scratch_ptr(int device);
 extern "C" size_t drhip_k_scratch_bytes(void);
@@ -317,6 +324,111 @@ int drhip_cumsum(int kind, const void* in, void* out, size_t n) {
     return 0;
 }
 
+// ---- operators of language models -----------------------------------------------
+
+// The launches count blocks in one dimension, of at most 2^32 threads
+static const int64_t kMostRows = int64_t(1) << 28, kMostBlocks = int64_t(1) << 23;
+
+static const char* attention_fault(const drhip_attention_t* a, int grad) {
+    if (a->batch < 0 || a->hq < 0 || a->hkv < 0 || a->lq < 0 || a->lk < 0) return "negative size";
+    if (a->hkv ? a->hq % a->hkv : a->hq) return "hq is not a multiple of hkv";
+    if (a->d < 1 || a->d > 128) return "head size outside 1..128";
+    if (a->lq >= 1 << 28 || a->lk >= 1 << 28) return "more than 2^28 rows";
+    const int64_t heads = (int64_t)a->batch * a->hq;
+    if (heads >= kMostBlocks || heads * (a->lq / 32 + 1) >= kMostBlocks || heads * (a->lk / 128 + 1) >= kMostBlocks)
+        return "more blocks than one launch holds";
+    if (a->prefix_value < 0) return "negative prefix";
+    if (heads && a->lq && (!a->q || !a->o || (a->lk && (!a->k || !a->v)))) return "null operand";
+    if (grad && heads && ((a->lq && (!a->dout || !a->dq || !a->lse)) || (a->lk && (!a->k || !a->v || !a->dk || !a->dv)))) return "null operand";
+    return nullptr;
+}
+
+int drhip_attention_work(const drhip_attention_t* a, int grad, uint64_t* bytes) {
+    if (!a || !bytes) return fail(DRHIP_EINVAL, "drhip_attention_work", "null argument");
+    const bool empty = a->batch <= 0 || a->hq <= 0;
+    drhip_attention_t b = *a;      // (the operands need not be there yet)
+    b.q = b.k = b.v = b.dout = (const float*)16;
+    b.o = b.lse = b.dq = b.dk = b.dv = (float*)16;
+    if (const char* why = attention_fault(&b, grad)) return fail(DRHIP_EINVAL, "drhip_attention_work", why);
+    *bytes = empty ? 0 : drhip_k_attention_work(a, grad);
+    return 0;
+}
+
+int drhip_attention(const drhip_attention_t* a) {
+    NEED_INIT();
+    if (!a) return fail(DRHIP_EINVAL, "drhip_attention", "null argument");
+    if (const char* why = attention_fault(a, 0)) return fail(DRHIP_EINVAL, "drhip_attention", why);
+    if (!a->batch || !a->hq || !a->lq) return 0;
+    const uint64_t need = drhip_k_attention_work(a, 0);
+    if (need && (!a->work || a->work_bytes < need)) return fail(DRHIP_EINVAL, "drhip_attention", "workspace too small");
+    if (int rc = drhip_k_attention(a, g_stream)) return fail(rc, "drhip_attention", hipGetErrorString((hipError_t)rc));
+    g_cnt.n_launches++;
+    return 0;
+}
+
+int drhip_attention_grad(const drhip_attention_t* a) {
+    NEED_INIT();
+    if (!a) return fail(DRHIP_EINVAL, "drhip_attention_grad", "null argument");
+    if (const char* why = attention_fault(a, 1)) return fail(DRHIP_EINVAL, "drhip_attention_grad", why);
+    if (!a->batch || !a->hq) return 0;
+    const uint64_t need = drhip_k_attention_work(a, 1);
+    if (need && (!a->work || a->work_bytes < need)) return fail(DRHIP_EINVAL, "drhip_attention_grad", "workspace too small");
+    if (int rc = drhip_k_attention_grad(a, g_stream)) return fail(rc, "drhip_attention_grad", hipGetErrorString((hipError_t)rc));
+    g_cnt.n_launches++;
+    return 0;
+}
+
+static const char* rotary_fault(const drhip_rotary_t* p) {
+    if (p->batch < 0 || p->heads < 0 || p->rows < 0) return "negative size";
+    if (p->d < 1 || p->d > 512) return "head size outside 1..512";
+    if (p->dims < 0 || p->dims > p->d || p->dims % 2) return "dims is not an even number of elements of a head";
+    if (p->d_pad < p->d || p->d_pad % 4) return "bad d_pad";
+    if ((int64_t)p->batch * p->rows >= kMostRows || (int64_t)p->batch * p->rows * (p->heads / 8 + 1) >= 4 * kMostBlocks || p->heads >= 1 << 20)
+        return "more rows than one launch holds";
+    return nullptr;
+}
+
+int drhip_rotary_work(const drhip_rotary_t* p, uint64_t* bytes) {
+    if (!p || !bytes) return fail(DRHIP_EINVAL, "drhip_rotary_work", "null argument");
+    if (const char* why = rotary_fault(p)) return fail(DRHIP_EINVAL, "drhip_rotary_work", why);
+    *bytes = p->heads ? drhip_k_rotary_work(p) : 0;
+    return 0;
+}
+
+int drhip_rotary(const drhip_rotary_t* p) {
+    NEED_INIT();
+    if (!p) return fail(DRHIP_EINVAL, "drhip_rotary", "null argument");
+    if (const char* why = rotary_fault(p)) return fail(DRHIP_EINVAL, "drhip_rotary", why);
+    if (!p->heads || (!p->dweight && (!p->batch || !p->rows))) return 0;
+    if ((int64_t)p->batch * p->rows && (!p->x || !p->y || (p->dweight && !p->dy))) return fail(DRHIP_EINVAL, "drhip_rotary", "null operand");
+    if (p->dweight) {
+        if (!p->weight) return fail(DRHIP_EINVAL, "drhip_rotary", "null operand");
+        if (!p->work || p->work_bytes < drhip_k_rotary_work(p)) return fail(DRHIP_EINVAL, "drhip_rotary", "workspace too small");
+    }
+    if (int rc = drhip_k_rotary(p, g_stream)) return fail(rc, "drhip_rotary", hipGetErrorString((hipError_t)rc));
+    g_cnt.n_launches++;
+    return 0;
+}
+
+int drhip_sample(const drhip_sample_t* p) {
+    NEED_INIT();
+    if (!p) return fail(DRHIP_EINVAL, "drhip_sample", "null argument");
+    if (p->batch < 0 || p->vocabulary < 1 || p->vocabulary >= 1 << 28 || p->batch >= kMostBlocks / 4) return fail(DRHIP_EINVAL, "drhip_sample", "bad size");
+    if (!(p->one >= 1.0) || p->one * p->vocabulary > 4611686018427387904.0) return fail(DRHIP_EINVAL, "drhip_sample", "weights would not fit 64 bits");
+    if (!p->batch) return 0;
+    if (!p->logits || !p->uniforms || !p->tokens) return fail(DRHIP_EINVAL, "drhip_sample", "null operand");
+    if (int rc = drhip_k_sample(p, g_stream)) return fail(rc, "drhip_sample", hipGetErrorString((hipError_t)rc));
+    g_cnt.n_launches++;
+    return 0;
+}
+
+int drhip_stream(void** stream) {
+    NEED_INIT();
+    if (!stream) return fail(DRHIP_EINVAL, "drhip_stream", "null out");
+    *stream = (void*)g_stream;
+    return 0;
+}
+
 // ---- compile / load --------------------------------------------------------
 
 int drhip_compile(const char* src, const char* name, const char* const* opts, int nopts,
@@ -517,6 +629,16 @@ int drhip_event_record(void* ev) {
 int drhip_event_sync(void* ev) {
     NEED_INIT();
     HIP_TRY(hipEventSynchronize((hipEvent_t)ev));
+    return 0;
+}
+
+int drhip_event_done(void* ev, int* done) {
+    NEED_INIT();
+    if (!ev || !done) return fail(DRHIP_EINVAL, "drhip_event_done", "null argument");
+    const hipError_t e = hipEventQuery((hipEvent_t)ev);
+    if (e == hipErrorNotReady) (void)hipGetLastError();
+    else if (e != hipSuccess) return fail((int)e, "hipEventQuery", hipGetErrorString(e));
+    *done = e == hipSuccess;
     return 0;
 }
 

@@ -1,0 +1,1127 @@
+// Attention on gfx950: forward (long and short query blocks), joining of split key ranges,
+// and the gradient.  Interface: drhip_attention_t in include/drhip.h.
+//
+//   x_ij = scale q_i . k_j            z_ij = cap tanh(x_ij / cap) - slope_h |p_i - j|
+//   o_i  = sum_j P_ij v_j,  P_ij = exp(z_ij - lse_i),  lse_i = log sum_j exp z_ij
+//   dV_j = sum_i P_ij dO_i            D_i = dO_i . o_i
+//   dX_ij = P_ij (dO_i . v_j - D_i) (1 - tanh^2(x_ij / cap))
+//   dQ_i = scale sum_j dX_ij k_j      dK_j = scale sum_i dX_ij q_i
+//
+// Sums run over the pairs that count: j below the row's limit (the sequence's length; for causal
+// rows max(p_i + 1, prefix) as well) and, with documents, of the row's own document.  A row
+// without pairs gives zeros and lse = -inf.  A pair that does not count contributes nothing
+// whatever its key holds: tiles are freed of values that are not finite when they are staged,
+// and the rows that held one are added by themselves, where their weight is not zero.
+//
+// Everything is float32 on v_mfma_f32_32x32x2f32 / 16x16x4f32 (products and sums exact to float32;
+// the statistics of the softmax are float32 too).
+#include "../../include/drhip.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef drhip_attention_t Args;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+constexpr int kThreads = 256;        // 4 waves
+constexpr int kRows = 128;           // query rows (or keys, in the dK/dV kernel) of a block: 32 for each wave
+constexpr int kTile = 32;            // keys (query rows) staged at a time
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh to about an ulp: an odd polynomial (own fit on |y| <= 0.55, relative error 1e-9) where
+// 1 - 2 / (e^2y + 1) would cancel, that form elsewhere
+__device__ __forceinline__ float tanh_(float y) {
+    const float a = fabsf(y), u = y * y;
+    const float p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, -0.0062742396257817745f, 0.021071678027510643f),
+                                         -0.05385230854153633f), 0.13332585990428925f), -0.33333316445350647f);
+    const float small = fmaf(y * u, p, y);
+    const float large = copysignf(1.0f - 2.0f / (exp2_(a * (2.0f * kLog2e)) + 1.0f), y);
+    return a <= 0.55f ? small : (a == a ? large : y);
+}
+
+__device__ __forceinline__ bool finite_(float x) { return fabsf(x) < __builtin_inff(); }
+
+__device__ __forceinline__ int clamp_(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// Four neighbouring elements of a row, zeros past its end; `wide`: rows are 16-byte aligned multiples of four
+__device__ __forceinline__ f32x4 load4(const float* row, int d, int size, bool ok, bool wide) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (wide) {
+        if (ok && d < size) x = *(const f32x4*)(row + d);
+    } else if (ok) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (d + c < size) x[c] = row[d + c];
+    }
+    return x;
+}
+
+// What a sequence says about its rows
+struct Seq {
+    int len, start, prefix;
+    const int32_t* docs;
+};
+
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+    Seq s;
+    s.len = a.lengths ? clamp_(a.lengths[b], 0, a.lk) : a.lk;
+    const int far = 1 << 30;      // positions stay far from the ends of int32
+    s.start = a.start ? clamp_(a.start[b], -far, far) : a.start_mode ? clamp_(a.start_value, -far, far) : s.len - a.lq;
+    s.prefix = a.prefix ? clamp_(a.prefix[b], 0, a.lk) : a.prefix_value;
+    s.docs = a.documents ? a.documents + (int64_t)b * a.documents_stride : nullptr;
+    return s;
+}
+
+// The keys that the row at position p may see are those below its limit, of its own document
+__device__ __forceinline__ int row_limit(const Args& a, const Seq& s, int p) {
+    int lim = s.len;
+    if (a.causal) {
+        const int seen = p + 1 > s.prefix ? p + 1 : s.prefix;
+        lim = clamp_(seen, 0, s.len);
+    }
+    if (s.docs && (p < 0 || p >= s.len)) lim = 0;      // a row without a document
+    return lim;
+}
+
+// Element index of accumulator tile c, row i (0..31): chosen so that the operand of the product
+// that contracts over tile rows is one vector per lane (NT = 4: 16 bytes, NT = 2: 8)
+template <int NT> __device__ __forceinline__ int elem(int i, int c) {
+    return NT == 4 ? 4 * i + c : NT == 2 ? 2 * i + c : 32 * c + i;
+}
+
+// Row of register v in a 32x32 accumulator, for the lanes of half h
+__device__ __forceinline__ int acc_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
+
+// A 32-row tile of a matrix on its way from memory to LDS.  Rows lie LD = 32 NT + 4 words apart: b128
+// reads of one column quad by 16 lanes then fall into 64 different banks.
+template <int NT> struct Tile {
+    static constexpr int LD = 32 * NT + 4;
+    static constexpr int QUADS = 8 * NT;                       // of a row
+    static constexpr int PASSES = kTile * QUADS / kThreads;    // NT
+    f32x4 r[PASSES];
+    __device__ __forceinline__ static int row(int p) { return (threadIdx.x + p * kThreads) / QUADS; }
+    __device__ __forceinline__ static int col(int p) { return (threadIdx.x + p * kThreads) % QUADS * 4; }
+    __device__ __forceinline__ void fetch(const float* base, int64_t stride, int first, int end, int size, bool wide) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int at = first + row(p);
+            r[p] = load4(base + at * stride, col(p), size, at < end, wide);
+        }
+    }
+    // Store the tile with its non-finite values as zeros; a row that had one is marked in *bad
+    __device__ __forceinline__ void stage(float* lds, unsigned* bad) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            f32x4 x = r[p];
+            const float worst = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+            const float nan = x[0] + x[1] + x[2] + x[3];
+            if (!(worst < __builtin_inff()) || nan != nan) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] = finite_(x[c]) ? x[c] : 0.f;
+                atomicOr(bad, 1u << row(p));
+            }
+            *(f32x4*)(lds + row(p) * LD + col(p)) = x;
+        }
+    }
+};
+
+// acc[row][col] += sum_d tile[row][d] own[col][d]: lane l holds column l % 32 of `own`, elements
+// 8t + 4h + c, and the tile is read in the same order
+template <int NT>
+__device__ __forceinline__ f32x16 product(const float* tile, const f32x4 (&own)[4 * NT], int lane) {
+    f32x16 acc;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+    const float* at = tile + (lane & 31) * Tile<NT>::LD + 4 * (lane >> 5);
+#pragma unroll
+    for (int t = 0; t < 4 * NT; ++t) {
+        const f32x4 x = *(const f32x4*)(at + 8 * t);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[c], own[t][c], acc, 0, 0, 0);
+    }
+    return acc;
+}
+
+// acc[c][i][col] += sum_row tile[row][elem(i, c)] w[row][col], w in the accumulator layout: register v
+// of the two halves is one step of two rows, so weights go from one product to the next without a move
+template <int NT>
+__device__ __forceinline__ void spread(f32x16 (&acc)[NT], const float* tile, const f32x16& w, int lane) {
+    const int i = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        const float* at = tile + acc_row(v, h) * Tile<NT>::LD;
+        float x[NT];
+        if constexpr (NT == 4) {
+            const f32x4 y = *(const f32x4*)(at + 4 * i);
+            x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
+        } else if constexpr (NT == 2) {
+            const float2 y = *(const float2*)(at + 2 * i);
+            x[0] = y.x, x[1] = y.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) x[c] = at[32 * c + i];
+        }
+#pragma unroll
+        for (int c = 0; c < NT; ++c) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[c], w[v], acc[c], 0, 0, 0);
+    }
+}
+
+// The part of `spread` that staging left out: elements that are not finite, of the rows in `bad`
+template <int NT>
+__device__ void spread_bad(f32x16 (&acc)[NT], unsigned bad, const float* base, int64_t stride, int size, const f32x16& w, int lane) {
+    const int h = lane >> 5;
+    while (bad) {
+        const int r = __builtin_ctz(bad);
+        bad &= bad - 1;
+        const int from = 4 * (r >> 3) + (r & 3);
+        float mine = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mine = v == from ? w[v] : mine;
+        const float weight = __shfl(mine, (lane & 31) + 32 * ((r >> 2) & 1));
+        const float* row = base + r * stride;
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int d = elem<NT>(acc_row(v, h), c);
+                const float x = d < size ? row[d] : 0.f;
+                if (!finite_(x) && weight != 0.f) acc[c][v] += weight * x;
+            }
+    }
+}
+
+// A lane's column of an accumulator, as the row of a matrix
+template <int NT>
+__device__ __forceinline__ void store_row(float* row, const f32x16 (&acc)[NT], float by, int size, bool wide, int h) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        if constexpr (NT == 4 || NT == 2) {
+            // rows 8u + 4h .. + 3 of all tiles are 4 NT neighbouring elements
+            const int d0 = NT * (8 * u + 4 * h);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                f32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[(4 * n + e) % NT][4 * u + (4 * n + e) / NT] * by;
+                const int d = d0 + 4 * n;
+                if (wide) {
+                    if (d < size) *(f32x4*)(row + d) = x;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < size) row[d + e] = x[e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const int d = 32 * c + 8 * u + 4 * h;
+                if (wide) {
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = acc[c][4 * u + e] * by;
+                    if (d < size) *(f32x4*)(row + d) = x;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < size) row[d + e] = acc[c][4 * u + e] * by;
+                }
+            }
+        }
+    }
+}
+
+// Score of one pair from its product, in units of log 2, and the factor of its derivative
+__device__ __forceinline__ float score(const Args& a, float x, float slope2, int p, int j) {
+    float z;
+    if (a.cap > 0.f)
+        z = a.cap * kLog2e * tanh_(x / a.cap);
+    else
+        z = x * kLog2e;
+    if (a.slopes) z -= slope2 * fabsf((float)(p - j));
+    return z;
+}
+
+struct Plan {
+    int few;         // 1: the kernel for few rows
+    int splits, chunk;
+    int wide;
+};
+
+// ---- forward, many rows ---------------------------------------------------------------------
+// A block owns 128 rows of the queries that share a key head (row = query head in the group x
+// query position), each wave 32 of them, one per column of its accumulators: S^T = K Q^T leaves the
+// scores of a row in one lane pair, so the softmax needs one exchange, and P^T in the layout that
+// O^T += V^T P^T reads.  Keys and values come 32 at a time through LDS, two buffers, fetched a tile ahead.
+template <int NT>
+__global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan, int tiles, float* part, float* part_lse) {
+    using T = Tile<NT>;
+    __shared__ __attribute__((aligned(16))) float lds[2][2][kTile * T::LD];
+    __shared__ unsigned bad[2][2];
+    __shared__ int ends[4], doc_range[2][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int heads = a.batch * a.hkv;
+    int id = blockIdx.x;
+    const int head = id % heads;
+    id /= heads;
+    const int split = id % plan.splits;
+    const int tile = tiles - 1 - id / plan.splits;          // the longest rows first
+    const int b = head / a.hkv, kh = head % a.hkv, group = a.hq / a.hkv;
+    const Seq s = sequence(a, b);
+    const bool wide = plan.wide;
+
+    const int rows = group * a.lq;
+    const int r = tile * kRows + wave * 32 + (lane & 31);
+    const bool valid = r < rows;
+    const int g = valid ? r / a.lq : 0, i = valid ? r - g * a.lq : 0;
+    const int qh = kh * group + g, p = s.start + i;
+    const int lim = valid ? row_limit(a, s, p) : 0;
+    const int doc = s.docs && lim > 0 ? s.docs[p] : 0;
+    const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
+
+    f32x4 own[4 * NT];
+    const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
+#pragma unroll
+    for (int t = 0; t < 4 * NT; ++t) {
+        own[t] = load4(qrow, 8 * t + 4 * h, a.d, valid, wide);
+        own[t] *= a.scale;
+    }
+
+    // range of limits (and documents) in the wave and in the block
+    int top = lim, low = valid ? lim : 0x7fffffff, dlo = lim > 0 ? doc : 0x7fffffff, dhi = lim > 0 ? doc : -0x7fffffff - 1;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        top = max(top, __shfl_xor(top, m));
+        low = min(low, __shfl_xor(low, m));
+        dlo = min(dlo, __shfl_xor(dlo, m));
+        dhi = max(dhi, __shfl_xor(dhi, m));
+    }
+    if (lane == 0) ends[wave] = top, doc_range[0][wave] = dlo, doc_range[1][wave] = dhi;
+    if (threadIdx.x < 4) (&bad[0][0])[threadIdx.x] = 0;
+    __syncthreads();
+    const int begin = split * plan.chunk;
+    int end = max(max(ends[0], ends[1]), max(ends[2], ends[3]));
+    dlo = min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3]));
+    dhi = max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3]));
+    if (end > begin + plan.chunk) end = begin + plan.chunk;
+
+    const float* kbase = a.k + b * a.k_stride[0] + kh * a.k_stride[1];
+    const float* vbase = a.v + b * a.v_stride[0] + kh * a.v_stride[1];
+    // the first key of the next tile that any row of the block may see
+    auto next = [&](int j0) {
+        if (s.docs)
+            for (; j0 < end; j0 += kTile) {
+                const int j = j0 + (lane & 31);
+                const int x = j < end ? s.docs[j] : 0;
+                if (__any(j < end && x >= dlo && x <= dhi)) break;
+            }
+        return j0;
+    };
+
+    f32x16 acc[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
+    float most = -__builtin_inff(), total = 0.f;      // running maximum of the row, sum over this lane's keys
+
+    T tk, tv;
+    int j0 = next(begin), buf = 0;
+    if (j0 < end) {
+        tk.fetch(kbase, a.k_stride[2], j0, s.len, a.d, wide);
+        tv.fetch(vbase, a.v_stride[2], j0, s.len, a.d, wide);
+        tk.stage(lds[0][0], &bad[0][0]);
+        tv.stage(lds[0][1], &bad[0][1]);
+    }
+    __syncthreads();
+    while (j0 < end) {
+        const int j1 = next(j0 + kTile);
+        if (j1 < end) {
+            tk.fetch(kbase, a.k_stride[2], j1, s.len, a.d, wide);
+            tv.fetch(vbase, a.v_stride[2], j1, s.len, a.d, wide);
+        }
+        if (j0 < top) {                                // some row of this wave sees the tile
+            f32x16 x = product<NT>(lds[buf][0], own, lane);
+            const unsigned kbad = bad[buf][0];
+            const bool whole = j0 + kTile <= low && !s.docs && !kbad;
+            float peak = most;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int j = j0 + acc_row(v, h);
+                float z = score(a, x[v], slope2, p, j);
+                if (!whole) {
+                    if (kbad >> acc_row(v, h) & 1) z = __builtin_nanf("");
+                    bool ok = j < lim;
+                    if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc;
+                    z = ok ? z : -__builtin_inff();
+                }
+                x[v] = z;
+                peak = z > peak || z != z ? z : peak;
+            }
+            const float other = __shfl_xor(peak, 32);
+            peak = other > peak || other != other ? other : peak;
+            const float ref = peak == -__builtin_inff() ? 0.f : peak;
+            const float shrink = exp2_(most - ref);
+            if (__any(shrink != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < NT; ++c)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) acc[c][v] *= shrink;
+                total *= shrink;
+            }
+            most = peak;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                x[v] = exp2_(x[v] - ref);
+                total += x[v];
+            }
+            spread<NT>(acc, lds[buf][1], x, lane);
+            const unsigned vbad = bad[buf][1];
+            if (vbad) spread_bad<NT>(acc, vbad, vbase + j0 * a.v_stride[2], a.v_stride[2], a.d, x, lane);
+        }
+        __syncthreads();                               // everyone is done with the marks of this buffer
+        if (threadIdx.x < 2) bad[buf][threadIdx.x] = 0;
+        buf ^= 1;
+        if (j1 < end) {
+            tk.stage(lds[buf][0], &bad[buf][0]);
+            tv.stage(lds[buf][1], &bad[buf][1]);
+        }
+        __syncthreads();
+        j0 = j1;
+    }
+
+    total += __shfl_xor(total, 32);
+    if (!valid) return;
+    const float by = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;      // (a NaN stays one)
+    const float lse = total == 0.f ? -__builtin_inff() : (most + __builtin_amdgcn_logf(total)) * kLn2;
+    if (part) {
+        const int64_t row = (((int64_t)split * a.batch + b) * a.hq + qh) * a.lq + i;
+        store_row<NT>(part + row * a.d, acc, by, a.d, wide, h);
+        if (h == 0) part_lse[row] = lse;
+    } else {
+        store_row<NT>(a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2], acc, by, a.d, wide, h);
+        if (h == 0 && a.lse) a.lse[((int64_t)b * a.hq + qh) * a.lq + i] = lse;
+    }
+}
+
+// ---- forward, few rows ----------------------------------------------------------------------
+// At most 16 NQ rows against a long key range (single tokens, with all query heads of a key head
+// together): bound by reading keys and values once.  No LDS: a wave takes 16 keys at a time, the blocks'
+// waves in turn, and its loads are the operands of v_mfma_f32_16x16x4f32 as they come (K: lane = key,
+// 16 bytes of its row; V: 16 neighbouring bytes of four rows each).  Key ranges of one sequence go to
+// `splits` blocks, whose results are joined by `attention_join`.
+template <int NB, int NQ>
+__global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, float* part, float* part_lse) {
+    constexpr int KS = 4 * NB;                 // 16-byte steps of a key row for each quarter of the wave
+    __shared__ __attribute__((aligned(16))) float merged[4][16][64 * NB + 4];
+    __shared__ float stat[4][2][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, h = lane >> 4;
+    const int heads = a.batch * a.hkv;
+    const int head = blockIdx.x % heads, split = blockIdx.x / heads;
+    const int b = head / a.hkv, kh = head % a.hkv, group = a.hq / a.hkv;
+    const Seq s = sequence(a, b);
+    const bool wide = plan.wide;
+    const int rows = group * a.lq;
+
+    f32x4 own[NQ][KS];
+    int lim[NQ], pos[NQ], doc[NQ];
+    float slope2[NQ];
+    int top = 0, low = 0x7fffffff;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = 16 * n + col;
+        const bool valid = r < rows;
+        const int g = valid ? r / a.lq : 0, i = valid ? r - g * a.lq : 0, qh = kh * group + g;
+        pos[n] = s.start + i;
+        lim[n] = valid ? row_limit(a, s, pos[n]) : 0;
+        doc[n] = s.docs && lim[n] > 0 ? s.docs[pos[n]] : 0;
+        slope2[n] = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
+        const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+            own[n][t] = load4(qrow, 16 * t + 4 * h, a.d, valid, wide);
+            own[n][t] *= a.scale;
+        }
+        top = max(top, lim[n]);
+        low = min(low, valid ? lim[n] : 0x7fffffff);
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+        top = max(top, __shfl_xor(top, m));
+        low = min(low, __shfl_xor(low, m));
+    }
+    const int begin = split * plan.chunk, end = min(begin + plan.chunk, top);
+    const float* kbase = a.k + b * a.k_stride[0] + kh * a.k_stride[1];
+    const float* vbase = a.v + b * a.v_stride[0] + kh * a.v_stride[1];
+
+    f32x4 acc[NQ][NB][4];
+    float most[NQ], total[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        most[n] = -__builtin_inff(), total[n] = 0.f;
+#pragma unroll
+        for (int e = 0; e < NB; ++e)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[n][e][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    f32x4 kx[KS], vx[4][NB];
+    auto fetch = [&](int j0) {
+        const int jk = j0 + col;
+        const float* krow = kbase + (int64_t)(jk < end ? jk : 0) * a.k_stride[2];
+#pragma unroll
+        for (int t = 0; t < KS; ++t) kx[t] = load4(krow, 16 * t + 4 * h, a.d, jk < end, wide);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int jv = j0 + 4 * h + v;
+            const float* vrow = vbase + (int64_t)(jv < end ? jv : 0) * a.v_stride[2];
+#pragma unroll
+            for (int e = 0; e < NB; ++e) vx[v][e] = load4(vrow, 64 * e + 4 * col, a.d, jv < end, wide);
+        }
+    };
+    int j0 = begin + 16 * wave;
+    if (j0 < end) fetch(j0);
+    while (j0 < end) {
+        f32x4 kc[KS], vc[4][NB];
+#pragma unroll
+        for (int t = 0; t < KS; ++t) kc[t] = kx[t];
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int e = 0; e < NB; ++e) vc[v][e] = vx[v][e];
+        const int j1 = j0 + 64;
+        if (j1 < end) fetch(j1);
+
+        // values that are not finite: taken out here, added by themselves below
+        bool kbad = false;
+        unsigned vbad = 0;
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) kbad = kbad || !finite_(kc[t][c]);
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int e = 0; e < NB; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (!finite_(vc[v][e][c])) {
+                        vc[v][e][c] = 0.f;
+                        vbad |= 1u << (4 * h + v);
+                    }
+        unsigned kmask = 0;
+        if (__any(kbad)) {                    // (a key's row is spread over four lanes)
+            const unsigned long long m = __ballot(kbad);
+            kmask = (unsigned)((m | m >> 16 | m >> 32 | m >> 48) & 0xffff);
+#pragma unroll
+            for (int t = 0; t < KS; ++t)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) kc[t][c] = finite_(kc[t][c]) ? kc[t][c] : 0.f;
+        }
+        if (__any(vbad != 0)) {
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) vbad |= __shfl_xor(vbad, m);
+        }
+        const bool whole = j0 + 16 <= low && !s.docs && !kmask;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < KS; ++t)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[t][c], own[n][t][c], x, 0, 0, 0);
+            float peak = most[n];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int j = j0 + 4 * h + v;
+                float z = score(a, x[v], slope2[n], pos[n], j);
+                if (!whole) {
+                    if (kmask >> (4 * h + v) & 1) z = __builtin_nanf("");
+                    bool ok = j < lim[n] && j < end;
+                    if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc[n];
+                    z = ok ? z : -__builtin_inff();
+                }
+                x[v] = z;
+                peak = z > peak || z != z ? z : peak;
+            }
+#pragma unroll
+            for (int m = 16; m < 64; m <<= 1) {
+                const float other = __shfl_xor(peak, m);
+                peak = other > peak || other != other ? other : peak;
+            }
+            const float ref = peak == -__builtin_inff() ? 0.f : peak;
+            const float shrink = exp2_(most[n] - ref);
+            if (__any(shrink != 1.f)) {
+                total[n] *= shrink;
+#pragma unroll
+                for (int e = 0; e < NB; ++e)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[n][e][c] *= shrink;
+            }
+            most[n] = peak;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                x[v] = exp2_(x[v] - ref);
+                total[n] += x[v];
+            }
+#pragma unroll
+            for (int e = 0; e < NB; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        acc[n][e][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vc[v][e][c], x[v], acc[n][e][c], 0, 0, 0);
+            for (unsigned m = vbad; m; m &= m - 1) {
+                const int key = __builtin_ctz(m);
+                float mine = 0.f;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) mine = v == (key & 3) ? x[v] : mine;
+                const float weight = __shfl(mine, col + 16 * (key >> 2));
+                const float* vrow = vbase + (int64_t)(j0 + key) * a.v_stride[2];
+#pragma unroll
+                for (int e = 0; e < NB; ++e)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            const int d = 64 * e + 4 * (4 * h + v) + c;
+                            const float y = d < a.d ? vrow[d] : 0.f;
+                            if (!finite_(y) && weight != 0.f) acc[n][e][c][v] += weight * y;
+                        }
+            }
+        }
+        j0 = j1;
+    }
+
+    // the four waves' results, one group of 16 rows at a time
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        float sum = total[n];
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (n) __syncthreads();
+        if (h == 0) stat[wave][0][col] = most[n], stat[wave][1][col] = sum;
+#pragma unroll
+        for (int e = 0; e < NB; ++e)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                f32x4 x;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] = acc[n][e][c][v];
+                *(f32x4*)&merged[wave][col][64 * e + 4 * (4 * h + v)] = x;
+            }
+        __syncthreads();
+        const int q = threadIdx.x >> 4;             // 16 threads for each row
+        const int r = 16 * n + q;
+        if (r < rows) {
+            float peak = -__builtin_inff();
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float z = stat[w][0][q];
+                peak = z > peak || z != z ? z : peak;
+            }
+            const float ref = peak == -__builtin_inff() ? 0.f : peak;
+            float f[4], sum4 = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                f[w] = exp2_(stat[w][0][q] - ref);
+                sum4 += f[w] * stat[w][1][q];
+            }
+            const float by = sum4 > 0.f ? 1.f / sum4 : sum4 == 0.f ? 0.f : sum4;
+            const float lse = sum4 == 0.f ? -__builtin_inff() : (peak + __builtin_amdgcn_logf(sum4)) * kLn2;
+            const int g = r / a.lq, i = r - g * a.lq, qh = kh * group + g;
+            const int64_t prow = (((int64_t)split * a.batch + b) * a.hq + qh) * a.lq + i;
+            float* row = part ? part + prow * a.d : a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2];
+            const int at = threadIdx.x & 15;
+#pragma unroll
+            for (int e = 0; e < NB; ++e) {
+                const int d = 64 * e + 4 * at;
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const f32x4 y = *(const f32x4*)&merged[w][q][d];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) x[c] += f[w] == 0.f ? 0.f : f[w] * y[c];
+                }
+                x *= by;
+                if (wide) {
+                    if (d < a.d) *(f32x4*)(row + d) = x;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (d + c < a.d) row[d + c] = x[c];
+                }
+            }
+            if (at == 0) {
+                if (part)
+                    part_lse[prow] = lse;
+                else if (a.lse)
+                    a.lse[((int64_t)b * a.hq + qh) * a.lq + i] = lse;
+            }
+        }
+    }
+}
+
+// Results of `splits` key ranges into one: a wave for each row
+__global__ __launch_bounds__(kThreads) void attention_join(Args a, int splits, const float* part, const float* part_lse) {
+    const int64_t rows = (int64_t)a.batch * a.hq * a.lq;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    float peak = -__builtin_inff();
+    for (int s = lane; s < splits; s += 64) {
+        const float z = part_lse[s * rows + row];
+        peak = z > peak || z != z ? z : peak;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const float other = __shfl_xor(peak, m);
+        peak = other > peak || other != other ? other : peak;
+    }
+    const float ref = peak == -__builtin_inff() ? 0.f : peak;
+    float sum = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int s = 0; s < splits; ++s) {
+        const float w = exp2_((part_lse[s * rows + row] - ref) * kLog2e);
+        if (w == 0.f) continue;
+        const float* from = part + (s * rows + row) * a.d;
+        sum += w;
+        if (lane < a.d) x0 += w * from[lane];
+        if (lane + 64 < a.d) x1 += w * from[lane + 64];
+    }
+    const float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    const int i = (int)(row % a.lq);
+    const int64_t bh = row / a.lq;
+    float* to = a.o + bh / a.hq * a.o_stride[0] + bh % a.hq * a.o_stride[1] + i * a.o_stride[2];
+    if (lane < a.d) to[lane] = x0 * by;
+    if (lane + 64 < a.d) to[lane + 64] = x1 * by;
+    if (lane == 0 && a.lse) a.lse[row] = sum == 0.f ? -__builtin_inff() : peak + __builtin_amdgcn_logf(sum) * kLn2;
+}
+
+// ---- gradient -------------------------------------------------------------------------------
+// Two kernels, each with all sums of one output in one place, so that results do not depend on timing:
+// dQ (rows own their sums, keys pass by, as in the forward kernel; writes D_i too) and dK, dV (keys own
+// their sums, rows pass by).  The scores are computed in both: seven products instead of five.
+template <int NT>
+__global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, int tiles, float* delta) {
+    using T = Tile<NT>;
+    __shared__ __attribute__((aligned(16))) float lds[2][2][kTile * T::LD];
+    __shared__ unsigned bad[2][2];
+    __shared__ int ends[4], doc_range[2][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int heads = a.batch * a.hkv;
+    const int head = blockIdx.x % heads, tile = tiles - 1 - blockIdx.x / heads;
+    const int b = head / a.hkv, kh = head % a.hkv, group = a.hq / a.hkv;
+    const Seq s = sequence(a, b);
+    const bool wide = plan.wide;
+    const int rows = group * a.lq;
+    const int r = tile * kRows + wave * 32 + (lane & 31);
+    const bool valid = r < rows;
+    const int g = valid ? r / a.lq : 0, i = valid ? r - g * a.lq : 0;
+    const int qh = kh * group + g, p = s.start + i;
+    const int64_t at = ((int64_t)b * a.hq + qh) * a.lq + i;
+    const float lse = valid ? a.lse[at] : -__builtin_inff();
+    const int lim = valid && lse != -__builtin_inff() ? row_limit(a, s, p) : 0;
+    const int doc = s.docs && lim > 0 ? s.docs[p] : 0;
+    const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f, lse2 = lse * kLog2e;
+
+    f32x4 own[4 * NT], dout[4 * NT];
+    const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
+    const float* grow = a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1] + i * a.dout_stride[2];
+    const float* orow = a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2];
+    float dot = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4 * NT; ++t) {
+        own[t] = load4(qrow, 8 * t + 4 * h, a.d, lim > 0, wide);
+        own[t] *= a.scale;
+        dout[t] = load4(grow, 8 * t + 4 * h, a.d, lim > 0, wide);
+        const f32x4 y = load4(orow, 8 * t + 4 * h, a.d, lim > 0, wide);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) dot += dout[t][c] * y[c];
+    }
+    dot += __shfl_xor(dot, 32);
+    if (valid && h == 0) delta[at] = dot;
+
+    int top = lim, low = valid ? lim : 0x7fffffff, dlo = lim > 0 ? doc : 0x7fffffff, dhi = lim > 0 ? doc : -0x7fffffff - 1;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        top = max(top, __shfl_xor(top, m));
+        low = min(low, __shfl_xor(low, m));
+        dlo = min(dlo, __shfl_xor(dlo, m));
+        dhi = max(dhi, __shfl_xor(dhi, m));
+    }
+    if (lane == 0) ends[wave] = top, doc_range[0][wave] = dlo, doc_range[1][wave] = dhi;
+    if (threadIdx.x < 4) (&bad[0][0])[threadIdx.x] = 0;
+    __syncthreads();
+    const int end = max(max(ends[0], ends[1]), max(ends[2], ends[3]));
+    dlo = min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3]));
+    dhi = max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3]));
+    const float* kbase = a.k + b * a.k_stride[0] + kh * a.k_stride[1];
+    const float* vbase = a.v + b * a.v_stride[0] + kh * a.v_stride[1];
+    auto next = [&](int j0) {
+        if (s.docs)
+            for (; j0 < end; j0 += kTile) {
+                const int j = j0 + (lane & 31);
+                const int x = j < end ? s.docs[j] : 0;
+                if (__any(j < end && x >= dlo && x <= dhi)) break;
+            }
+        return j0;
+    };
+    f32x16 acc[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
+    T tk, tv;
+    int j0 = next(0), buf = 0;
+    if (j0 < end) {
+        tk.fetch(kbase, a.k_stride[2], j0, s.len, a.d, wide);
+        tv.fetch(vbase, a.v_stride[2], j0, s.len, a.d, wide);
+        tk.stage(lds[0][0], &bad[0][0]);
+        tv.stage(lds[0][1], &bad[0][1]);
+    }
+    __syncthreads();
+    while (j0 < end) {
+        const int j1 = next(j0 + kTile);
+        if (j1 < end) {
+            tk.fetch(kbase, a.k_stride[2], j1, s.len, a.d, wide);
+            tv.fetch(vbase, a.v_stride[2], j1, s.len, a.d, wide);
+        }
+        if (j0 < top) {
+            f32x16 x = product<NT>(lds[buf][0], own, lane);
+            f32x16 y = product<NT>(lds[buf][1], dout, lane);
+            const unsigned kbad = bad[buf][0], vbad = bad[buf][1];
+            const bool whole = j0 + kTile <= low && !s.docs && !(kbad | vbad);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int j = j0 + acc_row(v, h);
+                float z, slope = a.scale;
+                if (a.cap > 0.f) {
+                    const float t = tanh_(x[v] / a.cap);
+                    z = a.cap * kLog2e * t;
+                    slope *= 1.f - t * t;
+                } else {
+                    z = x[v] * kLog2e;
+                }
+                if (a.slopes) z -= slope2 * fabsf((float)(p - j));
+                float w = exp2_(z - lse2) * (y[v] - dot) * slope;
+                if (!whole) {
+                    if ((kbad | vbad) >> acc_row(v, h) & 1) w = __builtin_nanf("");
+                    bool ok = j < lim;
+                    if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc;
+                    w = ok ? w : 0.f;
+                }
+                x[v] = w;
+            }
+            spread<NT>(acc, lds[buf][0], x, lane);
+            if (kbad) spread_bad<NT>(acc, kbad, kbase + j0 * a.k_stride[2], a.k_stride[2], a.d, x, lane);
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) bad[buf][threadIdx.x] = 0;
+        buf ^= 1;
+        if (j1 < end) {
+            tk.stage(lds[buf][0], &bad[buf][0]);
+            tv.stage(lds[buf][1], &bad[buf][1]);
+        }
+        __syncthreads();
+        j0 = j1;
+    }
+    if (valid) store_row<NT>(a.dq + b * a.dq_stride[0] + qh * a.dq_stride[1] + i * a.dq_stride[2], acc, 1.f, a.d, wide, h);
+}
+
+// `parts` > 1: the query heads of a key head go to different blocks, whose sums are added by `attention_add`
+template <int NT>
+__global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, int parts, const float* delta, float* part) {
+    using T = Tile<NT>;
+    __shared__ __attribute__((aligned(16))) float lds[2][2][kTile * T::LD];
+    __shared__ float stat[2][2][kTile];
+    __shared__ unsigned bad[2][2];
+    __shared__ int doc_range[2][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int heads = a.batch * a.hkv, group = a.hq / a.hkv;
+    int id = blockIdx.x;
+    const int head = id % heads;
+    id /= heads;
+    const int slice = id % parts, tile = id / parts;       // (causal: the first keys are seen by the most rows)
+    const int b = head / a.hkv, kh = head % a.hkv;
+    const Seq s = sequence(a, b);
+    const bool wide = plan.wide;
+    const int key0 = tile * kRows, j = key0 + wave * 32 + (lane & 31);
+    const bool valid = j < a.lk, counts = j < s.len;
+    const int doc = s.docs && counts ? s.docs[j] : 0;
+
+    f32x4 key[4 * NT], val[4 * NT];
+    const float* krow = a.k + b * a.k_stride[0] + kh * a.k_stride[1] + (int64_t)j * a.k_stride[2];
+    const float* vrow = a.v + b * a.v_stride[0] + kh * a.v_stride[1] + (int64_t)j * a.v_stride[2];
+#pragma unroll
+    for (int t = 0; t < 4 * NT; ++t) {
+        key[t] = load4(krow, 8 * t + 4 * h, a.d, counts, wide);
+        val[t] = load4(vrow, 8 * t + 4 * h, a.d, counts, wide);
+    }
+    f32x16 dk[NT], dv[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) dk[c][v] = 0.f, dv[c][v] = 0.f;
+
+    int dlo = counts ? doc : 0x7fffffff, dhi = counts ? doc : -0x7fffffff - 1;
+    if (s.docs) {
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            dlo = min(dlo, __shfl_xor(dlo, m));
+            dhi = max(dhi, __shfl_xor(dhi, m));
+        }
+    }
+    if (lane == 0) doc_range[0][wave] = dlo, doc_range[1][wave] = dhi;
+    if (threadIdx.x < 4) (&bad[0][0])[threadIdx.x] = 0;
+    __syncthreads();
+    dlo = min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3]));
+    dhi = max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3]));
+
+    // rows before `first` see none of the block's keys
+    int first = 0;
+    if (a.causal && key0 >= s.prefix) first = clamp_(key0 - s.start, 0, a.lq) & ~(kTile - 1);
+    if (key0 >= s.len) first = a.lq;
+    const int g0 = parts > 1 ? slice : 0, g1 = parts > 1 ? slice + 1 : group;
+    auto next = [&](int& g, int& i0) {     // to a tile of rows that may see a key of the block
+        for (; g < g1; ++g, i0 = first) {
+            for (; i0 < a.lq; i0 += kTile) {
+                if (!s.docs) return;
+                const int i = i0 + (lane & 31), p = s.start + i;
+                const bool in = i < a.lq && p >= 0 && p < s.len;
+                const int x = in ? s.docs[p] : 0;
+                if (__any(in && x >= dlo && x <= dhi)) return;
+            }
+        }
+    };
+    T tq, tg;
+    float mylse = 0.f, mydelta = 0.f;
+    auto fetch = [&](int g, int i0) {
+        const int qh = kh * group + g;
+        const int64_t at = ((int64_t)b * a.hq + qh) * a.lq;
+        const float* qbase = a.q + b * a.q_stride[0] + qh * a.q_stride[1];
+        const float* gbase = a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1];
+#pragma unroll
+        for (int x = 0; x < T::PASSES; ++x) {      // a row without pairs may hold anything
+            const int i = i0 + T::row(x);
+            const bool in = i < a.lq && a.lse[at + i] != -__builtin_inff();
+            tq.r[x] = load4(qbase + i * a.q_stride[2], T::col(x), a.d, in, wide);
+            tg.r[x] = load4(gbase + i * a.dout_stride[2], T::col(x), a.d, in, wide);
+        }
+        if (threadIdx.x < kTile) {
+            const int i = i0 + threadIdx.x;
+            mylse = i < a.lq ? a.lse[at + i] * kLog2e : -__builtin_inff();
+            if (mylse == -__builtin_inff()) mylse = __builtin_inff();    // weights of exp2(-inf) = 0
+            mydelta = i < a.lq ? delta[at + i] : 0.f;
+        }
+    };
+    auto stage = [&](int buf) {
+        tq.stage(lds[buf][0], &bad[buf][0]);
+        tg.stage(lds[buf][1], &bad[buf][1]);
+        if (threadIdx.x < kTile) stat[buf][0][threadIdx.x] = mylse, stat[buf][1][threadIdx.x] = mydelta;
+    };
+    int g = g0, i0 = first, buf = 0;
+    next(g, i0);
+    if (g < g1) {
+        fetch(g, i0);
+        stage(0);
+    }
+    __syncthreads();
+    while (g < g1) {
+        int ng = g, ni = i0 + kTile;
+        next(ng, ni);
+        if (ng < g1) fetch(ng, ni);
+        const int qh = kh * group + g;
+        const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
+        f32x16 x = product<NT>(lds[buf][0], key, lane);
+        f32x16 y = product<NT>(lds[buf][1], val, lane);
+        const unsigned qbad = bad[buf][0], gbad = bad[buf][1];
+        f32x16 w;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const int row = acc_row(v, h), i = i0 + row, p = s.start + i;
+            float z, slope = a.scale;
+            if (a.cap > 0.f) {
+                const float t = tanh_(x[v] * a.scale / a.cap);
+                z = a.cap * kLog2e * t;
+                slope *= 1.f - t * t;
+            } else {
+                z = x[v] * (a.scale * kLog2e);
+            }
+            if (a.slopes) z -= slope2 * fabsf((float)(p - j));
+            float weight = exp2_(z - stat[buf][0][row]);
+            float back = weight * (y[v] - stat[buf][1][row]) * slope;
+            bool ok = j < row_limit(a, s, p) && i < a.lq && stat[buf][0][row] != __builtin_inff();
+            if (s.docs) ok = ok && s.docs[ok ? p : 0] == doc;
+            if (qbad >> row & 1) weight = back = __builtin_nanf("");
+            if (gbad >> row & 1) back = __builtin_nanf("");
+            w[v] = ok ? weight : 0.f;
+            x[v] = ok ? back : 0.f;
+        }
+        spread<NT>(dv, lds[buf][1], w, lane);
+        spread<NT>(dk, lds[buf][0], x, lane);
+        if (gbad)
+            spread_bad<NT>(dv, gbad, a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1] + i0 * a.dout_stride[2], a.dout_stride[2], a.d, w, lane);
+        if (qbad)
+            spread_bad<NT>(dk, qbad, a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i0 * a.q_stride[2], a.q_stride[2], a.d, x, lane);
+        __syncthreads();
+        if (threadIdx.x < 2) bad[buf][threadIdx.x] = 0;
+        buf ^= 1;
+        if (ng < g1) stage(buf);
+        __syncthreads();
+        g = ng, i0 = ni;
+    }
+    if (!valid) return;
+    if (part) {
+        const int64_t rows = (int64_t)heads * a.lk;
+        float* to = part + (((int64_t)slice * 2) * rows + (int64_t)head * a.lk + j) * a.d;
+        store_row<NT>(to, dk, 1.f, a.d, wide, h);
+        store_row<NT>(to + rows * a.d, dv, 1.f, a.d, wide, h);
+    } else {
+        store_row<NT>(a.dk + b * a.dk_stride[0] + kh * a.dk_stride[1] + (int64_t)j * a.dk_stride[2], dk, 1.f, a.d, wide, h);
+        store_row<NT>(a.dv + b * a.dv_stride[0] + kh * a.dv_stride[1] + (int64_t)j * a.dv_stride[2], dv, 1.f, a.d, wide, h);
+    }
+}
+
+// dK and dV from the parts of the query heads, in their order; one row of one of them for each wave
+__global__ __launch_bounds__(kThreads) void attention_add(Args a, int parts, const float* part) {
+    const int64_t rows = (int64_t)a.batch * a.hkv * a.lk;
+    const int lane = threadIdx.x & 63;
+    int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= 2 * rows) return;
+    const float* from = part + row * a.d;
+    float x0 = 0.f, x1 = 0.f;
+    for (int n = 0; n < parts; ++n, from += 2 * rows * a.d) {
+        if (lane < a.d) x0 += from[lane];
+        if (lane + 64 < a.d) x1 += from[lane + 64];
+    }
+    const bool second = row >= rows;
+    if (second) row -= rows;
+    const int64_t* stride = second ? a.dv_stride : a.dk_stride;
+    const int64_t bh = row / a.lk;
+    float* to = (second ? a.dv : a.dk) + bh / a.hkv * stride[0] + bh % a.hkv * stride[1] + row % a.lk * stride[2];
+    if (lane < a.d) to[lane] = x0;
+    if (lane + 64 < a.d) to[lane + 64] = x1;
+}
+
+bool aligned(const void* p, const int64_t* stride) {
+    return (uintptr_t)p % 16 == 0 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
+}
+
+int row_tiles(const Args& a) { return (int)(((int64_t)(a.hq / a.hkv) * a.lq + kRows - 1) / kRows); }
+
+// Which forward kernel, and into how many key ranges.  Few rows: up to 32 rows of a key head, where the
+// 128-row blocks of the other kernel would be mostly empty.  Ranges: enough for `want` blocks (the
+// device holds 512 of either kernel), none shorter than `least` keys, whose work pays for joining.
+Plan plan_forward(const Args& a) {
+    Plan p;
+    p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride);
+    const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
+    p.few = rows <= 32;
+    const int64_t blocks = heads * (p.few ? 1 : row_tiles(a));
+    const int64_t want = p.few ? 2048 : 512;
+    const int least = p.few ? 256 : 512;
+    int64_t splits = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+    const int64_t most = (a.lk + least - 1) / least;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    p.chunk = (int)(((a.lk + splits - 1) / splits + 63) / 64 * 64);
+    if (p.chunk < 64) p.chunk = 64;
+    p.splits = a.lk > 0 ? (a.lk + p.chunk - 1) / p.chunk : 1;
+    return p;
+}
+
+// Query heads of a key head in blocks of their own: only where the keys alone give too few blocks
+int plan_parts(const Args& a) {
+    const int64_t blocks = (int64_t)a.batch * a.hkv * ((a.lk + kRows - 1) / kRows);
+    return a.hq > a.hkv && blocks < 512 ? a.hq / a.hkv : 1;
+}
+
+}  // namespace
+
+extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad) {
+    const uint64_t rows = (uint64_t)a->batch * a->hq * a->lq;
+    if (grad) {
+        const int parts = plan_parts(*a);
+        const uint64_t keys = (uint64_t)a->batch * a->hkv * a->lk * a->d;
+        return (rows * 4 + 255) / 256 * 256 + (parts > 1 ? keys * 8 * parts : 0);
+    }
+    const Plan p = plan_forward(*a);
+    return p.splits > 1 ? (rows * p.splits * 4 + 255) / 256 * 256 + rows * p.splits * a->d * 4 : 0;
+}
+
+extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
+    const Args& a = *args;
+    const Plan p = plan_forward(a);
+    const int64_t rows = (int64_t)a.batch * a.hq * a.lq, heads = (int64_t)a.batch * a.hkv;
+    float *part = nullptr, *part_lse = nullptr;
+    if (p.splits > 1) {
+        part_lse = (float*)a.work;
+        part = (float*)((char*)a.work + (rows * p.splits * 4 + 255) / 256 * 256);
+    }
+    if (p.few) {
+        const dim3 grid((unsigned)(heads * p.splits));
+        const bool two = (int64_t)(a.hq / a.hkv) * a.lq > 16;
+        if (a.d <= 64)
+            two ? attention_few<1, 2><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<1, 1><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
+        else
+            two ? attention_few<2, 2><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<2, 1><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
+    } else {
+        const int tiles = row_tiles(a);
+        const dim3 grid((unsigned)(heads * tiles * p.splits));
+        switch ((a.d + 31) / 32) {
+            case 1: attention_rows<1><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
+            case 2: attention_rows<2><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
+            case 3: attention_rows<3><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
+            default: attention_rows<4><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
+        }
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    if (p.splits > 1) {
+        attention_join<<<dim3((unsigned)((rows + 3) / 4)), kThreads, 0, s>>>(a, p.splits, part, part_lse);
+        e = hipGetLastError();
+    }
+    return (int)e;
+}
+
+extern "C" int drhip_k_attention_grad(const drhip_attention_t* args, hipStream_t s) {
+    const Args& a = *args;
+    const int64_t rows = (int64_t)a.batch * a.hq * a.lq, heads = (int64_t)a.batch * a.hkv;
+    float* delta = (float*)a.work;
+    const int parts = plan_parts(a);
+    float* part = parts > 1 ? (float*)((char*)a.work + (rows * 4 + 255) / 256 * 256) : nullptr;
+    Plan p{};
+    p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride) &&
+             aligned(a.dout, a.dout_stride) && aligned(a.dq, a.dq_stride) && aligned(a.dk, a.dk_stride) && aligned(a.dv, a.dv_stride);
+    const int tiles = row_tiles(a);
+    const int nt = (a.d + 31) / 32;
+    hipError_t e = hipSuccess;
+    if (rows > 0) {
+        const dim3 grid((unsigned)(heads * tiles));
+        switch (nt) {
+            case 1: attention_dq<1><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
+            case 2: attention_dq<2><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
+            case 3: attention_dq<3><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
+            default: attention_dq<4><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
+        }
+        e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    if (a.lk == 0 || heads == 0) return 0;
+    const dim3 grid((unsigned)(heads * parts * ((a.lk + kRows - 1) / kRows)));
+    switch (nt) {
+        case 1: attention_dkv<1><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
+        case 2: attention_dkv<2><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
+        case 3: attention_dkv<3><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
+        default: attention_dkv<4><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
+    }
+    e = hipGetLastError();
+    if (e != hipSuccess || parts == 1) return (int)e;
+    attention_add<<<dim3((unsigned)((2 * heads * a.lk + 3) / 4)), kThreads, 0, s>>>(a, parts, part);
+    return (int)hipGetLastError();
+}

@@ -1,0 +1,634 @@
+// Rotary positions (with the norm of each head in the same pass, and the gradient of both) and the
+// drawing of tokens, on gfx950.  Interfaces: drhip_rotary_t and drhip_sample_t in include/drhip.h.
+#include "../../include/drhip.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// ---- rotary positions -------------------------------------------------------------------------
+//
+//   y = R(position) (w * x * r),  r = (mean x^2 + eps)^-1/2      (without a weight: y = R x)
+//   R turns the pair (a, b) with number i by position * frequency_i / stretch; pairs are elements
+//   (i, i + dims/2) or (2i, 2i + 1); elements from `dims` on are left as they are
+//   gradient: g = R^T dy,  dx = r (w g - xhat mean(w g xhat)),  dw = sum over rows of g xhat,  xhat = r x
+//
+// Bound by memory: a row is read and written once.  A row belongs to a group of 2^k lanes, eight elements
+// each (the halves of four pairs); a group takes several heads of one token, so that the angles, which
+// need 64 bits (positions of a million turn by a million radians), are computed once for them.
+
+typedef drhip_rotary_t Rot;
+
+template <typename T> struct Vec4 { T v[4]; };
+
+template <typename T> __device__ __forceinline__ void load_quad(T (&x)[4], const T* p) {
+    *(Vec4<T>*)x = *(const Vec4<T>*)__builtin_assume_aligned(p, 16);
+}
+template <typename T> __device__ __forceinline__ void store_quad(T* p, const T (&x)[4]) {
+    *(Vec4<T>*)__builtin_assume_aligned(p, 16) = *(const Vec4<T>*)x;
+}
+
+// A lane's share of a row: pairs (a[n], b[n]) with number idx[n], and elements behind `dims`
+template <typename T, bool WIDE> struct Row {
+    T a[4], b[4], rest[8];
+    // number of the lane's pair n
+    __device__ __forceinline__ static int pair(const Rot& p, int lane, int lanes, int n) {
+        if (!WIDE) return lane + n * lanes;
+        const int half = p.dims / 2;
+        if (!p.interleaved) return 4 * lane + n;
+        return n < 2 ? 2 * lane + n : half / 2 + 2 * lane + n - 2;
+    }
+    __device__ __forceinline__ void load(const Rot& p, const T* row, int lane, int lanes, bool ok) {
+        const int half = p.dims / 2, behind = p.d - p.dims;
+        if constexpr (WIDE) {
+            T u[4] = {}, v[4] = {};
+            if (ok && 4 * lane < half) {
+                load_quad(u, row + 4 * lane);
+                load_quad(v, row + half + 4 * lane);
+            }
+            spread(p, u, v);
+            T s[4] = {}, t[4] = {};
+            if (behind) {
+                if (ok && 4 * lane < behind) load_quad(s, row + p.dims + 4 * lane);
+                if (ok && 4 * (lane + lanes) < behind) load_quad(t, row + p.dims + 4 * (lane + lanes));
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) rest[n] = s[n], rest[4 + n] = t[n];
+        } else {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int i = lane + n * lanes;
+                const bool in = ok && i < half;
+                a[n] = in ? row[p.interleaved ? 2 * i : i] : T(0);
+                b[n] = in ? row[p.interleaved ? 2 * i + 1 : half + i] : T(0);
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int i = lane + n * lanes;
+                rest[n] = ok && i < behind ? row[p.dims + i] : T(0);
+            }
+        }
+    }
+    __device__ __forceinline__ void spread(const Rot& p, const T (&u)[4], const T (&v)[4]) {
+        if (p.interleaved) {
+            a[0] = u[0], b[0] = u[1], a[1] = u[2], b[1] = u[3];
+            a[2] = v[0], b[2] = v[1], a[3] = v[2], b[3] = v[3];
+        } else {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) a[n] = u[n], b[n] = v[n];
+        }
+    }
+    __device__ __forceinline__ void store(const Rot& p, T* row, int lane, int lanes) const {
+        const int half = p.dims / 2, behind = p.d - p.dims;
+        if constexpr (WIDE) {
+            if (4 * lane < half) {
+                T u[4], v[4];
+                if (p.interleaved) {
+                    u[0] = a[0], u[1] = b[0], u[2] = a[1], u[3] = b[1];
+                    v[0] = a[2], v[1] = b[2], v[2] = a[3], v[3] = b[3];
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) u[n] = a[n], v[n] = b[n];
+                }
+                store_quad(row + 4 * lane, u);
+                store_quad(row + half + 4 * lane, v);
+            }
+            if (behind) {
+                T s[4], t[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) s[n] = rest[n], t[n] = rest[4 + n];
+                if (4 * lane < behind) store_quad(row + p.dims + 4 * lane, s);
+                if (4 * (lane + lanes) < behind) store_quad(row + p.dims + 4 * (lane + lanes), t);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int i = lane + n * lanes;
+                if (i < half) {
+                    row[p.interleaved ? 2 * i : i] = a[n];
+                    row[p.interleaved ? 2 * i + 1 : half + i] = b[n];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int i = lane + n * lanes;
+                if (i < behind) row[p.dims + i] = rest[n];
+            }
+        }
+    }
+    template <typename F> __device__ __forceinline__ void each(F f) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) f(a[n], n), f(b[n], 4 + n);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) f(rest[n], 8 + n);
+    }
+    __device__ __forceinline__ T& at(int n) { return n < 4 ? a[n] : n < 8 ? b[n - 4] : rest[n - 8]; }
+    __device__ __forceinline__ const T& at(int n) const { return n < 4 ? a[n] : n < 8 ? b[n - 4] : rest[n - 8]; }
+    __device__ __forceinline__ void turn(const T (&c)[4], const T (&s)[4]) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const T x = a[n], y = b[n];
+            a[n] = x * c[n] - y * s[n];
+            b[n] = y * c[n] + x * s[n];
+        }
+    }
+};
+
+__device__ __forceinline__ float root(float x) { return sqrtf(x); }
+__device__ __forceinline__ double root(double x) { return sqrt(x); }
+
+template <typename T> __device__ __forceinline__ T group_sum(T x, int lanes) {
+    for (int m = 1; m < lanes; m <<= 1) x += __shfl_xor(x, m);
+    return x;
+}
+
+// Frequencies of the lane's pairs: from the table, or base^(-2i / dims)
+template <typename T, bool WIDE>
+__device__ __forceinline__ void frequencies(const Rot& p, int lane, int lanes, double (&f)[4]) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int i = Row<T, WIDE>::pair(p, lane, lanes, n);
+        const bool in = i < p.dims / 2;
+        f[n] = p.frequencies ? (in ? p.frequencies[i] : 0.0) : exp2(i * p.step);
+        f[n] *= p.squeeze;
+    }
+}
+
+// cos and sin of position * f.  In float32 the angle is reduced to a part of a turn in 64 bits first.
+template <typename T>
+__device__ __forceinline__ void angles(const Rot& p, double position, const double (&f)[4], T (&c)[4], T (&s)[4]) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const double angle = position * f[n];
+        double x, y;
+        if constexpr (sizeof(T) == 4) {
+            const double turns = angle * 0.15915494309189533577;
+            float u, v;
+            sincospif((float)(2.0 * (turns - rint(turns))), &u, &v);
+            c[n] = v * (float)p.magnitude, s[n] = u * (float)(p.sign * p.magnitude);
+        } else {
+            sincos(angle, &x, &y);
+            c[n] = y * p.magnitude, s[n] = x * p.sign * p.magnitude;
+        }
+    }
+}
+
+__device__ __forceinline__ double position_of(const Rot& p, int b, int l) {
+    if (!p.positions) return (double)(p.first + l);
+    const int64_t at = b * p.positions_stride + l;
+    return p.positions_wide ? (double)((const int64_t*)p.positions)[at] : (double)((const int32_t*)p.positions)[at];
+}
+
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(Rot p, int lanes_log, int slots, int64_t groups) {
+    const int lanes = 1 << lanes_log;
+    const int64_t id = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> lanes_log;
+    const int lane = threadIdx.x & (lanes - 1);
+    const bool live = id < groups;
+    const int64_t g = live ? id : 0;
+    // a token's heads are taken by `slots` groups in turn, which are neighbours
+    const int slot = (int)(g % slots);
+    const int64_t token = g / slots;
+    const int b = (int)(token / p.rows), l = (int)(token % p.rows);
+    double f[4];
+    T c[4], s[4];
+    frequencies<T, WIDE>(p, lane, lanes, f);
+    angles<T>(p, position_of(p, b, l), f, c, s);
+    for (int h = slot; h < p.heads; h += slots) {
+        Row<T, WIDE> x;
+        x.load(p, (const T*)p.x + b * p.x_stride[0] + h * p.x_stride[1] + l * p.x_stride[2], lane, lanes, live);
+        if (p.weight) {
+            T sum = 0;
+            x.each([&](T& v, int) { sum += v * v; });
+            sum = group_sum(sum, lanes);
+            const T r = T(1) / root(sum / T(p.d) + T(p.eps));
+            Row<T, WIDE> w;
+            w.load(p, (const T*)p.weight + h * p.weight_stride, lane, lanes, true);
+            x.each([&](T& v, int n) { v = v * r * w.at(n); });
+        }
+        x.turn(c, s);
+        if (live) x.store(p, (T*)p.y + b * p.y_stride[0] + h * p.y_stride[1] + l * p.y_stride[2], lane, lanes);
+    }
+}
+
+// Gradient with a norm.  A block owns up to HEADS heads and every `slots`-th run of tokens, its groups one token
+// each; a lane keeps the sums of its elements of dw, the groups meet in LDS, the blocks in `rotary_dw`.
+constexpr int kHeads = 2;
+
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(kThreads) void rotary_grad_kernel(Rot p, int lanes_log, int slots) {
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    const int lanes = 1 << lanes_log, groups = kThreads >> lanes_log;
+    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
+    const int slot = blockIdx.x % slots, h0 = blockIdx.x / slots * kHeads;
+    const int64_t tokens = (int64_t)p.batch * p.rows;
+    double f[4];
+    frequencies<T, WIDE>(p, lane, lanes, f);
+    Row<T, WIDE> w[kHeads];
+    T sums[kHeads][16];
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+        w[k].load(p, (const T*)p.weight + (h0 + k) * p.weight_stride, lane, lanes, h0 + k < p.heads);
+#pragma unroll
+        for (int n = 0; n < 16; ++n) sums[k][n] = 0;
+    }
+    for (int64_t t0 = (int64_t)slot * groups; t0 < tokens; t0 += (int64_t)slots * groups) {
+        const int64_t token = t0 + group;
+        const bool live = token < tokens;
+        const int b = live ? (int)(token / p.rows) : 0, l = live ? (int)(token % p.rows) : 0;
+        T c[4], s[4];
+        angles<T>(p, position_of(p, b, l), f, c, s);
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+            const int h = h0 + k;
+            const bool in = live && h < p.heads;
+            Row<T, WIDE> x, g;
+            x.load(p, (const T*)p.x + b * p.x_stride[0] + h * p.x_stride[1] + l * p.x_stride[2], lane, lanes, in);
+            g.load(p, (const T*)p.dy + b * p.dy_stride[0] + h * p.dy_stride[1] + l * p.dy_stride[2], lane, lanes, in);
+            g.turn(c, s);
+            T square = 0, dot = 0;
+            x.each([&](T& v, int n) {
+                square += v * v;
+                dot += v * g.at(n) * w[k].at(n);
+            });
+            square = group_sum(square, lanes);
+            dot = group_sum(dot, lanes);
+            const T r = T(1) / root(square / T(p.d) + T(p.eps));
+            const T mean = dot * r * r / T(p.d);            // mean(w g xhat) r
+            Row<T, WIDE> out;
+            out.each([&](T& v, int n) {
+                const T hat = x.at(n) * r;
+                sums[k][n] += in ? g.at(n) * hat : T(0);
+                v = r * g.at(n) * w[k].at(n) - x.at(n) * r * mean;
+            });
+            if (in) out.store(p, (T*)p.y + b * p.y_stride[0] + h * p.y_stride[1] + l * p.y_stride[2], lane, lanes);
+        }
+    }
+    // [k][n][lane] summed over the groups in their order
+    T* lds = (T*)shared;
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+        if (k) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 16; ++n) lds[n * kThreads + threadIdx.x] = sums[k][n];
+        __syncthreads();
+        if (group == 0 && h0 + k < p.heads) {
+            Row<T, WIDE> total;
+            total.each([&](T& v, int n) {
+                T x = 0;
+                for (int j = 0; j < groups; ++j) x += lds[n * kThreads + j * lanes + lane];
+                v = x;
+            });
+            total.store(p, (T*)p.work + ((int64_t)slot * p.heads + h0 + k) * p.d_pad, lane, lanes);
+        }
+    }
+}
+
+// dw from the blocks' parts; a weight shared by the heads takes all of theirs
+template <typename T> __global__ __launch_bounds__(kThreads) void rotary_dw(Rot p, int slots) {
+    __shared__ double lds[4][64];
+    const int d = (int)blockIdx.x % ((p.d + 63) / 64) * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    const int head = blockIdx.x / ((p.d + 63) / 64);
+    const bool shared_weight = p.weight_stride == 0;
+    const int64_t count = shared_weight ? (int64_t)slots * p.heads : slots;
+    double sum = 0.0;
+    if (d < p.d)
+        for (int64_t n = part; n < count; n += 4)
+            sum += (double)((const T*)p.work)[(shared_weight ? n : n * p.heads + head) * p.d_pad + d];
+    lds[part][threadIdx.x & 63] = sum;
+    __syncthreads();
+    if (part == 0 && d < p.d) {
+        const int k = threadIdx.x & 63;
+        ((T*)p.dweight)[(int64_t)head * p.d + d] = (T)(((lds[0][k] + lds[1][k]) + lds[2][k]) + lds[3][k]);
+    }
+}
+
+int lanes_log_of(const Rot& p) {
+    const int half = p.dims / 2, behind = p.d - p.dims;
+    int lanes = (half + 3) / 4;
+    if ((behind + 7) / 8 > lanes) lanes = (behind + 7) / 8;
+    int log = 0;
+    while ((1 << log) < lanes) ++log;
+    return log;
+}
+
+bool quads(const void* p, const int64_t* stride, int n, int item) {
+    if (!p) return true;
+    if ((uintptr_t)p % 16) return false;
+    for (int i = 0; i < n; ++i)
+        if (stride[i] * item % 16) return false;
+    return true;
+}
+
+bool wide_of(const Rot& p) {
+    const int item = p.is_double ? 8 : 4, half = p.dims / 2;
+    return half % 4 == 0 && (p.d - p.dims) % 4 == 0 && quads(p.x, p.x_stride, 3, item) && quads(p.y, p.y_stride, 3, item) &&
+           quads(p.dy, p.dy_stride, 3, item) && quads(p.weight, &p.weight_stride, 1, item);
+}
+
+// Blocks for each pair of heads in the gradient: about 2048 in all (8 for a compute unit), and at least
+// eight tokens for each group, so that the parts of dw stay small against dx
+int grad_slots(const Rot& p) {
+    const int64_t sets = (p.heads + kHeads - 1) / kHeads, groups = kThreads >> lanes_log_of(p);
+    const int64_t runs = ((int64_t)p.batch * p.rows + groups - 1) / groups;
+    int64_t slots = 2048 / sets;
+    if (slots > (runs + 7) / 8) slots = (runs + 7) / 8;
+    return slots < 1 ? 1 : (int)slots;
+}
+
+template <typename T> void launch_rotary(const Rot& p, hipStream_t s) {
+    const int log = lanes_log_of(p);
+    const int64_t tokens = (int64_t)p.batch * p.rows;
+    int slots = (p.heads + 7) / 8;                           // eight heads share the angles ...
+    while (slots < p.heads && tokens * slots << log < 256 * 2048) slots = slots * 2 < p.heads ? slots * 2 : p.heads;  // ... where there are enough tokens
+    const int64_t groups = tokens * slots;
+    const unsigned blocks = (unsigned)(((groups << log) + kThreads - 1) / kThreads);
+    if (wide_of(p))
+        rotary_kernel<T, true><<<blocks, kThreads, 0, s>>>(p, log, slots, groups);
+    else
+        rotary_kernel<T, false><<<blocks, kThreads, 0, s>>>(p, log, slots, groups);
+}
+
+template <typename T> void launch_rotary_grad(const Rot& p, hipStream_t s) {
+    const int log = lanes_log_of(p), slots = grad_slots(p);
+    const unsigned blocks = (unsigned)(((p.heads + kHeads - 1) / kHeads) * slots);
+    const unsigned lds = 16 * kThreads * sizeof(T);
+    if (wide_of(p))
+        rotary_grad_kernel<T, true><<<blocks, kThreads, lds, s>>>(p, log, slots);
+    else
+        rotary_grad_kernel<T, false><<<blocks, kThreads, lds, s>>>(p, log, slots);
+    const unsigned parts = (unsigned)((p.d + 63) / 64 * (p.weight_stride ? p.heads : 1));
+    rotary_dw<T><<<parts, kThreads, 0, s>>>(p, slots);
+}
+
+// ---- drawing tokens ---------------------------------------------------------------------------
+//
+// Tokens in the order (logit falling, number rising); weights exp((logit - largest) / temperature).  top-k
+// keeps the first k, top-p the first ones until their weight reaches p of what is left, min-p those of at
+// least min_p of the largest weight: all three are beginnings of that order.  The token is the first one,
+// by number, at which the kept weight summed from token 0 exceeds u times all kept weight.
+//
+// Nothing is sorted: the ends of the kept beginnings are found digit by digit of the logits' bits (11, 11,
+// 10), from counts and weights of the digits.  Weights are 64-bit whole numbers (the largest 2^s, s such
+// that all fit; computed in float64), so that sums do not depend on their order.  A block for each row.
+
+typedef drhip_sample_t Smp;
+typedef unsigned long long u64;
+constexpr int kDraw = 1024;          // threads of a block
+constexpr int kBins = 2048;
+constexpr int kChunks = 2048;        // parts of a row whose weights are kept for the last search
+
+__device__ __forceinline__ unsigned key_of(float x) {
+    if (x != x) return 0;                                    // a NaN is below everything and never drawn
+    const unsigned u = __float_as_uint(x + 0.0f);            // (-0 and 0 are equal)
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+struct Weigher {
+    float top;
+    double by, one;       // 1 / temperature, 2^s
+    __device__ __forceinline__ double real(float x) const { return x == top ? 1.0 : x != x ? 0.0 : exp(((double)x - (double)top) * by); }
+    __device__ __forceinline__ u64 whole(double w) const { return (u64)(w * one + 0.5); }
+};
+
+// Sum over the threads before this one, and over all (four barriers; `lds`: 17 words)
+__device__ __forceinline__ u64 scan(u64 x, u64* lds, u64& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    u64 sum = x;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const u64 y = __shfl_up(sum, m);
+        if (lane >= m) sum += y;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = sum;
+    __syncthreads();
+    u64 before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kDraw / 64; ++w) {
+        if (w < wave) before += lds[w];
+        total += lds[w];
+    }
+    all = total;
+    return before + sum - x;
+}
+
+struct Found {
+    unsigned bin;
+    u64 before;       // of the bins above it
+};
+
+// The highest bins first: the one in which the running sum first reaches `want` (1 <= want <= all)
+__device__ __forceinline__ Found reach(const u64* hist, u64 want, u64* lds, Found* out) {
+    const int i = kBins - 1 - 2 * threadIdx.x;
+    const u64 x = hist[i], y = hist[i - 1];
+    u64 all;
+    const u64 before = scan(x + y, lds, all);
+    if (before < want && want <= before + x) *out = {(unsigned)i, before};
+    if (before + x < want && want <= before + x + y) *out = {(unsigned)(i - 1), before + x};
+    __syncthreads();
+    return *out;
+}
+
+// The key at which the running sum (of counts, or of weights) over falling keys first reaches `want`, over the
+// tokens with keys of at least `least`; before: the sum of the larger ones
+template <bool COUNT>
+__device__ unsigned select(const float* row, int v, unsigned least, u64 ties, unsigned tie_key, u64 want, const Weigher& weigh,
+                           u64* hist, u64* lds, Found* found, u64& before) {
+    unsigned prefix = 0;
+    before = 0;
+#pragma unroll
+    for (int level = 0; level < 3; ++level) {
+        const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
+        const int bits = level == 2 ? 10 : 11;
+        for (int i = threadIdx.x; i < kBins; i += kDraw) hist[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < v; i += kDraw) {
+            const float x = row[i];
+            const unsigned key = key_of(x);
+            if (key < least || key == tie_key) continue;
+            if (level && key >> (shift + bits) != prefix) continue;
+            atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], COUNT ? 1 : weigh.whole(weigh.real(x)));
+        }
+        // the tokens at the end of the top-k beginning are equal: as many as it keeps, at once
+        if (!COUNT && threadIdx.x == 0 && ties && (!level || tie_key >> (shift + bits) == prefix))
+            atomicAdd(&hist[tie_key >> shift & ((1u << bits) - 1)], ties * weigh.whole(weigh.real(value_of(tie_key))));
+        __syncthreads();
+        const Found f = reach(hist, want - before, lds, found);
+        before += f.before;
+        prefix = prefix << bits | f.bin;
+        __syncthreads();
+    }
+    return prefix;
+}
+
+__global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
+    __shared__ u64 hist[kBins], lds[kDraw / 64 + 1];
+    __shared__ unsigned marks[kChunks];
+    __shared__ Found found;
+    __shared__ int chunk_at;
+    __shared__ u64 chunk_before, chunk_tied;
+    if (threadIdx.x == 0) chunk_at = 0, chunk_before = 0, chunk_tied = 0, found = {0, 0};
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float* row = p.logits + b * p.logits_stride;
+    const int v = p.vocabulary;
+
+    // largest logit, lowest number first
+    u64 best = 0;
+    for (int i = threadIdx.x; i < v; i += kDraw) {
+        const u64 x = (u64)key_of(row[i]) << 32 | (unsigned)~i;
+        best = x > best ? x : best;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const u64 y = __shfl_xor(best, m);
+        best = y > best ? y : best;
+    }
+    if (lane == 0) lds[wave] = best;
+    __syncthreads();
+    best = 0;
+#pragma unroll
+    for (int w = 0; w < kDraw / 64; ++w) best = lds[w] > best ? lds[w] : best;
+    __syncthreads();
+    const unsigned top_key = (unsigned)(best >> 32);
+    const double temperature = p.temperature ? p.temperature[b] : p.temperature_all;
+    const bool none = top_key <= key_of(-__builtin_inff());
+    if (none || !(temperature > 0.0)) {
+        if (threadIdx.x == 0) p.tokens[b] = none ? -1 : (int64_t)(int)~(unsigned)best;
+        return;
+    }
+    Weigher weigh{value_of(top_key), 1.0 / temperature, p.one};
+    const int64_t k = p.top_k ? p.top_k[b] : p.top_k_all;
+    const double top_p = p.top_p ? p.top_p[b] : p.top_p_all;
+    double min_p = p.min_p ? p.min_p[b] : p.min_p_all;
+    if (!(min_p > 0.0)) min_p = 0.0;
+    if (min_p > 1.0) min_p = 1.0;
+
+    // end of what is kept: keys above `cut`, and the first `ties` tokens whose key it is
+    const unsigned no_key = ~0u;       // (of no number)
+    unsigned cut = 0;
+    u64 ties = ~0ull, before;
+    bool all = true;
+    if (k > 0 && k < v) {
+        cut = select<true>(row, v, 0, 0, no_key, (u64)k, weigh, hist, lds, &found, before);
+        ties = (u64)k - before;
+        all = false;
+    }
+    if (top_p < 1.0) {
+        // weight of the beginning so far
+        u64 sum = 0, weight;
+        for (int i = threadIdx.x; i < v; i += kDraw) {
+            const float x = row[i];
+            const unsigned key = key_of(x);
+            if (all || key > cut) sum += weigh.whole(weigh.real(x));
+        }
+        scan(sum, lds, weight);
+        const u64 tied = all ? 0 : ties * weigh.whole(weigh.real(value_of(cut)));
+        weight += tied;
+        const double goal = top_p * (double)weight;
+        u64 want = goal >= (double)weight ? weight : (u64)ceil(goal);
+        if (want < 1) want = 1;
+        const unsigned from = all ? 0 : cut;
+        const unsigned end = select<false>(row, v, from, all ? 0 : ties, all ? no_key : cut, want, weigh, hist, lds, &found, before);
+        const u64 each = weigh.whole(weigh.real(value_of(end)));
+        u64 n = each ? (want - before + each - 1) / each : 1;
+        if (!all && end == cut && n > ties) n = ties;
+        cut = end;
+        ties = n;
+        all = false;
+    }
+
+    // weights and ties of the parts of the row, then the part and the token in which the draw falls
+    const int chunk = max(512, ((v + kChunks - 1) / kChunks + 63) & ~63), chunks = (v + chunk - 1) / chunk;
+    for (int c = wave; c < chunks; c += kDraw / 64) {
+        u64 sum = 0;
+        unsigned tied = 0;
+        for (int i = c * chunk + lane; i < min(v, (c + 1) * chunk); i += 64) {
+            const float x = row[i];
+            const unsigned key = key_of(x);
+            if (!all && key < cut) continue;
+            const double w = weigh.real(x);
+            if (w < min_p) continue;
+            if (!all && key == cut) ++tied;
+            else sum += weigh.whole(w);
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            sum += __shfl_xor(sum, m);
+            tied += __shfl_xor(tied, m);
+        }
+        if (lane == 0) hist[c] = sum, marks[c] = tied;
+    }
+    __syncthreads();
+    const u64 each = all ? 0 : weigh.whole(weigh.real(value_of(cut)));
+    const int c0 = 2 * threadIdx.x;
+    const unsigned t0 = c0 < chunks ? marks[c0] : 0, t1 = c0 + 1 < chunks ? marks[c0 + 1] : 0;
+    u64 every;
+    const u64 tied_before = scan(t0 + t1, lds, every);
+    auto kept = [&](u64 from, u64 count) { return from >= ties ? 0 : (ties - from < count ? ties - from : count); };
+    const u64 w0 = c0 < chunks ? hist[c0] + each * kept(tied_before, t0) : 0;
+    const u64 w1 = c0 + 1 < chunks ? hist[c0 + 1] + each * kept(tied_before + t0, t1) : 0;
+    u64 weight;
+    const u64 weight_before = scan(w0 + w1, lds, weight);
+    const double u = p.uniforms_wide ? ((const double*)p.uniforms)[b] : (double)((const float*)p.uniforms)[b];
+    const double goal = u * (double)weight;
+    u64 target = goal > 0.0 ? (goal >= (double)weight ? weight - 1 : (u64)goal) : 0;
+    if (target >= weight) target = weight - 1;
+    if (weight_before <= target && target < weight_before + w0) chunk_at = c0, chunk_before = weight_before, chunk_tied = tied_before;
+    if (weight_before + w0 <= target && target < weight_before + w0 + w1) chunk_at = c0 + 1, chunk_before = weight_before + w0, chunk_tied = tied_before + t0;
+    __syncthreads();
+    if (wave) return;
+    u64 sum = chunk_before, tied = chunk_tied;
+    int token = 0;
+    const int first = chunk_at * chunk;
+    for (int i0 = first; i0 < min(v, first + chunk); i0 += 64) {
+        const int i = i0 + lane;
+        const float x = i < v ? row[i] : -__builtin_inff();
+        const unsigned key = key_of(x);
+        const double w = weigh.real(x);
+        bool in = i < v && (all || key >= cut) && w >= min_p;
+        const bool tie = in && !all && key == cut;
+        const u64 m = __ballot(tie);
+        if (tie) in = tied + __popcll(m & ((1ull << lane) - 1)) < ties;
+        tied += __popcll(m);
+        u64 run = in ? weigh.whole(w) : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const u64 y = __shfl_up(run, d);
+            if (lane >= d) run += y;
+        }
+        const u64 past = __ballot(sum + run > target);
+        if (past) {
+            token = i0 + __builtin_ctzll(past);
+            break;
+        }
+        sum += __shfl(run, 63);
+    }
+    if (lane == 0) p.tokens[b] = token;
+}
+
+}  // namespace
+
+extern "C" uint64_t drhip_k_rotary_work(const drhip_rotary_t* p) {
+    if (!p->dweight) return 0;
+    return (uint64_t)grad_slots(*p) * p->heads * p->d_pad * (p->is_double ? 8 : 4);
+}
+
+extern "C" int drhip_k_rotary(const drhip_rotary_t* p, hipStream_t s) {
+    if (p->dweight)
+        p->is_double ? launch_rotary_grad<double>(*p, s) : launch_rotary_grad<float>(*p, s);
+    else
+        p->is_double ? launch_rotary<double>(*p, s) : launch_rotary<float>(*p, s);
+    return (int)hipGetLastError();
+}
+
+extern "C" int drhip_k_sample(const drhip_sample_t* p, hipStream_t s) {
+    sample_kernel<<<p->batch, kDraw, 0, s>>>(*p);
+    return (int)hipGetLastError();
+}

@@ -309,10 +309,8 @@ class DelayArray(numpy.lib.mixins.NDArrayOperatorsMixin):
                 return res
         return NPArray(self._force()[key])
 
-    def __setitem__(self, key, item):
-        """Write into the materialised array.  A lazy right-hand side is handed
-        to the backend as one fused kernel writing straight into the destination
-        (the reference evaluates it to a temporary first, delayarray.py:114-121)."""
+    def _written(self):
+        """The materialised array, about to be written to."""
         arr = self._force()
         # written to by hand, the result is an array in its own right from now on: it
         # must not be recomputed (and the write lost) when one of its inputs changes,
@@ -330,6 +328,13 @@ class DelayArray(numpy.lib.mixins.NDArrayOperatorsMixin):
             own = d.get("_key")
             if own is not None and Memoiser._cache.get(own) is self:
                 Memoiser._cache.pop(own)
+        return arr
+
+    def __setitem__(self, key, item):
+        """Write into the materialised array.  A lazy right-hand side is handed
+        to the backend as one fused kernel writing straight into the destination
+        (the reference evaluates it to a temporary first, delayarray.py:114-121)."""
+        arr = self._written()
         key = _unwrap(key)
         check = getattr(arr, "check_writable", None)
         if check is not None:
@@ -1837,7 +1842,7 @@ for _name in ("empty", "empty_like", "eye", "identity", "ones", "ones_like", "ze
               "zeros_like", "full", "full_like", "array", "asarray", "asanyarray",
               "ascontiguousarray", "copy", "arange", "linspace", "logspace", "tri", "tril",
               "triu", "asmatrix", "frombuffer", "fromfile", "fromfunction", "fromiter",
-              "fromstring", "loadtxt", "geomspace", "vander"):
+              "fromstring", "loadtxt", "geomspace", "vander", "from_dlpack"):
     _fn = getattr(_backend.fallback, _name, None)
     if _fn is not None:
         globals()[_name] = cast(_fn)

@@ -8,6 +8,7 @@ returns views of the same buffer, as the front end's `__getitem__` /
 `__setitem__` expect (delayarray.py:114-128).  All data movement and compute
 goes through libdrhip; nothing here computes on the host.
 """
+import ctypes as C
 import numbers
 import warnings
 
@@ -57,6 +58,51 @@ class Buffer:
         if self.shadow:
             _free(self.shadow)
             self.shadow = None
+
+
+_LEAVING = []     # (event, owner) of borrowed memory whose last view is gone
+
+
+class Borrowed(Buffer):
+    """Device memory of another library, as `from_dlpack` takes it over.  `owner` is kept until
+    the work queued here when the last view went has run: the other library may hand the
+    memory out again as soon as its object is released.  The address never changes: updates
+    that read what they overwrite copy back instead of swapping allocations (hip._write)."""
+
+    __slots__ = ("owner",)
+
+    def __init__(self, nbytes, ptr, owner):
+        self.owner = None
+        super().__init__(nbytes, ptr)
+        self.owner = owner
+
+    def __del__(self, _free=hiprt.free, _rt=hiprt, _leaving=_LEAVING):
+        if self.shadow:
+            _free(self.shadow)
+            self.shadow = None
+        self.ptr = None
+        owner, self.owner = self.owner, None
+        if owner is None:
+            return
+        try:
+            _leaving.append((None if _rt.Graph.capturing else _rt.Event().record(), owner))
+        except Exception:       # interpreter shutdown: the process releases everything
+            return
+        release_borrowed()
+
+
+def release_borrowed():
+    """Let go of the borrowed memory that nothing queued uses any more."""
+    if hiprt.Graph.capturing:
+        return
+    for _ in range(len(_LEAVING)):
+        if not _LEAVING:        # (releasing an owner can run this again)
+            return
+        event, owner = _LEAVING.pop(0)
+        if event is None:
+            event = hiprt.Event().record()
+        if not event.done():
+            _LEAVING.append((event, owner))
 
 
 class _Placeholder(Buffer):
@@ -394,3 +440,58 @@ def placeholder(shape, dtype, strides=None, offset=0, buf=None):
     if buf is None:
         buf = _Placeholder((offset + size) * np.dtype(dtype).itemsize)
     return ndarray(shape, dtype, buf, offset, strides)
+
+
+# ---- arrays of other libraries (the DLPack protocol, as numpy.from_dlpack) -----------------
+
+class _DLTensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("device_type", C.c_int32), ("device_id", C.c_int32),
+                ("ndim", C.c_int32), ("code", C.c_uint8), ("bits", C.c_uint8),
+                ("lanes", C.c_uint16), ("shape", C.POINTER(C.c_int64)),
+                ("strides", C.POINTER(C.c_int64)), ("byte_offset", C.c_uint64)]
+
+
+_capsule_pointer = C.pythonapi.PyCapsule_GetPointer
+_capsule_pointer.restype = C.c_void_p
+_capsule_pointer.argtypes = [C.py_object, C.c_char_p]
+
+_DL_HOST, _DL_ROCM = (1, 3, 11), 10
+_DL_KINDS = {0: "int", 1: "uint", 2: "float", 6: "bool"}
+
+
+def from_dlpack(x):
+    """Array over the memory of another library's device array, without a copy (host arrays
+    are uploaded).  Work queued there before the call is waited for on the device; later
+    work, in either direction, is for the caller to order (`synchronize()`).  Take each array
+    over once and keep it: two arrays over one memory do not see each other's writes as
+    changes of a cached result."""
+    device_type, device = x.__dlpack_device__()
+    if device_type in _DL_HOST:
+        return ndarray.from_host(np.from_dlpack(x))
+    if device_type != _DL_ROCM:
+        raise BufferError(f"from_dlpack takes host arrays and arrays of a ROCm device, not of device type {int(device_type)}")
+    hiprt.init()
+    if device != hiprt.device():
+        raise BufferError(f"the array is on device {device}, this library runs on device {hiprt.device()}")
+    if hiprt.Graph.capturing:
+        raise RuntimeError("from_dlpack is not allowed while capturing a graph")
+    release_borrowed()
+    capsule = x.__dlpack__(stream=hiprt.stream())
+    t = _DLTensor.from_address(_capsule_pointer(capsule, b"dltensor"))
+    kind = _DL_KINDS.get(t.code)
+    name = "bool" if kind == "bool" else f"{kind}{t.bits}"
+    if kind is None or t.lanes != 1 or name not in SUPPORTED_DTYPES:
+        raise TypeError(f"dtype {name if kind else 'of DLPack code %d' % t.code} is not supported on the device")
+    dtype = np.dtype(name)
+    shape = tuple(t.shape[i] for i in range(t.ndim))
+    strides = tuple(t.strides[i] for i in range(t.ndim)) if t.strides else _contiguous_strides(shape)
+    lo = hi = 0
+    for d, s in zip(shape, strides):
+        lo, hi = lo + min(0, (d - 1) * s), hi + max(0, (d - 1) * s)
+    if 0 in shape:
+        lo, hi = 0, -1
+    ptr = (t.data or 0) + t.byte_offset + lo * dtype.itemsize
+    if ptr % dtype.itemsize:
+        raise BufferError("the array's elements are not aligned")
+    buf = Borrowed((hi - lo + 1) * dtype.itemsize, ptr, capsule)
+    return ndarray(shape, dtype, buf, -lo, strides)

@@ -27,7 +27,7 @@ import numpy
 
 from . import codegen as cg
 from . import hiprt
-from .devarray import Buffer, ndarray, placeholder  # noqa: F401
+from .devarray import Borrowed, Buffer, ndarray, placeholder, release_borrowed  # noqa: F401
 from .codegen import Program, dtype_code, code_dtype
 from .promote import result_dtype, scalar_descr
 from .visitor import Visitor
@@ -80,6 +80,7 @@ def is_ndarray(arr):
 
 def synchronize():
     hiprt.sync()
+    release_borrowed()
 
 
 # ---------------------------------------------------------------------------
@@ -493,7 +494,9 @@ class Replay:
 
     def _issue_all(self):
         for func, grid, lds, args, slot, scratch in self.launches:
-            if slot is None:
+            if grid is None:              # an operator of the library
+                func(args)
+            elif slot is None:
                 hiprt.launch(func, grid, _BLOCK_OF.get(func, cg.BLOCK), lds, args, len(args))
             else:
                 hiprt.launch_scratch(func, grid, _BLOCK_OF.get(func, cg.BLOCK), lds, args, len(args), slot, scratch)
@@ -649,6 +652,19 @@ def _issue(func, grid, args, slot=None, scratch=0):
     if _RECORDING is not None:
         _RECORDING.launches.append((func, grid, 0, args, slot, scratch))
     STATS["launches"] += 1
+
+
+def issue_operator(func, args, used, written):
+    """Launch (and record) one of the library's own operators: `func(args)` with a packed
+    argument struct; `used`: what it reads and writes, workspaces among it."""
+    func(args)
+    STATS["launches"] += 1
+    for arr in written:
+        arr.buf.touch()
+    if _RECORDING is not None:
+        _RECORDING.launches.append((func, None, None, args, None, 0))
+        _RECORDING.keep += used
+        _RECORDING.written += [(arr.buf, False) for arr in written]
 
 
 _SCRATCH_BYTES = hiprt.scratch_bytes()
@@ -1367,12 +1383,20 @@ def _write(plan, dst):
         if buf.shadow is None:
             buf.shadow = hiprt.malloc(max(buf.nbytes, 1))
             buf.shadow_region = None
+        borrowed = type(buf) is Borrowed       # its address is another library's too
+        if borrowed and _RECORDING is not None:
+            raise RuntimeError("hip.record(): an update that reads what it overwrites cannot be recorded "
+                               "for an array taken over from another library")
         if buf.shadow_region != plan.region:
             hiprt.memcpy_d2d(buf.shadow, buf.ptr, buf.nbytes)
         _fire(plan, [buf.shadow + off])
-        buf.ptr, buf.shadow = buf.shadow, buf.ptr
-        buf.shadow_region = plan.region
-        buf.version += 1
+        if borrowed:
+            hiprt.memcpy_d2d(buf.ptr, buf.shadow, buf.nbytes)
+            buf.touch()
+        else:
+            buf.ptr, buf.shadow = buf.shadow, buf.ptr
+            buf.shadow_region = plan.region
+            buf.version += 1
     if _RECORDING is not None:
         _RECORDING.keep += [dst] + plan.leaves
         _RECORDING.written.append((buf, plan.hazard))
@@ -1465,3 +1489,4 @@ def compile_source(source):
 # the `np` and `fallback` namespaces of the backend protocol live in arrayns.py (it
 # imports this module, hence the late import)
 from .arrayns import fallback, np  # noqa: E402,F401
+from . import hip_nn as operators  # noqa: E402,F401

@@ -8,6 +8,7 @@ raises.
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdrhip.so")
@@ -75,6 +76,13 @@ _SIGNATURES = {
     "drhip_copy_kernel": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_uint]),
     "drhip_matmul": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p] + [C.c_int64] * 6),
     "drhip_cumsum": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_size_t]),
+    "drhip_attention_work": (C.c_int, [C.c_char_p, C.c_int, C.POINTER(C.c_uint64)]),
+    "drhip_attention": (C.c_int, [C.c_char_p]),
+    "drhip_attention_grad": (C.c_int, [C.c_char_p]),
+    "drhip_rotary_work": (C.c_int, [C.c_char_p, C.POINTER(C.c_uint64)]),
+    "drhip_rotary": (C.c_int, [C.c_char_p]),
+    "drhip_sample": (C.c_int, [C.c_char_p]),
+    "drhip_stream": (C.c_int, [C.POINTER(C.c_void_p)]),
     "drhip_compile": (C.c_int, [C.c_char_p, C.c_char_p, C.POINTER(C.c_char_p), C.c_int,
                                 C.POINTER(C.c_void_p)]),
     "drhip_code_get": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(C.c_size_t)]),
@@ -95,12 +103,14 @@ _SIGNATURES = {
     "drhip_event_destroy": (C.c_int, [C.c_void_p]),
     "drhip_event_record": (C.c_int, [C.c_void_p]),
     "drhip_event_sync": (C.c_int, [C.c_void_p]),
+    "drhip_event_done": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
     "drhip_event_elapsed_ms": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_float)]),
     "drhip_counters": (C.c_int, [C.POINTER(Counters)]),
 }
 
 _lib = None
 _initialised = False
+_device = None
 
 
 def lib():
@@ -132,13 +142,20 @@ def _check(code):
 
 def init(device=None):
     """Initialise the device once; later calls are free."""
-    global _initialised
+    global _initialised, _device
     if _initialised:
         return
     if device is None:
         device = int(os.environ.get("DRHIP_DEVICE", "0"))
     _check(lib().drhip_init(device))
+    _device = device
     _initialised = True
+
+
+def device():
+    """Number of the device the library runs on."""
+    init()
+    return _device
 
 
 def device_info():
@@ -202,6 +219,57 @@ def matmul(is_double, a, b, c, m, n, k, lda, ldb, ldc):
 
 def cumsum(kind, src, dst, n):
     _check(_lib.drhip_cumsum(kind, src, dst, n))
+
+
+# The argument structs of the operators are packed as bytes (native alignment), in the order of
+# include/drhip.h; `work` and `work_bytes` are the last pointer and the word behind it.
+ATTENTION = struct.Struct("@15PQ25q10i2f")
+ROTARY = struct.Struct("@8PQ12q5d9i")
+SAMPLE = struct.Struct("@7Pq4d4i")
+
+
+def attention_work(args, grad):
+    n = C.c_uint64()
+    _check(lib().drhip_attention_work(args, int(grad), C.byref(n)))
+    return n.value
+
+
+def attention(args):
+    rc = _lib.drhip_attention(args)
+    if rc:
+        _check(rc)
+
+
+def attention_grad(args):
+    rc = _lib.drhip_attention_grad(args)
+    if rc:
+        _check(rc)
+
+
+def rotary_work(args):
+    n = C.c_uint64()
+    _check(lib().drhip_rotary_work(args, C.byref(n)))
+    return n.value
+
+
+def rotary(args):
+    rc = _lib.drhip_rotary(args)
+    if rc:
+        _check(rc)
+
+
+def sample(args):
+    rc = _lib.drhip_sample(args)
+    if rc:
+        _check(rc)
+
+
+def stream():
+    """Address of the library's stream, for other libraries to order their work with it."""
+    init()
+    p = C.c_void_p()
+    _check(_lib.drhip_stream(C.byref(p)))
+    return p.value
 
 
 def _opts_array(opts):
@@ -277,13 +345,17 @@ class Graph:
     def __init__(self, handle):
         self.h = handle
 
+    capturing = False
+
     @staticmethod
     def begin():
         init()
         _check(_lib.drhip_graph_begin())
+        Graph.capturing = True
 
     @staticmethod
     def end():
+        Graph.capturing = False
         h = C.c_void_p()
         _check(_lib.drhip_graph_end(C.byref(h)))
         return Graph(h.value)
@@ -314,6 +386,12 @@ class Event:
 
     def synchronize(self):
         _check(_lib.drhip_event_sync(self.h))
+
+    def done(self):
+        """Whether the work queued before the event's record has finished (does not wait)."""
+        x = C.c_int()
+        _check(_lib.drhip_event_done(self.h, C.byref(x)))
+        return bool(x.value)
 
     def elapsed_ms(self, later):
         ms = C.c_float()

@@ -113,6 +113,97 @@ int drhip_matmul(int is_double, const void* a, const void* b, void* c, int64_t m
  * eager, not part of the fused path. */
 int drhip_cumsum(int kind, const void* in_dev, void* out_dev, size_t n);
 
+/* ---- operators of language models ----------------------------------------
+ * No counterpart in the reference.  Device pointers and element strides of
+ * (batch, head, row); the last dimension is dense.  Arguments that a GPU array
+ * holds (lengths, positions ...) cannot be checked here: the kernels clamp
+ * them to what the arrays hold.  Nothing is allocated: `work` is device memory
+ * of at least the bytes that the *_work call of the same arguments gives (it is
+ * only written before it is read within the call), so that the calls can be
+ * captured. */
+
+/* Attention of q[batch][hq][lq][d] to k, v[batch][hkv][lk][d] (hq a multiple of
+ * hkv, d <= 128), float.  Row i stands at position start + i; key j counts for
+ * it if j < lengths (lk without), with `causal` if also j <= position or
+ * j < prefix, with `documents` if documents[j] = documents[position] (none at
+ * positions outside the sequence).
+ * Scores: scale q.k, with cap > 0 cap tanh(scale q.k / cap), with slopes less
+ * slopes[head] |position - j|.  o = softmax(scores) v, lse (may be NULL) the
+ * logarithm of the sum of their exponentials; a row without keys gives zeros
+ * and -inf.  drhip_attention_grad: dq, dk, dv from dout and the forward call's
+ * o and lse. */
+typedef struct drhip_attention_t {
+    const float *q, *k, *v;
+    float *o, *lse;               /* lse: dense [batch][hq][lq]                */
+    const float* dout;            /* gradient only, with dq, dk, dv            */
+    float *dq, *dk, *dv;
+    const int32_t *lengths, *start, *prefix; /* [batch] or NULL                */
+    const int32_t* documents;     /* [batch][lk] or NULL                       */
+    const float* slopes;          /* [hq] or NULL                              */
+    void* work;
+    uint64_t work_bytes;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+    int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+    int64_t documents_stride;
+    int32_t batch, hq, hkv, lq, lk, d;
+    int32_t causal;
+    int32_t start_mode;           /* 0: start = length - lq, 1: start_value (or the array) */
+    int32_t start_value, prefix_value;
+    float scale, cap;
+} drhip_attention_t;
+int drhip_attention_work(const drhip_attention_t* a, int grad, uint64_t* bytes);
+int drhip_attention(const drhip_attention_t* a);
+int drhip_attention_grad(const drhip_attention_t* a);
+
+/* Rotary positions of x[batch][heads][rows][d] (d <= 512), float or double: the
+ * pair of elements number i < dims/2 turns by sign * position * frequency_i *
+ * squeeze, frequency_i = 2^(i * step) or from the table, and is multiplied by
+ * magnitude.  With a weight (weight_stride 0: [d], else [heads][d]) rows are first
+ * divided by the root of their mean square + eps and multiplied by it.
+ * With dweight the call is the gradient of the latter (sign -1): from x and dy, dx
+ * goes to y and the weight's gradient, dense, to dweight. */
+typedef struct drhip_rotary_t {
+    const void* x;
+    void* y;
+    const void *weight, *dy;
+    void* dweight;
+    const void* positions;        /* int32 or int64 [batch or 1][rows]; NULL: first, first + 1 ... */
+    const double* frequencies;
+    void* work;
+    uint64_t work_bytes;
+    int64_t x_stride[3], y_stride[3], dy_stride[3];
+    int64_t weight_stride, positions_stride, first;
+    double step, squeeze, magnitude, sign, eps;
+    int32_t batch, heads, rows, d, dims, d_pad; /* d_pad: d rounded up to 4    */
+    int32_t interleaved, is_double, positions_wide;
+} drhip_rotary_t;
+int drhip_rotary_work(const drhip_rotary_t* p, uint64_t* bytes);
+int drhip_rotary(const drhip_rotary_t* p);
+
+/* One token for each row of logits[batch][vocabulary]: weights exp(logit /
+ * temperature), the top_k largest of them (0: all), the first of those that
+ * hold top_p of their weight, of these the ones of at least min_p of the
+ * largest; the token is the first by number at which their sum exceeds
+ * uniforms[row] of it.  temperature 0: the largest.  Equal logits: the lower
+ * number is the larger.  A row without a logit above -inf gives -1.  Parameters:
+ * an array of one for each row, or one for all.  `one` is the weight of the
+ * largest as a whole number, at most 2^62 / vocabulary. */
+typedef struct drhip_sample_t {
+    const float* logits;
+    const void* uniforms;         /* float or double [batch]                   */
+    int64_t* tokens;
+    const float *temperature, *top_p, *min_p;
+    const int32_t* top_k;
+    int64_t logits_stride;
+    double temperature_all, top_p_all, min_p_all, one;
+    int32_t top_k_all, batch, vocabulary, uniforms_wide;
+} drhip_sample_t;
+int drhip_sample(const drhip_sample_t* p);
+
+/* The library's stream (a hipStream_t), for ordering work of other libraries
+ * with it. */
+int drhip_stream(void** stream);
+
 /* ---- run-time compilation ----------------------------------------------
  * Replaces cupy.ElementwiseKernel(...) construction (cuda.py:35-43), i.e.
  * NVRTC + module load.  `src` is HIP C++ text holding one or more
@@ -180,6 +271,7 @@ int drhip_event_create(void** ev);
 int drhip_event_destroy(void* ev);
 int drhip_event_record(void* ev);            /* on the library stream      */
 int drhip_event_sync(void* ev);
+int drhip_event_done(void* ev, int* done);   /* 1 once the work before it is done */
 int drhip_event_elapsed_ms(void* start, void* stop, float* ms);
 
 /* Counters for the bench harness. */
