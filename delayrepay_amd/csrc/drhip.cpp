@@ -335,7 +335,7 @@ static const char* attention_fault(const drhip_attention_t* a, int grad) {
     if (a->d < 1 || a->d > 128) return "head size outside 1..128";
     if (a->lq >= 1 << 28 || a->lk >= 1 << 28) return "more than 2^28 rows";
     const int64_t heads = (int64_t)a->batch * a->hq;
-    if (heads >= kMostBlocks || heads * (a->lq / 32 + 1) >= kMostBlocks || heads * (a->lk / 128 + 1) >= kMostBlocks)
+    if (heads >= kMostBlocks || heads * (a->lq / 32 + 1) >= kMostBlocks || heads * (a->lk / 32 + 1) >= kMostBlocks)
         return "more blocks than one launch holds";
     if (a->prefix_value < 0) return "negative prefix";
     if (heads && a->lq && (!a->q || !a->o || (a->lk && (!a->k || !a->v)))) return "null operand";

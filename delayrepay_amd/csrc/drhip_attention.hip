@@ -248,23 +248,219 @@ __device__ __forceinline__ float score(const Args& a, float x, float slope2, int
     return z;
 }
 
+
 struct Plan {
-    int few;         // 1: the kernel for few rows
-    int splits, chunk;
-    int wide;
+    int few;             // the kernel for few rows
+    int waves;           // of a block of the other one
+    int splits, chunk;   // key ranges, and keys in one
+    int wide;            // rows can be read and written 16 bytes at a time
 };
 
-// ---- forward, many rows ---------------------------------------------------------------------
-// A block owns 128 rows of the queries that share a key head (row = query head in the group x
-// query position), each wave 32 of them, one per column of its accumulators: S^T = K Q^T leaves the
-// scores of a row in one lane pair, so the softmax needs one exchange, and P^T in the layout that
-// O^T += V^T P^T reads.  Keys and values come 32 at a time through LDS, two buffers, fetched a tile ahead.
+// ---- float32 products on bfloat16 matrix instructions ------------------------------------------
+// v_mfma_f32_32x32x16_bf16 does sixteen times the work of v_mfma_f32_32x32x2_f32 in half its cycles.  A
+// float32 number is the sum of three bfloat16 (8 bits each, rounded to nearest, the differences exact):
+// x = h + m + l up to 2^-27 |x|.  Of the nine products of two such sums the six largest are added, small
+// ones first; the others are below 2^-26 of the product, a quarter of float32's own rounding.  So the result is
+// that of float32 arithmetic at 16 x 2 / 6 = 2.7 times its rate.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+struct Three {
+    bf16x8 p[3];
+};
+
+__device__ __forceinline__ void split2(f32x2 x, int at, Three& out) {
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        const bf16x2 y = __builtin_convertvector(x, bf16x2);
+        out.p[n][at] = y[0], out.p[n][at + 1] = y[1];
+        if (n < 2) x = x - __builtin_convertvector(y, f32x2);
+    }
+}
+
+// (numbers past bfloat16's largest would round to infinity)
+__device__ __forceinline__ float in_range(float x) { return __builtin_amdgcn_fmed3f(x, -3.3895313892515355e38f, 3.3895313892515355e38f); }
+
+__device__ __forceinline__ f32x16 mac6(const Three& a, const Three& b, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
+// A 32-row tile in three planes, 16-byte chunks of eight numbers, in either of two orders.  Both are
+// read by consecutive lanes at consecutive chunks.
+//   by rows:    [plane][element / 8][row][element % 8]              (contracted over elements)
+//   by columns: [plane][group of eight rows][element][row in it]    (contracted over rows)
+// The row groups are those that a lane half holds in eight registers of an accumulator (acc_row), so that
+// weights go from one product to the next without a move.
+template <int NT> struct Planes {
+    static constexpr int PLANE = 32 * 32 * NT;        // numbers
+    static constexpr int BYTES = 3 * PLANE * 2;       // of a tile in one order
+    __device__ __forceinline__ static Three row_chunk(const char* tile, int row, int chunk) {
+        Three x;
+#pragma unroll
+        for (int n = 0; n < 3; ++n) x.p[n] = *(const bf16x8*)(tile + 2 * (n * PLANE + (chunk * 32 + row) * 8));
+        return x;
+    }
+    __device__ __forceinline__ static Three column_chunk(const char* tile, int group, int element) {
+        Three x;
+#pragma unroll
+        for (int n = 0; n < 3; ++n) x.p[n] = *(const bf16x8*)(tile + 2 * (n * PLANE + (group * 32 * NT + element) * 8));
+        return x;
+    }
+};
+
+// acc[row][col] = sum_d tile[row][d] own[col][d]: lane l holds elements 16t + 8h .. + 7 of column l % 32
+template <int NT> __device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[2 * NT], int lane) {
+    f32x16 acc;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2 * NT; ++t) acc = mac6(Planes<NT>::row_chunk(tile, lane & 31, 2 * t + (lane >> 5)), own[t], acc);
+    return acc;
+}
+
+// acc[c][i][col] += sum_row tile[row][32 c + i] w[row][col]
+template <int NT> __device__ __forceinline__ void spread6(f32x16 (&acc)[NT], const char* tile, const f32x16& w, int lane) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        Three x;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) split2(f32x2{w[8 * u + e], w[8 * u + e + 1]}, e, x);
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+            acc[c] = mac6(Planes<NT>::column_chunk(tile, 2 * u + (lane >> 5), 32 * c + (lane & 31)), x, acc[c]);
+    }
+}
+
 template <int NT>
-__global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan, int tiles, float* part, float* part_lse) {
-    using T = Tile<NT>;
-    __shared__ __attribute__((aligned(16))) float lds[2][2][kTile * T::LD];
-    __shared__ unsigned bad[2][2];
-    __shared__ int ends[4], doc_range[2][4];
+__device__ void spread6_bad(f32x16 (&acc)[NT], unsigned bad, const float* base, int64_t stride, int size, const f32x16& w, int lane) {
+    const int h = lane >> 5;
+    while (bad) {
+        const int r = __builtin_ctz(bad);
+        bad &= bad - 1;
+        const int from = 4 * (r >> 3) + (r & 3);
+        float mine = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mine = v == from ? w[v] : mine;
+        const float weight = __shfl(mine, (lane & 31) + 32 * ((r >> 2) & 1));
+        const float* row = base + r * stride;
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int d = 32 * c + acc_row(v, h);
+                const float x = d < size ? row[d] : 0.f;
+                if (!finite_(x) && weight != 0.f) acc[c][v] += weight * x;
+            }
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ void store_column(float* row, const f32x16 (&acc)[NT], float by, int size, bool wide, int h) {
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int d = 32 * c + 8 * u + 4 * h;
+            if (wide) {
+                f32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[c][4 * u + e] * by;
+                if (d < size) *(f32x4*)(row + d) = x;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < size) row[d + e] = acc[c][4 * u + e] * by;
+            }
+        }
+}
+
+// Keys by rows and values by columns, for every tile of 32 that holds a key of its sequence; rows behind
+// the sequence and values that are not finite are zeros, the rows that held one are marked.  Bound by memory:
+// 4 bytes read and 6 written for each number, once for all blocks that read the tile.
+template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Args a, int wide, int tiles, char* planes, unsigned* marks) {
+    __shared__ float lds[2][kTile][32 * NT + 1];
+    __shared__ unsigned bad[2];
+    const int tile = blockIdx.x % tiles, head = blockIdx.x / tiles;
+    const int b = head / a.hkv, kh = head % a.hkv;
+    const int len = sequence(a, b).len;
+    const int j0 = tile * kTile;
+    if (j0 >= len) return;
+    if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+    __syncthreads();
+    const float* base[2] = {a.k + b * a.k_stride[0] + kh * a.k_stride[1], a.v + b * a.v_stride[0] + kh * a.v_stride[1]};
+    const int64_t stride[2] = {a.k_stride[2], a.v_stride[2]};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int p = 0; p < NT; ++p) {
+            const int at = threadIdx.x + p * kThreads, row = at / (8 * NT), d = at % (8 * NT) * 4;
+            f32x4 x = load4(base[n] + (j0 + row) * stride[n], d, a.d, j0 + row < len, wide);
+            bool fine = true;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                fine = fine && finite_(x[c]);
+                lds[n][row][d + c] = finite_(x[c]) ? in_range(x[c]) : 0.f;
+            }
+            if (!fine) atomicOr(&bad[n], 1u << row);
+        }
+    __syncthreads();
+    char* to = planes + ((int64_t)head * tiles + tile) * 2 * Planes<NT>::BYTES;
+    if (threadIdx.x < 2) marks[((int64_t)head * tiles + tile) * 2 + threadIdx.x] = bad[threadIdx.x];
+    for (int at = threadIdx.x; at < 32 * 4 * NT; at += kThreads) {
+        Three x;
+        const int row = at & 31, chunk = at >> 5;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) split2(f32x2{lds[0][row][8 * chunk + e], lds[0][row][8 * chunk + e + 1]}, e, x);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) *(bf16x8*)(to + 2 * (n * Planes<NT>::PLANE + at * 8)) = x.p[n];
+        const int d = at % (32 * NT), group = at / (32 * NT);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const int r = acc_row(8 * (group >> 1) + e, group & 1);
+            split2(f32x2{lds[1][r][d], lds[1][r + 1][d]}, e, x);
+        }
+#pragma unroll
+        for (int n = 0; n < 3; ++n) *(bf16x8*)(to + Planes<NT>::BYTES + 2 * (n * Planes<NT>::PLANE + at * 8)) = x.p[n];
+    }
+}
+
+// `bytes` (a multiple of 1024) from memory to LDS without a register between, by the block's waves in turn
+template <int WAVES> __device__ __forceinline__ void copy_to_lds(char* lds, const char* from, int bytes) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int at = wave * 1024; at < bytes; at += WAVES * 1024)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + at + lane * 16),
+                                         (__attribute__((address_space(3))) void*)(lds + at), 16, 0, 0);
+}
+
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Whether the keys of a tile are of the lane's row's document, as bits in the order of the accumulator's registers
+__device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) {
+    unsigned m = 0;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        const int lo = __builtin_amdgcn_readlane(key_docs, acc_row(v, 0)), hi = __builtin_amdgcn_readlane(key_docs, acc_row(v, 1));
+        m |= ((h ? hi : lo) == doc ? 1u : 0u) << v;
+    }
+    return m;
+}
+
+// ---- forward, many rows ---------------------------------------------------------------------
+// A block owns 32 WAVES rows of the queries that share a key head (row = query head in the group x query
+// position), each wave 32 of them, one per column of its accumulators: S^T = K Q^T leaves the scores of a
+// row in one lane pair, so the softmax needs one exchange, and P^T in the layout that O^T += V^T P^T reads.
+// Keys and values come 32 at a time from the packed planes through LDS, two buffers, copied a tile ahead.
+template <int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, const char* planes, const unsigned* marks, float* part, float* part_lse) {
+    using P = Planes<NT>;
+    __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
+    __shared__ int ends[WAVES], doc_range[2][WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int heads = a.batch * a.hkv;
     int id = blockIdx.x;
@@ -277,7 +473,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan,
     const bool wide = plan.wide;
 
     const int rows = group * a.lq;
-    const int r = tile * kRows + wave * 32 + (lane & 31);
+    const int r = (tile * WAVES + wave) * 32 + (lane & 31);
     const bool valid = r < rows;
     const int g = valid ? r / a.lq : 0, i = valid ? r - g * a.lq : 0;
     const int qh = kh * group + g, p = s.start + i;
@@ -285,12 +481,18 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan,
     const int doc = s.docs && lim > 0 ? s.docs[p] : 0;
     const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
 
-    f32x4 own[4 * NT];
+    // scores come out in units of log 2, or with a cap as they are
+    const float scale = a.cap > 0.f ? a.scale : a.scale * kLog2e;
+    Three own[2 * NT];
     const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
 #pragma unroll
-    for (int t = 0; t < 4 * NT; ++t) {
-        own[t] = load4(qrow, 8 * t + 4 * h, a.d, valid, wide);
-        own[t] *= a.scale;
+    for (int t = 0; t < 2 * NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const f32x4 x = load4(qrow, 16 * t + 8 * h + e, a.d, valid, wide) * scale;
+            split2(f32x2{x[0], x[1]}, e, own[t]);
+            split2(f32x2{x[2], x[3]}, e + 2, own[t]);
+        }
     }
 
     // range of limits (and documents) in the wave and in the block
@@ -303,23 +505,30 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan,
         dhi = max(dhi, __shfl_xor(dhi, m));
     }
     if (lane == 0) ends[wave] = top, doc_range[0][wave] = dlo, doc_range[1][wave] = dhi;
-    if (threadIdx.x < 4) (&bad[0][0])[threadIdx.x] = 0;
     __syncthreads();
     const int begin = split * plan.chunk;
-    int end = max(max(ends[0], ends[1]), max(ends[2], ends[3]));
-    dlo = min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3]));
-    dhi = max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3]));
-    if (end > begin + plan.chunk) end = begin + plan.chunk;
+    int end = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        end = max(end, ends[w]);
+        dlo = min(dlo, doc_range[0][w]);
+        dhi = max(dhi, doc_range[1][w]);
+    }
+    end = __builtin_amdgcn_readfirstlane(min(end, begin + plan.chunk));
+    top = __builtin_amdgcn_readfirstlane(top);
+    low = __builtin_amdgcn_readfirstlane(low);
 
-    const float* kbase = a.k + b * a.k_stride[0] + kh * a.k_stride[1];
-    const float* vbase = a.v + b * a.v_stride[0] + kh * a.v_stride[1];
+    const int key_tiles = (a.lk + kTile - 1) / kTile;
+    const char* packed = planes + (int64_t)head * key_tiles * 2 * P::BYTES;
+    const unsigned* marked = marks + (int64_t)head * key_tiles * 2;
+    int docs_next = 0;
     // the first key of the next tile that any row of the block may see
     auto next = [&](int j0) {
         if (s.docs)
             for (; j0 < end; j0 += kTile) {
                 const int j = j0 + (lane & 31);
-                const int x = j < end ? s.docs[j] : 0;
-                if (__any(j < end && x >= dlo && x <= dhi)) break;
+                docs_next = j < end ? s.docs[j] : 0;
+                if (__any(j < end && docs_next >= dlo && docs_next <= dhi)) break;
             }
         return j0;
     };
@@ -331,41 +540,40 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan,
         for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
     float most = -__builtin_inff(), total = 0.f;      // running maximum of the row, sum over this lane's keys
 
-    T tk, tv;
     int j0 = next(begin), buf = 0;
-    if (j0 < end) {
-        tk.fetch(kbase, a.k_stride[2], j0, s.len, a.d, wide);
-        tv.fetch(vbase, a.v_stride[2], j0, s.len, a.d, wide);
-        tk.stage(lds[0][0], &bad[0][0]);
-        tv.stage(lds[0][1], &bad[0][1]);
-    }
-    __syncthreads();
+    if (j0 < end) copy_to_lds<WAVES>(lds[0], packed + (int64_t)(j0 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
     while (j0 < end) {
+        copies_done();
+        __syncthreads();                               // this tile is there, and everyone is done with the other buffer
+        const int docs = docs_next;
         const int j1 = next(j0 + kTile);
-        if (j1 < end) {
-            tk.fetch(kbase, a.k_stride[2], j1, s.len, a.d, wide);
-            tv.fetch(vbase, a.v_stride[2], j1, s.len, a.d, wide);
-        }
+        if (j1 < end) copy_to_lds<WAVES>(lds[buf ^ 1], packed + (int64_t)(j1 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
         if (j0 < top) {                                // some row of this wave sees the tile
-            f32x16 x = product<NT>(lds[buf][0], own, lane);
-            const unsigned kbad = bad[buf][0];
-            const bool whole = j0 + kTile <= low && !s.docs && !kbad;
+            const unsigned kbad = marked[j0 / kTile * 2], vbad = marked[j0 / kTile * 2 + 1];
+            f32x16 x = product6<NT>(lds[buf], own, lane);
+            if (a.cap > 0.f) {
+                const float by = 1.f / a.cap, to = a.cap * kLog2e;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] = to * tanh_(x[v] * by);
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(p - j0 - acc_row(v, h)));
+            }
+            if (j0 + kTile > low || s.docs || kbad) {
+                const unsigned same = s.docs ? same_document(docs, doc, h) : ~0u;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int row = acc_row(v, h);
+                    const bool ok = j0 + row < lim && (same >> v & 1);
+                    x[v] = kbad >> row & 1 ? __builtin_nanf("") : x[v];
+                    x[v] = ok ? x[v] : -__builtin_inff();
+                }
+            }
             float peak = most;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int j = j0 + acc_row(v, h);
-                float z = score(a, x[v], slope2, p, j);
-                if (!whole) {
-                    if (kbad >> acc_row(v, h) & 1) z = __builtin_nanf("");
-                    bool ok = j < lim;
-                    if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc;
-                    z = ok ? z : -__builtin_inff();
-                }
-                x[v] = z;
-                peak = z > peak || z != z ? z : peak;
-            }
-            const float other = __shfl_xor(peak, 32);
-            peak = other > peak || other != other ? other : peak;
+            for (int v = 0; v < 16; ++v) peak = fmaxf(peak, x[v]);          // (a NaN shows in the sum)
+            peak = fmaxf(peak, __shfl_xor(peak, 32));
             const float ref = peak == -__builtin_inff() ? 0.f : peak;
             const float shrink = exp2_(most - ref);
             if (__any(shrink != 1.f)) {
@@ -381,18 +589,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan,
                 x[v] = exp2_(x[v] - ref);
                 total += x[v];
             }
-            spread<NT>(acc, lds[buf][1], x, lane);
-            const unsigned vbad = bad[buf][1];
-            if (vbad) spread_bad<NT>(acc, vbad, vbase + j0 * a.v_stride[2], a.v_stride[2], a.d, x, lane);
+            spread6<NT>(acc, lds[buf] + P::BYTES, x, lane);
+            if (vbad)
+                spread6_bad<NT>(acc, vbad, a.v + b * a.v_stride[0] + kh * a.v_stride[1] + j0 * a.v_stride[2], a.v_stride[2], a.d, x, lane);
         }
-        __syncthreads();                               // everyone is done with the marks of this buffer
-        if (threadIdx.x < 2) bad[buf][threadIdx.x] = 0;
         buf ^= 1;
-        if (j1 < end) {
-            tk.stage(lds[buf][0], &bad[buf][0]);
-            tv.stage(lds[buf][1], &bad[buf][1]);
-        }
-        __syncthreads();
         j0 = j1;
     }
 
@@ -402,10 +603,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows(Args a, Plan plan,
     const float lse = total == 0.f ? -__builtin_inff() : (most + __builtin_amdgcn_logf(total)) * kLn2;
     if (part) {
         const int64_t row = (((int64_t)split * a.batch + b) * a.hq + qh) * a.lq + i;
-        store_row<NT>(part + row * a.d, acc, by, a.d, wide, h);
+        store_column<NT>(part + row * a.d, acc, by, a.d, wide, h);
         if (h == 0) part_lse[row] = lse;
     } else {
-        store_row<NT>(a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2], acc, by, a.d, wide, h);
+        store_column<NT>(a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2], acc, by, a.d, wide, h);
         if (h == 0 && a.lse) a.lse[((int64_t)b * a.hq + qh) * a.lq + i] = lse;
     }
 }
@@ -1015,16 +1216,18 @@ bool aligned(const void* p, const int64_t* stride) {
 int row_tiles(const Args& a) { return (int)(((int64_t)(a.hq / a.hkv) * a.lq + kRows - 1) / kRows); }
 
 // Which forward kernel, and into how many key ranges.  Few rows: up to 32 rows of a key head, where the
-// 128-row blocks of the other kernel would be mostly empty.  Ranges: enough for `want` blocks (the
-// device holds 512 of either kernel), none shorter than `least` keys, whose work pays for joining.
+// blocks of the other kernel would be mostly empty.  Blocks of eight waves share each tile among 256 rows, of
+// four where that leaves compute units without a block.  Ranges: enough for `want` blocks, none shorter than
+// `least` keys, whose work pays for joining.
 Plan plan_forward(const Args& a) {
     Plan p;
     p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride);
     const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
     p.few = rows <= 32;
-    const int64_t blocks = heads * (p.few ? 1 : row_tiles(a));
-    const int64_t want = p.few ? 2048 : 512;
-    const int least = p.few ? 256 : 512;
+    p.waves = heads * ((rows + 255) / 256) >= 256 ? 8 : 4;
+    const int64_t blocks = heads * (p.few ? 1 : (rows + 32 * p.waves - 1) / (32 * p.waves));
+    const int64_t want = p.few ? 2048 : 256;
+    const int least = 256;
     int64_t splits = blocks >= want ? 1 : (want + blocks - 1) / blocks;
     const int64_t most = (a.lk + least - 1) / least;
     if (splits > most) splits = most;
@@ -1033,6 +1236,34 @@ Plan plan_forward(const Args& a) {
     if (p.chunk < 64) p.chunk = 64;
     p.splits = a.lk > 0 ? (a.lk + p.chunk - 1) / p.chunk : 1;
     return p;
+}
+
+uint64_t up(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// The forward call's workspace: marks, planes, the ranges' lse and results
+struct Room {
+    uint64_t planes, lse, part, all;
+};
+
+Room room_forward(const Args& a, const Plan& p) {
+    const uint64_t rows = (uint64_t)a.batch * a.hq * a.lq, tiles = (uint64_t)a.batch * a.hkv * ((a.lk + kTile - 1) / kTile);
+    Room r;
+    r.planes = p.few ? 0 : up(tiles * 8);
+    r.lse = r.planes + (p.few ? 0 : up(tiles * 2 * 6144 * ((a.d + 31) / 32)));
+    r.part = r.lse + (p.splits > 1 ? up(rows * p.splits * 4) : 0);
+    r.all = r.part + (p.splits > 1 ? rows * p.splits * a.d * 4 : 0);
+    return r;
+}
+
+template <int NT> void launch_rows(const Args& a, const Plan& p, char* planes, unsigned* marks, float* part, float* part_lse, hipStream_t s) {
+    const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
+    const int key_tiles = (a.lk + kTile - 1) / kTile, tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
+    if (key_tiles) attention_pack<NT><<<dim3((unsigned)(heads * key_tiles)), kThreads, 0, s>>>(a, p.wide, key_tiles, planes, marks);
+    const dim3 grid((unsigned)(heads * tiles * p.splits));
+    if (p.waves == 8)
+        attention_rows<NT, 8><<<grid, 512, 0, s>>>(a, p, tiles, planes, marks, part, part_lse);
+    else
+        attention_rows<NT, 4><<<grid, 256, 0, s>>>(a, p, tiles, planes, marks, part, part_lse);
 }
 
 // Query heads of a key head in blocks of their own: only where the keys alone give too few blocks
@@ -1050,19 +1281,17 @@ extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad)
         const uint64_t keys = (uint64_t)a->batch * a->hkv * a->lk * a->d;
         return (rows * 4 + 255) / 256 * 256 + (parts > 1 ? keys * 8 * parts : 0);
     }
-    const Plan p = plan_forward(*a);
-    return p.splits > 1 ? (rows * p.splits * 4 + 255) / 256 * 256 + rows * p.splits * a->d * 4 : 0;
+    return room_forward(*a, plan_forward(*a)).all;
 }
 
 extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
     const Args& a = *args;
     const Plan p = plan_forward(a);
     const int64_t rows = (int64_t)a.batch * a.hq * a.lq, heads = (int64_t)a.batch * a.hkv;
-    float *part = nullptr, *part_lse = nullptr;
-    if (p.splits > 1) {
-        part_lse = (float*)a.work;
-        part = (float*)((char*)a.work + (rows * p.splits * 4 + 255) / 256 * 256);
-    }
+    const Room room = room_forward(a, p);
+    char* work = (char*)a.work;
+    float* part = p.splits > 1 ? (float*)(work + room.part) : nullptr;
+    float* part_lse = p.splits > 1 ? (float*)(work + room.lse) : nullptr;
     if (p.few) {
         const dim3 grid((unsigned)(heads * p.splits));
         const bool two = (int64_t)(a.hq / a.hkv) * a.lq > 16;
@@ -1071,13 +1300,13 @@ extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
         else
             two ? attention_few<2, 2><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<2, 1><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
     } else {
-        const int tiles = row_tiles(a);
-        const dim3 grid((unsigned)(heads * tiles * p.splits));
+        unsigned* marks = (unsigned*)work;
+        char* planes = work + room.planes;
         switch ((a.d + 31) / 32) {
-            case 1: attention_rows<1><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
-            case 2: attention_rows<2><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
-            case 3: attention_rows<3><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
-            default: attention_rows<4><<<grid, kThreads, 0, s>>>(a, p, tiles, part, part_lse); break;
+            case 1: launch_rows<1>(a, p, planes, marks, part, part_lse, s); break;
+            case 2: launch_rows<2>(a, p, planes, marks, part, part_lse, s); break;
+            case 3: launch_rows<3>(a, p, planes, marks, part, part_lse, s); break;
+            default: launch_rows<4>(a, p, planes, marks, part, part_lse, s); break;
         }
     }
     hipError_t e = hipGetLastError();
