@@ -41,7 +41,7 @@ __device__ __forceinline__ float tanh_(float y) {
     const float p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, -0.0062742396257817745f, 0.021071678027510643f),
                                          -0.05385230854153633f), 0.13332585990428925f), -0.33333316445350647f);
     const float small = fmaf(y * u, p, y);
-    const float large = copysignf(1.0f - 2.0f / (exp2_(a * (2.0f * kLog2e)) + 1.0f), y);
+    const float large = copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(exp2_(a * (2.0f * kLog2e)) + 1.0f), y);
     return a <= 0.55f ? small : (a == a ? large : y);
 }
 
@@ -175,8 +175,9 @@ __device__ __forceinline__ void spread(f32x16 (&acc)[NT], const float* tile, con
 // The part of `spread` that staging left out: elements that are not finite, of the rows in `bad`
 template <int NT>
 __device__ void spread_bad(f32x16 (&acc)[NT], unsigned bad, const float* base, int64_t stride, int size, const f32x16& w, int lane) {
-    const int h = lane >> 5;
     while (bad) {
+        int h = lane >> 5;
+        asm volatile("" : "+v"(h));      // (nothing of this rare path is computed ahead of it and kept in registers)
         const int r = __builtin_ctz(bad);
         bad &= bad - 1;
         const int from = 4 * (r >> 3) + (r & 3);
@@ -314,33 +315,60 @@ template <int NT> struct Planes {
     }
 };
 
+// Nothing is moved across the end of a step of six matrix instructions, which has the chunks of the next
+// one on their way from LDS: 24 registers of chunks at a time.  Left to the compiler's own order the loads of
+// a whole tile come first, and what they displace goes to scratch memory, whose waits are also waits for the
+// next tile's copies.
+__device__ __forceinline__ void step_ends() { __builtin_amdgcn_sched_barrier(0); }
+
 // acc[row][col] = sum_d tile[row][d] own[col][d]: lane l holds elements 16t + 8h .. + 7 of column l % 32
 template <int NT> __device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[2 * NT], int lane) {
     f32x16 acc;
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+    const int h = lane >> 5, row = lane & 31;
+    Three x = Planes<NT>::row_chunk(tile, row, h);
 #pragma unroll
-    for (int t = 0; t < 2 * NT; ++t) acc = mac6(Planes<NT>::row_chunk(tile, lane & 31, 2 * t + (lane >> 5)), own[t], acc);
+    for (int t = 0; t < 2 * NT; ++t) {
+        Three y = x;
+        if (t + 1 < 2 * NT) y = Planes<NT>::row_chunk(tile, row, 2 * (t + 1) + h);
+        acc = mac6(x, own[t], acc);
+        x = y;
+        step_ends();
+    }
     return acc;
 }
 
 // acc[c][i][col] += sum_row tile[row][32 c + i] w[row][col]
 template <int NT> __device__ __forceinline__ void spread6(f32x16 (&acc)[NT], const char* tile, const f32x16& w, int lane) {
+    const int h = lane >> 5, i = lane & 31;
+    Three x = Planes<NT>::column_chunk(tile, h, i), by[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        Three x;
+    for (int e = 0; e < 8; e += 2) split2(f32x2{w[e], w[e + 1]}, e, by[0]);
+    step_ends();
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) split2(f32x2{w[8 * u + e], w[8 * u + e + 1]}, e, x);
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
-            acc[c] = mac6(Planes<NT>::column_chunk(tile, 2 * u + (lane >> 5), 32 * c + (lane & 31)), x, acc[c]);
-    }
+        for (int c = 0; c < NT; ++c) {
+            Three y = x;
+            if (c + 1 < NT) y = Planes<NT>::column_chunk(tile, 2 * u + h, 32 * (c + 1) + i);
+            else if (u == 0) y = Planes<NT>::column_chunk(tile, 2 + h, i);
+            if (u == 0) {                 // the second half's weights are split between the first one's products
+#pragma unroll
+                for (int e = 8 * c / NT; e < 8 * (c + 1) / NT; ++e)
+                    if (e % 2 == 0) split2(f32x2{w[8 + e], w[9 + e]}, e, by[1]);
+            }
+            acc[c] = mac6(x, by[u], acc[c]);
+            x = y;
+            step_ends();
+        }
 }
 
 template <int NT>
 __device__ void spread6_bad(f32x16 (&acc)[NT], unsigned bad, const float* base, int64_t stride, int size, const f32x16& w, int lane) {
-    const int h = lane >> 5;
     while (bad) {
+        int h = lane >> 5;
+        asm volatile("" : "+v"(h));      // (nothing of this rare path is computed ahead of it and kept in registers)
         const int r = __builtin_ctz(bad);
         bad &= bad - 1;
         const int from = 4 * (r >> 3) + (r & 3);
@@ -354,8 +382,9 @@ __device__ void spread6_bad(f32x16 (&acc)[NT], unsigned bad, const float* base, 
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 const int d = 32 * c + acc_row(v, h);
-                const float x = d < size ? row[d] : 0.f;
-                if (!finite_(x) && weight != 0.f) acc[c][v] += weight * x;
+                const float x = row[d < size ? d : 0], y = weight * x;
+                acc[c][v] += !finite_(x) && d < size && weight != 0.f ? y : 0.f;
+                if (v % 2) step_ends();
             }
     }
 }
@@ -554,19 +583,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
             if (a.cap > 0.f) {
                 const float by = 1.f / a.cap, to = a.cap * kLog2e;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] = to * tanh_(x[v] * by);
+                for (int v = 0; v < 16; ++v) {
+                    x[v] = to * tanh_(x[v] * by);
+                    if (v & 1) step_ends();
+                }
             }
             if (a.slopes) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(p - j0 - acc_row(v, h)));
+                for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(p - j0 - 4 * h - acc_row(v, 0)));
             }
             if (j0 + kTile > low || s.docs || kbad) {
                 const unsigned same = s.docs ? same_document(docs, doc, h) : ~0u;
+                const unsigned nans = kbad >> 4 * h;
+                const int left = lim - j0 - 4 * h;
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const int row = acc_row(v, h);
-                    const bool ok = j0 + row < lim && (same >> v & 1);
-                    x[v] = kbad >> row & 1 ? __builtin_nanf("") : x[v];
+                    const bool ok = acc_row(v, 0) < left && (same >> v & 1);
+                    x[v] = nans >> acc_row(v, 0) & 1 ? __builtin_nanf("") : x[v];
                     x[v] = ok ? x[v] : -__builtin_inff();
                 }
             }
