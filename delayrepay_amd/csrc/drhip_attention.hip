@@ -481,9 +481,10 @@ __device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) 
 }
 
 // ---- forward, many rows ---------------------------------------------------------------------
-// A block owns 32 WAVES rows of the queries that share a key head (row = query head in the group x query
-// position), each wave 32 of them, one per column of its accumulators: S^T = K Q^T leaves the scores of a
-// row in one lane pair, so the softmax needs one exchange, and P^T in the layout that O^T += V^T P^T reads.
+// A block owns 32 WAVES rows of the queries that share a key head (query positions one after the other, the
+// heads of a position together, so that the rows of a block see nearly the same keys), each wave 32 of them, one
+// per column of its accumulators: S^T = K Q^T leaves the scores of a row in one lane pair, so the softmax
+// needs one exchange, and P^T in the layout that O^T += V^T P^T reads.
 // Keys and values come 32 at a time from the packed planes through LDS, two buffers, copied a tile ahead.
 template <int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, const char* planes, const unsigned* marks, float* part, float* part_lse) {
@@ -504,7 +505,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     const int rows = group * a.lq;
     const int r = (tile * WAVES + wave) * 32 + (lane & 31);
     const bool valid = r < rows;
-    const int g = valid ? r / a.lq : 0, i = valid ? r - g * a.lq : 0;
+    const int i = valid ? r / group : 0, g = valid ? r - i * group : 0;
     const int qh = kh * group + g, p = s.start + i;
     const int lim = valid ? row_limit(a, s, p) : 0;
     const int doc = s.docs && lim > 0 ? s.docs[p] : 0;
@@ -636,7 +637,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     const float lse = total == 0.f ? -__builtin_inff() : (most + __builtin_amdgcn_logf(total)) * kLn2;
     if (part) {
         const int64_t row = (((int64_t)split * a.batch + b) * a.hq + qh) * a.lq + i;
-        store_column<NT>(part + row * a.d, acc, by, a.d, wide, h);
+        if (total != 0.f) store_column<NT>(part + row * a.d, acc, by, a.d, wide, h);     // (the join reads no others)
         if (h == 0) part_lse[row] = lse;
     } else {
         store_column<NT>(a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2], acc, by, a.d, wide, h);
@@ -1251,7 +1252,7 @@ int row_tiles(const Args& a) { return (int)(((int64_t)(a.hq / a.hkv) * a.lq + kR
 // Which forward kernel, and into how many key ranges.  Few rows: up to 32 rows of a key head, where the
 // blocks of the other kernel would be mostly empty.  Blocks of eight waves share each tile among 256 rows, of
 // four where that leaves compute units without a block.  Ranges: enough for `want` blocks, none shorter than
-// `least` keys, whose work pays for joining.
+// `least` keys, whose work pays for joining; causal blocks are of unequal length, so two for a compute unit.
 Plan plan_forward(const Args& a) {
     Plan p;
     p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride);
@@ -1259,7 +1260,7 @@ Plan plan_forward(const Args& a) {
     p.few = rows <= 32;
     p.waves = heads * ((rows + 255) / 256) >= 256 ? 8 : 4;
     const int64_t blocks = heads * (p.few ? 1 : (rows + 32 * p.waves - 1) / (32 * p.waves));
-    const int64_t want = p.few ? 2048 : 256;
+    const int64_t want = p.few ? 2048 : a.causal ? 512 : 256;
     const int least = 256;
     int64_t splits = blocks >= want ? 1 : (want + blocks - 1) / blocks;
     const int64_t most = (a.lk + least - 1) / least;
