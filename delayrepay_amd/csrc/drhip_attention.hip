@@ -36,13 +36,19 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 
 // tanh to about an ulp: an odd polynomial (own fit on |y| <= 0.55, relative error 1e-9) where
 // 1 - 2 / (e^2y + 1) would cancel, that form elsewhere
-__device__ __forceinline__ float tanh_(float y) {
-    const float a = fabsf(y), u = y * y;
+constexpr float kSmall = 0.55f;
+
+__device__ __forceinline__ float tanh_small(float y) {
+    const float u = y * y;
     const float p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, -0.0062742396257817745f, 0.021071678027510643f),
                                          -0.05385230854153633f), 0.13332585990428925f), -0.33333316445350647f);
-    const float small = fmaf(y * u, p, y);
+    return fmaf(y * u, p, y);
+}
+
+__device__ __forceinline__ float tanh_(float y) {
+    const float a = fabsf(y);
     const float large = copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(exp2_(a * (2.0f * kLog2e)) + 1.0f), y);
-    return a <= 0.55f ? small : (a == a ? large : y);
+    return a <= kSmall ? tanh_small(y) : (a == a ? large : y);
 }
 
 __device__ __forceinline__ bool finite_(float x) { return fabsf(x) < __builtin_inff(); }
@@ -321,6 +327,29 @@ template <int NT> struct Planes {
 // next tile's copies.
 __device__ __forceinline__ void step_ends() { __builtin_amdgcn_sched_barrier(0); }
 
+// tanh(x * by); scores are mostly small against their cap, and then a third of the work is enough
+__device__ __forceinline__ void tanh_tile(f32x16& x, float by) {
+    float most = 0.f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        x[v] *= by;
+        most = fmaxf(most, fabsf(x[v]));
+    }
+    if (__any(most > kSmall)) {             // (a NaN stays one either way)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            x[v] = tanh_(x[v]);
+            if (v & 1) step_ends();
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            x[v] = tanh_small(x[v]);
+            if (v & 1) step_ends();
+        }
+    }
+}
+
 // acc[row][col] = sum_d tile[row][d] own[col][d]: lane l holds elements 16t + 8h .. + 7 of column l % 32
 template <int NT> __device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[2 * NT], int lane) {
     f32x16 acc;
@@ -496,8 +525,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     int id = blockIdx.x;
     const int head = id % heads;
     id /= heads;
-    const int split = id % plan.splits;
-    const int tile = tiles - 1 - id / plan.splits;          // the longest rows first
+    // The longest rows first, range by range: blocks go to the shader engines in turn, so that ranges of one tile
+    // next to each other would give all first ranges, the long ones, to half of them (1.7 times the time)
+    const int tile = tiles - 1 - id % tiles, split = id / tiles;
     const int b = head / a.hkv, kh = head % a.hkv, group = a.hq / a.hkv;
     const Seq s = sequence(a, b);
     const bool wide = plan.wide;
@@ -550,8 +580,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
 
     const int key_tiles = (a.lk + kTile - 1) / kTile;
     const char* packed = planes + (int64_t)head * key_tiles * 2 * P::BYTES;
-    const unsigned* marked = marks + (int64_t)head * key_tiles * 2;
+    const uint2* marked = (const uint2*)marks + (int64_t)head * key_tiles;
     int docs_next = 0;
+    uint2 marks_next = {0, 0};                        // (read ahead of the copies: a wait for it would wait for them)
     // the first key of the next tile that any row of the block may see
     auto next = [&](int j0) {
         if (s.docs)
@@ -571,23 +602,26 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     float most = -__builtin_inff(), total = 0.f;      // running maximum of the row, sum over this lane's keys
 
     int j0 = next(begin), buf = 0;
-    if (j0 < end) copy_to_lds<WAVES>(lds[0], packed + (int64_t)(j0 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
+    if (j0 < end) {
+        marks_next = marked[j0 / kTile];
+        copy_to_lds<WAVES>(lds[0], packed + (int64_t)(j0 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
+    }
     while (j0 < end) {
         copies_done();
         __syncthreads();                               // this tile is there, and everyone is done with the other buffer
         const int docs = docs_next;
+        const unsigned kbad = __builtin_amdgcn_readfirstlane(marks_next.x), vbad = __builtin_amdgcn_readfirstlane(marks_next.y);
         const int j1 = next(j0 + kTile);
-        if (j1 < end) copy_to_lds<WAVES>(lds[buf ^ 1], packed + (int64_t)(j1 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
+        if (j1 < end) {
+            marks_next = marked[j1 / kTile];
+            copy_to_lds<WAVES>(lds[buf ^ 1], packed + (int64_t)(j1 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
+        }
         if (j0 < top) {                                // some row of this wave sees the tile
-            const unsigned kbad = marked[j0 / kTile * 2], vbad = marked[j0 / kTile * 2 + 1];
             f32x16 x = product6<NT>(lds[buf], own, lane);
             if (a.cap > 0.f) {
-                const float by = 1.f / a.cap, to = a.cap * kLog2e;
+                tanh_tile(x, 1.f / a.cap);
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    x[v] = to * tanh_(x[v] * by);
-                    if (v & 1) step_ends();
-                }
+                for (int v = 0; v < 16; ++v) x[v] *= a.cap * kLog2e;
             }
             if (a.slopes) {
 #pragma unroll
