@@ -20,6 +20,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -95,154 +97,8 @@ __device__ __forceinline__ int row_limit(const Args& a, const Seq& s, int p) {
     return lim;
 }
 
-// Element index of accumulator tile c, row i (0..31): chosen so that the operand of the product
-// that contracts over tile rows is one vector per lane (NT = 4: 16 bytes, NT = 2: 8)
-template <int NT> __device__ __forceinline__ int elem(int i, int c) {
-    return NT == 4 ? 4 * i + c : NT == 2 ? 2 * i + c : 32 * c + i;
-}
-
 // Row of register v in a 32x32 accumulator, for the lanes of half h
 __device__ __forceinline__ int acc_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
-
-// A 32-row tile of a matrix on its way from memory to LDS.  Rows lie LD = 32 NT + 4 words apart: b128
-// reads of one column quad by 16 lanes then fall into 64 different banks.
-template <int NT> struct Tile {
-    static constexpr int LD = 32 * NT + 4;
-    static constexpr int QUADS = 8 * NT;                       // of a row
-    static constexpr int PASSES = kTile * QUADS / kThreads;    // NT
-    f32x4 r[PASSES];
-    __device__ __forceinline__ static int row(int p) { return (threadIdx.x + p * kThreads) / QUADS; }
-    __device__ __forceinline__ static int col(int p) { return (threadIdx.x + p * kThreads) % QUADS * 4; }
-    __device__ __forceinline__ void fetch(const float* base, int64_t stride, int first, int end, int size, bool wide) {
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            const int at = first + row(p);
-            r[p] = load4(base + at * stride, col(p), size, at < end, wide);
-        }
-    }
-    // Store the tile with its non-finite values as zeros; a row that had one is marked in *bad
-    __device__ __forceinline__ void stage(float* lds, unsigned* bad) {
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            f32x4 x = r[p];
-            const float worst = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-            const float nan = x[0] + x[1] + x[2] + x[3];
-            if (!(worst < __builtin_inff()) || nan != nan) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[c] = finite_(x[c]) ? x[c] : 0.f;
-                atomicOr(bad, 1u << row(p));
-            }
-            *(f32x4*)(lds + row(p) * LD + col(p)) = x;
-        }
-    }
-};
-
-// acc[row][col] += sum_d tile[row][d] own[col][d]: lane l holds column l % 32 of `own`, elements
-// 8t + 4h + c, and the tile is read in the same order
-template <int NT>
-__device__ __forceinline__ f32x16 product(const float* tile, const f32x4 (&own)[4 * NT], int lane) {
-    f32x16 acc;
-#pragma unroll
-    for (int v = 0; v < 16; ++v) acc[v] = 0.f;
-    const float* at = tile + (lane & 31) * Tile<NT>::LD + 4 * (lane >> 5);
-#pragma unroll
-    for (int t = 0; t < 4 * NT; ++t) {
-        const f32x4 x = *(const f32x4*)(at + 8 * t);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[c], own[t][c], acc, 0, 0, 0);
-    }
-    return acc;
-}
-
-// acc[c][i][col] += sum_row tile[row][elem(i, c)] w[row][col], w in the accumulator layout: register v
-// of the two halves is one step of two rows, so weights go from one product to the next without a move
-template <int NT>
-__device__ __forceinline__ void spread(f32x16 (&acc)[NT], const float* tile, const f32x16& w, int lane) {
-    const int i = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-        const float* at = tile + acc_row(v, h) * Tile<NT>::LD;
-        float x[NT];
-        if constexpr (NT == 4) {
-            const f32x4 y = *(const f32x4*)(at + 4 * i);
-            x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
-        } else if constexpr (NT == 2) {
-            const float2 y = *(const float2*)(at + 2 * i);
-            x[0] = y.x, x[1] = y.y;
-        } else {
-#pragma unroll
-            for (int c = 0; c < NT; ++c) x[c] = at[32 * c + i];
-        }
-#pragma unroll
-        for (int c = 0; c < NT; ++c) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[c], w[v], acc[c], 0, 0, 0);
-    }
-}
-
-// The part of `spread` that staging left out: elements that are not finite, of the rows in `bad`
-template <int NT>
-__device__ void spread_bad(f32x16 (&acc)[NT], unsigned bad, const float* base, int64_t stride, int size, const f32x16& w, int lane) {
-    while (bad) {
-        int h = lane >> 5;
-        asm volatile("" : "+v"(h));      // (nothing of this rare path is computed ahead of it and kept in registers)
-        const int r = __builtin_ctz(bad);
-        bad &= bad - 1;
-        const int from = 4 * (r >> 3) + (r & 3);
-        float mine = 0.f;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) mine = v == from ? w[v] : mine;
-        const float weight = __shfl(mine, (lane & 31) + 32 * ((r >> 2) & 1));
-        const float* row = base + r * stride;
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int d = elem<NT>(acc_row(v, h), c);
-                const float x = d < size ? row[d] : 0.f;
-                if (!finite_(x) && weight != 0.f) acc[c][v] += weight * x;
-            }
-    }
-}
-
-// A lane's column of an accumulator, as the row of a matrix
-template <int NT>
-__device__ __forceinline__ void store_row(float* row, const f32x16 (&acc)[NT], float by, int size, bool wide, int h) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        if constexpr (NT == 4 || NT == 2) {
-            // rows 8u + 4h .. + 3 of all tiles are 4 NT neighbouring elements
-            const int d0 = NT * (8 * u + 4 * h);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                f32x4 x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = acc[(4 * n + e) % NT][4 * u + (4 * n + e) / NT] * by;
-                const int d = d0 + 4 * n;
-                if (wide) {
-                    if (d < size) *(f32x4*)(row + d) = x;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < size) row[d + e] = x[e];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-                const int d = 32 * c + 8 * u + 4 * h;
-                if (wide) {
-                    f32x4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = acc[c][4 * u + e] * by;
-                    if (d < size) *(f32x4*)(row + d) = x;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < size) row[d + e] = acc[c][4 * u + e] * by;
-                }
-            }
-        }
-    }
-}
 
 // Score of one pair from its product, in units of log 2, and the factor of its derivative
 __device__ __forceinline__ float score(const Args& a, float x, float slope2, int p, int j) {
@@ -350,8 +206,14 @@ __device__ __forceinline__ void tanh_tile(f32x16& x, float by) {
     }
 }
 
-// acc[row][col] = sum_d tile[row][d] own[col][d]: lane l holds elements 16t + 8h .. + 7 of column l % 32
-template <int NT> __device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[2 * NT], int lane) {
+struct Nothing {
+    __device__ __forceinline__ void operator()(int) const {}
+};
+
+// acc[row][col] = sum_d tile[row][d] own[col][d]: lane l holds elements 16t + 8h .. + 7 of column l % 32.
+// between(t) is vector work that step t's matrix instructions hide (here and below).
+template <int NT, typename F = Nothing>
+__device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[2 * NT], int lane, F between = F()) {
     f32x16 acc;
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[v] = 0.f;
@@ -362,18 +224,26 @@ template <int NT> __device__ __forceinline__ f32x16 product6(const char* tile, c
         Three y = x;
         if (t + 1 < 2 * NT) y = Planes<NT>::row_chunk(tile, row, 2 * (t + 1) + h);
         acc = mac6(x, own[t], acc);
+        between(t);
         x = y;
         step_ends();
     }
     return acc;
 }
 
-// acc[c][i][col] += sum_row tile[row][32 c + i] w[row][col]
-template <int NT> __device__ __forceinline__ void spread6(f32x16 (&acc)[NT], const char* tile, const f32x16& w, int lane) {
-    const int h = lane >> 5, i = lane & 31;
-    Three x = Planes<NT>::column_chunk(tile, h, i), by[2];
+__device__ __forceinline__ Three split8(const f32x16& w, int from) {
+    Three x;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) split2(f32x2{w[e], w[e + 1]}, e, by[0]);
+    for (int e = 0; e < 8; e += 2) split2(f32x2{w[from + e], w[from + e + 1]}, e, x);
+    return x;
+}
+
+// acc[c][i][col] += sum_row tile[row][32 c + i] w[row][col]; `lo`: the first eight registers of w, split.
+// The others are split between the products of those, then comes between(c).
+template <int NT, typename F = Nothing>
+__device__ __forceinline__ void spread6(f32x16 (&acc)[NT], const char* tile, const Three& lo, const f32x16& w, int lane, F between = F()) {
+    const int h = lane >> 5, i = lane & 31;
+    Three x = Planes<NT>::column_chunk(tile, h, i), hi;
     step_ends();
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -382,12 +252,14 @@ template <int NT> __device__ __forceinline__ void spread6(f32x16 (&acc)[NT], con
             Three y = x;
             if (c + 1 < NT) y = Planes<NT>::column_chunk(tile, 2 * u + h, 32 * (c + 1) + i);
             else if (u == 0) y = Planes<NT>::column_chunk(tile, 2 + h, i);
-            if (u == 0) {                 // the second half's weights are split between the first one's products
+            if (u == 0) {
 #pragma unroll
                 for (int e = 8 * c / NT; e < 8 * (c + 1) / NT; ++e)
-                    if (e % 2 == 0) split2(f32x2{w[8 + e], w[9 + e]}, e, by[1]);
+                    if (e % 2 == 0) split2(f32x2{w[8 + e], w[9 + e]}, e, hi);
+            } else {
+                between(c);
             }
-            acc[c] = mac6(x, by[u], acc[c]);
+            acc[c] = mac6(x, u == 0 ? lo : hi, acc[c]);
             x = y;
             step_ends();
         }
@@ -418,6 +290,24 @@ __device__ void spread6_bad(f32x16 (&acc)[NT], unsigned bad, const float* base, 
     }
 }
 
+// The same where there are no registers to spare: the elements of a lane's column that become NaN are kept as bits
+template <int NT>
+__device__ void note_bad(unsigned (*poison)[NT], unsigned bad, const float* base, int64_t stride, int size, const f32x16& w, int lane) {
+    while (bad) {
+        const int r = __builtin_ctz(bad);
+        bad &= bad - 1;
+        const int from = 4 * (r >> 3) + (r & 3);
+        float mine = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mine = v == from ? w[v] : mine;
+        const float weight = __shfl(mine, (lane & 31) + 32 * ((r >> 2) & 1));
+        const float* row = base + r * stride;
+        if (weight != 0.f && lane < 32)
+            for (int d = 0; d < size; ++d)
+                if (!finite_(row[d])) poison[lane][d >> 5] |= 1u << (d & 31);
+    }
+}
+
 template <int NT>
 __device__ __forceinline__ void store_column(float* row, const f32x16 (&acc)[NT], float by, int size, bool wide, int h) {
 #pragma unroll
@@ -438,53 +328,92 @@ __device__ __forceinline__ void store_column(float* row, const f32x16 (&acc)[NT]
         }
 }
 
-// Keys by rows and values by columns, for every tile of 32 that holds a key of its sequence; rows behind
-// the sequence and values that are not finite are zeros, the rows that held one are marked.  Bound by memory:
-// 4 bytes read and 6 written for each number, once for all blocks that read the tile.
-template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Args a, int wide, int tiles, char* planes, unsigned* marks) {
-    __shared__ float lds[2][kTile][32 * NT + 1];
-    __shared__ unsigned bad[2];
-    const int tile = blockIdx.x % tiles, head = blockIdx.x / tiles;
-    const int b = head / a.hkv, kh = head % a.hkv;
-    const int len = sequence(a, b).len;
-    const int j0 = tile * kTile;
-    if (j0 >= len) return;
-    if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+// One matrix to be packed: keys and values up to their sequence's length, or q and dO, of which a row
+// without pairs counts as zeros.  With dO goes D = rowsum(dO o).
+struct Pack {
+    const float* x;
+    int64_t stride[3];
+    int heads, tiles, keys;         // tiles of 32 rows of one head
+    char *by_rows, *by_columns;     // (either may be null)
+    unsigned* marks;
+    float* delta;
+};
+struct Packs {
+    Pack job[4];
+};
+
+// Matrices in planes, for every tile that counts; values that are not finite become zeros and their rows
+// are marked.  Bound by memory: 4 bytes read and 6 written (in each order) for each number, once for all blocks
+// that read the tile.
+template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Args a, Packs packs, int wide) {
+    __shared__ float lds[kTile][32 * NT + 1];
+    __shared__ unsigned bad;
+    int id = blockIdx.x, n = 0;
+    while (id >= a.batch * packs.job[n].heads * packs.job[n].tiles) {
+        id -= a.batch * packs.job[n].heads * packs.job[n].tiles;
+        ++n;
+    }
+    const Pack& job = packs.job[n];
+    const int tile = id % job.tiles, head = id / job.tiles;
+    const int b = head / job.heads, nh = head % job.heads;
+    const int first = tile * kTile;
+    const int end = job.keys ? sequence(a, b).len : a.lq;
+    if (first >= end) return;
+    if (threadIdx.x == 0) bad = 0;
     __syncthreads();
-    const float* base[2] = {a.k + b * a.k_stride[0] + kh * a.k_stride[1], a.v + b * a.v_stride[0] + kh * a.v_stride[1]};
-    const int64_t stride[2] = {a.k_stride[2], a.v_stride[2]};
+    const float* base = job.x + b * job.stride[0] + nh * job.stride[1];
+    const float* lse = job.keys ? nullptr : a.lse + (int64_t)head * a.lq;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int p = 0; p < NT; ++p) {
+        const int at = threadIdx.x + p * kThreads, row = at / (8 * NT), d = at % (8 * NT) * 4, i = first + row;
+        const bool in = i < end && !(lse && lse[i] == -__builtin_inff());
+        const f32x4 x = load4(base + i * job.stride[2], d, a.d, in, wide);
+        bool fine = true;
 #pragma unroll
-        for (int p = 0; p < NT; ++p) {
-            const int at = threadIdx.x + p * kThreads, row = at / (8 * NT), d = at % (8 * NT) * 4;
-            f32x4 x = load4(base[n] + (j0 + row) * stride[n], d, a.d, j0 + row < len, wide);
-            bool fine = true;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                fine = fine && finite_(x[c]);
-                lds[n][row][d + c] = finite_(x[c]) ? in_range(x[c]) : 0.f;
-            }
-            if (!fine) atomicOr(&bad[n], 1u << row);
+        for (int c = 0; c < 4; ++c) {
+            fine = fine && finite_(x[c]);
+            lds[row][d + c] = finite_(x[c]) ? in_range(x[c]) : 0.f;
         }
+        if (!fine) atomicOr(&bad, 1u << row);
+    }
     __syncthreads();
-    char* to = planes + ((int64_t)head * tiles + tile) * 2 * Planes<NT>::BYTES;
-    if (threadIdx.x < 2) marks[((int64_t)head * tiles + tile) * 2 + threadIdx.x] = bad[threadIdx.x];
+    const int64_t place = (int64_t)head * job.tiles + tile;
+    if (threadIdx.x == 0) job.marks[place] = bad;
+    char* by_rows = job.by_rows ? job.by_rows + place * Planes<NT>::BYTES : nullptr;
+    char* by_columns = job.by_columns ? job.by_columns + place * Planes<NT>::BYTES : nullptr;
     for (int at = threadIdx.x; at < 32 * 4 * NT; at += kThreads) {
         Three x;
-        const int row = at & 31, chunk = at >> 5;
+        if (by_rows) {
+            const int row = at & 31, chunk = at >> 5;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) split2(f32x2{lds[0][row][8 * chunk + e], lds[0][row][8 * chunk + e + 1]}, e, x);
+            for (int e = 0; e < 8; e += 2) split2(f32x2{lds[row][8 * chunk + e], lds[row][8 * chunk + e + 1]}, e, x);
 #pragma unroll
-        for (int n = 0; n < 3; ++n) *(bf16x8*)(to + 2 * (n * Planes<NT>::PLANE + at * 8)) = x.p[n];
-        const int d = at % (32 * NT), group = at / (32 * NT);
+            for (int k = 0; k < 3; ++k) *(bf16x8*)(by_rows + 2 * (k * Planes<NT>::PLANE + at * 8)) = x.p[k];
+        }
+        if (by_columns) {
+            const int d = at % (32 * NT), group = at / (32 * NT);
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const int r = acc_row(8 * (group >> 1) + e, group & 1);
-            split2(f32x2{lds[1][r][d], lds[1][r + 1][d]}, e, x);
+            for (int e = 0; e < 8; e += 2) {
+                const int r = acc_row(8 * (group >> 1) + e, group & 1);
+                split2(f32x2{lds[r][d], lds[r + 1][d]}, e, x);
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *(bf16x8*)(by_columns + 2 * (k * Planes<NT>::PLANE + at * 8)) = x.p[k];
+        }
+    }
+    if (job.delta) {                      // eight lanes for each row
+        const int row = threadIdx.x >> 3, i = first + row;
+        const bool in = i < end && lse[i] != -__builtin_inff();
+        const float* orow = a.o + b * a.o_stride[0] + nh * a.o_stride[1] + i * a.o_stride[2];
+        float sum = 0.f;
+        for (int d = 4 * (threadIdx.x & 7); d < a.d; d += 32) {
+            const f32x4 y = load4(orow, d, a.d, in, wide);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum = fmaf(lds[row][d + c], y[c], sum);
         }
 #pragma unroll
-        for (int n = 0; n < 3; ++n) *(bf16x8*)(to + Planes<NT>::BYTES + 2 * (n * Planes<NT>::PLANE + at * 8)) = x.p[n];
+        for (int m = 1; m < 8; m <<= 1) sum += __shfl_xor(sum, m);
+        if ((threadIdx.x & 7) == 0 && i < end) job.delta[(int64_t)head * a.lq + i] = sum;
     }
 }
 
@@ -509,6 +438,14 @@ __device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) 
     return m;
 }
 
+// What the kernels read of the packed matrices
+struct Packed {
+    const char *key_rows, *key_columns, *value_rows, *value_columns;
+    const char *query_rows, *query_columns, *grad_rows, *grad_columns;
+    const unsigned *key_marks, *value_marks, *query_marks, *grad_marks;
+    float* delta;
+};
+
 // ---- forward, many rows ---------------------------------------------------------------------
 // A block owns 32 WAVES rows of the queries that share a key head (query positions one after the other, the
 // heads of a position together, so that the rows of a block see nearly the same keys), each wave 32 of them, one
@@ -516,7 +453,7 @@ __device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) 
 // needs one exchange, and P^T in the layout that O^T += V^T P^T reads.
 // Keys and values come 32 at a time from the packed planes through LDS, two buffers, copied a tile ahead.
 template <int NT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, const char* planes, const unsigned* marks, float* part, float* part_lse) {
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, Packed in, float* part, float* part_lse) {
     using P = Planes<NT>;
     __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
     __shared__ int ends[WAVES], doc_range[2][WAVES];
@@ -579,10 +516,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     low = __builtin_amdgcn_readfirstlane(low);
 
     const int key_tiles = (a.lk + kTile - 1) / kTile;
-    const char* packed = planes + (int64_t)head * key_tiles * 2 * P::BYTES;
-    const uint2* marked = (const uint2*)marks + (int64_t)head * key_tiles;
+    unsigned marks_next[2] = {0, 0};
+    const int64_t place = (int64_t)head * key_tiles;
+    auto copy = [&](int to, int j) {                  // (marks are read ahead of the copies: a wait for them would wait for these)
+        marks_next[0] = in.key_marks[place + j / kTile];
+        marks_next[1] = in.value_marks[place + j / kTile];
+        copy_to_lds<WAVES>(lds[to], in.key_rows + (place + j / kTile) * P::BYTES, P::BYTES);
+        copy_to_lds<WAVES>(lds[to] + P::BYTES, in.value_columns + (place + j / kTile) * P::BYTES, P::BYTES);
+    };
     int docs_next = 0;
-    uint2 marks_next = {0, 0};                        // (read ahead of the copies: a wait for it would wait for them)
     // the first key of the next tile that any row of the block may see
     auto next = [&](int j0) {
         if (s.docs)
@@ -602,20 +544,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     float most = -__builtin_inff(), total = 0.f;      // running maximum of the row, sum over this lane's keys
 
     int j0 = next(begin), buf = 0;
-    if (j0 < end) {
-        marks_next = marked[j0 / kTile];
-        copy_to_lds<WAVES>(lds[0], packed + (int64_t)(j0 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
-    }
+    if (j0 < end) copy(0, j0);
     while (j0 < end) {
         copies_done();
         __syncthreads();                               // this tile is there, and everyone is done with the other buffer
         const int docs = docs_next;
-        const unsigned kbad = __builtin_amdgcn_readfirstlane(marks_next.x), vbad = __builtin_amdgcn_readfirstlane(marks_next.y);
+        const unsigned kbad = __builtin_amdgcn_readfirstlane(marks_next[0]), vbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
         const int j1 = next(j0 + kTile);
-        if (j1 < end) {
-            marks_next = marked[j1 / kTile];
-            copy_to_lds<WAVES>(lds[buf ^ 1], packed + (int64_t)(j1 / kTile) * 2 * P::BYTES, 2 * P::BYTES);
-        }
+        if (j1 < end) copy(buf ^ 1, j1);
         if (j0 < top) {                                // some row of this wave sees the tile
             f32x16 x = product6<NT>(lds[buf], own, lane);
             if (a.cap > 0.f) {
@@ -657,7 +593,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
                 x[v] = exp2_(x[v] - ref);
                 total += x[v];
             }
-            spread6<NT>(acc, lds[buf] + P::BYTES, x, lane);
+            spread6<NT>(acc, lds[buf] + P::BYTES, split8(x, 0), x, lane);
             if (vbad)
                 spread6_bad<NT>(acc, vbad, a.v + b * a.v_stride[0] + kh * a.v_stride[1] + j0 * a.v_stride[2], a.v_stride[2], a.d, x, lane);
         }
@@ -973,13 +909,14 @@ __global__ __launch_bounds__(kThreads) void attention_join(Args a, int splits, c
 
 // ---- gradient -------------------------------------------------------------------------------
 // Two kernels, each with all sums of one output in one place, so that results do not depend on timing:
-// dQ (rows own their sums, keys pass by, as in the forward kernel; writes D_i too) and dK, dV (keys own
-// their sums, rows pass by).  The scores are computed in both: seven products instead of five.
-template <int NT>
-__global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, int tiles, float* delta) {
-    using T = Tile<NT>;
-    __shared__ __attribute__((aligned(16))) float lds[2][2][kTile * T::LD];
-    __shared__ unsigned bad[2][2];
+// dQ (rows own their sums, keys pass by, as in the forward kernel) and dK, dV (keys own their sums, rows pass
+// by).  The scores are computed in both: seven products instead of five.  A wave holds two matrices of 32
+// columns in planes and its sums, more than 256 registers, so there is one for each SIMD, and what it does on
+// the vector unit stands between its matrix instructions.
+template <int NT, bool CAP>
+__global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, int tiles, Packed in) {
+    using P = Planes<NT>;
+    __shared__ __attribute__((aligned(16))) char lds[2][3 * P::BYTES];
     __shared__ int ends[4], doc_range[2][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int heads = a.batch * a.hkv;
@@ -988,32 +925,34 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
     const Seq s = sequence(a, b);
     const bool wide = plan.wide;
     const int rows = group * a.lq;
-    const int r = tile * kRows + wave * 32 + (lane & 31);
+    const int r = (tile * 4 + wave) * 32 + (lane & 31);
     const bool valid = r < rows;
-    const int g = valid ? r / a.lq : 0, i = valid ? r - g * a.lq : 0;
+    const int i = valid ? r / group : 0, g = valid ? r - i * group : 0;
     const int qh = kh * group + g, p = s.start + i;
     const int64_t at = ((int64_t)b * a.hq + qh) * a.lq + i;
     const float lse = valid ? a.lse[at] : -__builtin_inff();
     const int lim = valid && lse != -__builtin_inff() ? row_limit(a, s, p) : 0;
     const int doc = s.docs && lim > 0 ? s.docs[p] : 0;
-    const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f, lse2 = lse * kLog2e;
+    const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
+    const float lse2 = lse == -__builtin_inff() ? __builtin_inff() : lse * kLog2e;       // (weights of exp2(-inf) = 0)
+    const float dot = lim > 0 ? in.delta[at] : 0.f;
 
-    f32x4 own[4 * NT], dout[4 * NT];
+    const float scale = CAP ? a.scale : a.scale * kLog2e;
+    Three own[2 * NT], dout[2 * NT];
     const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
     const float* grow = a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1] + i * a.dout_stride[2];
-    const float* orow = a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2];
-    float dot = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4 * NT; ++t) {
-        own[t] = load4(qrow, 8 * t + 4 * h, a.d, lim > 0, wide);
-        own[t] *= a.scale;
-        dout[t] = load4(grow, 8 * t + 4 * h, a.d, lim > 0, wide);
-        const f32x4 y = load4(orow, 8 * t + 4 * h, a.d, lim > 0, wide);
+    for (int t = 0; t < 2 * NT; ++t) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) dot += dout[t][c] * y[c];
+        for (int e = 0; e < 8; e += 4) {
+            const f32x4 x = load4(qrow, 16 * t + 8 * h + e, a.d, lim > 0, wide) * scale;
+            split2(f32x2{x[0], x[1]}, e, own[t]);
+            split2(f32x2{x[2], x[3]}, e + 2, own[t]);
+            const f32x4 y = load4(grow, 16 * t + 8 * h + e, a.d, lim > 0, wide);
+            split2(f32x2{y[0], y[1]}, e, dout[t]);
+            split2(f32x2{y[2], y[3]}, e + 2, dout[t]);
+        }
     }
-    dot += __shfl_xor(dot, 32);
-    if (valid && h == 0) delta[at] = dot;
 
     int top = lim, low = valid ? lim : 0x7fffffff, dlo = lim > 0 ? doc : 0x7fffffff, dhi = lim > 0 ? doc : -0x7fffffff - 1;
 #pragma unroll
@@ -1024,92 +963,109 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
         dhi = max(dhi, __shfl_xor(dhi, m));
     }
     if (lane == 0) ends[wave] = top, doc_range[0][wave] = dlo, doc_range[1][wave] = dhi;
-    if (threadIdx.x < 4) (&bad[0][0])[threadIdx.x] = 0;
     __syncthreads();
-    const int end = max(max(ends[0], ends[1]), max(ends[2], ends[3]));
-    dlo = min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3]));
-    dhi = max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3]));
-    const float* kbase = a.k + b * a.k_stride[0] + kh * a.k_stride[1];
-    const float* vbase = a.v + b * a.v_stride[0] + kh * a.v_stride[1];
+    int end = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        end = max(end, ends[w]);
+        dlo = min(dlo, doc_range[0][w]);
+        dhi = max(dhi, doc_range[1][w]);
+    }
+    end = __builtin_amdgcn_readfirstlane(end);
+    top = __builtin_amdgcn_readfirstlane(top);
+    low = __builtin_amdgcn_readfirstlane(low);
+
+    int docs_next = 0;
     auto next = [&](int j0) {
         if (s.docs)
             for (; j0 < end; j0 += kTile) {
                 const int j = j0 + (lane & 31);
-                const int x = j < end ? s.docs[j] : 0;
-                if (__any(j < end && x >= dlo && x <= dhi)) break;
+                docs_next = j < end ? s.docs[j] : 0;
+                if (__any(j < end && docs_next >= dlo && docs_next <= dhi)) break;
             }
         return j0;
+    };
+    unsigned marks_next[2] = {0, 0};
+    const int64_t place = (int64_t)head * ((a.lk + kTile - 1) / kTile);
+    auto copy = [&](int to, int j) {
+        const int64_t n = place + j / kTile;
+        marks_next[0] = in.key_marks[n];
+        marks_next[1] = in.value_marks[n];
+        copy_to_lds<4>(lds[to], in.key_rows + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(lds[to] + P::BYTES, in.value_rows + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(lds[to] + 2 * P::BYTES, in.key_columns + n * P::BYTES, P::BYTES);
     };
     f32x16 acc[NT];
 #pragma unroll
     for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int v = 0; v < 16; ++v) acc[c][v] = 0.f;
-    T tk, tv;
     int j0 = next(0), buf = 0;
-    if (j0 < end) {
-        tk.fetch(kbase, a.k_stride[2], j0, s.len, a.d, wide);
-        tv.fetch(vbase, a.v_stride[2], j0, s.len, a.d, wide);
-        tk.stage(lds[0][0], &bad[0][0]);
-        tv.stage(lds[0][1], &bad[0][1]);
-    }
-    __syncthreads();
+    if (j0 < end) copy(0, j0);
     while (j0 < end) {
+        copies_done();
+        __syncthreads();
+        const int docs = docs_next;
+        const unsigned kbad = __builtin_amdgcn_readfirstlane(marks_next[0]), vbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
         const int j1 = next(j0 + kTile);
-        if (j1 < end) {
-            tk.fetch(kbase, a.k_stride[2], j1, s.len, a.d, wide);
-            tv.fetch(vbase, a.v_stride[2], j1, s.len, a.d, wide);
-        }
+        if (j1 < end) copy(buf ^ 1, j1);
         if (j0 < top) {
-            f32x16 x = product<NT>(lds[buf][0], own, lane);
-            f32x16 y = product<NT>(lds[buf][1], dout, lane);
-            const unsigned kbad = bad[buf][0], vbad = bad[buf][1];
-            const bool whole = j0 + kTile <= low && !s.docs && !(kbad | vbad);
+            f32x16 x = product6<NT>(lds[buf], own, lane);
+            f32x16 slope;                              // of the capped scores
+            if constexpr (CAP) {
+                tanh_tile(x, 1.f / a.cap);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int j = j0 + acc_row(v, h);
-                float z, slope = a.scale;
-                if (a.cap > 0.f) {
-                    const float t = tanh_(x[v] / a.cap);
-                    z = a.cap * kLog2e * t;
-                    slope *= 1.f - t * t;
-                } else {
-                    z = x[v] * kLog2e;
+                for (int v = 0; v < 16; ++v) {
+                    slope[v] = fmaf(-x[v], x[v], 1.f);
+                    x[v] *= a.cap * kLog2e;
                 }
-                if (a.slopes) z -= slope2 * fabsf((float)(p - j));
-                float w = exp2_(z - lse2) * (y[v] - dot) * slope;
-                if (!whole) {
-                    if ((kbad | vbad) >> acc_row(v, h) & 1) w = __builtin_nanf("");
-                    bool ok = j < lim;
-                    if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc;
-                    w = ok ? w : 0.f;
-                }
-                x[v] = w;
             }
-            spread<NT>(acc, lds[buf][0], x, lane);
-            if (kbad) spread_bad<NT>(acc, kbad, kbase + j0 * a.k_stride[2], a.k_stride[2], a.d, x, lane);
+            if (a.slopes) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(p - j0 - 4 * h - acc_row(v, 0)));
+            }
+            const bool whole = j0 + kTile <= low && !s.docs && !(kbad | vbad);
+            if (!whole) {
+                const unsigned same = s.docs ? same_document(docs, doc, h) : ~0u;
+                const unsigned nans = kbad >> 4 * h;
+                const int left = lim - j0 - 4 * h;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const bool ok = acc_row(v, 0) < left && (same >> v & 1);
+                    x[v] = nans >> acc_row(v, 0) & 1 ? __builtin_nanf("") : x[v];
+                    x[v] = ok ? x[v] : -__builtin_inff();
+                }
+            }
+            f32x16 y = product6<NT>(lds[buf] + P::BYTES, dout, lane, [&](int t) {
+#pragma unroll
+                for (int v = 16 * t / (2 * NT); v < 16 * (t + 1) / (2 * NT); ++v) x[v] = exp2_(x[v] - lse2);
+            });
+            if (vbad) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) y[v] = vbad >> 4 * h >> acc_row(v, 0) & 1 ? __builtin_nanf("") : y[v];
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v) x[v] = x[v] == 0.f ? 0.f : x[v] * (y[v] - dot) * (CAP ? slope[v] : 1.f);
+            spread6<NT>(acc, lds[buf] + 2 * P::BYTES, split8(x, 0), x, lane);
+            if (kbad)
+                spread6_bad<NT>(acc, kbad, a.k + b * a.k_stride[0] + kh * a.k_stride[1] + j0 * a.k_stride[2], a.k_stride[2], a.d, x, lane);
         }
-        __syncthreads();
-        if (threadIdx.x < 2) bad[buf][threadIdx.x] = 0;
         buf ^= 1;
-        if (j1 < end) {
-            tk.stage(lds[buf][0], &bad[buf][0]);
-            tv.stage(lds[buf][1], &bad[buf][1]);
-        }
-        __syncthreads();
         j0 = j1;
     }
-    if (valid) store_row<NT>(a.dq + b * a.dq_stride[0] + qh * a.dq_stride[1] + i * a.dq_stride[2], acc, 1.f, a.d, wide, h);
+    if (valid) store_column<NT>(a.dq + b * a.dq_stride[0] + qh * a.dq_stride[1] + i * a.dq_stride[2], acc, a.scale, a.d, wide, h);
 }
 
-// `parts` > 1: the query heads of a key head go to different blocks, whose sums are added by `attention_add`
-template <int NT>
-__global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, int parts, const float* delta, float* part) {
-    using T = Tile<NT>;
-    __shared__ __attribute__((aligned(16))) float lds[2][2][kTile * T::LD];
-    __shared__ float stat[2][2][kTile];
-    __shared__ unsigned bad[2][2];
+// `parts` > 1: the query heads of a key head go to different blocks, whose sums are added by `attention_add`.
+// A tile of rows is read in both orders, 4 x 24 KB for heads of 128, too much for two buffers: the tile by rows has
+// two, the one by columns, which is needed later, is copied while the first products run.
+template <int NT, bool CAP>
+__global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, int parts, Packed in, float* part) {
+    using P = Planes<NT>;
+    __shared__ __attribute__((aligned(16))) char rows_lds[2][2 * P::BYTES], columns_lds[2 * P::BYTES];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][kTile];
     __shared__ int doc_range[2][4];
+    __shared__ unsigned poison[2][kRows][NT];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int heads = a.batch * a.hkv, group = a.hq / a.hkv;
     int id = blockIdx.x;
@@ -1122,14 +1078,24 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     const int key0 = tile * kRows, j = key0 + wave * 32 + (lane & 31);
     const bool valid = j < a.lk, counts = j < s.len;
     const int doc = s.docs && counts ? s.docs[j] : 0;
+    // the first row that sees the key
+    const int need = !counts ? 0x7fffffff : a.causal && j >= s.prefix ? max(j - s.start, 0) : 0;
 
-    f32x4 key[4 * NT], val[4 * NT];
+    const float scale = CAP ? a.scale : a.scale * kLog2e;
+    Three key[2 * NT], val[2 * NT];
     const float* krow = a.k + b * a.k_stride[0] + kh * a.k_stride[1] + (int64_t)j * a.k_stride[2];
     const float* vrow = a.v + b * a.v_stride[0] + kh * a.v_stride[1] + (int64_t)j * a.v_stride[2];
 #pragma unroll
-    for (int t = 0; t < 4 * NT; ++t) {
-        key[t] = load4(krow, 8 * t + 4 * h, a.d, counts, wide);
-        val[t] = load4(vrow, 8 * t + 4 * h, a.d, counts, wide);
+    for (int t = 0; t < 2 * NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const f32x4 x = load4(krow, 16 * t + 8 * h + e, a.d, counts, wide) * scale;
+            split2(f32x2{x[0], x[1]}, e, key[t]);
+            split2(f32x2{x[2], x[3]}, e + 2, key[t]);
+            const f32x4 y = load4(vrow, 16 * t + 8 * h + e, a.d, counts, wide);
+            split2(f32x2{y[0], y[1]}, e, val[t]);
+            split2(f32x2{y[2], y[3]}, e + 2, val[t]);
+        }
     }
     f32x16 dk[NT], dv[NT];
 #pragma unroll
@@ -1137,16 +1103,16 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
 #pragma unroll
         for (int v = 0; v < 16; ++v) dk[c][v] = 0.f, dv[c][v] = 0.f;
 
-    int dlo = counts ? doc : 0x7fffffff, dhi = counts ? doc : -0x7fffffff - 1;
-    if (s.docs) {
+    int dlo = counts ? doc : 0x7fffffff, dhi = counts ? doc : -0x7fffffff - 1, all = need;
 #pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            dlo = min(dlo, __shfl_xor(dlo, m));
-            dhi = max(dhi, __shfl_xor(dhi, m));
-        }
+    for (int m = 1; m < 32; m <<= 1) {
+        dlo = min(dlo, __shfl_xor(dlo, m));
+        dhi = max(dhi, __shfl_xor(dhi, m));
+        all = max(all, __shfl_xor(all, m));
     }
+    all = __builtin_amdgcn_readfirstlane(all);             // from this row on every key of the wave is seen
     if (lane == 0) doc_range[0][wave] = dlo, doc_range[1][wave] = dhi;
-    if (threadIdx.x < 4) (&bad[0][0])[threadIdx.x] = 0;
+    for (int n = threadIdx.x; n < 2 * kRows * NT; n += kThreads) (&poison[0][0][0])[n] = 0;
     __syncthreads();
     dlo = min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3]));
     dhi = max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3]));
@@ -1156,103 +1122,146 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     if (a.causal && key0 >= s.prefix) first = clamp_(key0 - s.start, 0, a.lq) & ~(kTile - 1);
     if (key0 >= s.len) first = a.lq;
     const int g0 = parts > 1 ? slice : 0, g1 = parts > 1 ? slice + 1 : group;
+    int docs_next = 0;
     auto next = [&](int& g, int& i0) {     // to a tile of rows that may see a key of the block
         for (; g < g1; ++g, i0 = first) {
             for (; i0 < a.lq; i0 += kTile) {
                 if (!s.docs) return;
                 const int i = i0 + (lane & 31), p = s.start + i;
-                const bool in = i < a.lq && p >= 0 && p < s.len;
-                const int x = in ? s.docs[p] : 0;
-                if (__any(in && x >= dlo && x <= dhi)) return;
+                const bool there = i < a.lq && p >= 0 && p < s.len;
+                docs_next = there ? s.docs[p] : 0;
+                if (__any(there && docs_next >= dlo && docs_next <= dhi)) return;
             }
         }
     };
-    T tq, tg;
-    float mylse = 0.f, mydelta = 0.f;
-    auto fetch = [&](int g, int i0) {
-        const int qh = kh * group + g;
-        const int64_t at = ((int64_t)b * a.hq + qh) * a.lq;
-        const float* qbase = a.q + b * a.q_stride[0] + qh * a.q_stride[1];
-        const float* gbase = a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1];
-#pragma unroll
-        for (int x = 0; x < T::PASSES; ++x) {      // a row without pairs may hold anything
-            const int i = i0 + T::row(x);
-            const bool in = i < a.lq && a.lse[at + i] != -__builtin_inff();
-            tq.r[x] = load4(qbase + i * a.q_stride[2], T::col(x), a.d, in, wide);
-            tg.r[x] = load4(gbase + i * a.dout_stride[2], T::col(x), a.d, in, wide);
-        }
+    const int row_tiles = (a.lq + kTile - 1) / kTile;
+    auto place = [&](int g, int i0) { return ((int64_t)b * a.hq + kh * group + g) * row_tiles + i0 / kTile; };
+    unsigned marks_next[2] = {0, 0};
+    float lse_next = 0.f, delta_next = 0.f;
+    auto copy_rows = [&](int to, int g, int i0) {
+        const int64_t n = place(g, i0);
+        marks_next[0] = in.query_marks[n];
+        marks_next[1] = in.grad_marks[n];
         if (threadIdx.x < kTile) {
             const int i = i0 + threadIdx.x;
-            mylse = i < a.lq ? a.lse[at + i] * kLog2e : -__builtin_inff();
-            if (mylse == -__builtin_inff()) mylse = __builtin_inff();    // weights of exp2(-inf) = 0
-            mydelta = i < a.lq ? delta[at + i] : 0.f;
+            const int64_t at = ((int64_t)b * a.hq + kh * group + g) * a.lq + i;
+            lse_next = i < a.lq ? a.lse[at] * kLog2e : -__builtin_inff();
+            delta_next = i < a.lq ? in.delta[at] : 0.f;
+        }
+        copy_to_lds<4>(rows_lds[to], in.query_rows + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(rows_lds[to] + P::BYTES, in.grad_rows + n * P::BYTES, P::BYTES);
+    };
+    auto stage_stat = [&](int to) {           // weights of rows without pairs: exp2(x - inf) = 0
+        if (threadIdx.x < kTile) {
+            stat[to][0][threadIdx.x] = lse_next == -__builtin_inff() ? __builtin_inff() : lse_next;
+            stat[to][1][threadIdx.x] = delta_next;
         }
     };
-    auto stage = [&](int buf) {
-        tq.stage(lds[buf][0], &bad[buf][0]);
-        tg.stage(lds[buf][1], &bad[buf][1]);
-        if (threadIdx.x < kTile) stat[buf][0][threadIdx.x] = mylse, stat[buf][1][threadIdx.x] = mydelta;
-    };
+    unsigned any_bad = 0;
     int g = g0, i0 = first, buf = 0;
     next(g, i0);
     if (g < g1) {
-        fetch(g, i0);
-        stage(0);
+        copy_rows(0, g, i0);
+        stage_stat(0);
     }
-    __syncthreads();
     while (g < g1) {
+        copies_done();
+        __syncthreads();                      // the tile by rows is there, everyone is done with the last one
+        const int docs = docs_next;
+        const unsigned qbad = __builtin_amdgcn_readfirstlane(marks_next[0]), gbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
+        const int64_t n = place(g, i0);
+        copy_to_lds<4>(columns_lds, in.query_columns + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(columns_lds + P::BYTES, in.grad_columns + n * P::BYTES, P::BYTES);
         int ng = g, ni = i0 + kTile;
         next(ng, ni);
-        if (ng < g1) fetch(ng, ni);
+        const bool more = ng < g1;
+        if (more) copy_rows(buf ^ 1, ng, ni);
+
         const int qh = kh * group + g;
-        const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
-        f32x16 x = product<NT>(lds[buf][0], key, lane);
-        f32x16 y = product<NT>(lds[buf][1], val, lane);
-        const unsigned qbad = bad[buf][0], gbad = bad[buf][1];
-        f32x16 w;
+        f32x16 x = product6<NT>(rows_lds[buf], key, lane), slope;
+        if constexpr (CAP) {
+            tanh_tile(x, 1.f / a.cap);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const int row = acc_row(v, h), i = i0 + row, p = s.start + i;
-            float z, slope = a.scale;
-            if (a.cap > 0.f) {
-                const float t = tanh_(x[v] * a.scale / a.cap);
-                z = a.cap * kLog2e * t;
-                slope *= 1.f - t * t;
-            } else {
-                z = x[v] * (a.scale * kLog2e);
+            for (int v = 0; v < 16; ++v) {
+                slope[v] = fmaf(-x[v], x[v], 1.f);
+                x[v] *= a.cap * kLog2e;
             }
-            if (a.slopes) z -= slope2 * fabsf((float)(p - j));
-            float weight = exp2_(z - stat[buf][0][row]);
-            float back = weight * (y[v] - stat[buf][1][row]) * slope;
-            bool ok = j < row_limit(a, s, p) && i < a.lq && stat[buf][0][row] != __builtin_inff();
-            if (s.docs) ok = ok && s.docs[ok ? p : 0] == doc;
-            if (qbad >> row & 1) weight = back = __builtin_nanf("");
-            if (gbad >> row & 1) back = __builtin_nanf("");
-            w[v] = ok ? weight : 0.f;
-            x[v] = ok ? back : 0.f;
         }
-        spread<NT>(dv, lds[buf][1], w, lane);
-        spread<NT>(dk, lds[buf][0], x, lane);
+        if (a.slopes) {
+            const float slope2 = a.slopes[qh] * kLog2e;
+            const int apart = s.start + i0 + 4 * h - j;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(apart + acc_row(v, 0)));
+        }
+        if (i0 < all || s.docs || qbad) {
+            const unsigned same = s.docs ? same_document(docs, doc, h) : ~0u;
+            const unsigned nans = qbad >> 4 * h;
+            const int from = need - i0 - 4 * h;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const bool ok = acc_row(v, 0) >= from && counts && (same >> v & 1);
+                x[v] = nans >> acc_row(v, 0) & 1 ? __builtin_nanf("") : x[v];
+                x[v] = ok ? x[v] : -__builtin_inff();
+            }
+        }
+        Three lo;                             // weights of the first eight registers, split as they come
+        f32x16 y = product6<NT>(rows_lds[buf] + P::BYTES, val, lane, [&](int t) {
+#pragma unroll
+            for (int v = 16 * t / (2 * NT); v < 16 * (t + 1) / (2 * NT); ++v) {
+                x[v] = x[v] == -__builtin_inff() ? 0.f : exp2_(x[v] - stat[buf][0][acc_row(v, h)]);      // (the row's lse may be NaN)
+                if (v < 8 && v % 2) split2(f32x2{x[v - 1], x[v]}, v - 1, lo);
+            }
+        });
+        if (gbad) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) y[v] = gbad >> 4 * h >> acc_row(v, 0) & 1 ? __builtin_nanf("") : y[v];
+        }
+        // the copies by columns are done when no more are under way than every wave queued after them, for the
+        // next tile's rows: two matrices of 6 NT kilobytes, of which a wave takes a quarter, rounded down
+        if (more)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (6 * NT / 4)) : "memory");
+        else
+            copies_done();
+        if (more) stage_stat(buf ^ 1);
+        __syncthreads();
+        Three dlow;
+        spread6<NT>(dv, columns_lds + P::BYTES, lo, x, lane, [&](int c) {
+#pragma unroll
+            for (int e = 16 * c / NT; e < 16 * (c + 1) / NT; ++e) {
+                y[e] = x[e] == 0.f ? 0.f : x[e] * (y[e] - stat[buf][1][acc_row(e, h)]) * (CAP ? slope[e] : 1.f);
+                if (e < 8 && e % 2) split2(f32x2{y[e - 1], y[e]}, e - 1, dlow);
+            }
+        });
+        spread6<NT>(dk, columns_lds, dlow, y, lane);
         if (gbad)
-            spread_bad<NT>(dv, gbad, a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1] + i0 * a.dout_stride[2], a.dout_stride[2], a.d, w, lane);
+            note_bad<NT>(&poison[1][wave * 32], gbad, a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1] + i0 * a.dout_stride[2], a.dout_stride[2], a.d, x, lane);
         if (qbad)
-            spread_bad<NT>(dk, qbad, a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i0 * a.q_stride[2], a.q_stride[2], a.d, x, lane);
-        __syncthreads();
-        if (threadIdx.x < 2) bad[buf][threadIdx.x] = 0;
+            note_bad<NT>(&poison[0][wave * 32], qbad, a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i0 * a.q_stride[2], a.q_stride[2], a.d, y, lane);
+        any_bad |= gbad | qbad;
         buf ^= 1;
-        if (ng < g1) stage(buf);
-        __syncthreads();
         g = ng, i0 = ni;
+    }
+    if (any_bad) {
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            const unsigned no_dk = poison[0][wave * 32 + (lane & 31)][c], no_dv = poison[1][wave * 32 + (lane & 31)][c];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                dk[c][v] = no_dk >> acc_row(v, h) & 1 ? __builtin_nanf("") : dk[c][v];
+                dv[c][v] = no_dv >> acc_row(v, h) & 1 ? __builtin_nanf("") : dv[c][v];
+            }
+        }
     }
     if (!valid) return;
     if (part) {
         const int64_t rows = (int64_t)heads * a.lk;
         float* to = part + (((int64_t)slice * 2) * rows + (int64_t)head * a.lk + j) * a.d;
-        store_row<NT>(to, dk, 1.f, a.d, wide, h);
-        store_row<NT>(to + rows * a.d, dv, 1.f, a.d, wide, h);
+        store_column<NT>(to, dk, a.scale, a.d, wide, h);
+        store_column<NT>(to + rows * a.d, dv, 1.f, a.d, wide, h);
     } else {
-        store_row<NT>(a.dk + b * a.dk_stride[0] + kh * a.dk_stride[1] + (int64_t)j * a.dk_stride[2], dk, 1.f, a.d, wide, h);
-        store_row<NT>(a.dv + b * a.dv_stride[0] + kh * a.dv_stride[1] + (int64_t)j * a.dv_stride[2], dv, 1.f, a.d, wide, h);
+        store_column<NT>(a.dk + b * a.dk_stride[0] + kh * a.dk_stride[1] + (int64_t)j * a.dk_stride[2], dk, a.scale, a.d, wide, h);
+        store_column<NT>(a.dv + b * a.dv_stride[0] + kh * a.dv_stride[1] + (int64_t)j * a.dv_stride[2], dv, 1.f, a.d, wide, h);
     }
 }
 
@@ -1308,30 +1317,113 @@ Plan plan_forward(const Args& a) {
 
 uint64_t up(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// The forward call's workspace: marks, planes, the ranges' lse and results
+// Workspaces, as offsets; packed matrices first
 struct Room {
-    uint64_t planes, lse, part, all;
+    Packed packed;              // (offsets from null)
+    uint64_t lse, part, all;
 };
+
+// One array of `bytes` behind the others
+template <typename T> T* next_room(uint64_t& at, uint64_t bytes) {
+    T* p = (T*)at;
+    at += up(bytes);
+    return p;
+}
 
 Room room_forward(const Args& a, const Plan& p) {
     const uint64_t rows = (uint64_t)a.batch * a.hq * a.lq, tiles = (uint64_t)a.batch * a.hkv * ((a.lk + kTile - 1) / kTile);
-    Room r;
-    r.planes = p.few ? 0 : up(tiles * 8);
-    r.lse = r.planes + (p.few ? 0 : up(tiles * 2 * 6144 * ((a.d + 31) / 32)));
-    r.part = r.lse + (p.splits > 1 ? up(rows * p.splits * 4) : 0);
-    r.all = r.part + (p.splits > 1 ? rows * p.splits * a.d * 4 : 0);
+    const uint64_t planes = tiles * 6144 * ((a.d + 31) / 32);
+    Room r{};
+    uint64_t at = 0;
+    if (!p.few) {
+        r.packed.key_marks = next_room<unsigned>(at, tiles * 4);
+        r.packed.value_marks = next_room<unsigned>(at, tiles * 4);
+        r.packed.key_rows = next_room<char>(at, planes);
+        r.packed.value_columns = next_room<char>(at, planes);
+    }
+    r.lse = at;
+    if (p.splits > 1) next_room<float>(at, rows * p.splits * 4);
+    r.part = at;
+    if (p.splits > 1) next_room<float>(at, rows * p.splits * a.d * 4);
+    r.all = at;
     return r;
 }
 
-template <int NT> void launch_rows(const Args& a, const Plan& p, char* planes, unsigned* marks, float* part, float* part_lse, hipStream_t s) {
+Room room_grad(const Args& a, int parts) {
+    const uint64_t rows = (uint64_t)a.batch * a.hq * a.lq, nt = (a.d + 31) / 32;
+    const uint64_t keys = (uint64_t)a.batch * a.hkv * ((a.lk + kTile - 1) / kTile), queries = (uint64_t)a.batch * a.hq * ((a.lq + kTile - 1) / kTile);
+    Room r{};
+    uint64_t at = 0;
+    r.packed.delta = next_room<float>(at, rows * 4);
+    r.packed.key_marks = next_room<unsigned>(at, keys * 4);
+    r.packed.value_marks = next_room<unsigned>(at, keys * 4);
+    r.packed.query_marks = next_room<unsigned>(at, queries * 4);
+    r.packed.grad_marks = next_room<unsigned>(at, queries * 4);
+    r.packed.key_rows = next_room<char>(at, keys * 6144 * nt);
+    r.packed.key_columns = next_room<char>(at, keys * 6144 * nt);
+    r.packed.value_rows = next_room<char>(at, keys * 6144 * nt);
+    r.packed.query_rows = next_room<char>(at, queries * 6144 * nt);
+    r.packed.query_columns = next_room<char>(at, queries * 6144 * nt);
+    r.packed.grad_rows = next_room<char>(at, queries * 6144 * nt);
+    r.packed.grad_columns = next_room<char>(at, queries * 6144 * nt);
+    r.part = at;
+    if (parts > 1) next_room<float>(at, (uint64_t)parts * 2 * a.batch * a.hkv * a.lk * a.d * 4);
+    r.all = at;
+    return r;
+}
+
+// The packed matrices of a room whose memory begins at `work`
+Packed packed_at(const Room& room, char* work) {
+    Packed p = room.packed;
+    auto move = [&](auto*& x) { x = (std::remove_reference_t<decltype(x)>)(work + (uint64_t)x); };
+    move(p.key_rows), move(p.key_columns), move(p.value_rows), move(p.value_columns);
+    move(p.query_rows), move(p.query_columns), move(p.grad_rows), move(p.grad_columns);
+    move(p.key_marks), move(p.value_marks), move(p.query_marks), move(p.grad_marks), move(p.delta);
+    return p;
+}
+
+Pack pack_of(const float* x, const int64_t* stride, int heads, int rows, int keys, const char* by_rows, const char* by_columns, const unsigned* marks, float* delta) {
+    return Pack{x, {stride[0], stride[1], stride[2]}, heads, (rows + kTile - 1) / kTile, keys, (char*)by_rows, (char*)by_columns, (unsigned*)marks, delta};
+}
+
+template <int NT> void launch_rows(const Args& a, const Plan& p, const Packed& in, float* part, float* part_lse, hipStream_t s) {
     const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
     const int key_tiles = (a.lk + kTile - 1) / kTile, tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
-    if (key_tiles) attention_pack<NT><<<dim3((unsigned)(heads * key_tiles)), kThreads, 0, s>>>(a, p.wide, key_tiles, planes, marks);
+    Packs packs{};
+    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key_rows, nullptr, in.key_marks, nullptr);
+    packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, nullptr, in.value_columns, in.value_marks, nullptr);
+    if (key_tiles) attention_pack<NT><<<dim3((unsigned)(2 * heads * key_tiles)), kThreads, 0, s>>>(a, packs, p.wide);
     const dim3 grid((unsigned)(heads * tiles * p.splits));
     if (p.waves == 8)
-        attention_rows<NT, 8><<<grid, 512, 0, s>>>(a, p, tiles, planes, marks, part, part_lse);
+        attention_rows<NT, 8><<<grid, 512, 0, s>>>(a, p, tiles, in, part, part_lse);
     else
-        attention_rows<NT, 4><<<grid, 256, 0, s>>>(a, p, tiles, planes, marks, part, part_lse);
+        attention_rows<NT, 4><<<grid, 256, 0, s>>>(a, p, tiles, in, part, part_lse);
+}
+
+template <int NT> void launch_grad(const Args& a, const Plan& p, int parts, const Packed& in, float* part, hipStream_t s) {
+    const int64_t heads = (int64_t)a.batch * a.hkv;
+    const int key_tiles = (a.lk + kTile - 1) / kTile, query_tiles = (a.lq + kTile - 1) / kTile, tiles = row_tiles(a);
+    Packs packs{};
+    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key_rows, in.key_columns, in.key_marks, nullptr);
+    packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, in.value_rows, nullptr, in.value_marks, nullptr);
+    packs.job[2] = pack_of(a.q, a.q_stride, a.hq, a.lq, 0, in.query_rows, in.query_columns, in.query_marks, nullptr);
+    packs.job[3] = pack_of(a.dout, a.dout_stride, a.hq, a.lq, 0, in.grad_rows, in.grad_columns, in.grad_marks, in.delta);
+    const int64_t blocks = 2 * heads * key_tiles + 2 * (int64_t)a.batch * a.hq * query_tiles;
+    attention_pack<NT><<<dim3((unsigned)blocks), kThreads, 0, s>>>(a, packs, p.wide);
+    const dim3 rows_grid((unsigned)(heads * tiles)), keys_grid((unsigned)(heads * parts * ((a.lk + kRows - 1) / kRows)));
+    if (a.lq) {
+        if (a.cap > 0.f)
+            attention_dq<NT, true><<<rows_grid, kThreads, 0, s>>>(a, p, tiles, in);
+        else
+            attention_dq<NT, false><<<rows_grid, kThreads, 0, s>>>(a, p, tiles, in);
+    }
+    if (a.lk) {
+        if (a.cap > 0.f)
+            attention_dkv<NT, true><<<keys_grid, kThreads, 0, s>>>(a, p, parts, in, part);
+        else
+            attention_dkv<NT, false><<<keys_grid, kThreads, 0, s>>>(a, p, parts, in, part);
+    }
+    if (a.lk && parts > 1) attention_add<<<dim3((unsigned)((2 * heads * a.lk + 3) / 4)), kThreads, 0, s>>>(a, parts, part);
 }
 
 // Query heads of a key head in blocks of their own: only where the keys alone give too few blocks
@@ -1343,13 +1435,7 @@ int plan_parts(const Args& a) {
 }  // namespace
 
 extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad) {
-    const uint64_t rows = (uint64_t)a->batch * a->hq * a->lq;
-    if (grad) {
-        const int parts = plan_parts(*a);
-        const uint64_t keys = (uint64_t)a->batch * a->hkv * a->lk * a->d;
-        return (rows * 4 + 255) / 256 * 256 + (parts > 1 ? keys * 8 * parts : 0);
-    }
-    return room_forward(*a, plan_forward(*a)).all;
+    return grad ? room_grad(*a, plan_parts(*a)).all : room_forward(*a, plan_forward(*a)).all;
 }
 
 extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
@@ -1368,13 +1454,12 @@ extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
         else
             two ? attention_few<2, 2><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<2, 1><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
     } else {
-        unsigned* marks = (unsigned*)work;
-        char* planes = work + room.planes;
+        const Packed in = packed_at(room, work);
         switch ((a.d + 31) / 32) {
-            case 1: launch_rows<1>(a, p, planes, marks, part, part_lse, s); break;
-            case 2: launch_rows<2>(a, p, planes, marks, part, part_lse, s); break;
-            case 3: launch_rows<3>(a, p, planes, marks, part, part_lse, s); break;
-            default: launch_rows<4>(a, p, planes, marks, part, part_lse, s); break;
+            case 1: launch_rows<1>(a, p, in, part, part_lse, s); break;
+            case 2: launch_rows<2>(a, p, in, part, part_lse, s); break;
+            case 3: launch_rows<3>(a, p, in, part, part_lse, s); break;
+            default: launch_rows<4>(a, p, in, part, part_lse, s); break;
         }
     }
     hipError_t e = hipGetLastError();
@@ -1388,37 +1473,20 @@ extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
 
 extern "C" int drhip_k_attention_grad(const drhip_attention_t* args, hipStream_t s) {
     const Args& a = *args;
-    const int64_t rows = (int64_t)a.batch * a.hq * a.lq, heads = (int64_t)a.batch * a.hkv;
-    float* delta = (float*)a.work;
     const int parts = plan_parts(a);
-    float* part = parts > 1 ? (float*)((char*)a.work + (rows * 4 + 255) / 256 * 256) : nullptr;
+    const Room room = room_grad(a, parts);
+    char* work = (char*)a.work;
+    const Packed in = packed_at(room, work);
+    float* part = parts > 1 ? (float*)(work + room.part) : nullptr;
     Plan p{};
     p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride) &&
              aligned(a.dout, a.dout_stride) && aligned(a.dq, a.dq_stride) && aligned(a.dk, a.dk_stride) && aligned(a.dv, a.dv_stride);
-    const int tiles = row_tiles(a);
-    const int nt = (a.d + 31) / 32;
-    hipError_t e = hipSuccess;
-    if (rows > 0) {
-        const dim3 grid((unsigned)(heads * tiles));
-        switch (nt) {
-            case 1: attention_dq<1><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
-            case 2: attention_dq<2><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
-            case 3: attention_dq<3><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
-            default: attention_dq<4><<<grid, kThreads, 0, s>>>(a, p, tiles, delta); break;
-        }
-        e = hipGetLastError();
-        if (e != hipSuccess) return (int)e;
+    if (!a.lq && !a.lk) return 0;
+    switch ((a.d + 31) / 32) {
+        case 1: launch_grad<1>(a, p, parts, in, part, s); break;
+        case 2: launch_grad<2>(a, p, parts, in, part, s); break;
+        case 3: launch_grad<3>(a, p, parts, in, part, s); break;
+        default: launch_grad<4>(a, p, parts, in, part, s); break;
     }
-    if (a.lk == 0 || heads == 0) return 0;
-    const dim3 grid((unsigned)(heads * parts * ((a.lk + kRows - 1) / kRows)));
-    switch (nt) {
-        case 1: attention_dkv<1><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
-        case 2: attention_dkv<2><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
-        case 3: attention_dkv<3><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
-        default: attention_dkv<4><<<grid, kThreads, 0, s>>>(a, p, parts, delta, part); break;
-    }
-    e = hipGetLastError();
-    if (e != hipSuccess || parts == 1) return (int)e;
-    attention_add<<<dim3((unsigned)((2 * heads * a.lk + 3) / 4)), kThreads, 0, s>>>(a, parts, part);
     return (int)hipGetLastError();
 }
