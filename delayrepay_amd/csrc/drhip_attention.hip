@@ -427,6 +427,14 @@ template <int WAVES> __device__ __forceinline__ void copy_to_lds(char* lds, cons
 
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// A barrier that leaves copies under way (__syncthreads waits for all of them): what the waves wrote to LDS
+// themselves is there after it
+__device__ __forceinline__ void barrier_only() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // Whether the keys of a tile are of the lane's row's document, as bits in the order of the accumulator's registers
 __device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) {
     unsigned m = 0;
@@ -1145,7 +1153,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
         if (threadIdx.x < kTile) {
             const int i = i0 + threadIdx.x;
             const int64_t at = ((int64_t)b * a.hq + kh * group + g) * a.lq + i;
-            lse_next = i < a.lq ? a.lse[at] * kLog2e : -__builtin_inff();
+            lse_next = i < a.lq ? a.lse[at] : -__builtin_inff();       // (used when it has come: a wait now would be for all copies)
             delta_next = i < a.lq ? in.delta[at] : 0.f;
         }
         copy_to_lds<4>(rows_lds[to], in.query_rows + n * P::BYTES, P::BYTES);
@@ -1153,7 +1161,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     };
     auto stage_stat = [&](int to) {           // weights of rows without pairs: exp2(x - inf) = 0
         if (threadIdx.x < kTile) {
-            stat[to][0][threadIdx.x] = lse_next == -__builtin_inff() ? __builtin_inff() : lse_next;
+            stat[to][0][threadIdx.x] = lse_next == -__builtin_inff() ? __builtin_inff() : lse_next * kLog2e;
             stat[to][1][threadIdx.x] = delta_next;
         }
     };
@@ -1169,12 +1177,13 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
         __syncthreads();                      // the tile by rows is there, everyone is done with the last one
         const int docs = docs_next;
         const unsigned qbad = __builtin_amdgcn_readfirstlane(marks_next[0]), gbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
-        const int64_t n = place(g, i0);
-        copy_to_lds<4>(columns_lds, in.query_columns + n * P::BYTES, P::BYTES);
-        copy_to_lds<4>(columns_lds + P::BYTES, in.grad_columns + n * P::BYTES, P::BYTES);
         int ng = g, ni = i0 + kTile;
         next(ng, ni);
         const bool more = ng < g1;
+        const int64_t n = place(g, i0);
+        const float slope2 = a.slopes ? a.slopes[kh * group + __builtin_amdgcn_readfirstlane(g)] * kLog2e : 0.f;
+        copy_to_lds<4>(columns_lds, in.query_columns + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(columns_lds + P::BYTES, in.grad_columns + n * P::BYTES, P::BYTES);
         if (more) copy_rows(buf ^ 1, ng, ni);
 
         const int qh = kh * group + g;
@@ -1188,7 +1197,6 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
             }
         }
         if (a.slopes) {
-            const float slope2 = a.slopes[qh] * kLog2e;
             const int apart = s.start + i0 + 4 * h - j;
 #pragma unroll
             for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(apart + acc_row(v, 0)));
@@ -1223,7 +1231,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
         else
             copies_done();
         if (more) stage_stat(buf ^ 1);
-        __syncthreads();
+        barrier_only();
         Three dlow;
         spread6<NT>(dv, columns_lds + P::BYTES, lo, x, lane, [&](int c) {
 #pragma unroll
