@@ -154,25 +154,36 @@ __device__ __forceinline__ f32x16 mac6(const Three& a, const Three& b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
 
-// A 32-row tile in three planes, 16-byte chunks of eight numbers, in either of two orders.  Both are
-// read by consecutive lanes at consecutive chunks.
-//   by rows:    [plane][element / 8][row][element % 8]              (contracted over elements)
-//   by columns: [plane][group of eight rows][element][row in it]    (contracted over rows)
-// The row groups are those that a lane half holds in eight registers of an accumulator (acc_row), so that
-// weights go from one product to the next without a move.
+// A 32-row tile in three planes: [plane][element / 8][row][element % 8], 16-byte chunks of eight elements of a
+// row, those of odd chunks with the row's bit 2 turned.  A product contracts over elements (row_chunk: a lane
+// takes a chunk of its row, consecutive lanes consecutive chunks) or over rows (column_chunk: a lane takes
+// eight rows of its element with transposing reads, of which 16 lanes read four rows of two chunks; the turned bit
+// puts these into different banks).  The eight rows are those that a lane half holds in eight registers
+// of an accumulator (acc_row), so that weights go from one product to the next without a move.
 template <int NT> struct Planes {
-    static constexpr int PLANE = 32 * 32 * NT;        // numbers
-    static constexpr int BYTES = 3 * PLANE * 2;       // of a tile in one order
-    __device__ __forceinline__ static Three row_chunk(const char* tile, int row, int chunk) {
+    static constexpr int PLANE = 2 * 32 * 32 * NT;    // bytes
+    static constexpr int BYTES = 3 * PLANE;           // of a tile
+    __device__ __forceinline__ static int place(int row, int chunk) { return (chunk * 32 + (row ^ 4 * (chunk & 1))) * 16; }
+    __device__ __forceinline__ static Three row_chunk(const char* tile, int row, int t, int h) {
         Three x;
+        const char* at = tile + place(row, h) + 1024 * t;
 #pragma unroll
-        for (int n = 0; n < 3; ++n) x.p[n] = *(const bf16x8*)(tile + 2 * (n * PLANE + (chunk * 32 + row) * 8));
+        for (int n = 0; n < 3; ++n) x.p[n] = *(const bf16x8*)(at + n * PLANE);
         return x;
     }
-    __device__ __forceinline__ static Three column_chunk(const char* tile, int group, int element) {
+    // element 32 c + lane % 32, rows acc_row(8u .. 8u + 7, lane / 32)
+    __device__ __forceinline__ static Three column_chunk(const char* tile, int u, int c, int lane) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const int l = lane & 15, odd = l >> 1 & 1, row = (4 * (lane >> 5) + (l >> 2)) ^ 4 * odd;
+        const char* at = tile + ((2 * (lane >> 4 & 1) + odd) * 32 + row) * 16 + (l & 1) * 8 + 2048 * c + 256 * u;
         Three x;
 #pragma unroll
-        for (int n = 0; n < 3; ++n) x.p[n] = *(const bf16x8*)(tile + 2 * (n * PLANE + (group * 32 * NT + element) * 8));
+        for (int n = 0; n < 3; ++n) {
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + n * PLANE));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + n * PLANE + 128));
+            x.p[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
         return x;
     }
 };
@@ -218,11 +229,11 @@ __device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[v] = 0.f;
     const int h = lane >> 5, row = lane & 31;
-    Three x = Planes<NT>::row_chunk(tile, row, h);
+    Three x = Planes<NT>::row_chunk(tile, row, 0, h);
 #pragma unroll
     for (int t = 0; t < 2 * NT; ++t) {
         Three y = x;
-        if (t + 1 < 2 * NT) y = Planes<NT>::row_chunk(tile, row, 2 * (t + 1) + h);
+        if (t + 1 < 2 * NT) y = Planes<NT>::row_chunk(tile, row, t + 1, h);
         acc = mac6(x, own[t], acc);
         between(t);
         x = y;
@@ -242,16 +253,15 @@ __device__ __forceinline__ Three split8(const f32x16& w, int from) {
 // The others are split between the products of those, then comes between(c).
 template <int NT, typename F = Nothing>
 __device__ __forceinline__ void spread6(f32x16 (&acc)[NT], const char* tile, const Three& lo, const f32x16& w, int lane, F between = F()) {
-    const int h = lane >> 5, i = lane & 31;
-    Three x = Planes<NT>::column_chunk(tile, h, i), hi;
+    Three x = Planes<NT>::column_chunk(tile, 0, 0, lane), hi;
     step_ends();
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
             Three y = x;
-            if (c + 1 < NT) y = Planes<NT>::column_chunk(tile, 2 * u + h, 32 * (c + 1) + i);
-            else if (u == 0) y = Planes<NT>::column_chunk(tile, 2 + h, i);
+            if (c + 1 < NT) y = Planes<NT>::column_chunk(tile, u, c + 1, lane);
+            else if (u == 0) y = Planes<NT>::column_chunk(tile, 1, 0, lane);
             if (u == 0) {
 #pragma unroll
                 for (int e = 8 * c / NT; e < 8 * (c + 1) / NT; ++e)
@@ -334,7 +344,7 @@ struct Pack {
     const float* x;
     int64_t stride[3];
     int heads, tiles, keys;         // tiles of 32 rows of one head
-    char *by_rows, *by_columns;     // (either may be null)
+    char* planes;
     unsigned* marks;
     float* delta;
 };
@@ -343,8 +353,7 @@ struct Packs {
 };
 
 // Matrices in planes, for every tile that counts; values that are not finite become zeros and their rows
-// are marked.  Bound by memory: 4 bytes read and 6 written (in each order) for each number, once for all blocks
-// that read the tile.
+// are marked.  Bound by memory: 4 bytes read and 6 written for each number, once for all blocks that read the tile.
 template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Args a, Packs packs, int wide) {
     __shared__ float lds[kTile][32 * NT + 1];
     __shared__ unsigned bad;
@@ -379,27 +388,14 @@ template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Arg
     __syncthreads();
     const int64_t place = (int64_t)head * job.tiles + tile;
     if (threadIdx.x == 0) job.marks[place] = bad;
-    char* by_rows = job.by_rows ? job.by_rows + place * Planes<NT>::BYTES : nullptr;
-    char* by_columns = job.by_columns ? job.by_columns + place * Planes<NT>::BYTES : nullptr;
+    char* to = job.planes + place * Planes<NT>::BYTES;
     for (int at = threadIdx.x; at < 32 * 4 * NT; at += kThreads) {
         Three x;
-        if (by_rows) {
-            const int row = at & 31, chunk = at >> 5;
+        const int row = at & 31, chunk = at >> 5;
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) split2(f32x2{lds[row][8 * chunk + e], lds[row][8 * chunk + e + 1]}, e, x);
+        for (int e = 0; e < 8; e += 2) split2(f32x2{lds[row][8 * chunk + e], lds[row][8 * chunk + e + 1]}, e, x);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) *(bf16x8*)(by_rows + 2 * (k * Planes<NT>::PLANE + at * 8)) = x.p[k];
-        }
-        if (by_columns) {
-            const int d = at % (32 * NT), group = at / (32 * NT);
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const int r = acc_row(8 * (group >> 1) + e, group & 1);
-                split2(f32x2{lds[r][d], lds[r + 1][d]}, e, x);
-            }
-#pragma unroll
-            for (int k = 0; k < 3; ++k) *(bf16x8*)(by_columns + 2 * (k * Planes<NT>::PLANE + at * 8)) = x.p[k];
-        }
+        for (int k = 0; k < 3; ++k) *(bf16x8*)(to + k * Planes<NT>::PLANE + Planes<NT>::place(row, chunk)) = x.p[k];
     }
     if (job.delta) {                      // eight lanes for each row
         const int row = threadIdx.x >> 3, i = first + row;
@@ -427,14 +423,6 @@ template <int WAVES> __device__ __forceinline__ void copy_to_lds(char* lds, cons
 
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// A barrier that leaves copies under way (__syncthreads waits for all of them): what the waves wrote to LDS
-// themselves is there after it
-__device__ __forceinline__ void barrier_only() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // Whether the keys of a tile are of the lane's row's document, as bits in the order of the accumulator's registers
 __device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) {
     unsigned m = 0;
@@ -448,8 +436,7 @@ __device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) 
 
 // What the kernels read of the packed matrices
 struct Packed {
-    const char *key_rows, *key_columns, *value_rows, *value_columns;
-    const char *query_rows, *query_columns, *grad_rows, *grad_columns;
+    const char *key, *value, *query, *grad;
     const unsigned *key_marks, *value_marks, *query_marks, *grad_marks;
     float* delta;
 };
@@ -529,8 +516,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     auto copy = [&](int to, int j) {                  // (marks are read ahead of the copies: a wait for them would wait for these)
         marks_next[0] = in.key_marks[place + j / kTile];
         marks_next[1] = in.value_marks[place + j / kTile];
-        copy_to_lds<WAVES>(lds[to], in.key_rows + (place + j / kTile) * P::BYTES, P::BYTES);
-        copy_to_lds<WAVES>(lds[to] + P::BYTES, in.value_columns + (place + j / kTile) * P::BYTES, P::BYTES);
+        copy_to_lds<WAVES>(lds[to], in.key + (place + j / kTile) * P::BYTES, P::BYTES);
+        copy_to_lds<WAVES>(lds[to] + P::BYTES, in.value + (place + j / kTile) * P::BYTES, P::BYTES);
     };
     int docs_next = 0;
     // the first key of the next tile that any row of the block may see
@@ -924,7 +911,7 @@ __global__ __launch_bounds__(kThreads) void attention_join(Args a, int splits, c
 template <int NT, bool CAP>
 __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, int tiles, Packed in) {
     using P = Planes<NT>;
-    __shared__ __attribute__((aligned(16))) char lds[2][3 * P::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
     __shared__ int ends[4], doc_range[2][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int heads = a.batch * a.hkv;
@@ -999,9 +986,8 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
         const int64_t n = place + j / kTile;
         marks_next[0] = in.key_marks[n];
         marks_next[1] = in.value_marks[n];
-        copy_to_lds<4>(lds[to], in.key_rows + n * P::BYTES, P::BYTES);
-        copy_to_lds<4>(lds[to] + P::BYTES, in.value_rows + n * P::BYTES, P::BYTES);
-        copy_to_lds<4>(lds[to] + 2 * P::BYTES, in.key_columns + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(lds[to], in.key + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(lds[to] + P::BYTES, in.value + n * P::BYTES, P::BYTES);
     };
     f32x16 acc[NT];
 #pragma unroll
@@ -1054,7 +1040,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
             }
 #pragma unroll
             for (int v = 0; v < 16; ++v) x[v] = x[v] == 0.f ? 0.f : x[v] * (y[v] - dot) * (CAP ? slope[v] : 1.f);
-            spread6<NT>(acc, lds[buf] + 2 * P::BYTES, split8(x, 0), x, lane);
+            spread6<NT>(acc, lds[buf], split8(x, 0), x, lane);
             if (kbad)
                 spread6_bad<NT>(acc, kbad, a.k + b * a.k_stride[0] + kh * a.k_stride[1] + j0 * a.k_stride[2], a.k_stride[2], a.d, x, lane);
         }
@@ -1065,12 +1051,10 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
 }
 
 // `parts` > 1: the query heads of a key head go to different blocks, whose sums are added by `attention_add`.
-// A tile of rows is read in both orders, 4 x 24 KB for heads of 128, too much for two buffers: the tile by rows has
-// two, the one by columns, which is needed later, is copied while the first products run.
 template <int NT, bool CAP>
 __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, int parts, Packed in, float* part) {
     using P = Planes<NT>;
-    __shared__ __attribute__((aligned(16))) char rows_lds[2][2 * P::BYTES], columns_lds[2 * P::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
     __shared__ __attribute__((aligned(16))) float stat[2][2][kTile];
     __shared__ int doc_range[2][4];
     __shared__ unsigned poison[2][kRows][NT];
@@ -1146,7 +1130,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     auto place = [&](int g, int i0) { return ((int64_t)b * a.hq + kh * group + g) * row_tiles + i0 / kTile; };
     unsigned marks_next[2] = {0, 0};
     float lse_next = 0.f, delta_next = 0.f;
-    auto copy_rows = [&](int to, int g, int i0) {
+    auto copy = [&](int to, int g, int i0) {
         const int64_t n = place(g, i0);
         marks_next[0] = in.query_marks[n];
         marks_next[1] = in.grad_marks[n];
@@ -1156,8 +1140,8 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
             lse_next = i < a.lq ? a.lse[at] : -__builtin_inff();       // (used when it has come: a wait now would be for all copies)
             delta_next = i < a.lq ? in.delta[at] : 0.f;
         }
-        copy_to_lds<4>(rows_lds[to], in.query_rows + n * P::BYTES, P::BYTES);
-        copy_to_lds<4>(rows_lds[to] + P::BYTES, in.grad_rows + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(lds[to], in.query + n * P::BYTES, P::BYTES);
+        copy_to_lds<4>(lds[to] + P::BYTES, in.grad + n * P::BYTES, P::BYTES);
     };
     auto stage_stat = [&](int to) {           // weights of rows without pairs: exp2(x - inf) = 0
         if (threadIdx.x < kTile) {
@@ -1168,26 +1152,21 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     unsigned any_bad = 0;
     int g = g0, i0 = first, buf = 0;
     next(g, i0);
-    if (g < g1) {
-        copy_rows(0, g, i0);
-        stage_stat(0);
-    }
+    if (g < g1) copy(0, g, i0);
     while (g < g1) {
         copies_done();
-        __syncthreads();                      // the tile by rows is there, everyone is done with the last one
+        stage_stat(buf);
+        __syncthreads();                      // this tile is there, and everyone is done with the other buffer
         const int docs = docs_next;
         const unsigned qbad = __builtin_amdgcn_readfirstlane(marks_next[0]), gbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
         int ng = g, ni = i0 + kTile;
         next(ng, ni);
         const bool more = ng < g1;
-        const int64_t n = place(g, i0);
         const float slope2 = a.slopes ? a.slopes[kh * group + __builtin_amdgcn_readfirstlane(g)] * kLog2e : 0.f;
-        copy_to_lds<4>(columns_lds, in.query_columns + n * P::BYTES, P::BYTES);
-        copy_to_lds<4>(columns_lds + P::BYTES, in.grad_columns + n * P::BYTES, P::BYTES);
-        if (more) copy_rows(buf ^ 1, ng, ni);
+        if (more) copy(buf ^ 1, ng, ni);
 
         const int qh = kh * group + g;
-        f32x16 x = product6<NT>(rows_lds[buf], key, lane), slope;
+        f32x16 x = product6<NT>(lds[buf], key, lane), slope;
         if constexpr (CAP) {
             tanh_tile(x, 1.f / a.cap);
 #pragma unroll
@@ -1213,7 +1192,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
             }
         }
         Three lo;                             // weights of the first eight registers, split as they come
-        f32x16 y = product6<NT>(rows_lds[buf] + P::BYTES, val, lane, [&](int t) {
+        f32x16 y = product6<NT>(lds[buf] + P::BYTES, val, lane, [&](int t) {
 #pragma unroll
             for (int v = 16 * t / (2 * NT); v < 16 * (t + 1) / (2 * NT); ++v) {
                 x[v] = x[v] == -__builtin_inff() ? 0.f : exp2_(x[v] - stat[buf][0][acc_row(v, h)]);      // (the row's lse may be NaN)
@@ -1224,23 +1203,15 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
 #pragma unroll
             for (int v = 0; v < 16; ++v) y[v] = gbad >> 4 * h >> acc_row(v, 0) & 1 ? __builtin_nanf("") : y[v];
         }
-        // the copies by columns are done when no more are under way than every wave queued after them, for the
-        // next tile's rows: two matrices of 6 NT kilobytes, of which a wave takes a quarter, rounded down
-        if (more)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (6 * NT / 4)) : "memory");
-        else
-            copies_done();
-        if (more) stage_stat(buf ^ 1);
-        barrier_only();
         Three dlow;
-        spread6<NT>(dv, columns_lds + P::BYTES, lo, x, lane, [&](int c) {
+        spread6<NT>(dv, lds[buf] + P::BYTES, lo, x, lane, [&](int c) {
 #pragma unroll
             for (int e = 16 * c / NT; e < 16 * (c + 1) / NT; ++e) {
                 y[e] = x[e] == 0.f ? 0.f : x[e] * (y[e] - stat[buf][1][acc_row(e, h)]) * (CAP ? slope[e] : 1.f);
                 if (e < 8 && e % 2) split2(f32x2{y[e - 1], y[e]}, e - 1, dlow);
             }
         });
-        spread6<NT>(dk, columns_lds, dlow, y, lane);
+        spread6<NT>(dk, lds[buf], dlow, y, lane);
         if (gbad)
             note_bad<NT>(&poison[1][wave * 32], gbad, a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1] + i0 * a.dout_stride[2], a.dout_stride[2], a.d, x, lane);
         if (qbad)
@@ -1346,8 +1317,8 @@ Room room_forward(const Args& a, const Plan& p) {
     if (!p.few) {
         r.packed.key_marks = next_room<unsigned>(at, tiles * 4);
         r.packed.value_marks = next_room<unsigned>(at, tiles * 4);
-        r.packed.key_rows = next_room<char>(at, planes);
-        r.packed.value_columns = next_room<char>(at, planes);
+        r.packed.key = next_room<char>(at, planes);
+        r.packed.value = next_room<char>(at, planes);
     }
     r.lse = at;
     if (p.splits > 1) next_room<float>(at, rows * p.splits * 4);
@@ -1367,13 +1338,10 @@ Room room_grad(const Args& a, int parts) {
     r.packed.value_marks = next_room<unsigned>(at, keys * 4);
     r.packed.query_marks = next_room<unsigned>(at, queries * 4);
     r.packed.grad_marks = next_room<unsigned>(at, queries * 4);
-    r.packed.key_rows = next_room<char>(at, keys * 6144 * nt);
-    r.packed.key_columns = next_room<char>(at, keys * 6144 * nt);
-    r.packed.value_rows = next_room<char>(at, keys * 6144 * nt);
-    r.packed.query_rows = next_room<char>(at, queries * 6144 * nt);
-    r.packed.query_columns = next_room<char>(at, queries * 6144 * nt);
-    r.packed.grad_rows = next_room<char>(at, queries * 6144 * nt);
-    r.packed.grad_columns = next_room<char>(at, queries * 6144 * nt);
+    r.packed.key = next_room<char>(at, keys * 6144 * nt);
+    r.packed.value = next_room<char>(at, keys * 6144 * nt);
+    r.packed.query = next_room<char>(at, queries * 6144 * nt);
+    r.packed.grad = next_room<char>(at, queries * 6144 * nt);
     r.part = at;
     if (parts > 1) next_room<float>(at, (uint64_t)parts * 2 * a.batch * a.hkv * a.lk * a.d * 4);
     r.all = at;
@@ -1384,22 +1352,21 @@ Room room_grad(const Args& a, int parts) {
 Packed packed_at(const Room& room, char* work) {
     Packed p = room.packed;
     auto move = [&](auto*& x) { x = (std::remove_reference_t<decltype(x)>)(work + (uint64_t)x); };
-    move(p.key_rows), move(p.key_columns), move(p.value_rows), move(p.value_columns);
-    move(p.query_rows), move(p.query_columns), move(p.grad_rows), move(p.grad_columns);
+    move(p.key), move(p.value), move(p.query), move(p.grad);
     move(p.key_marks), move(p.value_marks), move(p.query_marks), move(p.grad_marks), move(p.delta);
     return p;
 }
 
-Pack pack_of(const float* x, const int64_t* stride, int heads, int rows, int keys, const char* by_rows, const char* by_columns, const unsigned* marks, float* delta) {
-    return Pack{x, {stride[0], stride[1], stride[2]}, heads, (rows + kTile - 1) / kTile, keys, (char*)by_rows, (char*)by_columns, (unsigned*)marks, delta};
+Pack pack_of(const float* x, const int64_t* stride, int heads, int rows, int keys, const char* planes, const unsigned* marks, float* delta = nullptr) {
+    return Pack{x, {stride[0], stride[1], stride[2]}, heads, (rows + kTile - 1) / kTile, keys, (char*)planes, (unsigned*)marks, delta};
 }
 
 template <int NT> void launch_rows(const Args& a, const Plan& p, const Packed& in, float* part, float* part_lse, hipStream_t s) {
     const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
     const int key_tiles = (a.lk + kTile - 1) / kTile, tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
     Packs packs{};
-    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key_rows, nullptr, in.key_marks, nullptr);
-    packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, nullptr, in.value_columns, in.value_marks, nullptr);
+    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key, in.key_marks);
+    packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, in.value, in.value_marks);
     if (key_tiles) attention_pack<NT><<<dim3((unsigned)(2 * heads * key_tiles)), kThreads, 0, s>>>(a, packs, p.wide);
     const dim3 grid((unsigned)(heads * tiles * p.splits));
     if (p.waves == 8)
@@ -1412,10 +1379,10 @@ template <int NT> void launch_grad(const Args& a, const Plan& p, int parts, cons
     const int64_t heads = (int64_t)a.batch * a.hkv;
     const int key_tiles = (a.lk + kTile - 1) / kTile, query_tiles = (a.lq + kTile - 1) / kTile, tiles = row_tiles(a);
     Packs packs{};
-    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key_rows, in.key_columns, in.key_marks, nullptr);
-    packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, in.value_rows, nullptr, in.value_marks, nullptr);
-    packs.job[2] = pack_of(a.q, a.q_stride, a.hq, a.lq, 0, in.query_rows, in.query_columns, in.query_marks, nullptr);
-    packs.job[3] = pack_of(a.dout, a.dout_stride, a.hq, a.lq, 0, in.grad_rows, in.grad_columns, in.grad_marks, in.delta);
+    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key, in.key_marks);
+    packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, in.value, in.value_marks);
+    packs.job[2] = pack_of(a.q, a.q_stride, a.hq, a.lq, 0, in.query, in.query_marks);
+    packs.job[3] = pack_of(a.dout, a.dout_stride, a.hq, a.lq, 0, in.grad, in.grad_marks, in.delta);
     const int64_t blocks = 2 * heads * key_tiles + 2 * (int64_t)a.batch * a.hq * query_tiles;
     attention_pack<NT><<<dim3((unsigned)blocks), kThreads, 0, s>>>(a, packs, p.wide);
     const dim3 rows_grid((unsigned)(heads * tiles)), keys_grid((unsigned)(heads * parts * ((a.lk + kRows - 1) / kRows)));
