@@ -155,18 +155,18 @@ __device__ __forceinline__ f32x16 mac6(const Three& a, const Three& b, f32x16 c)
 }
 
 // A 32-row tile in three planes: [plane][element / 8][row][element % 8], 16-byte chunks of eight elements of a
-// row, those of odd chunks with the row's bit 2 turned.  A product contracts over elements (row_chunk: a lane
+// row, whose bits 2 and 3 are turned by the chunk's number.  A product contracts over elements (row_chunk: a lane
 // takes a chunk of its row, consecutive lanes consecutive chunks) or over rows (column_chunk: a lane takes
-// eight rows of its element with transposing reads, of which 16 lanes read four rows of two chunks; the turned bit
-// puts these into different banks).  The eight rows are those that a lane half holds in eight registers
+// eight rows of its element with transposing reads, of which 32 lanes read four rows of four chunks; the turned
+// bits put these into different banks).  The eight rows are those that a lane half holds in eight registers
 // of an accumulator (acc_row), so that weights go from one product to the next without a move.
 template <int NT> struct Planes {
     static constexpr int PLANE = 2 * 32 * 32 * NT;    // bytes
     static constexpr int BYTES = 3 * PLANE;           // of a tile
-    __device__ __forceinline__ static int place(int row, int chunk) { return (chunk * 32 + (row ^ 4 * (chunk & 1))) * 16; }
+    __device__ __forceinline__ static int place(int row, int chunk) { return (chunk * 32 + (row ^ 4 * (chunk & 3))) * 16; }
     __device__ __forceinline__ static Three row_chunk(const char* tile, int row, int t, int h) {
         Three x;
-        const char* at = tile + place(row, h) + 1024 * t;
+        const char* at = tile + place(row, h + 2 * (t & 1)) + 2048 * (t / 2);
 #pragma unroll
         for (int n = 0; n < 3; ++n) x.p[n] = *(const bf16x8*)(at + n * PLANE);
         return x;
@@ -175,13 +175,14 @@ template <int NT> struct Planes {
     __device__ __forceinline__ static Three column_chunk(const char* tile, int u, int c, int lane) {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const int l = lane & 15, odd = l >> 1 & 1, row = (4 * (lane >> 5) + (l >> 2)) ^ 4 * odd;
-        const char* at = tile + ((2 * (lane >> 4 & 1) + odd) * 32 + row) * 16 + (l & 1) * 8 + 2048 * c + 256 * u;
+        const int l = lane & 15, chunk = 2 * (lane >> 4 & 1) + (l >> 1 & 1);
+        const char* at = tile + place(4 * (lane >> 5) + (l >> 2), chunk) + (l & 1) * 8 + 2048 * c + 256 * u;
+        const int other = place(8 + 4 * (lane >> 5) + (l >> 2), chunk) - place(4 * (lane >> 5) + (l >> 2), chunk);
         Three x;
 #pragma unroll
         for (int n = 0; n < 3; ++n) {
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + n * PLANE));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + n * PLANE + 128));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + other + n * PLANE));
             x.p[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
         return x;
@@ -193,6 +194,18 @@ template <int NT> struct Planes {
 // a whole tile come first, and what they displace goes to scratch memory, whose waits are also waits for the
 // next tile's copies.
 __device__ __forceinline__ void step_ends() { __builtin_amdgcn_sched_barrier(0); }
+
+// MIX: the order within a step is reads of LDS, then matrix instructions with vector instructions behind each, which
+// run while it does (a matrix instruction that waits for the one before it holds up all that come after).  For
+// kernels with one wave on each SIMD; two waves fill each other's gaps, and the order costs registers.
+template <int READS> __device__ __forceinline__ void mix_step() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+    for (int n = 0; n < 6; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 7, 0);
+    }
+}
 
 // tanh(x * by); scores are mostly small against their cap, and then a third of the work is enough
 __device__ __forceinline__ void tanh_tile(f32x16& x, float by) {
@@ -223,7 +236,7 @@ struct Nothing {
 
 // acc[row][col] = sum_d tile[row][d] own[col][d]: lane l holds elements 16t + 8h .. + 7 of column l % 32.
 // between(t) is vector work that step t's matrix instructions hide (here and below).
-template <int NT, typename F = Nothing>
+template <int NT, bool MIX, typename F = Nothing>
 __device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[2 * NT], int lane, F between = F()) {
     f32x16 acc;
 #pragma unroll
@@ -237,6 +250,7 @@ __device__ __forceinline__ f32x16 product6(const char* tile, const Three (&own)[
         acc = mac6(x, own[t], acc);
         between(t);
         x = y;
+        if (MIX) mix_step<3>();
         step_ends();
     }
     return acc;
@@ -251,7 +265,7 @@ __device__ __forceinline__ Three split8(const f32x16& w, int from) {
 
 // acc[c][i][col] += sum_row tile[row][32 c + i] w[row][col]; `lo`: the first eight registers of w, split.
 // The others are split between the products of those, then comes between(c).
-template <int NT, typename F = Nothing>
+template <int NT, bool MIX, typename F = Nothing>
 __device__ __forceinline__ void spread6(f32x16 (&acc)[NT], const char* tile, const Three& lo, const f32x16& w, int lane, F between = F()) {
     Three x = Planes<NT>::column_chunk(tile, 0, 0, lane), hi;
     step_ends();
@@ -271,6 +285,7 @@ __device__ __forceinline__ void spread6(f32x16 (&acc)[NT], const char* tile, con
             }
             acc[c] = mac6(x, u == 0 ? lo : hi, acc[c]);
             x = y;
+            if (MIX) mix_step<6>();
             step_ends();
         }
 }
@@ -413,12 +428,16 @@ template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Arg
     }
 }
 
-// `bytes` (a multiple of 1024) from memory to LDS without a register between, by the block's waves in turn
+// `bytes` (a multiple of 1024) from memory to LDS without a register between, by the block's waves in turn.
+// As instructions that the compiler does not know for writes to LDS: it would wait for them ahead of the next
+// read of LDS, though that is one of the other buffer.  They have no result in registers; copies_done() and a
+// barrier stand before the first read of what they write.  (m0 is the compiler's own register, which these kernels
+// use for nothing else.)
 template <int WAVES> __device__ __forceinline__ void copy_to_lds(char* lds, const char* from, int bytes) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     for (int at = wave * 1024; at < bytes; at += WAVES * 1024)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + at + lane * 16),
-                                         (__attribute__((address_space(3))) void*)(lds + at), 16, 0, 0);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to + at)), "v"(from + at + lane * 16) : "memory");
 }
 
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -548,7 +567,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
         const int j1 = next(j0 + kTile);
         if (j1 < end) copy(buf ^ 1, j1);
         if (j0 < top) {                                // some row of this wave sees the tile
-            f32x16 x = product6<NT>(lds[buf], own, lane);
+            f32x16 x = product6<NT, false>(lds[buf], own, lane);
             if (a.cap > 0.f) {
                 tanh_tile(x, 1.f / a.cap);
 #pragma unroll
@@ -588,7 +607,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
                 x[v] = exp2_(x[v] - ref);
                 total += x[v];
             }
-            spread6<NT>(acc, lds[buf] + P::BYTES, split8(x, 0), x, lane);
+            spread6<NT, false>(acc, lds[buf] + P::BYTES, split8(x, 0), x, lane);
             if (vbad)
                 spread6_bad<NT>(acc, vbad, a.v + b * a.v_stride[0] + kh * a.v_stride[1] + j0 * a.v_stride[2], a.v_stride[2], a.d, x, lane);
         }
@@ -1004,7 +1023,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
         const int j1 = next(j0 + kTile);
         if (j1 < end) copy(buf ^ 1, j1);
         if (j0 < top) {
-            f32x16 x = product6<NT>(lds[buf], own, lane);
+            f32x16 x = product6<NT, true>(lds[buf], own, lane);
             f32x16 slope;                              // of the capped scores
             if constexpr (CAP) {
                 tanh_tile(x, 1.f / a.cap);
@@ -1030,7 +1049,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
                     x[v] = ok ? x[v] : -__builtin_inff();
                 }
             }
-            f32x16 y = product6<NT>(lds[buf] + P::BYTES, dout, lane, [&](int t) {
+            f32x16 y = product6<NT, true>(lds[buf] + P::BYTES, dout, lane, [&](int t) {
 #pragma unroll
                 for (int v = 16 * t / (2 * NT); v < 16 * (t + 1) / (2 * NT); ++v) x[v] = exp2_(x[v] - lse2);
             });
@@ -1040,7 +1059,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
             }
 #pragma unroll
             for (int v = 0; v < 16; ++v) x[v] = x[v] == 0.f ? 0.f : x[v] * (y[v] - dot) * (CAP ? slope[v] : 1.f);
-            spread6<NT>(acc, lds[buf], split8(x, 0), x, lane);
+            spread6<NT, true>(acc, lds[buf], split8(x, 0), x, lane);
             if (kbad)
                 spread6_bad<NT>(acc, kbad, a.k + b * a.k_stride[0] + kh * a.k_stride[1] + j0 * a.k_stride[2], a.k_stride[2], a.d, x, lane);
         }
@@ -1166,7 +1185,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
         if (more) copy(buf ^ 1, ng, ni);
 
         const int qh = kh * group + g;
-        f32x16 x = product6<NT>(lds[buf], key, lane), slope;
+        f32x16 x = product6<NT, true>(lds[buf], key, lane), slope;
         if constexpr (CAP) {
             tanh_tile(x, 1.f / a.cap);
 #pragma unroll
@@ -1191,11 +1210,18 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
                 x[v] = ok ? x[v] : -__builtin_inff();
             }
         }
+        f32x16 row_lse, row_delta;            // (read ahead: inside a choice a read would be a branch)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const f32x4 e = *(const f32x4*)&stat[buf][0][8 * u + 4 * h], f = *(const f32x4*)&stat[buf][1][8 * u + 4 * h];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) row_lse[4 * u + c] = e[c], row_delta[4 * u + c] = f[c];
+        }
         Three lo;                             // weights of the first eight registers, split as they come
-        f32x16 y = product6<NT>(lds[buf] + P::BYTES, val, lane, [&](int t) {
+        f32x16 y = product6<NT, true>(lds[buf] + P::BYTES, val, lane, [&](int t) {
 #pragma unroll
             for (int v = 16 * t / (2 * NT); v < 16 * (t + 1) / (2 * NT); ++v) {
-                x[v] = x[v] == -__builtin_inff() ? 0.f : exp2_(x[v] - stat[buf][0][acc_row(v, h)]);      // (the row's lse may be NaN)
+                x[v] = x[v] == -__builtin_inff() ? 0.f : exp2_(x[v] - row_lse[v]);      // (the row's lse may be NaN)
                 if (v < 8 && v % 2) split2(f32x2{x[v - 1], x[v]}, v - 1, lo);
             }
         });
@@ -1204,14 +1230,14 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
             for (int v = 0; v < 16; ++v) y[v] = gbad >> 4 * h >> acc_row(v, 0) & 1 ? __builtin_nanf("") : y[v];
         }
         Three dlow;
-        spread6<NT>(dv, lds[buf] + P::BYTES, lo, x, lane, [&](int c) {
+        spread6<NT, true>(dv, lds[buf] + P::BYTES, lo, x, lane, [&](int c) {
 #pragma unroll
             for (int e = 16 * c / NT; e < 16 * (c + 1) / NT; ++e) {
-                y[e] = x[e] == 0.f ? 0.f : x[e] * (y[e] - stat[buf][1][acc_row(e, h)]) * (CAP ? slope[e] : 1.f);
+                y[e] = x[e] == 0.f ? 0.f : x[e] * (y[e] - row_delta[e]) * (CAP ? slope[e] : 1.f);
                 if (e < 8 && e % 2) split2(f32x2{y[e - 1], y[e]}, e - 1, dlow);
             }
         });
-        spread6<NT>(dk, lds[buf], dlow, y, lane);
+        spread6<NT, true>(dk, lds[buf], dlow, y, lane);
         if (gbad)
             note_bad<NT>(&poison[1][wave * 32], gbad, a.dout + b * a.dout_stride[0] + qh * a.dout_stride[1] + i0 * a.dout_stride[2], a.dout_stride[2], a.d, x, lane);
         if (qbad)
