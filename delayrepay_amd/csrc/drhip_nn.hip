@@ -371,15 +371,20 @@ template <typename T> void launch_rotary_grad(const Rot& p, hipStream_t s) {
 // least min_p of the largest weight: all three are beginnings of that order.  The token is the first one,
 // by number, at which the kept weight summed from token 0 exceeds u times all kept weight.
 //
-// Nothing is sorted: the ends of the kept beginnings are found digit by digit of the logits' bits (11, 11,
-// 10), from counts and weights of the digits.  Weights are 64-bit whole numbers (the largest 2^s, s such
-// that all fit; computed in float64), so that sums do not depend on their order.  A block for each row.
+// A block for each row.  The row is not sorted: one pass finds the largest logit and counts (for top-k), or a
+// second one sums the weights (for top-p), of the logits' first 13 bits; only the tokens of the digit where a
+// beginning ends, or the few kept ones themselves, go to LDS and are sorted there.  Where more share a digit than
+// LDS holds (many equal logits) the end is found digit by digit over the whole row instead.  Weights are
+// 64-bit whole numbers (the largest 2^s, s such that all fit, computed in float64), so that sums do not
+// depend on their order.
 
 typedef drhip_sample_t Smp;
 typedef unsigned long long u64;
 constexpr int kDraw = 1024;          // threads of a block
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;          // of a digit of 11 bits
+constexpr int kCoarse = 8192;        // of the first 13 bits
 constexpr int kChunks = 2048;        // parts of a row whose weights are kept for the last search
+constexpr int kList = 2048;          // tokens that LDS holds
 
 __device__ __forceinline__ unsigned key_of(float x) {
     if (x != x) return 0;                                    // a NaN is below everything and never drawn
@@ -389,15 +394,50 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float value_of(unsigned key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+// Position in the order as one number: larger is earlier
+__device__ __forceinline__ u64 rank_of(float x, int i) { return (u64)key_of(x) << 32 | (unsigned)~i; }
 
 struct Weigher {
     float top;
-    double by, one;       // 1 / temperature, 2^s
-    __device__ __forceinline__ double real(float x) const { return x == top ? 1.0 : x != x ? 0.0 : exp(((double)x - (double)top) * by); }
-    __device__ __forceinline__ u64 whole(double w) const { return (u64)(w * one + 0.5); }
+    double by, one;       // log2(e) / temperature, 2^s
+    // 2^t for t <= 0: t = n + f, |f| <= 1/2, and a polynomial of degree 10 (own fit, relative error 6e-16)
+    __device__ __forceinline__ double real(float x) const {
+        if (x == top) return 1.0;
+        const double t = ((double)x - (double)top) * by, n = rint(t), f = t - n;
+        double p = 7.070977711584016e-09;
+        p = fma(p, f, 1.0205905398548696e-07);
+        p = fma(p, f, 1.3215451632925122e-06);
+        p = fma(p, f, 1.5252672924951426e-05);
+        p = fma(p, f, 0.00015403530424779803);
+        p = fma(p, f, 0.0013333558200794376);
+        p = fma(p, f, 0.00961812910761866);
+        p = fma(p, f, 0.05550410866465167);
+        p = fma(p, f, 0.24022650695910075);
+        p = fma(p, f, 0.6931471805599462);
+        p = fma(p, f, 1.0);
+        return t > -1000.0 ? ldexp(p, (int)n) : 0.0;         // (also where t is NaN: x is)
+    }
+    // nearest whole number of w * 2^s <= 2^52: the low bits of its sum with 2^52
+    __device__ __forceinline__ u64 whole(double w) const {
+        const double x = fma(w, one, 4503599627370496.0);
+        return (u64)__double_as_longlong(x) - 0x4330000000000000ull;
+    }
 };
 
-// Sum over the threads before this one, and over all (four barriers; `lds`: 17 words)
+// f(number, logit) for every token, eight loads at a time under way
+template <typename F> __device__ __forceinline__ void each_token(const float* row, int v, F f) {
+    int i = threadIdx.x;
+    for (; i + 7 * kDraw < v; i += 8 * kDraw) {
+        float x[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x[n] = row[i + n * kDraw];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) f(i + n * kDraw, x[n]);
+    }
+    for (; i < v; i += kDraw) f(i, row[i]);
+}
+
+// Sum over the threads before this one, and over all (`lds`: 17 words)
 __device__ __forceinline__ u64 scan(u64 x, u64* lds, u64& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 sum = x;
@@ -421,23 +461,32 @@ __device__ __forceinline__ u64 scan(u64 x, u64* lds, u64& all) {
 
 struct Found {
     unsigned bin;
-    u64 before;       // of the bins above it
+    u64 before, inside;       // of the bins above it, and its own
 };
 
-// The highest bins first: the one in which the running sum first reaches `want` (1 <= want <= all)
-__device__ __forceinline__ Found reach(const u64* hist, u64 want, u64* lds, Found* out) {
-    const int i = kBins - 1 - 2 * threadIdx.x;
-    const u64 x = hist[i], y = hist[i - 1];
-    u64 all;
-    const u64 before = scan(x + y, lds, all);
-    if (before < want && want <= before + x) *out = {(unsigned)i, before};
-    if (before + x < want && want <= before + x + y) *out = {(unsigned)(i - 1), before + x};
+// The highest bins first: the one in which the running sum first reaches `want(all)`, between 1 and all
+template <int BINS, typename T, typename W> __device__ __forceinline__ Found reach(const T* hist, W want_of, u64* lds, Found* out) {
+    constexpr int PER = BINS / kDraw;
+    const int first = BINS - 1 - PER * threadIdx.x;
+    u64 sum = 0;
+#pragma unroll
+    for (int n = 0; n < PER; ++n) sum += hist[first - n];
+    u64 all, before = scan(sum, lds, all);
+    const u64 want = want_of(all);
+    if (before < want && want <= before + sum) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const u64 x = hist[first - n];
+            if (before < want && want <= before + x) *out = {(unsigned)(first - n), before, x};
+            before += x;
+        }
+    }
     __syncthreads();
     return *out;
 }
 
 // The key at which the running sum (of counts, or of weights) over falling keys first reaches `want`, over the
-// tokens with keys of at least `least`; before: the sum of the larger ones
+// tokens with keys of at least `least` and, in place of those with `tie_key`, `ties` of them; before: the sum of the larger ones
 template <bool COUNT>
 __device__ unsigned select(const float* row, int v, unsigned least, u64 ties, unsigned tie_key, u64 want, const Weigher& weigh,
                            u64* hist, u64* lds, Found* found, u64& before) {
@@ -456,11 +505,11 @@ __device__ unsigned select(const float* row, int v, unsigned least, u64 ties, un
             if (level && key >> (shift + bits) != prefix) continue;
             atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], COUNT ? 1 : weigh.whole(weigh.real(x)));
         }
-        // the tokens at the end of the top-k beginning are equal: as many as it keeps, at once
         if (!COUNT && threadIdx.x == 0 && ties && (!level || tie_key >> (shift + bits) == prefix))
             atomicAdd(&hist[tie_key >> shift & ((1u << bits) - 1)], ties * weigh.whole(weigh.real(value_of(tie_key))));
         __syncthreads();
-        const Found f = reach(hist, want - before, lds, found);
+        const u64 rest = want - before;
+        const Found f = reach<kBins>(hist, [&](u64) { return rest; }, lds, found);
         before += f.before;
         prefix = prefix << bits | f.bin;
         __syncthreads();
@@ -468,23 +517,60 @@ __device__ unsigned select(const float* row, int v, unsigned least, u64 ties, un
     return prefix;
 }
 
+// Sorts n entries, largest first, in place (a bitonic network over the next power of two)
+__device__ __forceinline__ void sort_down(u64* list, int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += kDraw) list[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+            for (int t = threadIdx.x; t < size >> 1; t += kDraw) {
+                const int a = 2 * t - (t & (j - 1)), b = a + j;      // pairs j apart
+                const u64 x = list[a], y = list[b];
+                if ((x < y) == !(a & k)) list[a] = y, list[b] = x;
+            }
+            __syncthreads();
+        }
+}
+
 __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
-    __shared__ u64 hist[kBins], lds[kDraw / 64 + 1];
+    __shared__ u64 coarse[kCoarse];            // weights of the first 13 bits, or counts, or the digits of `select`
+    __shared__ u64 list[kList], weights[kList], parts[kChunks], lds[kDraw / 64 + 1];
     __shared__ unsigned marks[kChunks];
     __shared__ Found found;
-    __shared__ int chunk_at;
-    __shared__ u64 chunk_before, chunk_tied;
-    if (threadIdx.x == 0) chunk_at = 0, chunk_before = 0, chunk_tied = 0, found = {0, 0};
+    __shared__ int listed, chunk_at;
+    __shared__ u64 chunk_before, chunk_tied, cut_rank;
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float* row = p.logits + b * p.logits_stride;
     const int v = p.vocabulary;
+    const double temperature = p.temperature ? p.temperature[b] : p.temperature_all;
+    const int64_t k = p.top_k ? p.top_k[b] : p.top_k_all;
+    const double top_p = p.top_p ? p.top_p[b] : p.top_p_all;
+    const bool counted = k > 0 && k < v && temperature > 0.0, cut_p = top_p < 1.0;
+    double min_p = p.min_p ? p.min_p[b] : p.min_p_all;
+    if (!(min_p > 0.0)) min_p = 0.0;
+    if (min_p > 1.0) min_p = 1.0;
+    const double u = p.uniforms_wide ? ((const double*)p.uniforms)[b] : (double)((const float*)p.uniforms)[b];
 
-    // largest logit, lowest number first
+    // largest logit, lowest number first, and how many tokens have each beginning of 13 bits
+    unsigned* counts = (unsigned*)coarse;
+    if (counted)
+        for (int i = threadIdx.x; i < kCoarse; i += kDraw) counts[i] = 0;
+    if (threadIdx.x == 0) listed = 0, chunk_at = 0, chunk_before = 0, chunk_tied = 0, cut_rank = 0, found = {0, 0, 0};
+    __syncthreads();
     u64 best = 0;
-    for (int i = threadIdx.x; i < v; i += kDraw) {
-        const u64 x = (u64)key_of(row[i]) << 32 | (unsigned)~i;
-        best = x > best ? x : best;
-    }
+    if (counted)
+        each_token(row, v, [&](int i, float x) {
+            const u64 r = rank_of(x, i);
+            best = r > best ? r : best;
+            atomicAdd(&counts[r >> 51], 1u);
+        });
+    else
+        each_token(row, v, [&](int i, float x) {
+            const u64 r = rank_of(x, i);
+            best = r > best ? r : best;
+        });
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
         const u64 y = __shfl_xor(best, m);
@@ -497,86 +583,193 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     for (int w = 0; w < kDraw / 64; ++w) best = lds[w] > best ? lds[w] : best;
     __syncthreads();
     const unsigned top_key = (unsigned)(best >> 32);
-    const double temperature = p.temperature ? p.temperature[b] : p.temperature_all;
     const bool none = top_key <= key_of(-__builtin_inff());
     if (none || !(temperature > 0.0)) {
         if (threadIdx.x == 0) p.tokens[b] = none ? -1 : (int64_t)(int)~(unsigned)best;
         return;
     }
-    Weigher weigh{value_of(top_key), 1.0 / temperature, p.one};
-    const int64_t k = p.top_k ? p.top_k[b] : p.top_k_all;
-    const double top_p = p.top_p ? p.top_p[b] : p.top_p_all;
-    double min_p = p.min_p ? p.min_p[b] : p.min_p_all;
-    if (!(min_p > 0.0)) min_p = 0.0;
-    if (min_p > 1.0) min_p = 1.0;
+    const Weigher weigh{value_of(top_key), 1.4426950408889634074 / temperature, p.one};
 
-    // end of what is kept: keys above `cut`, and the first `ties` tokens whose key it is
+    // end of what is kept: ranks of at least `cut`; where that is not known, keys above `cut_key`, and the first
+    // `ties` tokens whose key it is
     const unsigned no_key = ~0u;       // (of no number)
-    unsigned cut = 0;
-    u64 ties = ~0ull, before;
-    bool all = true;
-    if (k > 0 && k < v) {
-        cut = select<true>(row, v, 0, 0, no_key, (u64)k, weigh, hist, lds, &found, before);
+    u64 cut = 0, ties = ~0ull;
+    unsigned cut_key = 0;
+    bool by_key = false;
+    u64 before;
+
+    if (counted) {
+        const Found f = reach<kCoarse>(counts, [&](u64) { return (u64)k; }, lds, &found);
+        const unsigned from = f.bin;
+        if (f.before + f.inside <= kList) {
+            // everything kept fits LDS: sort it, cut it, and draw from it
+            const int n = (int)(f.before + f.inside);
+            each_token(row, v, [&](int i, float x) {
+                const u64 r = rank_of(x, i);
+                if (r >> 51 >= from) list[atomicAdd(&listed, 1)] = r;
+            });
+            __syncthreads();
+            sort_down(list, n);
+            const int keep = (int)k < n ? (int)k : n, at = 2 * threadIdx.x;
+            double w[2];
+            u64 x[2], all;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                w[e] = at + e < keep ? weigh.real(value_of((unsigned)(list[at + e] >> 32))) : 0.0;
+                x[e] = at + e < keep ? weigh.whole(w[e]) : 0;
+            }
+            u64 sum = scan(x[0] + x[1], lds, all);
+            const double goal = top_p * (double)all;
+            u64 want = !cut_p || goal >= (double)all ? all : (u64)ceil(goal);
+            if (want < 1) want = 1;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bool in = at + e < keep && sum < want && w[e] >= min_p;
+                sum += x[e];
+                x[e] = in ? x[e] : 0;
+                if (at + e < keep) weights[at + e] = x[e];
+            }
+            scan(x[0] + x[1], lds, all);
+            const double aim = u * (double)all;
+            u64 target = aim > 0.0 ? (aim >= (double)all ? all - 1 : (u64)aim) : 0;
+            if (target >= all) target = all - 1;
+            __syncthreads();
+            // the weight of the kept tokens with lower numbers
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (!x[e]) continue;
+                const unsigned mine = (unsigned)list[at + e];
+                u64 lower = 0;
+                for (int j = 0; j < keep; ++j)
+                    if ((unsigned)list[j] > mine) lower += weights[j];       // (numbers are kept as ~i)
+                if (lower <= target && target < lower + x[e]) p.tokens[b] = (int64_t)(int)~mine;
+            }
+            return;
+        }
+        __syncthreads();
+        cut_key = select<true>(row, v, 0, 0, no_key, (u64)k, weigh, coarse, lds, &found, before);
         ties = (u64)k - before;
-        all = false;
+        by_key = true;
     }
-    if (top_p < 1.0) {
-        // weight of the beginning so far
+    // weights of the parts of the row, of tokens that are kept for certain
+    const int chunk = max(512, ((v + kChunks - 1) / kChunks + 63) & ~63), chunks = (v + chunk - 1) / chunk;
+    bool done = false;
+    if (cut_p && !by_key) {
+        for (int i = threadIdx.x; i < kCoarse; i += kDraw) coarse[i] = 0;
+        __syncthreads();
+        each_token(row, v, [&](int, float x) {
+            const u64 w = weigh.whole(weigh.real(x));
+            if (w) atomicAdd(&coarse[key_of(x) >> 19], w);
+        });
+        __syncthreads();
+        u64 want = 0;
+        const Found f = reach<kCoarse>(coarse, [&](u64 all) {
+            const double goal = top_p * (double)all;
+            want = goal >= (double)all ? all : (u64)ceil(goal);
+            return want < 1 ? (want = 1) : want;
+        }, lds, &found);
+        // the tokens of the digit in which the beginning ends go to the list, if there is room; those of larger ones are kept
+        for (int c = wave; c < chunks; c += kDraw / 64) {
+            u64 sum = 0;
+            for (int i = c * chunk + lane; i < min(v, (c + 1) * chunk); i += 64) {
+                const float x = row[i];
+                const unsigned digit = key_of(x) >> 19;
+                if (digit == f.bin) {
+                    const int at = atomicAdd(&listed, 1);
+                    if (at < kList) list[at] = rank_of(x, i);
+                } else if (digit > f.bin) {
+                    const double w = weigh.real(x);
+                    if (w >= min_p) sum += weigh.whole(w);
+                }
+            }
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+            if (lane == 0) parts[c] = sum;
+        }
+        __syncthreads();
+        const int n = listed;
+        if (n <= kList) {
+            sort_down(list, n);
+            const int at = 2 * threadIdx.x;
+            u64 x[2], all;
+            double w[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                w[e] = at + e < n ? weigh.real(value_of((unsigned)(list[at + e] >> 32))) : 0.0;
+                x[e] = at + e < n ? weigh.whole(w[e]) : 0;
+            }
+            u64 sum = f.before + scan(x[0] + x[1], lds, all);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bool in = at + e < n && sum < want;
+                sum += x[e];
+                if (!in) continue;
+                if (sum >= want || at + e == n - 1) cut_rank = list[at + e];      // the last one that is kept
+                if (w[e] >= min_p) atomicAdd(&parts[(int)~(unsigned)list[at + e] / chunk], x[e]);
+            }
+            __syncthreads();
+            cut = cut_rank;
+            done = true;
+        } else {
+            cut_key = select<false>(row, v, 0, 0, no_key, want, weigh, coarse, lds, &found, before);
+            const u64 each = weigh.whole(weigh.real(value_of(cut_key)));
+            ties = each ? (want - before + each - 1) / each : 1;
+            by_key = true;
+        }
+    } else if (cut_p) {
+        // the part p of the weight of the top-k beginning, which may end among its last, equal tokens
         u64 sum = 0, weight;
         for (int i = threadIdx.x; i < v; i += kDraw) {
             const float x = row[i];
-            const unsigned key = key_of(x);
-            if (all || key > cut) sum += weigh.whole(weigh.real(x));
+            if (key_of(x) > cut_key) sum += weigh.whole(weigh.real(x));
         }
         scan(sum, lds, weight);
-        const u64 tied = all ? 0 : ties * weigh.whole(weigh.real(value_of(cut)));
-        weight += tied;
+        weight += ties * weigh.whole(weigh.real(value_of(cut_key)));
         const double goal = top_p * (double)weight;
         u64 want = goal >= (double)weight ? weight : (u64)ceil(goal);
         if (want < 1) want = 1;
-        const unsigned from = all ? 0 : cut;
-        const unsigned end = select<false>(row, v, from, all ? 0 : ties, all ? no_key : cut, want, weigh, hist, lds, &found, before);
+        const unsigned end = select<false>(row, v, cut_key, ties, cut_key, want, weigh, coarse, lds, &found, before);
         const u64 each = weigh.whole(weigh.real(value_of(end)));
         u64 n = each ? (want - before + each - 1) / each : 1;
-        if (!all && end == cut && n > ties) n = ties;
-        cut = end;
+        if (end == cut_key && n > ties) n = ties;
+        cut_key = end;
         ties = n;
-        all = false;
     }
 
-    // weights and ties of the parts of the row, then the part and the token in which the draw falls
-    const int chunk = max(512, ((v + kChunks - 1) / kChunks + 63) & ~63), chunks = (v + chunk - 1) / chunk;
-    for (int c = wave; c < chunks; c += kDraw / 64) {
-        u64 sum = 0;
-        unsigned tied = 0;
-        for (int i = c * chunk + lane; i < min(v, (c + 1) * chunk); i += 64) {
-            const float x = row[i];
-            const unsigned key = key_of(x);
-            if (!all && key < cut) continue;
-            const double w = weigh.real(x);
-            if (w < min_p) continue;
-            if (!all && key == cut) ++tied;
-            else sum += weigh.whole(w);
-        }
+    if (!done)
+        for (int c = wave; c < chunks; c += kDraw / 64) {
+            u64 sum = 0;
+            unsigned tied = 0;
+            for (int i = c * chunk + lane; i < min(v, (c + 1) * chunk); i += 64) {
+                const float x = row[i];
+                const unsigned key = key_of(x);
+                if (by_key && key < cut_key) continue;
+                const double w = weigh.real(x);
+                if (w < min_p) continue;
+                if (by_key && key == cut_key) ++tied;
+                else sum += weigh.whole(w);
+            }
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            sum += __shfl_xor(sum, m);
-            tied += __shfl_xor(tied, m);
+            for (int m = 1; m < 64; m <<= 1) {
+                sum += __shfl_xor(sum, m);
+                tied += __shfl_xor(tied, m);
+            }
+            if (lane == 0) parts[c] = sum, marks[c] = tied;
         }
-        if (lane == 0) hist[c] = sum, marks[c] = tied;
-    }
+    else
+        for (int c = threadIdx.x; c < chunks; c += kDraw) marks[c] = 0;
     __syncthreads();
-    const u64 each = all ? 0 : weigh.whole(weigh.real(value_of(cut)));
+    // the part and the token in which the draw falls
+    const u64 each = by_key ? weigh.whole(weigh.real(value_of(cut_key))) : 0;
     const int c0 = 2 * threadIdx.x;
     const unsigned t0 = c0 < chunks ? marks[c0] : 0, t1 = c0 + 1 < chunks ? marks[c0 + 1] : 0;
     u64 every;
     const u64 tied_before = scan(t0 + t1, lds, every);
     auto kept = [&](u64 from, u64 count) { return from >= ties ? 0 : (ties - from < count ? ties - from : count); };
-    const u64 w0 = c0 < chunks ? hist[c0] + each * kept(tied_before, t0) : 0;
-    const u64 w1 = c0 + 1 < chunks ? hist[c0 + 1] + each * kept(tied_before + t0, t1) : 0;
+    const u64 w0 = c0 < chunks ? parts[c0] + each * kept(tied_before, t0) : 0;
+    const u64 w1 = c0 + 1 < chunks ? parts[c0 + 1] + each * kept(tied_before + t0, t1) : 0;
     u64 weight;
     const u64 weight_before = scan(w0 + w1, lds, weight);
-    const double u = p.uniforms_wide ? ((const double*)p.uniforms)[b] : (double)((const float*)p.uniforms)[b];
     const double goal = u * (double)weight;
     u64 target = goal > 0.0 ? (goal >= (double)weight ? weight - 1 : (u64)goal) : 0;
     if (target >= weight) target = weight - 1;
@@ -592,8 +785,8 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         const float x = i < v ? row[i] : -__builtin_inff();
         const unsigned key = key_of(x);
         const double w = weigh.real(x);
-        bool in = i < v && (all || key >= cut) && w >= min_p;
-        const bool tie = in && !all && key == cut;
+        bool in = i < v && (by_key ? key >= cut_key : rank_of(x, i) >= cut) && w >= min_p;
+        const bool tie = in && by_key && key == cut_key;
         const u64 m = __ballot(tie);
         if (tie) in = tied + __popcll(m & ((1ull << lane) - 1)) < ties;
         tied += __popcll(m);
