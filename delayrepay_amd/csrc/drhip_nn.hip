@@ -385,6 +385,7 @@ constexpr int kBins = 2048;          // of a digit of 11 bits
 constexpr int kCoarse = 8192;        // of the first 13 bits
 constexpr int kChunks = 2048;        // parts of a row whose weights are kept for the last search
 constexpr int kList = 2048;          // tokens that LDS holds
+constexpr int kFew = 128;            // of which so many are ordered by comparing all
 
 __device__ __forceinline__ unsigned key_of(float x) {
     if (x != x) return 0;                                    // a NaN is below everything and never drawn
@@ -402,8 +403,8 @@ struct Weigher {
     double by, one;       // log2(e) / temperature, 2^s
     // 2^t for t <= 0: t = n + f, |f| <= 1/2, and a polynomial of degree 10 (own fit, relative error 6e-16)
     __device__ __forceinline__ double real(float x) const {
-        if (x == top) return 1.0;
-        const double t = ((double)x - (double)top) * by, n = rint(t), f = t - n;
+        if (top == __builtin_inff()) return x == top ? 1.0 : 0.0;
+        const double t = fmax(((double)x - (double)top) * by, -1000.0), n = rint(t), f = t - n;      // (-1000 also for a NaN)
         double p = 7.070977711584016e-09;
         p = fma(p, f, 1.0205905398548696e-07);
         p = fma(p, f, 1.3215451632925122e-06);
@@ -415,7 +416,7 @@ struct Weigher {
         p = fma(p, f, 0.24022650695910075);
         p = fma(p, f, 0.6931471805599462);
         p = fma(p, f, 1.0);
-        return t > -1000.0 ? ldexp(p, (int)n) : 0.0;         // (also where t is NaN: x is)
+        return ldexp(p, (int)n);
     }
     // nearest whole number of w * 2^s <= 2^52: the low bits of its sum with 2^52
     __device__ __forceinline__ u64 whole(double w) const {
@@ -435,6 +436,18 @@ template <typename F> __device__ __forceinline__ void each_token(const float* ro
         for (int n = 0; n < 8; ++n) f(i + n * kDraw, x[n]);
     }
     for (; i < v; i += kDraw) f(i, row[i]);
+}
+
+// The same for one part of the row by one wave, from number `first` to `end`
+template <typename F> __device__ __forceinline__ void each_of_part(const float* row, int first, int end, F f) {
+    for (int i0 = first + (threadIdx.x & 63); i0 < end; i0 += 512) {
+        float x[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x[n] = row[min(i0 + 64 * n, end - 1)];
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+            if (i0 + 64 * n < end) f(i0 + 64 * n, x[n]);
+    }
 }
 
 // Sum over the threads before this one, and over all (`lds`: 17 words)
@@ -536,7 +549,7 @@ __device__ __forceinline__ void sort_down(u64* list, int n) {
 
 __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     __shared__ u64 coarse[kCoarse];            // weights of the first 13 bits, or counts, or the digits of `select`
-    __shared__ u64 list[kList], weights[kList], parts[kChunks], lds[kDraw / 64 + 1];
+    __shared__ u64 list[kList], weights[kFew], parts[kChunks], lds[kDraw / 64 + 1];
     __shared__ unsigned marks[kChunks];
     __shared__ Found found;
     __shared__ int listed, chunk_at;
@@ -598,63 +611,98 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     bool by_key = false;
     u64 before;
 
+    // weights of the parts of the row, of tokens that are known to be kept
+    const int chunk = max(512, ((v + kChunks - 1) / kChunks + 63) & ~63), chunks = (v + chunk - 1) / chunk;
+    bool done = false;
+    // The list's n tokens, of which the first `most` in the order count and of these the ones before whose weight,
+    // with `ahead` of others, stays below want(their weight): added to the parts, the last one is the end of what is kept.
+    // Up to kFew tokens, each compares itself with all (n reads of LDS for each), more are sorted; 50 tokens take 3 us less so, 270 take 3 us more.
+    auto keep_listed = [&](int n, int most, u64 ahead, auto want_of) {
+        const int keep = most < n ? most : n;
+        const bool few = n <= kFew;
+        u64 rank[2] = {0, 0}, x[2] = {0, 0}, sum = 0, all;
+        double w[2] = {0.0, 0.0};
+        int place = 2 * threadIdx.x;
+        if (few) {
+            const int me = threadIdx.x;
+            if (me < n) {
+                rank[0] = list[me];
+                w[0] = weigh.real(value_of((unsigned)(rank[0] >> 32)));
+                weights[me] = x[0] = weigh.whole(w[0]);
+            } else if (me < n + 8) {
+                list[me] = 0;                // (the loop below goes to a multiple of eight)
+            }
+            __syncthreads();
+            if (me < n) {
+                place = 0;
+                for (int j = 0; j < n; j += 8) {
+                    u64 r[8], y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[e] = list[j + e], y[e] = weights[j + e];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        sum += r[e] > rank[0] ? y[e] : 0;
+                        place += r[e] > rank[0];
+                    }
+                }
+                if (place >= keep) x[0] = 0;
+            } else {
+                place = keep;
+            }
+            scan(x[0], lds, all);
+        } else {
+            sort_down(list, n);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (place + e < keep) {
+                    rank[e] = list[place + e];
+                    w[e] = weigh.real(value_of((unsigned)(rank[e] >> 32)));
+                    x[e] = weigh.whole(w[e]);
+                }
+            sum = scan(x[0] + x[1], lds, all);
+        }
+        const u64 want = want_of(all);
+        sum += ahead;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (few && e) break;
+            const bool in = place + e < keep && sum < want;
+            sum += x[e];
+            if (!in) continue;
+            if (sum >= want || place + e == keep - 1) cut_rank = rank[e];
+            if (w[e] >= min_p) atomicAdd(&parts[(int)~(unsigned)rank[e] / chunk], x[e]);
+        }
+        __syncthreads();
+        cut = cut_rank;
+        done = true;
+    };
+    auto part_of = [&](u64 all) {            // top-p of a weight, at least the first token
+        const double goal = top_p * (double)all;
+        const u64 want = !cut_p || goal >= (double)all ? all : (u64)ceil(goal);
+        return want < 1 ? (u64)1 : want;
+    };
+
     if (counted) {
         const Found f = reach<kCoarse>(counts, [&](u64) { return (u64)k; }, lds, &found);
         const unsigned from = f.bin;
         if (f.before + f.inside <= kList) {
-            // everything kept fits LDS: sort it, cut it, and draw from it
-            const int n = (int)(f.before + f.inside);
+            for (int c = threadIdx.x; c < chunks; c += kDraw) parts[c] = 0;
             each_token(row, v, [&](int i, float x) {
                 const u64 r = rank_of(x, i);
                 if (r >> 51 >= from) list[atomicAdd(&listed, 1)] = r;
             });
             __syncthreads();
-            sort_down(list, n);
-            const int keep = (int)k < n ? (int)k : n, at = 2 * threadIdx.x;
-            double w[2];
-            u64 x[2], all;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                w[e] = at + e < keep ? weigh.real(value_of((unsigned)(list[at + e] >> 32))) : 0.0;
-                x[e] = at + e < keep ? weigh.whole(w[e]) : 0;
-            }
-            u64 sum = scan(x[0] + x[1], lds, all);
-            const double goal = top_p * (double)all;
-            u64 want = !cut_p || goal >= (double)all ? all : (u64)ceil(goal);
-            if (want < 1) want = 1;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const bool in = at + e < keep && sum < want && w[e] >= min_p;
-                sum += x[e];
-                x[e] = in ? x[e] : 0;
-                if (at + e < keep) weights[at + e] = x[e];
-            }
-            scan(x[0] + x[1], lds, all);
-            const double aim = u * (double)all;
-            u64 target = aim > 0.0 ? (aim >= (double)all ? all - 1 : (u64)aim) : 0;
-            if (target >= all) target = all - 1;
-            __syncthreads();
-            // the weight of the kept tokens with lower numbers
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (!x[e]) continue;
-                const unsigned mine = (unsigned)list[at + e];
-                u64 lower = 0;
-                for (int j = 0; j < keep; ++j)
-                    if ((unsigned)list[j] > mine) lower += weights[j];       // (numbers are kept as ~i)
-                if (lower <= target && target < lower + x[e]) p.tokens[b] = (int64_t)(int)~mine;
-            }
-            return;
+            keep_listed((int)(f.before + f.inside), (int)k, 0, part_of);
         }
+    }
+    if (counted && !done) {
         __syncthreads();
         cut_key = select<true>(row, v, 0, 0, no_key, (u64)k, weigh, coarse, lds, &found, before);
         ties = (u64)k - before;
         by_key = true;
     }
-    // weights of the parts of the row, of tokens that are kept for certain
-    const int chunk = max(512, ((v + kChunks - 1) / kChunks + 63) & ~63), chunks = (v + chunk - 1) / chunk;
-    bool done = false;
-    if (cut_p && !by_key) {
+    if (done) {
+    } else if (cut_p && !by_key) {
         for (int i = threadIdx.x; i < kCoarse; i += kDraw) coarse[i] = 0;
         __syncthreads();
         each_token(row, v, [&](int, float x) {
@@ -663,16 +711,11 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         });
         __syncthreads();
         u64 want = 0;
-        const Found f = reach<kCoarse>(coarse, [&](u64 all) {
-            const double goal = top_p * (double)all;
-            want = goal >= (double)all ? all : (u64)ceil(goal);
-            return want < 1 ? (want = 1) : want;
-        }, lds, &found);
+        const Found f = reach<kCoarse>(coarse, [&](u64 all) { return want = part_of(all); }, lds, &found);
         // the tokens of the digit in which the beginning ends go to the list, if there is room; those of larger ones are kept
         for (int c = wave; c < chunks; c += kDraw / 64) {
             u64 sum = 0;
-            for (int i = c * chunk + lane; i < min(v, (c + 1) * chunk); i += 64) {
-                const float x = row[i];
+            each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](int i, float x) {
                 const unsigned digit = key_of(x) >> 19;
                 if (digit == f.bin) {
                     const int at = atomicAdd(&listed, 1);
@@ -681,35 +724,16 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
                     const double w = weigh.real(x);
                     if (w >= min_p) sum += weigh.whole(w);
                 }
-            }
+            });
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
             if (lane == 0) parts[c] = sum;
         }
         __syncthreads();
         const int n = listed;
+        __syncthreads();
         if (n <= kList) {
-            sort_down(list, n);
-            const int at = 2 * threadIdx.x;
-            u64 x[2], all;
-            double w[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                w[e] = at + e < n ? weigh.real(value_of((unsigned)(list[at + e] >> 32))) : 0.0;
-                x[e] = at + e < n ? weigh.whole(w[e]) : 0;
-            }
-            u64 sum = f.before + scan(x[0] + x[1], lds, all);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const bool in = at + e < n && sum < want;
-                sum += x[e];
-                if (!in) continue;
-                if (sum >= want || at + e == n - 1) cut_rank = list[at + e];      // the last one that is kept
-                if (w[e] >= min_p) atomicAdd(&parts[(int)~(unsigned)list[at + e] / chunk], x[e]);
-            }
-            __syncthreads();
-            cut = cut_rank;
-            done = true;
+            keep_listed(n, n, f.before, [&](u64) { return want; });
         } else {
             cut_key = select<false>(row, v, 0, 0, no_key, want, weigh, coarse, lds, &found, before);
             const u64 each = weigh.whole(weigh.real(value_of(cut_key)));
@@ -725,9 +749,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         }
         scan(sum, lds, weight);
         weight += ties * weigh.whole(weigh.real(value_of(cut_key)));
-        const double goal = top_p * (double)weight;
-        u64 want = goal >= (double)weight ? weight : (u64)ceil(goal);
-        if (want < 1) want = 1;
+        const u64 want = part_of(weight);
         const unsigned end = select<false>(row, v, cut_key, ties, cut_key, want, weigh, coarse, lds, &found, before);
         const u64 each = weigh.whole(weigh.real(value_of(end)));
         u64 n = each ? (want - before + each - 1) / each : 1;
@@ -740,15 +762,19 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         for (int c = wave; c < chunks; c += kDraw / 64) {
             u64 sum = 0;
             unsigned tied = 0;
-            for (int i = c * chunk + lane; i < min(v, (c + 1) * chunk); i += 64) {
-                const float x = row[i];
-                const unsigned key = key_of(x);
-                if (by_key && key < cut_key) continue;
-                const double w = weigh.real(x);
-                if (w < min_p) continue;
-                if (by_key && key == cut_key) ++tied;
-                else sum += weigh.whole(w);
-            }
+            if (by_key)
+                each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](int, float x) {
+                    const unsigned key = key_of(x);
+                    const double w = weigh.real(x);
+                    if (key < cut_key || w < min_p) return;
+                    if (key == cut_key) ++tied;
+                    else sum += weigh.whole(w);
+                });
+            else
+                each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](int, float x) {
+                    const double w = weigh.real(x);
+                    sum += w >= min_p ? weigh.whole(w) : 0;
+                });
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) {
                 sum += __shfl_xor(sum, m);
@@ -778,32 +804,34 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     __syncthreads();
     if (wave) return;
     u64 sum = chunk_before, tied = chunk_tied;
-    int token = 0;
-    const int first = chunk_at * chunk;
-    for (int i0 = first; i0 < min(v, first + chunk); i0 += 64) {
-        const int i = i0 + lane;
-        const float x = i < v ? row[i] : -__builtin_inff();
-        const unsigned key = key_of(x);
-        const double w = weigh.real(x);
-        bool in = i < v && (by_key ? key >= cut_key : rank_of(x, i) >= cut) && w >= min_p;
-        const bool tie = in && by_key && key == cut_key;
-        const u64 m = __ballot(tie);
-        if (tie) in = tied + __popcll(m & ((1ull << lane) - 1)) < ties;
-        tied += __popcll(m);
-        u64 run = in ? weigh.whole(w) : 0;
+    int token = -1;
+    const int first = chunk_at * chunk, end = min(v, first + chunk);
+    for (int i1 = first; i1 < end && token < 0; i1 += 512) {
+        float x[8];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const u64 y = __shfl_up(run, d);
-            if (lane >= d) run += y;
+        for (int n = 0; n < 8; ++n) x[n] = row[min(i1 + 64 * n + lane, end - 1)];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const int i = i1 + 64 * n + lane;
+            const unsigned key = key_of(x[n]);
+            const double w = weigh.real(x[n]);
+            bool in = i < end && (by_key ? key >= cut_key : rank_of(x[n], i) >= cut) && w >= min_p;
+            const bool tie = in && by_key && key == cut_key;
+            const u64 m = __ballot(tie);
+            if (tie) in = tied + __popcll(m & ((1ull << lane) - 1)) < ties;
+            tied += __popcll(m);
+            u64 run = in ? weigh.whole(w) : 0;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const u64 y = __shfl_up(run, d);
+                if (lane >= d) run += y;
+            }
+            const u64 past = __ballot(sum + run > target);
+            if (past && token < 0) token = i1 + 64 * n + __builtin_ctzll(past);
+            sum += __shfl(run, 63);
         }
-        const u64 past = __ballot(sum + run > target);
-        if (past) {
-            token = i0 + __builtin_ctzll(past);
-            break;
-        }
-        sum += __shfl(run, 63);
     }
-    if (lane == 0) p.tokens[b] = token;
+    if (lane == 0) p.tokens[b] = token < 0 ? first : token;       // (one is always found: target < weight)
 }
 
 }  // namespace
