@@ -41,6 +41,18 @@ template <typename T, bool WIDE> struct Row {
         if (!p.interleaved) return 4 * lane + n;
         return n < 2 ? 2 * lane + n : half / 2 + 2 * lane + n - 2;
     }
+    // which element at(n) is; -1 for none
+    __device__ __forceinline__ static int element(const Rot& p, int lane, int lanes, int n) {
+        const int half = p.dims / 2;
+        if (n >= 8) {
+            const int i = WIDE ? 4 * (lane + (n >= 12 ? lanes : 0)) + (n & 3) : lane + (n - 8) * lanes;
+            return i < p.d - p.dims ? p.dims + i : -1;
+        }
+        const bool second = n >= 4;
+        const int i = pair(p, lane, lanes, n & 3);
+        if ((WIDE ? 4 * lane : i) >= half) return -1;
+        return p.interleaved ? 2 * i + second : i + (second ? half : 0);
+    }
     __device__ __forceinline__ void load(const Rot& p, const T* row, int lane, int lanes, bool ok) {
         const int half = p.dims / 2, behind = p.d - p.dims;
         if constexpr (WIDE) {
@@ -275,15 +287,14 @@ __global__ __launch_bounds__(kThreads) void rotary_grad_kernel(Rot p, int lanes_
 #pragma unroll
         for (int n = 0; n < 16; ++n) lds[n * kThreads + threadIdx.x] = sums[k][n];
         __syncthreads();
-        if (group == 0 && h0 + k < p.heads) {
-            Row<T, WIDE> total;
-            total.each([&](T& v, int n) {
-                T x = 0;
-                for (int j = 0; j < groups; ++j) x += lds[n * kThreads + j * lanes + lane];
-                v = x;
-            });
-            total.store(p, (T*)p.work + ((int64_t)slot * p.heads + h0 + k) * p.d_pad, lane, lanes);
-        }
+        if (h0 + k < p.heads)
+            for (int o = threadIdx.x; o < 16 << lanes_log; o += kThreads) {
+                const int n = o >> lanes_log, i = Row<T, WIDE>::element(p, o & (lanes - 1), lanes, n);
+                T total = 0;
+#pragma unroll 8
+                for (int j = 0; j < groups; ++j) total += lds[n * kThreads + j * lanes + (o & (lanes - 1))];
+                if (i >= 0) ((T*)p.work)[((int64_t)slot * p.heads + h0 + k) * p.d_pad + i] = total;
+            }
     }
 }
 
@@ -329,13 +340,13 @@ bool wide_of(const Rot& p) {
            quads(p.dy, p.dy_stride, 3, item) && quads(p.weight, &p.weight_stride, 1, item);
 }
 
-// Blocks for each pair of heads in the gradient: about 2048 in all (8 for a compute unit), and at least
-// eight tokens for each group, so that the parts of dw stay small against dx
+// Blocks for each pair of heads in the gradient: up to 2048 in all (8 for a compute unit), and two tokens
+// for each group, so that the parts of dw, a row for each block and head, stay below a thirtieth of dx
 int grad_slots(const Rot& p) {
     const int64_t sets = (p.heads + kHeads - 1) / kHeads, groups = kThreads >> lanes_log_of(p);
     const int64_t runs = ((int64_t)p.batch * p.rows + groups - 1) / groups;
     int64_t slots = 2048 / sets;
-    if (slots > (runs + 7) / 8) slots = (runs + 7) / 8;
+    if (slots > (runs + 1) / 2) slots = (runs + 1) / 2;
     return slots < 1 ? 1 : (int)slots;
 }
 
