@@ -635,7 +635,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
 // waves in turn, and its loads are the operands of v_mfma_f32_16x16x4f32 as they come (K: lane = key,
 // 16 bytes of its row; V: 16 neighbouring bytes of four rows each).  Key ranges of one sequence go to
 // `splits` blocks, whose results are joined by `attention_join`.
-template <int NB, int NQ>
+template <int NB, int NQ, bool WIDE>
 __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, float* part, float* part_lse) {
     constexpr int KS = 4 * NB;                 // 16-byte steps of a key row for each quarter of the wave
     __shared__ __attribute__((aligned(16))) float merged[4][16][64 * NB + 4];
@@ -645,7 +645,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
     const int head = blockIdx.x % heads, split = blockIdx.x / heads;
     const int b = head / a.hkv, kh = head % a.hkv, group = a.hq / a.hkv;
     const Seq s = sequence(a, b);
-    const bool wide = plan.wide;
+    constexpr bool wide = WIDE;       // (apart, for the size of the code: short calls wait for it)
     const int rows = group * a.lq;
 
     f32x4 own[NQ][KS];
@@ -690,49 +690,41 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
             for (int c = 0; c < 4; ++c) acc[n][e][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     f32x4 kx[KS], vx[4][NB];
-    auto fetch = [&](int j0) {
-        const int jk = j0 + col;
-        const float* krow = kbase + (int64_t)(jk < end ? jk : 0) * a.k_stride[2];
+    // Past the end of the range and of the row the last values are read again: such keys do not count, and such
+    // elements meet zeros of q or are not stored.
+    auto quad = [&](const float* row, int d) {
+        if constexpr (WIDE) return *(const f32x4*)(row + min(d, a.d - 4));
+        f32x4 x;
 #pragma unroll
-        for (int t = 0; t < KS; ++t) kx[t] = load4(krow, 16 * t + 4 * h, a.d, jk < end, wide);
+        for (int c = 0; c < 4; ++c) x[c] = row[min(d + c, a.d - 1)];
+        return x;
+    };
+    auto fetch_keys = [&](int j0) {
+        const float* krow = kbase + (int64_t)min(j0 + col, end - 1) * a.k_stride[2];
+#pragma unroll
+        for (int t = 0; t < KS; ++t) kx[t] = quad(krow, 16 * t + 4 * h);
+    };
+    auto fetch_values = [&](int j0) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-            const int jv = j0 + 4 * h + v;
-            const float* vrow = vbase + (int64_t)(jv < end ? jv : 0) * a.v_stride[2];
+            const float* vrow = vbase + (int64_t)min(j0 + 4 * h + v, end - 1) * a.v_stride[2];
 #pragma unroll
-            for (int e = 0; e < NB; ++e) vx[v][e] = load4(vrow, 64 * e + 4 * col, a.d, jv < end, wide);
+            for (int e = 0; e < NB; ++e) vx[v][e] = quad(vrow, 64 * e + 4 * col);
         }
     };
     int j0 = begin + 16 * wave;
-    if (j0 < end) fetch(j0);
+    if (j0 < end) {
+        fetch_keys(j0);
+        fetch_values(j0);
+    }
     while (j0 < end) {
-        f32x4 kc[KS], vc[4][NB];
-#pragma unroll
-        for (int t = 0; t < KS; ++t) kc[t] = kx[t];
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-#pragma unroll
-            for (int e = 0; e < NB; ++e) vc[v][e] = vx[v][e];
         const int j1 = j0 + 64;
-        if (j1 < end) fetch(j1);
-
-        // values that are not finite: taken out here, added by themselves below
+        // keys that are not finite become zeros, and their scores NaN
         bool kbad = false;
-        unsigned vbad = 0;
 #pragma unroll
         for (int t = 0; t < KS; ++t)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) kbad = kbad || !finite_(kc[t][c]);
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-#pragma unroll
-            for (int e = 0; e < NB; ++e)
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (!finite_(vc[v][e][c])) {
-                        vc[v][e][c] = 0.f;
-                        vbad |= 1u << (4 * h + v);
-                    }
+            for (int c = 0; c < 4; ++c) kbad = kbad || !finite_(kx[t][c]);
         unsigned kmask = 0;
         if (__any(kbad)) {                    // (a key's row is spread over four lanes)
             const unsigned long long m = __ballot(kbad);
@@ -740,32 +732,33 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
 #pragma unroll
             for (int t = 0; t < KS; ++t)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) kc[t][c] = finite_(kc[t][c]) ? kc[t][c] : 0.f;
+                for (int c = 0; c < 4; ++c) kx[t][c] = finite_(kx[t][c]) ? kx[t][c] : 0.f;
         }
-        if (__any(vbad != 0)) {
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) vbad |= __shfl_xor(vbad, m);
-        }
-        const bool whole = j0 + 16 <= low && !s.docs && !kmask;
+        f32x4 x[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            x[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < KS; ++t)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) x = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[t][c], own[n][t][c], x, 0, 0, 0);
+                for (int c = 0; c < 4; ++c) x[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[t][c], own[n][t][c], x[n], 0, 0, 0);
+        }
+        if (j1 < end) fetch_keys(j1);         // (values follow when they are used up: each is a step ahead)
+        const bool whole = j0 + 16 <= low && !s.docs && !kmask;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
             float peak = most[n];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 const int j = j0 + 4 * h + v;
-                float z = score(a, x[v], slope2[n], pos[n], j);
+                float z = score(a, x[n][v], slope2[n], pos[n], j);
                 if (!whole) {
                     if (kmask >> (4 * h + v) & 1) z = __builtin_nanf("");
                     bool ok = j < lim[n] && j < end;
                     if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc[n];
                     z = ok ? z : -__builtin_inff();
                 }
-                x[v] = z;
+                x[n][v] = z;
                 peak = z > peak || z != z ? z : peak;
             }
 #pragma unroll
@@ -785,32 +778,57 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
             most[n] = peak;
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                x[v] = exp2_(x[v] - ref);
-                total[n] += x[v];
+                x[n][v] = exp2_(x[n][v] - ref);
+                total[n] += x[n][v];
             }
+        }
+        // values that are not finite become zeros here and are added by themselves below
+        unsigned vbad = 0;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int e = 0; e < NB; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (!finite_(vx[v][e][c])) {
+                        vx[v][e][c] = 0.f;
+                        vbad |= 1u << (4 * h + v);
+                    }
+        if (__any(vbad != 0)) {
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) vbad |= __shfl_xor(vbad, m);
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
             for (int e = 0; e < NB; ++e)
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
                     for (int v = 0; v < 4; ++v)
-                        acc[n][e][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vc[v][e][c], x[v], acc[n][e][c], 0, 0, 0);
-            for (unsigned m = vbad; m; m &= m - 1) {
-                const int key = __builtin_ctz(m);
+                        acc[n][e][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[v][e][c], x[n][v], acc[n][e][c], 0, 0, 0);
+        if (j1 < end) fetch_values(j1);
+        for (unsigned m = vbad; m; m &= m - 1) {
+            const int key = __builtin_ctz(m);
+            if (j0 + key >= end) break;              // (the last key again)
+            int hh = h;
+            asm volatile("" : "+v"(hh));             // (nothing of this is computed ahead and kept)
+            const float* vrow = vbase + (int64_t)(j0 + key) * a.v_stride[2];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
                 float mine = 0.f;
 #pragma unroll
-                for (int v = 0; v < 4; ++v) mine = v == (key & 3) ? x[v] : mine;
+                for (int v = 0; v < 4; ++v) mine = v == (key & 3) ? x[n][v] : mine;
                 const float weight = __shfl(mine, col + 16 * (key >> 2));
-                const float* vrow = vbase + (int64_t)(j0 + key) * a.v_stride[2];
 #pragma unroll
                 for (int e = 0; e < NB; ++e)
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
-                            const int d = 64 * e + 4 * (4 * h + v) + c;
-                            const float y = d < a.d ? vrow[d] : 0.f;
-                            if (!finite_(y) && weight != 0.f) acc[n][e][c][v] += weight * y;
+                            const int d = 64 * e + 4 * (4 * hh + v) + c;
+                            const float y = vrow[d < a.d ? d : 0], z = weight * y;
+                            acc[n][e][c][v] += !finite_(y) && d < a.d && weight != 0.f ? z : 0.f;
                         }
             }
         }
@@ -904,13 +922,25 @@ __global__ __launch_bounds__(kThreads) void attention_join(Args a, int splits, c
     }
     const float ref = peak == -__builtin_inff() ? 0.f : peak;
     float sum = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float w = exp2_((part_lse[s * rows + row] - ref) * kLog2e);
-        if (w == 0.f) continue;
-        const float* from = part + (s * rows + row) * a.d;
-        sum += w;
-        if (lane < a.d) x0 += w * from[lane];
-        if (lane + 64 < a.d) x1 += w * from[lane + 64];
+    const int d0 = lane < a.d ? lane : 0, d1 = lane + 64 < a.d ? lane + 64 : 0;
+    for (int s0 = 0; s0 < splits; s0 += 64) {
+        const float mine = s0 + lane < splits ? exp2_((part_lse[(s0 + lane) * rows + row] - ref) * kLog2e) : 0.f;
+        const int n = min(64, splits - s0);
+        for (int s1 = 0; s1 < n; s1 += 8) {                   // eight ranges' loads under way
+            float w[8], y0[8], y1[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = __shfl(mine, s1 + e);
+                const float* from = part + (min(s0 + s1 + e, splits - 1) * rows + row) * a.d;
+                y0[e] = from[d0], y1[e] = from[d1];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {                     // (a range without keys has nothing there)
+                sum += w[e];
+                x0 += w[e] == 0.f ? 0.f : w[e] * y0[e];
+                x1 += w[e] == 0.f ? 0.f : w[e] * y1[e];
+            }
+        }
     }
     const float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
     const int i = (int)(row % a.lq);
@@ -1299,8 +1329,10 @@ int row_tiles(const Args& a) { return (int)(((int64_t)(a.hq / a.hkv) * a.lq + kR
 
 // Which forward kernel, and into how many key ranges.  Few rows: up to 32 rows of a key head, where the
 // blocks of the other kernel would be mostly empty.  Blocks of eight waves share each tile among 256 rows, of
-// four where that leaves compute units without a block.  Ranges: enough for `want` blocks, none shorter than
-// `least` keys, whose work pays for joining; causal blocks are of unequal length, so two for a compute unit.
+// four where that leaves compute units without a block.  Ranges: enough for a block on each compute unit (two,
+// as causal blocks are of unequal length), none shorter than 256 keys, whose work pays for joining.  For few rows,
+// two blocks for each compute unit with ranges of 128 keys or more, and up to eight, since sequences are of
+// unequal length, as long as ranges have 512.
 Plan plan_forward(const Args& a) {
     Plan p;
     p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride);
@@ -1308,11 +1340,17 @@ Plan plan_forward(const Args& a) {
     p.few = rows <= 32;
     p.waves = heads * ((rows + 255) / 256) >= 256 ? 8 : 4;
     const int64_t blocks = heads * (p.few ? 1 : (rows + 32 * p.waves - 1) / (32 * p.waves));
-    const int64_t want = p.few ? 2048 : a.causal ? 512 : 256;
-    const int least = 256;
-    int64_t splits = blocks >= want ? 1 : (want + blocks - 1) / blocks;
-    const int64_t most = (a.lk + least - 1) / least;
-    if (splits > most) splits = most;
+    int64_t splits;
+    if (p.few) {
+        splits = (512 + blocks - 1) / blocks;
+        const int64_t fine = (2048 + blocks - 1) / blocks, most = (a.lk + 127) / 128, long_ranges = a.lk / 512;
+        if (splits < fine) splits = fine < long_ranges ? fine : long_ranges > splits ? long_ranges : splits;
+        if (splits > most) splits = most;
+    } else {
+        const int64_t want = a.causal ? 512 : 256, most = (a.lk + 255) / 256;
+        splits = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+        if (splits > most) splits = most;
+    }
     if (splits < 1) splits = 1;
     p.chunk = (int)(((a.lk + splits - 1) / splits + 63) / 64 * 64);
     if (p.chunk < 64) p.chunk = 64;
@@ -1401,6 +1439,15 @@ template <int NT> void launch_rows(const Args& a, const Plan& p, const Packed& i
         attention_rows<NT, 4><<<grid, 256, 0, s>>>(a, p, tiles, in, part, part_lse);
 }
 
+template <bool WIDE> void launch_few(const Args& a, const Plan& p, float* part, float* part_lse, hipStream_t s) {
+    const dim3 grid((unsigned)(a.batch * a.hkv * p.splits));
+    const bool two = (int64_t)(a.hq / a.hkv) * a.lq > 16;
+    if (a.d <= 64)
+        two ? attention_few<1, 2, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<1, 1, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
+    else
+        two ? attention_few<2, 2, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<2, 1, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
+}
+
 template <int NT> void launch_grad(const Args& a, const Plan& p, int parts, const Packed& in, float* part, hipStream_t s) {
     const int64_t heads = (int64_t)a.batch * a.hkv;
     const int key_tiles = (a.lk + kTile - 1) / kTile, query_tiles = (a.lq + kTile - 1) / kTile, tiles = row_tiles(a);
@@ -1448,12 +1495,7 @@ extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
     float* part = p.splits > 1 ? (float*)(work + room.part) : nullptr;
     float* part_lse = p.splits > 1 ? (float*)(work + room.lse) : nullptr;
     if (p.few) {
-        const dim3 grid((unsigned)(heads * p.splits));
-        const bool two = (int64_t)(a.hq / a.hkv) * a.lq > 16;
-        if (a.d <= 64)
-            two ? attention_few<1, 2><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<1, 1><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
-        else
-            two ? attention_few<2, 2><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<2, 1><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
+        p.wide ? launch_few<true>(a, p, part, part_lse, s) : launch_few<false>(a, p, part, part_lse, s);
     } else {
         const Packed in = packed_at(room, work);
         switch ((a.d + 31) / 32) {
