@@ -19,8 +19,12 @@ def _strides(x):
     return x._strides[:3]
 
 
+def _steps(x):
+    return None if x is None else x._strides
+
+
 def _ptr(x):
-    return 0 if x is None else x.ptr
+    return 0 if x is None else x.buf.ptr + x.offset * x.dtype.itemsize
 
 
 def _reach(x):
@@ -49,9 +53,12 @@ def _places(outs, shapes, dtype, used, same=None):
     in their last axis or share memory with an operand (`same`: one that may be exactly the output)."""
     places = []
     for i, (out, shape) in enumerate(zip(outs, shapes)):
-        direct = out is not None and not (out.shape and out.shape[-1] > 1 and out._strides[-1] != 1)
+        if out is None:
+            places.append(ndarray(shape, dtype))
+            continue
+        direct = not (out.shape[-1] > 1 and out._strides[-1] != 1)
         if direct:
-            others = used + [o for n, o in enumerate(outs) if n != i]
+            others = used if len(outs) == 1 else used + [o for n, o in enumerate(outs) if n != i]
             if same is not None and out._strides == same._strides and out.ptr == same.ptr:
                 others = [u for u in others if u is not same]
             direct = _apart(out, others)
@@ -70,38 +77,63 @@ def _contiguous(x):
     return x if x is None or x.is_contiguous else x.copy()
 
 
-def _run(func, packer, fields, ints, work, used, written):
-    """Call one operator with `work` bytes of workspace between its two runs of fields."""
-    buf = None
+# What depends on geometry and options alone -> (its part of the argument struct, workspace bytes).  Addresses are
+# not part of it, and no workspace is kept.
+_PLANS = {}
+_PLANS_MAX = 1024
+
+
+def _plan(key, head, tail, fields, make, work_of):
+    """The remembered plan, or a new one: `make()` gives the tail's fields, work_of(args) the workspace."""
+    plan = _PLANS.get(key)
+    if plan is None:
+        packed = tail.pack(*make())
+        plan = packed, work_of(head.pack(*fields, 0, 0) + packed)
+        if len(_PLANS) >= _PLANS_MAX:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
+
+
+def _run(func, head, fields, plan, used, written):
+    """Call one operator, with a workspace from the pool where it needs one."""
+    tail, work = plan
     if work:
         buf = Buffer(work)
-    args = packer.pack(*fields, buf.ptr if buf else 0, work, *ints)
-    hip.issue_operator(func, args, used + written + ([buf] if buf else []), written)
+        hip.issue_operator(func, head.pack(*fields, buf.ptr, work) + tail, used + written + [buf], written)
+    else:
+        hip.issue_operator(func, head.pack(*fields, 0, 0) + tail, used + written, written)
 
 
-def _attention_args(q, k, v, o, lse, dout, grads, how):
+_NONE = (0, 0, 0)
+
+
+def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
     def index(x):
         return _contiguous(x) if isinstance(x, ndarray) else None
     lengths, start, prefix = how.lengths, how.start, how.prefix
     if isinstance(lengths, int):       # a number: the rows behind it do not exist
         k, v = k[:, :, :lengths], v[:, :, :lengths]
-    arrays = [index(lengths), index(start), index(prefix),
-              None if how.documents is None else _dense(how.documents),
-              None if how.slopes is None else _contiguous(how.slopes)]
-    if isinstance(lengths, int) and arrays[3] is not None:
-        arrays[3] = arrays[3][:, :lengths]
-    none = (0, 0, 0)
+    documents = None if how.documents is None else _dense(how.documents)
+    if isinstance(lengths, int) and documents is not None:
+        documents = documents[:, :lengths]
+    arrays = [index(lengths), index(start), index(prefix), documents, None if how.slopes is None else _contiguous(how.slopes)]
     fields = (q.ptr, k.ptr, v.ptr, o.ptr, _ptr(lse), _ptr(dout), *[_ptr(g) for g in grads], *[_ptr(x) for x in arrays])
-    lk = k.shape[2]
-    far = (1 << 31) - 1
-    ints = (*_strides(q), *_strides(k), *_strides(v), *_strides(o),
-            *(none if dout is None else _strides(dout)), *[s for g in grads for s in (none if g is None else _strides(g))],
-            0 if arrays[3] is None else arrays[3]._strides[0],
-            q.shape[0], q.shape[1], k.shape[1], q.shape[2], lk, q.shape[3], int(how.causal),
-            0 if start is None else 1, max(-far, min(far, start)) if isinstance(start, int) else 0,
-            min(prefix, lk) if isinstance(prefix, int) else 0,
-            how.scale, how.cap or 0.0)
-    return fields, ints, [x for x in arrays if x is not None]
+    key = (func, q.shape, q._strides, k.shape, k._strides, v._strides, o._strides, _steps(dout),
+           *[_steps(g) for g in grads], _steps(documents), how.causal,
+           start if isinstance(start, int) else start is None, prefix if isinstance(prefix, int) else None, how.scale, how.cap)
+
+    def make():
+        lk, far = k.shape[2], (1 << 31) - 1
+        return (*_strides(q), *_strides(k), *_strides(v), *_strides(o),
+                *(_NONE if dout is None else _strides(dout)), *[s for g in grads for s in (_NONE if g is None else _strides(g))],
+                0 if documents is None else documents._strides[0],
+                q.shape[0], q.shape[1], k.shape[1], q.shape[2], lk, q.shape[3], int(how.causal),
+                0 if start is None else 1, max(-far, min(far, start)) if isinstance(start, int) else 0,
+                min(prefix, lk) if isinstance(prefix, int) else 0,
+                how.scale, how.cap or 0.0)
+    plan = _plan(key, hiprt.ATTENTION_HEAD, hiprt.ATTENTION_TAIL, fields, make, lambda args: hiprt.attention_work(args, grad))
+    _run(func, hiprt.ATTENTION_HEAD, fields, plan, used + [x for x in arrays if x is not None], written)
 
 
 def attention(q, k, v, how, outs):
@@ -111,10 +143,7 @@ def attention(q, k, v, how, outs):
     places = _places(outs, shapes, _F32, [q, k, v] + masks)
     if len(places) > 1 and not places[1].is_contiguous:
         places[1] = ndarray(shapes[1], _F32)
-    o, lse = places[0], places[1] if len(places) > 1 else None
-    fields, ints, arrays = _attention_args(q, k, v, o, lse, None, (None, None, None), how)
-    probe = hiprt.ATTENTION.pack(*fields, 0, 0, *ints)
-    _run(hiprt.attention, hiprt.ATTENTION, fields, ints, hiprt.attention_work(probe, False), [q, k, v] + arrays, places)
+    _attention(hiprt.attention, False, q, k, v, places[0], places[1] if len(places) > 1 else None, None, (None, None, None), how, [q, k, v], places)
     return _give(outs, places)
 
 
@@ -129,9 +158,7 @@ def attention_grad(dout, q, k, v, o, lse, how, outs):
         for g in places[1:]:
             if how.lengths < k.shape[2]:
                 hip.assign(g[:, :, how.lengths:], 0.0)
-    fields, ints, arrays = _attention_args(q, k, v, o, lse, dout, grads, how)
-    probe = hiprt.ATTENTION.pack(*fields, 0, 0, *ints)
-    _run(hiprt.attention_grad, hiprt.ATTENTION, fields, ints, hiprt.attention_work(probe, True), used + arrays, places)
+    _attention(hiprt.attention_grad, True, q, k, v, o, lse, dout, grads, how, used, places)
     return _give(outs, places)
 
 
@@ -149,17 +176,21 @@ def _rotary(x, how, outs, sign, dy=None):
     places = _places(outs, shapes, rows.dtype, used, same=dy if grad else rows)
     if grad and not places[1].is_contiguous:
         places[1] = ndarray(shapes[1], rows.dtype)
-    none = (0, 0, 0)
     fields = (rows.ptr, places[0].ptr, _ptr(weight), dy.ptr if grad else 0, places[1].ptr if grad else 0, _ptr(positions), _ptr(frequencies))
-    ints = (*_strides(rows), *_strides(places[0]), *(_strides(dy) if grad else none),
-            weight._strides[0] if per_head else 0,
-            positions._strides[0] if positions is not None and len(positions.shape) == 2 else 0, how.first,
-            -2.0 * math.log2(how.base) / max(how.dims, 1), 1.0 / how.stretch, how.magnitude, sign, how.eps,
-            batch, heads, count, size, how.dims, (size + 3) // 4 * 4,
-            int(how.interleaved), int(rows.dtype.itemsize == 8),
-            int(positions is not None and positions.dtype.itemsize == 8))
-    work = hiprt.rotary_work(hiprt.ROTARY.pack(*fields, 0, 0, *ints)) if grad else 0
-    _run(hiprt.rotary, hiprt.ROTARY, fields, ints, work, used, places)
+    key = (grad, sign, rows.shape, rows._strides, places[0]._strides, _steps(dy), rows.dtype.itemsize, per_head and weight._strides,
+           None if positions is None else (positions.shape, positions._strides, positions.dtype.itemsize),
+           how.first, how.base, how.dims, how.stretch, how.magnitude, how.eps, how.interleaved)
+
+    def make():
+        return (*_strides(rows), *_strides(places[0]), *(_strides(dy) if grad else _NONE),
+                weight._strides[0] if per_head else 0,
+                positions._strides[0] if positions is not None and len(positions.shape) == 2 else 0, how.first,
+                -2.0 * math.log2(how.base) / max(how.dims, 1), 1.0 / how.stretch, how.magnitude, sign, how.eps,
+                batch, heads, count, size, how.dims, (size + 3) // 4 * 4,
+                int(how.interleaved), int(rows.dtype.itemsize == 8),
+                int(positions is not None and positions.dtype.itemsize == 8))
+    plan = _plan(key, hiprt.ROTARY_HEAD, hiprt.ROTARY_TAIL, fields, make, hiprt.rotary_work)
+    _run(hiprt.rotary, hiprt.ROTARY_HEAD, fields, plan, used, places)
     return _give(outs, places)
 
 
@@ -181,7 +212,7 @@ def sample(logits, uniforms, temperature, top_k, top_p, min_p, outs):
     used = [x for x in (logits, uniforms, t, k, p, m) if x is not None]
     places = _places(outs, [(batch,)], numpy.dtype(numpy.int64), used)
     one = 2.0 ** min(52, 62 - max(1, (vocabulary - 1).bit_length()))      # (float64 holds it)
-    args = hiprt.SAMPLE.pack(logits.ptr, uniforms.ptr, places[0].ptr, _ptr(t), _ptr(p), _ptr(m), _ptr(k), logits._strides[0],
-                             t_all, p_all, m_all, one, min(k_all, vocabulary), batch, vocabulary, int(uniforms.dtype.itemsize == 8))
+    args = hiprt.SAMPLE_HEAD.pack(logits.ptr, uniforms.ptr, places[0].ptr, _ptr(t), _ptr(p), _ptr(m), _ptr(k)) \
+        + hiprt.SAMPLE_TAIL.pack(logits._strides[0], t_all, p_all, m_all, one, min(k_all, vocabulary), batch, vocabulary, int(uniforms.dtype.itemsize == 8))
     hip.issue_operator(hiprt.sample, args, used + places, places)
     return _give(outs, places)

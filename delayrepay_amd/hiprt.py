@@ -226,6 +226,10 @@ def cumsum(kind, src, dst, n):
 ATTENTION = struct.Struct("@15PQ25q10i2f")
 ROTARY = struct.Struct("@8PQ12q5d9i")
 SAMPLE = struct.Struct("@7Pq4d4i")
+# the same in two pieces: addresses, and what depends on geometry and options alone
+ATTENTION_HEAD, ATTENTION_TAIL = struct.Struct("@15PQ"), struct.Struct("@25q10i2f")
+ROTARY_HEAD, ROTARY_TAIL = struct.Struct("@8PQ"), struct.Struct("@12q5d9i")
+SAMPLE_HEAD, SAMPLE_TAIL = struct.Struct("@7P"), struct.Struct("@q4d4i")
 
 
 def attention_work(args, grad):

@@ -33,6 +33,8 @@ MAX_ROTARY_HEAD = 512
 # ---- arguments -------------------------------------------------------------------------------
 
 def _array(x, name):
+    if type(x) is NPArray:          # (the common kinds first, here and below: a short call is bound by its checks)
+        return x.array
     if isinstance(x, DelayArray):
         return x._force()
     if _backend.is_ndarray(x):
@@ -61,6 +63,8 @@ def _integers(x, name, shape, number=True):
     """None, a whole number, or an int32 array of `shape` (int64 arrays are converted)."""
     if x is None:
         return None
+    if type(x) is NPArray and x.dtype == _INTS[0] and x.shape == shape:
+        return x.array
     if isinstance(x, (numbers.Integral, numpy.integer)) and not isinstance(x, (bool, numpy.bool_)):
         if not number:
             raise TypeError(f"{name} is an integer array")
@@ -73,6 +77,8 @@ def _integers(x, name, shape, number=True):
 
 
 def _number(x, name, low=-math.inf, above=False):
+    if type(x) is float and low < x < math.inf:
+        return x
     if isinstance(x, (bool, numpy.bool_)) or not isinstance(x, (numbers.Real, numpy.floating, numpy.integer)):
         raise TypeError(f"{name} is a number, not a {type(x).__name__}")
     x = float(x)
@@ -91,14 +97,17 @@ def _targets(out, shapes, dtypes):
         raise ValueError(f"out names {len(shapes)} array{'s' if len(shapes) > 1 else ''}, not {len(outs)}")
     arrays = []
     for i, (x, shape, dtype) in enumerate(zip(outs, shapes, dtypes)):
-        name = "out" if len(outs) == 1 else f"out[{i}]"
-        if isinstance(x, DelayArray):
+        name = "out" if len(outs) == 1 else "out[%d]" % i
+        if type(x) is NPArray:
+            arr = x.array
+        elif isinstance(x, DelayArray):
             arr = x._force()
         elif _backend.is_ndarray(x):
             arr = x
         else:
             raise TypeError(f"{name} is an array, not a {type(x).__name__}")
-        _shaped(arr, name, shape)
+        if arr.shape != shape:
+            _shaped(arr, name, shape)
         if arr.dtype != dtype:
             raise TypeError(f"{name} is {dtype}, not {arr.dtype}")
         check = getattr(arr, "check_writable", None)
@@ -217,7 +226,7 @@ class _Turn:
             raise ValueError(f"dims is an even number of a head's {size} elements, not {dims!r}")
         self.dims = int(self.dims)
         self.positions, self.first = None, 0
-        if isinstance(positions, (numbers.Integral, numpy.integer)) and not isinstance(positions, (bool, numpy.bool_)):
+        if type(positions) is not NPArray and isinstance(positions, (numbers.Integral, numpy.integer)) and not isinstance(positions, (bool, numpy.bool_)):
             self.first = int(positions)
             if abs(self.first) >= 1 << 52:
                 raise ValueError("positions lie below 2**52")
@@ -309,6 +318,8 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     def part(x, name, none, low, high, above):
         if x is None:
             return none
+        if type(x) is float and low < x <= high:
+            return x
         if isinstance(x, (numbers.Real, numpy.floating, numpy.integer)) and not isinstance(x, bool):
             x = float(x)
             if not low <= x <= high or (above and x == low):
