@@ -361,6 +361,7 @@ struct Pack {
     int heads, tiles, keys;         // tiles of 32 rows of one head
     char* planes;
     unsigned* marks;
+    int2* docs;                     // least and largest document of a tile
     float* delta;
 };
 struct Packs {
@@ -368,7 +369,7 @@ struct Packs {
 };
 
 // Matrices in planes, for every tile that counts; values that are not finite become zeros and their rows
-// are marked.  Bound by memory: 4 bytes read and 6 written for each number, once for all blocks that read the tile.
+// are marked; with documents, their range in the tile is noted.  Bound by memory: 4 bytes read and 6 written for each number, once for all blocks that read the tile.
 template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Args a, Packs packs, int wide) {
     __shared__ float lds[kTile][32 * NT + 1];
     __shared__ unsigned bad;
@@ -403,6 +404,18 @@ template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Arg
     __syncthreads();
     const int64_t place = (int64_t)head * job.tiles + tile;
     if (threadIdx.x == 0) job.marks[place] = bad;
+    if (job.docs && threadIdx.x < 64) {
+        const Seq s = sequence(a, b);
+        const int i = first + (threadIdx.x & 31), j = job.keys ? i : s.start + i;
+        const bool in = i < end && j >= 0 && j < s.len;
+        int lo = in ? s.docs[j] : 0x7fffffff, hi = in ? lo : -0x7fffffff - 1;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            lo = min(lo, __shfl_xor(lo, m));
+            hi = max(hi, __shfl_xor(hi, m));
+        }
+        if (threadIdx.x == 0) job.docs[place] = make_int2(lo, hi);
+    }
     char* to = job.planes + place * Planes<NT>::BYTES;
     for (int at = threadIdx.x; at < 32 * 4 * NT; at += kThreads) {
         Three x;
@@ -457,7 +470,29 @@ __device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) 
 struct Packed {
     const char *key, *value, *query, *grad;
     const unsigned *key_marks, *value_marks, *query_marks, *grad_marks;
+    const int2 *key_docs, *query_docs;
     float* delta;
+};
+
+// The next of `count` tiles from t on that may hold a document in [lo, hi], 64 tiles at a look
+struct Active {
+    const int2* ranges;
+    int count, lo, hi, group;
+    unsigned long long mask;
+    __device__ __forceinline__ int next(int t) {
+        while (t < count) {
+            if (t >> 6 != group) {
+                group = t >> 6;
+                const int mine = (group << 6) + (threadIdx.x & 63);
+                const int2 r = ranges[mine < count ? mine : 0];
+                mask = __ballot(mine < count && r.x <= hi && r.y >= lo);
+            }
+            const unsigned long long left = mask >> (t & 63);
+            if (left) return t + __builtin_ctzll(left);
+            t = (group + 1) << 6;
+        }
+        return count;
+    }
 };
 
 // ---- forward, many rows ---------------------------------------------------------------------
@@ -529,25 +564,22 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     top = __builtin_amdgcn_readfirstlane(top);
     low = __builtin_amdgcn_readfirstlane(low);
 
+    int docs_next = 0;
+    // the first key of the next tile that any row of the block may see
     const int key_tiles = (a.lk + kTile - 1) / kTile;
-    unsigned marks_next[2] = {0, 0};
     const int64_t place = (int64_t)head * key_tiles;
+    Active active{in.key_docs + place, (end + kTile - 1) / kTile, dlo, dhi, -1, 0};
+    auto next = [&](int j0) {
+        if (!s.docs) return j0;
+        return __builtin_amdgcn_readfirstlane(active.next(j0 / kTile)) * kTile;
+    };
+    unsigned marks_next[2] = {0, 0};
     auto copy = [&](int to, int j) {                  // (marks are read ahead of the copies: a wait for them would wait for these)
         marks_next[0] = in.key_marks[place + j / kTile];
         marks_next[1] = in.value_marks[place + j / kTile];
+        if (s.docs) docs_next = s.docs[min(j + (lane & 31), s.len - 1)];
         copy_to_lds<WAVES>(lds[to], in.key + (place + j / kTile) * P::BYTES, P::BYTES);
         copy_to_lds<WAVES>(lds[to] + P::BYTES, in.value + (place + j / kTile) * P::BYTES, P::BYTES);
-    };
-    int docs_next = 0;
-    // the first key of the next tile that any row of the block may see
-    auto next = [&](int j0) {
-        if (s.docs)
-            for (; j0 < end; j0 += kTile) {
-                const int j = j0 + (lane & 31);
-                docs_next = j < end ? s.docs[j] : 0;
-                if (__any(j < end && docs_next >= dlo && docs_next <= dhi)) break;
-            }
-        return j0;
     };
 
     f32x16 acc[NT];
@@ -1020,24 +1052,22 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
     low = __builtin_amdgcn_readfirstlane(low);
 
     int docs_next = 0;
+    const int key_tiles = (a.lk + kTile - 1) / kTile;
+    const int64_t place = (int64_t)head * key_tiles;
+    Active active{in.key_docs + place, (end + kTile - 1) / kTile, dlo, dhi, -1, 0};
     auto next = [&](int j0) {
-        if (s.docs)
-            for (; j0 < end; j0 += kTile) {
-                const int j = j0 + (lane & 31);
-                docs_next = j < end ? s.docs[j] : 0;
-                if (__any(j < end && docs_next >= dlo && docs_next <= dhi)) break;
-            }
-        return j0;
+        if (!s.docs) return j0;
+        return __builtin_amdgcn_readfirstlane(active.next(j0 / kTile)) * kTile;
     };
     unsigned marks_next[2] = {0, 0};
-    const int64_t place = (int64_t)head * ((a.lk + kTile - 1) / kTile);
-    auto copy = [&](int to, int j) {
-        const int64_t n = place + j / kTile;
-        marks_next[0] = in.key_marks[n];
-        marks_next[1] = in.value_marks[n];
-        copy_to_lds<4>(lds[to], in.key + n * P::BYTES, P::BYTES);
-        copy_to_lds<4>(lds[to] + P::BYTES, in.value + n * P::BYTES, P::BYTES);
+    auto copy = [&](int to, int j) {                  // (marks are read ahead of the copies: a wait for them would wait for these)
+        marks_next[0] = in.key_marks[place + j / kTile];
+        marks_next[1] = in.value_marks[place + j / kTile];
+        if (s.docs) docs_next = s.docs[min(j + (lane & 31), s.len - 1)];
+        copy_to_lds<4>(lds[to], in.key + (place + j / kTile) * P::BYTES, P::BYTES);
+        copy_to_lds<4>(lds[to] + P::BYTES, in.value + (place + j / kTile) * P::BYTES, P::BYTES);
     };
+
     f32x16 acc[NT];
 #pragma unroll
     for (int c = 0; c < NT; ++c)
@@ -1164,18 +1194,14 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     if (key0 >= s.len) first = a.lq;
     const int g0 = parts > 1 ? slice : 0, g1 = parts > 1 ? slice + 1 : group;
     int docs_next = 0;
+    const int row_tiles = (a.lq + kTile - 1) / kTile;
+    Active active{in.query_docs + (int64_t)b * a.hq * row_tiles, row_tiles, dlo, dhi, -1, 0};      // (the same for every head)
     auto next = [&](int& g, int& i0) {     // to a tile of rows that may see a key of the block
         for (; g < g1; ++g, i0 = first) {
-            for (; i0 < a.lq; i0 += kTile) {
-                if (!s.docs) return;
-                const int i = i0 + (lane & 31), p = s.start + i;
-                const bool there = i < a.lq && p >= 0 && p < s.len;
-                docs_next = there ? s.docs[p] : 0;
-                if (__any(there && docs_next >= dlo && docs_next <= dhi)) return;
-            }
+            if (s.docs) i0 = __builtin_amdgcn_readfirstlane(active.next(i0 / kTile)) * kTile;
+            if (i0 < a.lq) return;
         }
     };
-    const int row_tiles = (a.lq + kTile - 1) / kTile;
     auto place = [&](int g, int i0) { return ((int64_t)b * a.hq + kh * group + g) * row_tiles + i0 / kTile; };
     unsigned marks_next[2] = {0, 0};
     float lse_next = 0.f, delta_next = 0.f;
@@ -1183,6 +1209,10 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
         const int64_t n = place(g, i0);
         marks_next[0] = in.query_marks[n];
         marks_next[1] = in.grad_marks[n];
+        if (s.docs) {
+            const int i = i0 + (lane & 31), p = s.start + i;
+            docs_next = i < a.lq && p >= 0 && p < s.len ? s.docs[p] : 0;
+        }
         if (threadIdx.x < kTile) {
             const int i = i0 + threadIdx.x;
             const int64_t at = ((int64_t)b * a.hq + kh * group + g) * a.lq + i;
@@ -1381,6 +1411,7 @@ Room room_forward(const Args& a, const Plan& p) {
     if (!p.few) {
         r.packed.key_marks = next_room<unsigned>(at, tiles * 4);
         r.packed.value_marks = next_room<unsigned>(at, tiles * 4);
+        r.packed.key_docs = next_room<int2>(at, a.documents ? tiles * 8 : 0);
         r.packed.key = next_room<char>(at, planes);
         r.packed.value = next_room<char>(at, planes);
     }
@@ -1402,6 +1433,8 @@ Room room_grad(const Args& a, int parts) {
     r.packed.value_marks = next_room<unsigned>(at, keys * 4);
     r.packed.query_marks = next_room<unsigned>(at, queries * 4);
     r.packed.grad_marks = next_room<unsigned>(at, queries * 4);
+    r.packed.key_docs = next_room<int2>(at, a.documents ? keys * 8 : 0);
+    r.packed.query_docs = next_room<int2>(at, a.documents ? queries * 8 : 0);
     r.packed.key = next_room<char>(at, keys * 6144 * nt);
     r.packed.value = next_room<char>(at, keys * 6144 * nt);
     r.packed.query = next_room<char>(at, queries * 6144 * nt);
@@ -1417,19 +1450,19 @@ Packed packed_at(const Room& room, char* work) {
     Packed p = room.packed;
     auto move = [&](auto*& x) { x = (std::remove_reference_t<decltype(x)>)(work + (uint64_t)x); };
     move(p.key), move(p.value), move(p.query), move(p.grad);
-    move(p.key_marks), move(p.value_marks), move(p.query_marks), move(p.grad_marks), move(p.delta);
+    move(p.key_marks), move(p.value_marks), move(p.query_marks), move(p.grad_marks), move(p.key_docs), move(p.query_docs), move(p.delta);
     return p;
 }
 
-Pack pack_of(const float* x, const int64_t* stride, int heads, int rows, int keys, const char* planes, const unsigned* marks, float* delta = nullptr) {
-    return Pack{x, {stride[0], stride[1], stride[2]}, heads, (rows + kTile - 1) / kTile, keys, (char*)planes, (unsigned*)marks, delta};
+Pack pack_of(const float* x, const int64_t* stride, int heads, int rows, int keys, const char* planes, const unsigned* marks, const int2* docs = nullptr, float* delta = nullptr) {
+    return Pack{x, {stride[0], stride[1], stride[2]}, heads, (rows + kTile - 1) / kTile, keys, (char*)planes, (unsigned*)marks, (int2*)docs, delta};
 }
 
 template <int NT> void launch_rows(const Args& a, const Plan& p, const Packed& in, float* part, float* part_lse, hipStream_t s) {
     const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
     const int key_tiles = (a.lk + kTile - 1) / kTile, tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
     Packs packs{};
-    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key, in.key_marks);
+    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key, in.key_marks, a.documents ? in.key_docs : nullptr);
     packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, in.value, in.value_marks);
     if (key_tiles) attention_pack<NT><<<dim3((unsigned)(2 * heads * key_tiles)), kThreads, 0, s>>>(a, packs, p.wide);
     const dim3 grid((unsigned)(heads * tiles * p.splits));
@@ -1452,10 +1485,10 @@ template <int NT> void launch_grad(const Args& a, const Plan& p, int parts, cons
     const int64_t heads = (int64_t)a.batch * a.hkv;
     const int key_tiles = (a.lk + kTile - 1) / kTile, query_tiles = (a.lq + kTile - 1) / kTile, tiles = row_tiles(a);
     Packs packs{};
-    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key, in.key_marks);
+    packs.job[0] = pack_of(a.k, a.k_stride, a.hkv, a.lk, 1, in.key, in.key_marks, a.documents ? in.key_docs : nullptr);
     packs.job[1] = pack_of(a.v, a.v_stride, a.hkv, a.lk, 1, in.value, in.value_marks);
-    packs.job[2] = pack_of(a.q, a.q_stride, a.hq, a.lq, 0, in.query, in.query_marks);
-    packs.job[3] = pack_of(a.dout, a.dout_stride, a.hq, a.lq, 0, in.grad, in.grad_marks, in.delta);
+    packs.job[2] = pack_of(a.q, a.q_stride, a.hq, a.lq, 0, in.query, in.query_marks, a.documents ? in.query_docs : nullptr);
+    packs.job[3] = pack_of(a.dout, a.dout_stride, a.hq, a.lq, 0, in.grad, in.grad_marks, nullptr, in.delta);
     const int64_t blocks = 2 * heads * key_tiles + 2 * (int64_t)a.batch * a.hq * query_tiles;
     attention_pack<NT><<<dim3((unsigned)blocks), kThreads, 0, s>>>(a, packs, p.wide);
     const dim3 rows_grid((unsigned)(heads * tiles)), keys_grid((unsigned)(heads * parts * ((a.lk + kRows - 1) / kRows)));
