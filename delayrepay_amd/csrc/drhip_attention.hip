@@ -112,6 +112,11 @@ __device__ __forceinline__ float score(const Args& a, float x, float slope2, int
 }
 
 
+// How the rows of a key head's gradient are spread over blocks: `count` parts, (query heads) x `ranges` of `span` rows
+struct Parts {
+    int count, ranges, span;
+};
+
 struct Plan {
     int few;             // the kernel for few rows
     int waves;           // of a block of the other one
@@ -1129,9 +1134,10 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
     if (valid) store_column<NT>(a.dq + b * a.dq_stride[0] + qh * a.dq_stride[1] + i * a.dq_stride[2], acc, a.scale, a.d, wide, h);
 }
 
-// `parts` > 1: the query heads of a key head go to different blocks, whose sums are added by `attention_add`.
+// More than one part: the query heads of a key head, and ranges of `span` rows of them, go to different blocks,
+// whose sums are added by `attention_add`.
 template <int NT, bool CAP>
-__global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, int parts, Packed in, float* part) {
+__global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, Parts parts, Packed in, float* part) {
     using P = Planes<NT>;
     __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
     __shared__ __attribute__((aligned(16))) float stat[2][2][kTile];
@@ -1142,7 +1148,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     int id = blockIdx.x;
     const int head = id % heads;
     id /= heads;
-    const int slice = id % parts, tile = id / parts;       // (causal: the first keys are seen by the most rows)
+    const int slice = id % parts.count, tile = id / parts.count;       // (causal: the first keys are seen by the most rows)
     const int b = head / a.hkv, kh = head % a.hkv;
     const Seq s = sequence(a, b);
     const bool wide = plan.wide;
@@ -1192,14 +1198,16 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     int first = 0;
     if (a.causal && key0 >= s.prefix) first = clamp_(key0 - s.start, 0, a.lq) & ~(kTile - 1);
     if (key0 >= s.len) first = a.lq;
-    const int g0 = parts > 1 ? slice : 0, g1 = parts > 1 ? slice + 1 : group;
+    const int g0 = parts.count > 1 ? slice / parts.ranges : 0, g1 = parts.count > 1 ? g0 + 1 : group;
+    const int rows_end = min(a.lq, (slice % parts.ranges + 1) * parts.span);
+    first = max(first, slice % parts.ranges * parts.span);
     int docs_next = 0;
     const int row_tiles = (a.lq + kTile - 1) / kTile;
-    Active active{in.query_docs + (int64_t)b * a.hq * row_tiles, row_tiles, dlo, dhi, -1, 0};      // (the same for every head)
+    Active active{in.query_docs + (int64_t)b * a.hq * row_tiles, (rows_end + kTile - 1) / kTile, dlo, dhi, -1, 0};      // (the same for every head)
     auto next = [&](int& g, int& i0) {     // to a tile of rows that may see a key of the block
         for (; g < g1; ++g, i0 = first) {
             if (s.docs) i0 = __builtin_amdgcn_readfirstlane(active.next(i0 / kTile)) * kTile;
-            if (i0 < a.lq) return;
+            if (i0 < rows_end) return;
         }
     };
     auto place = [&](int g, int i0) { return ((int64_t)b * a.hq + kh * group + g) * row_tiles + i0 / kTile; };
@@ -1360,7 +1368,8 @@ int row_tiles(const Args& a) { return (int)(((int64_t)(a.hq / a.hkv) * a.lq + kR
 // Which forward kernel, and into how many key ranges.  Few rows: up to 32 rows of a key head, where the
 // blocks of the other kernel would be mostly empty.  Blocks of eight waves share each tile among 256 rows, of
 // four where that leaves compute units without a block.  Ranges: enough for a block on each compute unit (two,
-// as causal blocks are of unequal length), none shorter than 256 keys, whose work pays for joining.  For few rows,
+// as causal blocks are of unequal length; not with documents, whose rows see a part of the keys alone: 60 us
+// against 85 for three sequences of 1111), none shorter than 256 keys, whose work pays for joining.  For few rows,
 // two blocks for each compute unit with ranges of 128 keys or more, and up to eight, since sequences are of
 // unequal length, as long as ranges have 512.
 Plan plan_forward(const Args& a) {
@@ -1377,7 +1386,7 @@ Plan plan_forward(const Args& a) {
         if (splits < fine) splits = fine < long_ranges ? fine : long_ranges > splits ? long_ranges : splits;
         if (splits > most) splits = most;
     } else {
-        const int64_t want = a.causal ? 512 : 256, most = (a.lk + 255) / 256;
+        const int64_t want = a.causal && !a.documents ? 512 : 256, most = (a.lk + 255) / 256;
         splits = blocks >= want ? 1 : (want + blocks - 1) / blocks;
         if (splits > most) splits = most;
     }
@@ -1423,7 +1432,7 @@ Room room_forward(const Args& a, const Plan& p) {
     return r;
 }
 
-Room room_grad(const Args& a, int parts) {
+Room room_grad(const Args& a, const Parts& parts) {
     const uint64_t rows = (uint64_t)a.batch * a.hq * a.lq, nt = (a.d + 31) / 32;
     const uint64_t keys = (uint64_t)a.batch * a.hkv * ((a.lk + kTile - 1) / kTile), queries = (uint64_t)a.batch * a.hq * ((a.lq + kTile - 1) / kTile);
     Room r{};
@@ -1440,7 +1449,7 @@ Room room_grad(const Args& a, int parts) {
     r.packed.query = next_room<char>(at, queries * 6144 * nt);
     r.packed.grad = next_room<char>(at, queries * 6144 * nt);
     r.part = at;
-    if (parts > 1) next_room<float>(at, (uint64_t)parts * 2 * a.batch * a.hkv * a.lk * a.d * 4);
+    if (parts.count > 1) next_room<float>(at, (uint64_t)parts.count * 2 * a.batch * a.hkv * a.lk * a.d * 4);
     r.all = at;
     return r;
 }
@@ -1481,7 +1490,7 @@ template <bool WIDE> void launch_few(const Args& a, const Plan& p, float* part, 
         two ? attention_few<2, 2, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<2, 1, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
 }
 
-template <int NT> void launch_grad(const Args& a, const Plan& p, int parts, const Packed& in, float* part, hipStream_t s) {
+template <int NT> void launch_grad(const Args& a, const Plan& p, const Parts& parts, const Packed& in, float* part, hipStream_t s) {
     const int64_t heads = (int64_t)a.batch * a.hkv;
     const int key_tiles = (a.lk + kTile - 1) / kTile, query_tiles = (a.lq + kTile - 1) / kTile, tiles = row_tiles(a);
     Packs packs{};
@@ -1491,7 +1500,7 @@ template <int NT> void launch_grad(const Args& a, const Plan& p, int parts, cons
     packs.job[3] = pack_of(a.dout, a.dout_stride, a.hq, a.lq, 0, in.grad, in.grad_marks, nullptr, in.delta);
     const int64_t blocks = 2 * heads * key_tiles + 2 * (int64_t)a.batch * a.hq * query_tiles;
     attention_pack<NT><<<dim3((unsigned)blocks), kThreads, 0, s>>>(a, packs, p.wide);
-    const dim3 rows_grid((unsigned)(heads * tiles)), keys_grid((unsigned)(heads * parts * ((a.lk + kRows - 1) / kRows)));
+    const dim3 rows_grid((unsigned)(heads * tiles)), keys_grid((unsigned)(heads * parts.count * ((a.lk + kRows - 1) / kRows)));
     if (a.lq) {
         if (a.cap > 0.f)
             attention_dq<NT, true><<<rows_grid, kThreads, 0, s>>>(a, p, tiles, in);
@@ -1504,13 +1513,25 @@ template <int NT> void launch_grad(const Args& a, const Plan& p, int parts, cons
         else
             attention_dkv<NT, false><<<keys_grid, kThreads, 0, s>>>(a, p, parts, in, part);
     }
-    if (a.lk && parts > 1) attention_add<<<dim3((unsigned)((2 * heads * a.lk + 3) / 4)), kThreads, 0, s>>>(a, parts, part);
+    if (a.lk && parts.count > 1) attention_add<<<dim3((unsigned)((2 * heads * a.lk + 3) / 4)), kThreads, 0, s>>>(a, parts.count, part);
 }
 
-// Query heads of a key head in blocks of their own: only where the keys alone give too few blocks
-int plan_parts(const Args& a) {
+// Query heads of a key head go to blocks of their own where the keys alone give fewer than two blocks to a
+// compute unit, and ranges of rows as well where that leaves some without one
+Parts plan_parts(const Args& a) {
     const int64_t blocks = (int64_t)a.batch * a.hkv * ((a.lk + kRows - 1) / kRows);
-    return a.hq > a.hkv && blocks < 512 ? a.hq / a.hkv : 1;
+    const int group = a.hq / a.hkv;
+    Parts p{1, 1, a.lq > 0 ? (a.lq + kTile - 1) / kTile * kTile : kTile};
+    if (blocks >= 512 || blocks == 0) return p;
+    int64_t ranges = 256 / (blocks * group);
+    if (ranges > a.lq / kRows) ranges = a.lq / kRows;
+    if (ranges < 1) ranges = 1;
+    p.span = (int)(((a.lq + ranges - 1) / ranges + kTile - 1) / kTile * kTile);
+    if (p.span < kTile) p.span = kTile;
+    p.ranges = (int)(((int64_t)a.lq + p.span - 1) / p.span);
+    if (p.ranges < 1) p.ranges = 1;
+    p.count = group * p.ranges;
+    return p;
 }
 
 }  // namespace
@@ -1549,11 +1570,11 @@ extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
 
 extern "C" int drhip_k_attention_grad(const drhip_attention_t* args, hipStream_t s) {
     const Args& a = *args;
-    const int parts = plan_parts(a);
+    const Parts parts = plan_parts(a);
     const Room room = room_grad(a, parts);
     char* work = (char*)a.work;
     const Packed in = packed_at(room, work);
-    float* part = parts > 1 ? (float*)(work + room.part) : nullptr;
+    float* part = parts.count > 1 ? (float*)(work + room.part) : nullptr;
     Plan p{};
     p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride) &&
              aligned(a.dout, a.dout_stride) && aligned(a.dq, a.dq_stride) && aligned(a.dk, a.dk_stride) && aligned(a.dv, a.dv_stride);
