@@ -1386,7 +1386,7 @@ Plan plan_forward(const Args& a) {
         if (splits < fine) splits = fine < long_ranges ? fine : long_ranges > splits ? long_ranges : splits;
         if (splits > most) splits = most;
     } else {
-        const int64_t want = a.causal && !a.documents ? 512 : 256, most = (a.lk + 255) / 256;
+        const int64_t want = a.documents ? 64 : a.causal ? 512 : 256, most = (a.lk + 255) / 256;
         splits = blocks >= want ? 1 : (want + blocks - 1) / blocks;
         if (splits > most) splits = most;
     }

@@ -584,18 +584,20 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         for (int i = threadIdx.x; i < kCoarse; i += kDraw) counts[i] = 0;
     if (threadIdx.x == 0) listed = 0, chunk_at = 0, chunk_before = 0, chunk_tied = 0, cut_rank = 0, found = {0, 0, 0};
     __syncthreads();
-    u64 best = 0;
+    float most = -__builtin_inff();
+    int where = 0;
+    auto larger = [&](int i, float x) {
+        where = x > most ? i : where;
+        most = x > most ? x : most;
+    };
     if (counted)
         each_token(row, v, [&](int i, float x) {
-            const u64 r = rank_of(x, i);
-            best = r > best ? r : best;
-            atomicAdd(&counts[r >> 51], 1u);
+            larger(i, x);
+            atomicAdd(&counts[key_of(x) >> 19], 1u);
         });
     else
-        each_token(row, v, [&](int i, float x) {
-            const u64 r = rank_of(x, i);
-            best = r > best ? r : best;
-        });
+        each_token(row, v, larger);
+    u64 best = rank_of(most, where);
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
         const u64 y = __shfl_xor(best, m);
