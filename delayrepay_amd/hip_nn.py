@@ -121,7 +121,7 @@ def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
     fields = (q.ptr, k.ptr, v.ptr, o.ptr, _ptr(lse), _ptr(dout), *[_ptr(g) for g in grads], *[_ptr(x) for x in arrays])
     key = (func, q.shape, q._strides, k.shape, k._strides, v._strides, o._strides, _steps(dout),
            *[_steps(g) for g in grads], _steps(documents), how.causal,
-           start if isinstance(start, int) else start is None, prefix if isinstance(prefix, int) else None, how.scale, how.cap)
+           start if isinstance(start, int) else "last" if start is None else "array", prefix if isinstance(prefix, int) else None, how.scale, how.cap)
 
     def make():
         lk, far = k.shape[2], (1 << 31) - 1

@@ -192,6 +192,14 @@ def test_strides_and_alignment(lq):
         assert np.all(x.get()[..., :1] == 7) and np.all(x.get()[..., 49:] == 7)
 
 
+def test_options_that_follow_each_other():
+    """What is remembered of a call's geometry is told apart by every option of it."""
+    q, k, v, g = _normal(21, (2, 2, 5, 16), (2, 2, 9, 16), (2, 2, 9, 16), (2, 2, 5, 16))
+    for how in (dict(), dict(start=1), dict(start=0), dict(start=np.array([1, 3], np.int32)), dict(prefix=1), dict(prefix=0), dict(prefix=np.array([7, 6], np.int32)),
+                dict(cap=1.0), dict(scale=1.0), dict(start=1), dict()):
+        _check(q, k, v, g, causal=True, **how)
+
+
 def test_results_over_operands():
     q, k, v = _normal(10, (2, 4, 150, 32), (2, 4, 150, 32), (2, 4, 150, 32))
     want = nn_oracle.attention(q, k, v, causal=True)
