@@ -571,7 +571,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     const int v = p.vocabulary;
     const double temperature = p.temperature ? p.temperature[b] : p.temperature_all;
     const int64_t k = p.top_k ? p.top_k[b] : p.top_k_all;
-    const double top_p = p.top_p ? p.top_p[b] : p.top_p_all;
+    const double top_p = fmax(p.top_p ? p.top_p[b] : p.top_p_all, 0.0);      // (conversions of negative numbers below have no defined result)
     const bool counted = k > 0 && k < v && temperature > 0.0, cut_p = top_p < 1.0;
     double min_p = p.min_p ? p.min_p[b] : p.min_p_all;
     if (!(min_p > 0.0)) min_p = 0.0;
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         if (threadIdx.x == 0) p.tokens[b] = none ? -1 : (int64_t)(int)~(unsigned)best;
         return;
     }
-    const Weigher weigh{value_of(top_key), 1.4426950408889634074 / temperature, p.one};
+    const Weigher weigh{value_of(top_key), fmin(1.4426950408889634074 / temperature, 1e300), p.one};      // (finite: the largest is 0 apart from itself)
 
     // end of what is kept: ranks of at least `cut`; where that is not known, keys above `cut_key`, and the first
     // `ties` tokens whose key it is

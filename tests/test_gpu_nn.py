@@ -397,6 +397,21 @@ def test_sample_with_parameters_for_each_row():
     assert nn.sample(dr.array(np.zeros((0, 5), f)), dr.array(np.zeros(0))).shape == (0,)
 
 
+@pytest.mark.parametrize("vocabulary", [40, 5000])
+def test_sample_with_parameters_at_their_ends(vocabulary):
+    """Out of range in an array: the nearest in it.  The smallest temperatures leave the largest logits."""
+    rs = np.random.RandomState(3)
+    logits = np.round(rs.standard_normal((6, vocabulary)) * 2).astype(np.float32)
+    u = rs.rand(6)
+    f = np.float32
+    _draws(logits, u, top_p=np.array([0.0, -0.5, -1e30, -2.0, 1.5, INF], f))
+    _draws(logits, u, top_p=np.array([0.0, -0.5, -1e30, -2.0, 1.5, INF], f), top_k=30)
+    _draws(logits, u, top_p=np.array([0.0, -0.5, -1e30, -2.0, 1.5, INF], f), top_k=min(vocabulary - 1, 3000), temperature=1e30)      # (nearly equal weights)
+    for temperature in (5e-324, 1e-300, 1e-45, np.full(6, 1e-45, f), np.full(6, np.finfo(f).max)):
+        _draws(logits, u, temperature=temperature)
+        _draws(logits, u, temperature=temperature, top_k=5, top_p=0.5, min_p=0.9)
+
+
 def test_sample_from_the_device_generator():
     """The generator's lazy numbers are evaluated for the call; frequencies follow the weights: of 20000 draws
     each share is within five standard deviations."""
