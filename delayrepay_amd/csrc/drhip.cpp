@@ -391,7 +391,7 @@ static const char* rotary_fault(const drhip_rotary_t* p) {
 int drhip_rotary_work(const drhip_rotary_t* p, uint64_t* bytes) {
     if (!p || !bytes) return fail(DRHIP_EINVAL, "drhip_rotary_work", "null argument");
     if (const char* why = rotary_fault(p)) return fail(DRHIP_EINVAL, "drhip_rotary_work", why);
-    *bytes = p->heads ? drhip_k_rotary_work(p) : 0;
+    *bytes = drhip_k_rotary_work(p);
     return 0;
 }
 
@@ -399,11 +399,12 @@ int drhip_rotary(const drhip_rotary_t* p) {
     NEED_INIT();
     if (!p) return fail(DRHIP_EINVAL, "drhip_rotary", "null argument");
     if (const char* why = rotary_fault(p)) return fail(DRHIP_EINVAL, "drhip_rotary", why);
-    if (!p->heads || (!p->dweight && (!p->batch || !p->rows))) return 0;
-    if ((int64_t)p->batch * p->rows && (!p->x || !p->y || (p->dweight && !p->dy))) return fail(DRHIP_EINVAL, "drhip_rotary", "null operand");
+    if (!p->dweight && (!p->heads || !p->batch || !p->rows)) return 0;
+    if ((int64_t)p->batch * p->rows * p->heads && (!p->x || !p->y || (p->dweight && !p->dy))) return fail(DRHIP_EINVAL, "drhip_rotary", "null operand");
     if (p->dweight) {
         if (!p->weight) return fail(DRHIP_EINVAL, "drhip_rotary", "null operand");
-        if (!p->work || p->work_bytes < drhip_k_rotary_work(p)) return fail(DRHIP_EINVAL, "drhip_rotary", "workspace too small");
+        const uint64_t need = drhip_k_rotary_work(p);
+        if (need && (!p->work || p->work_bytes < need)) return fail(DRHIP_EINVAL, "drhip_rotary", "workspace too small");
     }
     if (int rc = drhip_k_rotary(p, g_stream)) return fail(rc, "drhip_rotary", hipGetErrorString((hipError_t)rc));
     g_cnt.n_launches++;

@@ -343,7 +343,7 @@ bool wide_of(const Rot& p) {
 // Blocks for each pair of heads in the gradient: up to 2048 in all (8 for a compute unit), and two tokens
 // for each group, so that the parts of dw, a row for each block and head, stay below a thirtieth of dx
 int grad_slots(const Rot& p) {
-    const int64_t sets = (p.heads + kHeads - 1) / kHeads, groups = kThreads >> lanes_log_of(p);
+    const int64_t sets = p.heads ? (p.heads + kHeads - 1) / kHeads : 1, groups = kThreads >> lanes_log_of(p);
     const int64_t runs = ((int64_t)p.batch * p.rows + groups - 1) / groups;
     int64_t slots = 2048 / sets;
     if (slots > (runs + 1) / 2) slots = (runs + 1) / 2;
@@ -368,12 +368,13 @@ template <typename T> void launch_rotary_grad(const Rot& p, hipStream_t s) {
     const int log = lanes_log_of(p), slots = grad_slots(p);
     const unsigned blocks = (unsigned)(((p.heads + kHeads - 1) / kHeads) * slots);
     const unsigned lds = 16 * kThreads * sizeof(T);
-    if (wide_of(p))
+    if (!blocks) {      // no heads: a weight for all of them has a gradient of zeros
+    } else if (wide_of(p))
         rotary_grad_kernel<T, true><<<blocks, kThreads, lds, s>>>(p, log, slots);
     else
         rotary_grad_kernel<T, false><<<blocks, kThreads, lds, s>>>(p, log, slots);
     const unsigned parts = (unsigned)((p.d + 63) / 64 * (p.weight_stride ? p.heads : 1));
-    rotary_dw<T><<<parts, kThreads, 0, s>>>(p, slots);
+    if (parts) rotary_dw<T><<<parts, kThreads, 0, s>>>(p, slots);
 }
 
 // ---- drawing tokens ---------------------------------------------------------------------------

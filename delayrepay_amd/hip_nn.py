@@ -167,6 +167,8 @@ def _rotary(x, how, outs, sign, dy=None):
     batch, heads, count, size = rows.shape
     weight = None if how.weight is None else _dense(how.weight)
     per_head = weight is not None and len(weight.shape) == 2
+    if per_head and heads > 1 and weight._strides[0] == 0:       # (a pitch of 0 is the sign of one weight for all)
+        weight = weight.copy()
     positions = None if how.positions is None else _dense(how.positions)
     frequencies = None if how.frequencies is None else _contiguous(how.frequencies)
     used = [a for a in (x, dy, weight, positions, frequencies) if a is not None]

@@ -336,6 +336,23 @@ def test_rotary_in_place_views_and_empty():
     assert dx.shape == (2, 3, 0, 8) and not dw.get().any()
 
 
+def test_rotary_weights_of_no_heads_and_of_equal_heads():
+    """No heads: a gradient of zeros, written over what stood there.  One row of weights broadcast to the heads: a gradient for each."""
+    ones = dr.array(np.ones(8, np.float32))
+    dw = dr.array(np.full(8, 7, np.float32))
+    empty = dr.array(np.zeros((2, 0, 3, 8), np.float32))
+    nn.rotary_grad(empty, empty, 0, weight=ones, out=(dr.array(np.zeros((2, 0, 3, 8), np.float32)), dw))
+    assert not dw.get().any()
+    assert nn.rotary_grad(empty, empty, 0, weight=dr.array(np.zeros((0, 8), np.float32)))[1].shape == (0, 8)
+    x, g, w = _normal(22, (2, 5, 6, 64), (2, 5, 6, 64), (64,))
+    dev = [dr.array(a) for a in (g, x)]
+    same = dr.broadcast_to(dr.array(w)[None], (5, 64))
+    each = dr.array(np.tile(w, (5, 1)))
+    for a, b in zip(nn.rotary_grad(*dev, 3, weight=same), nn.rotary_grad(*dev, 3, weight=each)):
+        assert a.shape == b.shape and a.get().tobytes() == b.get().tobytes()
+    assert nn.rotary(dev[1], 3, weight=same).get().tobytes() == nn.rotary(dev[1], 3, weight=each).get().tobytes()
+
+
 # ---- tokens ----------------------------------------------------------------------------------
 
 def _draws(logits, u, **how):
