@@ -335,9 +335,12 @@ static const char* attention_fault(const drhip_attention_t* a, int grad) {
     if (a->d < 1 || a->d > 128) return "head size outside 1..128";
     if (a->lq >= 1 << 28 || a->lk >= 1 << 28) return "more than 2^28 rows";
     const int64_t heads = (int64_t)a->batch * a->hq;
-    if (heads >= kMostBlocks || heads * (a->lq / 32 + 1) >= kMostBlocks || heads * (a->lk / 32 + 1) >= kMostBlocks)
+    // (one launch packs keys and values, in the gradient q and dout as well)
+    const int64_t most = grad ? kMostBlocks / 2 : kMostBlocks;
+    if (heads >= most || heads * (a->lq / 32 + 1) >= most || heads * (a->lk / 32 + 1) >= most)
         return "more blocks than one launch holds";
     if (a->prefix_value < 0) return "negative prefix";
+    if (!(a->scale >= -0x1p100f && a->scale <= 0x1p100f) || !(a->cap <= 0.f || (a->cap >= 0x1p-100f && a->cap <= 0x1p100f))) return "scale or cap outside 2^100";
     if (heads && a->lq && (!a->q || !a->o || (a->lk && (!a->k || !a->v)))) return "null operand";
     if (grad && heads && ((a->lq && (!a->dout || !a->dq || !a->lse)) || (a->lk && (!a->k || !a->v || !a->dk || !a->dv)))) return "null operand";
     return nullptr;

@@ -124,12 +124,12 @@ def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
            start if isinstance(start, int) else "last" if start is None else "array", prefix if isinstance(prefix, int) else None, how.scale, how.cap)
 
     def make():
-        lk, far = k.shape[2], (1 << 31) - 1
+        lk = k.shape[2]
         return (*_strides(q), *_strides(k), *_strides(v), *_strides(o),
                 *(_NONE if dout is None else _strides(dout)), *[s for g in grads for s in (_NONE if g is None else _strides(g))],
                 0 if documents is None else documents._strides[0],
                 q.shape[0], q.shape[1], k.shape[1], q.shape[2], lk, q.shape[3], int(how.causal),
-                0 if start is None else 1, max(-far, min(far, start)) if isinstance(start, int) else 0,
+                0 if start is None else 1, start if isinstance(start, int) else 0,
                 min(prefix, lk) if isinstance(prefix, int) else 0,
                 how.scale, how.cap or 0.0)
     plan = _plan(key, hiprt.ATTENTION_HEAD, hiprt.ATTENTION_TAIL, fields, make, lambda args: hiprt.attention_work(args, grad))
@@ -167,7 +167,7 @@ def _rotary(x, how, outs, sign, dy=None):
     batch, heads, count, size = rows.shape
     weight = None if how.weight is None else _dense(how.weight)
     per_head = weight is not None and len(weight.shape) == 2
-    if per_head and heads > 1 and weight._strides[0] == 0:       # (a pitch of 0 is the sign of one weight for all)
+    if per_head and heads != 1 and weight._strides[0] == 0:       # (a pitch of 0 is the sign of one weight for all)
         weight = weight.copy()
     positions = None if how.positions is None else _dense(how.positions)
     frequencies = None if how.frequencies is None else _contiguous(how.frequencies)

@@ -28,6 +28,8 @@ _INTS = (numpy.dtype(numpy.int32), numpy.dtype(numpy.int64))
 
 MAX_HEAD = 128           # elements of an attention head
 MAX_ROTARY_HEAD = 512
+_FAR = 1 << 30            # positions of rows are nearer to 0
+_LARGE = 2.0 ** 100       # scales and caps are smaller, and caps larger than its inverse: their products fit float32
 
 
 # ---- arguments -------------------------------------------------------------------------------
@@ -137,10 +139,14 @@ class _Mask:
     def __init__(self, q, k, scale, causal, start, lengths, prefix, documents, slopes, cap):
         batch, lk = k.shape[0], k.shape[2]
         self.scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else _number(scale, "scale")
+        if abs(self.scale) > _LARGE:
+            raise ValueError(f"scale lies within 2**100 of 0, not at {self.scale:g}")
         if not isinstance(causal, (bool, numpy.bool_)):
             raise TypeError("causal is True or False")
         self.causal = bool(causal)
         self.start = _integers(start, "start", (batch,))
+        if isinstance(self.start, int) and abs(self.start) > _FAR:
+            raise ValueError(f"start lies within 2**30 of 0, not at {self.start}")
         self.lengths = _integers(lengths, "lengths", (batch,))
         if isinstance(self.lengths, int) and not 0 <= self.lengths <= lk:
             raise ValueError(f"lengths lies in [0, {lk}], the rows of k, not {self.lengths}")
@@ -152,6 +158,8 @@ class _Mask:
         self.documents = _integers(documents, "documents", (batch, lk), number=False)
         self.slopes = None if slopes is None else _shaped(_floats(slopes, "slopes", 1), "slopes", (q.shape[1],))
         self.cap = None if cap is None else _number(cap, "cap", 0.0, above=True)
+        if cap is not None and not 1 / _LARGE <= self.cap <= _LARGE:
+            raise ValueError(f"cap lies between 2**-100 and 2**100, not at {self.cap:g}")
 
 
 def _heads(q, k, v):

@@ -157,6 +157,10 @@ REFUSALS = """
     refused(ValueError, "slopes", A, q, k, k, slopes=f(2))
     refused(ValueError, "cap", A, q, k, k, cap=0.0)
     refused(ValueError, "cap", A, q, k, k, cap=float("inf"))
+    refused(ValueError, "cap lies", A, q, k, k, cap=1e-50)
+    refused(ValueError, "cap lies", A, q, k, k, cap=1e35)
+    refused(ValueError, "scale lies", A, q, k, k, scale=-1e39)
+    refused(ValueError, "start lies", A, q, k, k, start=1 << 31)
     refused(ValueError, "scale", A, q, k, k, scale=float("nan"))
     refused(TypeError, "causal", A, q, k, k, causal=1)
     refused(ValueError, "out", A, q, k, k, out=f(2, 4, 3, 9))
@@ -213,17 +217,19 @@ def test_the_library_refuses_what_its_launches_cannot_hold():
     import ctypes
     from delayrepay_amd import hiprt
 
-    def attention(batch=1, hq=2, hkv=1, lq=3, lk=3, d=8, prefix=0):
-        args = hiprt.ATTENTION.pack(*[0] * 15, 0, *[0] * 25, batch, hq, hkv, lq, lk, d, 0, 0, 0, prefix, 1.0, 0.0)
+    def attention(batch=1, hq=2, hkv=1, lq=3, lk=3, d=8, prefix=0, scale=1.0, cap=0.0, grad=1):
+        args = hiprt.ATTENTION.pack(*[0] * 15, 0, *[0] * 25, batch, hq, hkv, lq, lk, d, 0, 0, 0, prefix, scale, cap)
         n = ctypes.c_uint64()
-        return hiprt.lib().drhip_attention_work(args, 1, ctypes.byref(n))
+        return hiprt.lib().drhip_attention_work(args, grad, ctypes.byref(n))
 
     def rotary(batch=1, heads=2, rows=3, d=8, dims=8, pad=8):
         args = hiprt.ROTARY.pack(*[0] * 8, 0, *[0] * 12, 0.0, 1.0, 1.0, 1.0, 0.0, batch, heads, rows, d, dims, pad, 0, 0, 0)
         n = ctypes.c_uint64()
         return hiprt.lib().drhip_rotary_work(args, ctypes.byref(n))
     assert attention() == 0 and rotary() == 0
-    for bad in (dict(hq=3, hkv=2), dict(d=129), dict(d=0), dict(lq=-1), dict(lk=1 << 28), dict(batch=1 << 23), dict(batch=1 << 20, lq=1 << 20), dict(prefix=-1)):
+    for bad in (dict(hq=3, hkv=2), dict(d=129), dict(d=0), dict(lq=-1), dict(lk=1 << 28), dict(batch=1 << 23), dict(batch=1 << 20, lq=1 << 20), dict(prefix=-1), dict(batch=1 << 21),
+                dict(scale=1e38), dict(scale=float("nan")), dict(cap=1e-38), dict(cap=float("inf"))):
         assert attention(**bad) == 20002, bad
+    assert attention(batch=1 << 21, grad=0) == 0          # (fewer matrices to pack)
     for bad in (dict(d=513, pad=516), dict(dims=7), dict(dims=10), dict(pad=6), dict(rows=-1), dict(batch=1 << 20, rows=1 << 20)):
         assert rotary(**bad) == 20002, bad
