@@ -113,7 +113,7 @@ def _targets(out, shapes, dtypes):
         if arr.dtype != dtype:
             raise TypeError(f"{name} is {dtype}, not {arr.dtype}")
         check = getattr(arr, "check_writable", None)
-        if check is not None:
+        if check is not None and arr.size:      # (an empty array has pitches of 0 by itself)
             check()
         arrays.append(arr)
     for x in outs:                    # (only once all of them are known to be right)
