@@ -1021,19 +1021,27 @@ template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(
 }
 
 // ---- gradient -------------------------------------------------------------------------------
-// Two kernels, each with all sums of one output in one place, so that results do not depend on timing:
+// Two kinds of blocks, each with all sums of one output in one place, so that results do not depend on timing:
 // dQ (rows own their sums, keys pass by, as in the forward kernel) and dK, dV (keys own their sums, rows pass
 // by).  The scores are computed in both: seven products instead of five.  A wave holds two matrices of 32
 // columns in planes and its sums, more than 256 registers, so there is one for each SIMD, and what it does on
 // the vector unit stands between its matrix instructions.
+template <int NT> struct GradLds {
+    __attribute__((aligned(16))) char tile[2][2 * Planes<NT>::BYTES];
+    __attribute__((aligned(16))) float stat[2][2][kTile];
+    int ends[4], doc_range[2][4];
+    unsigned poison[2][kRows][NT];
+};
+
 template <int NT, bool CAP>
-__global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, int tiles, Packed in) {
+__device__ __forceinline__ void grad_dq(const Args& a, const Plan& plan, int tiles, const Packed& in, int block, GradLds<NT>& shared) {
     using P = Planes<NT>;
-    __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
-    __shared__ int ends[4], doc_range[2][4];
+    auto& lds = shared.tile;
+    auto& ends = shared.ends;
+    auto& doc_range = shared.doc_range;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int heads = a.batch * a.hkv;
-    const int head = blockIdx.x % heads, tile = tiles - 1 - blockIdx.x / heads;
+    const int head = block % heads, tile = tiles - 1 - block / heads;
     const int b = head / a.hkv, kh = head % a.hkv, group = a.hq / a.hkv;
     const Seq s = sequence(a, b);
     const bool wide = plan.wide;
@@ -1169,15 +1177,15 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dq(Args a, Plan plan, i
 // More than one part: the query heads of a key head, and ranges of `span` rows of them, go to different blocks,
 // whose sums are added by `attention_add`.
 template <int NT, bool CAP>
-__global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, Parts parts, Packed in, float* part) {
+__device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const Parts& parts, const Packed& in, float* part, int block, GradLds<NT>& shared) {
     using P = Planes<NT>;
-    __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][kTile];
-    __shared__ int doc_range[2][4];
-    __shared__ unsigned poison[2][kRows][NT];
+    auto& lds = shared.tile;
+    auto& stat = shared.stat;
+    auto& doc_range = shared.doc_range;
+    auto& poison = shared.poison;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int heads = a.batch * a.hkv, group = a.hq / a.hkv;
-    int id = blockIdx.x;
+    int id = block;
     const int head = id % heads;
     id /= heads;
     const int slice = id % parts.count, tile = id / parts.count;       // (causal: the first keys are seen by the most rows)
@@ -1370,6 +1378,21 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(Args a, Plan plan, 
     }
 }
 
+// Both in one launch, the longer dK, dV blocks first: neither waits for the other's last blocks (3 sequences of
+// 517 rows, 6 heads of 64: 43 us, in two launches 68; 2 of 2048 rows, 16 heads of 128: 702 and 710).  The two take their
+// arguments from copies: of one the compiler would read all values ahead of the choice and keep them, a hundred
+// scalar registers more than there are.  Mixing the two kinds block by block costs 5%: an XCD's L2 then holds
+// neither's matrices.
+template <int NT, bool CAP>
+__global__ __launch_bounds__(kThreads, 1) void attention_grad(Args a, Args same, Plan plan, Parts parts, Packed in, Packed same_in, int row_tiles, int dq_sets, int sets, float* part) {
+    __shared__ GradLds<NT> shared;
+    const int keys = a.batch * a.hkv * (sets - dq_sets);
+    if ((int)blockIdx.x < keys)
+        grad_dkv<NT, CAP>(a, plan, parts, in, part, blockIdx.x, shared);
+    else
+        grad_dq<NT, CAP>(same, plan, row_tiles, same_in, blockIdx.x - keys, shared);
+}
+
 // dK and dV from the parts of the query heads, in their order; one row of one of them for each wave
 __global__ __launch_bounds__(kThreads) void attention_add(Args a, int parts, const float* part) {
     const int64_t rows = (int64_t)a.batch * a.hkv * a.lk;
@@ -1532,19 +1555,12 @@ template <int NT> void launch_grad(const Args& a, const Plan& p, const Parts& pa
     packs.job[3] = pack_of(a.dout, a.dout_stride, a.hq, a.lq, 0, in.grad, in.grad_marks, nullptr, in.delta);
     const int64_t blocks = 2 * heads * key_tiles + 2 * (int64_t)a.batch * a.hq * query_tiles;
     attention_pack<NT><<<dim3((unsigned)blocks), kThreads, 0, s>>>(a, packs, p.wide);
-    const dim3 rows_grid((unsigned)(heads * tiles)), keys_grid((unsigned)(heads * parts.count * ((a.lk + kRows - 1) / kRows)));
-    if (a.lq) {
-        if (a.cap > 0.f)
-            attention_dq<NT, true><<<rows_grid, kThreads, 0, s>>>(a, p, tiles, in);
-        else
-            attention_dq<NT, false><<<rows_grid, kThreads, 0, s>>>(a, p, tiles, in);
-    }
-    if (a.lk) {
-        if (a.cap > 0.f)
-            attention_dkv<NT, true><<<keys_grid, kThreads, 0, s>>>(a, p, parts, in, part);
-        else
-            attention_dkv<NT, false><<<keys_grid, kThreads, 0, s>>>(a, p, parts, in, part);
-    }
+    const int dq_sets = a.lq ? tiles : 0, sets = dq_sets + parts.count * ((a.lk + kRows - 1) / kRows);
+    const dim3 grid((unsigned)(heads * sets));
+    if (a.cap > 0.f)
+        attention_grad<NT, true><<<grid, kThreads, 0, s>>>(a, a, p, parts, in, in, tiles, dq_sets, sets, part);
+    else
+        attention_grad<NT, false><<<grid, kThreads, 0, s>>>(a, a, p, parts, in, in, tiles, dq_sets, sets, part);
     if (a.lk && parts.count > 1) attention_add<<<dim3((unsigned)((2 * heads * a.lk + 3) / 4)), kThreads, 0, s>>>(a, parts.count, part);
 }
 
