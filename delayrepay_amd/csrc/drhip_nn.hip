@@ -414,10 +414,15 @@ __device__ __forceinline__ u64 rank_of(float x, int i) { return (u64)key_of(x) <
 struct Weigher {
     float top;
     double by, one;       // log2(e) / temperature, 2^s
+    // log2 of a weight: rises with the logit, 0 for the largest, -1000 for what is far from it and for a NaN
+    __device__ __forceinline__ double power(float x) const {
+        if (top == __builtin_inff()) return x == top ? 0.0 : -1000.0;
+        return fmax(((double)x - (double)top) * by, -1000.0);
+    }
     // 2^t for t <= 0: t = n + f, |f| <= 1/2, and a polynomial of degree 10 (own fit, relative error 6e-16)
-    __device__ __forceinline__ double real(float x) const {
-        if (top == __builtin_inff()) return x == top ? 1.0 : 0.0;
-        const double t = fmax(((double)x - (double)top) * by, -1000.0), n = rint(t), f = t - n;      // (-1000 also for a NaN)
+    __device__ __forceinline__ double real(float x) const { return real_of(power(x)); }
+    __device__ __forceinline__ double real_of(double t) const {
+        const double n = rint(t), f = t - n;
         double p = 7.070977711584016e-09;
         p = fma(p, f, 1.0205905398548696e-07);
         p = fma(p, f, 1.3215451632925122e-06);
@@ -718,28 +723,69 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     }
     if (done) {
     } else if (cut_p && !by_key) {
+        // The weights by their logarithm in equal steps, down to 2^-s of the largest: a step holds few tokens, in
+        // the logits' own bits hundreds (sorting those took 8 us of 50)
+        const double steps = (kCoarse - 1) / (double)(ilogb(p.one) + 2);
+        auto step_of = [&](double t) { return kCoarse - 1 + max((int)(t * steps), 1 - kCoarse); };
         for (int i = threadIdx.x; i < kCoarse; i += kDraw) coarse[i] = 0;
         __syncthreads();
-        each_token(row, v, [&](int, float x) {
-            const u64 w = weigh.whole(weigh.real(x));
-            if (w) atomicAdd(&coarse[key_of(x) >> 19], w);
-        });
+        for (int i = threadIdx.x; i < v; i += 4 * kDraw) {           // (four at a time: one waits for its own products)
+            float x[4];
+            u64 w[4];
+            int at[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) x[n] = row[min(i + n * kDraw, v - 1)];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const double t = weigh.power(x[n]);
+                w[n] = i + n * kDraw < v ? weigh.whole(weigh.real_of(t)) : 0;
+                at[n] = step_of(t);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (w[n]) atomicAdd(&coarse[at[n]], w[n]);
+        }
         __syncthreads();
         u64 want = 0;
         const Found f = reach<kCoarse>(coarse, [&](u64 all) { return want = part_of(all); }, lds, &found);
-        // the tokens of the digit in which the beginning ends go to the list, if there is room; those of larger ones are kept
+        // The tokens of the step in which the beginning ends go to the list, if there is room; those of larger ones are
+        // kept: a wave packs them together first, as most are not
+        float* mine = (float*)coarse + wave * 512;
         for (int c = wave; c < chunks; c += kDraw / 64) {
             u64 sum = 0;
-            each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](int i, float x) {
-                const unsigned digit = key_of(x) >> 19;
-                if (digit == f.bin) {
-                    const int at = atomicAdd(&listed, 1);
-                    if (at < kList) list[at] = rank_of(x, i);
-                } else if (digit > f.bin) {
-                    const double w = weigh.real(x);
+            const int end = min(v, (c + 1) * chunk);
+            for (int i0 = c * chunk; i0 < end; i0 += 512) {
+                float x[8];
+                int at[8], kept = 0, ending = 0;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) x[n] = row[min(i0 + 64 * n + lane, end - 1)];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    at[n] = i0 + 64 * n + lane < end ? step_of(weigh.power(x[n])) : -1;
+                    const u64 m = __ballot(at[n] > (int)f.bin);
+                    if (at[n] > (int)f.bin) mine[kept + __popcll(m & ((1ull << lane) - 1))] = x[n];
+                    kept += __popcll(m);
+                    ending += __popcll(__ballot(at[n] == (int)f.bin));
+                }
+                __builtin_amdgcn_wave_barrier();
+                for (int j = lane; j < kept; j += 64) {
+                    const double w = weigh.real(mine[j]);
                     if (w >= min_p) sum += weigh.whole(w);
                 }
-            });
+                __builtin_amdgcn_wave_barrier();
+                if (!ending) continue;
+                int to = 0;
+                if (lane == 0) to = atomicAdd(&listed, ending);
+                to = __builtin_amdgcn_readfirstlane(to);
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const bool in = at[n] == (int)f.bin;
+                    const u64 m = __ballot(in);
+                    const int k = to + __popcll(m & ((1ull << lane) - 1));
+                    if (in && k < kList) list[k] = rank_of(x[n], i0 + 64 * n + lane);
+                    to += __popcll(m);
+                }
+            }
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
             if (lane == 0) parts[c] = sum;
