@@ -398,6 +398,7 @@ constexpr int kBins = 2048;          // of a digit of 11 bits
 constexpr int kCoarse = 8192;        // of the first 13 bits
 constexpr int kChunks = 2048;        // parts of a row whose weights are kept for the last search
 constexpr int kList = 2048;          // tokens that LDS holds
+constexpr int kHead = 16384;
 constexpr int kFew = 128;            // of which so many are ordered by comparing all
 
 __device__ __forceinline__ unsigned key_of(float x) {
@@ -414,28 +415,33 @@ __device__ __forceinline__ u64 rank_of(float x, int i) { return (u64)key_of(x) <
 struct Weigher {
     float top;
     double by, one;       // log2(e) / temperature, 2^s
-    // log2 of a weight: rises with the logit, 0 for the largest, -1000 for what is far from it and for a NaN
-    __device__ __forceinline__ double power(float x) const {
-        if (top == __builtin_inff()) return x == top ? 0.0 : -1000.0;
-        return fmax(((double)x - (double)top) * by, -1000.0);
+    const double* roots;  // 2^(j/64)
+    // log2 of a weight in 64ths, and the rest: t = k / 64 + rest.  Rises with the logit, is 0 for the largest, and
+    // -64000 for what is far from it and for a NaN.
+    struct Power {
+        int k;
+        double rest;
+    };
+    __device__ __forceinline__ Power power(float x) const {
+        double t;
+        if (top == __builtin_inff()) t = x == top ? 0.0 : -1000.0;
+        else t = fmax(((double)x - (double)top) * by, -1000.0);
+        const double shift = 105553116266496.0, u = t + shift;        // 1.5 * 2^46, whose last bit is 1/64 ...
+        return {(int)(unsigned)__double_as_longlong(u), t - (u - shift)};
     }
-    // 2^t for t <= 0: t = n + f, |f| <= 1/2, and a polynomial of degree 10 (own fit, relative error 6e-16)
-    __device__ __forceinline__ double real(float x) const { return real_of(power(x)); }
-    __device__ __forceinline__ double real_of(double t) const {
-        const double n = rint(t), f = t - n;
-        double p = 7.070977711584016e-09;
-        p = fma(p, f, 1.0205905398548696e-07);
-        p = fma(p, f, 1.3215451632925122e-06);
-        p = fma(p, f, 1.5252672924951426e-05);
-        p = fma(p, f, 0.00015403530424779803);
-        p = fma(p, f, 0.0013333558200794376);
-        p = fma(p, f, 0.00961812910761866);
-        p = fma(p, f, 0.05550410866465167);
-        p = fma(p, f, 0.24022650695910075);
-        p = fma(p, f, 0.6931471805599462);
+    // 2^t: |rest| <= 1/128, a polynomial of degree 4 (own fit, relative error 5e-15) times a root times a power of two; no
+    // conversions, which take four times as long as a product
+    __device__ __forceinline__ double real_of(const Power& t) const {
+        const double f = t.rest;
+        double p = 0.009618138509201629;
+        p = fma(p, f, 0.05550419004645178);
+        p = fma(p, f, 0.24022650695902897);
+        p = fma(p, f, 0.6931471805593244);
         p = fma(p, f, 1.0);
-        return ldexp(p, (int)n);
+        const double root = roots[t.k & 63];
+        return p * __longlong_as_double(__double_as_longlong(root) + ((long long)(t.k >> 6) << 52));
     }
+    __device__ __forceinline__ double real(float x) const { return real_of(power(x)); }
     // nearest whole number of w * 2^s <= 2^52: the low bits of its sum with 2^52
     __device__ __forceinline__ u64 whole(double w) const {
         const double x = fma(w, one, 4503599627370496.0);
@@ -443,9 +449,9 @@ struct Weigher {
     }
 };
 
-// f(number, logit) for every token, eight loads at a time under way
-template <typename F> __device__ __forceinline__ void each_token(const float* row, int v, F f) {
-    int i = threadIdx.x;
+// f(number, logit) for the tokens from `first` to `v`, eight loads at a time under way
+template <typename F> __device__ __forceinline__ void each_token(const float* row, int first, int v, F f) {
+    int i = first + threadIdx.x;
     for (; i + 7 * kDraw < v; i += 8 * kDraw) {
         float x[8];
 #pragma unroll
@@ -468,15 +474,44 @@ template <typename F> __device__ __forceinline__ void each_of_part(const float* 
     }
 }
 
+// x of another lane of the same 16 (or, with CTRL 0x142 and 0x143, of the last lane of the 16 or 32 before) without
+// LDS; 0 where there is none and in rows of 16 that ROWS leaves out
+template <int CTRL, int ROWS = 15> __device__ __forceinline__ u64 moved(u64 x) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, ROWS, 15, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(x >> 32), CTRL, ROWS, 15, false);
+    return (u64)hi << 32 | lo;
+}
+
+__device__ __forceinline__ u64 of_lane(u64 x, int lane) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, lane);
+}
+
+// f over the wave's values, in every lane: neighbours, pairs, fours and eights of 16 lanes, then the four rows
+template <typename F> __device__ __forceinline__ u64 of_wave(u64 x, F f) {
+    x = f(x, moved<0xb1>(x));
+    x = f(x, moved<0x4e>(x));
+    x = f(x, moved<0x141>(x));
+    x = f(x, moved<0x140>(x));
+    return f(f(of_lane(x, 0), of_lane(x, 16)), f(of_lane(x, 32), of_lane(x, 48)));
+}
+__device__ __forceinline__ u64 wave_sum(u64 x) {
+    return of_wave(x, [](u64 a, u64 b) { return a + b; });
+}
+
+// Sum over the wave's lanes up to this one
+__device__ __forceinline__ u64 wave_scan(u64 x) {
+    x += moved<0x111>(x);
+    x += moved<0x112>(x);
+    x += moved<0x114>(x);
+    x += moved<0x118>(x);
+    x += moved<0x142, 10>(x);
+    return x + moved<0x143, 12>(x);
+}
+
 // Sum over the threads before this one, and over all (`lds`: 17 words)
 __device__ __forceinline__ u64 scan(u64 x, u64* lds, u64& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u64 sum = x;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const u64 y = __shfl_up(sum, m);
-        if (lane >= m) sum += y;
-    }
+    const u64 sum = wave_scan(x);
     __syncthreads();
     if (lane == 63) lds[wave] = sum;
     __syncthreads();
@@ -569,6 +604,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     __shared__ u64 coarse[kCoarse];            // weights of the first 13 bits, or counts, or the digits of `select`
     __shared__ u64 list[kList], weights[kFew], parts[kChunks], lds[kDraw / 64 + 1];
     __shared__ unsigned marks[kChunks];
+    __shared__ double roots[64];
     __shared__ Found found;
     __shared__ int listed, chunk_at;
     __shared__ u64 chunk_before, chunk_tied, cut_rank;
@@ -596,19 +632,31 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         where = x > most ? i : where;
         most = x > most ? x : most;
     };
-    if (counted)
-        each_token(row, v, [&](int i, float x) {
+    // Of a long row the first kHead tokens say from which digit on a token can be one of the first k, so that the others
+    // that are go to the list at once, and only kHead are read again
+    const int head = v >= 4 * kHead && k * (v / kHead) <= kList / 2 ? kHead : v;
+    if (counted) {
+        each_token(row, 0, head, [&](int i, float x) {
             larger(i, x);
             atomicAdd(&counts[key_of(x) >> 19], 1u);
         });
-    else
-        each_token(row, v, larger);
+        if (head < v) {
+            __syncthreads();
+            const unsigned least = reach<kCoarse>(counts, [&](u64) { return (u64)k; }, lds, &found).bin;
+            each_token(row, head, v, [&](int i, float x) {
+                larger(i, x);
+                const unsigned digit = key_of(x) >> 19;
+                atomicAdd(&counts[digit], 1u);
+                if (digit >= least) {
+                    const int at = atomicAdd(&listed, 1);
+                    if (at < kList) list[at] = rank_of(x, i);
+                }
+            });
+        }
+    } else
+        each_token(row, 0, v, larger);
     u64 best = rank_of(most, where);
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const u64 y = __shfl_xor(best, m);
-        best = y > best ? y : best;
-    }
+    best = of_wave(best, [](u64 a, u64 b) { return a > b ? a : b; });
     if (lane == 0) lds[wave] = best;
     __syncthreads();
     best = 0;
@@ -621,7 +669,9 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         if (threadIdx.x == 0) p.tokens[b] = none ? -1 : (int64_t)(int)~(unsigned)best;
         return;
     }
-    const Weigher weigh{value_of(top_key), fmin(1.4426950408889634074 / temperature, 1e300), p.one};      // (finite: the largest is 0 apart from itself)
+    if (threadIdx.x < 64) roots[threadIdx.x] = exp2(threadIdx.x / 64.0);
+    __syncthreads();
+    const Weigher weigh{value_of(top_key), fmin(1.4426950408889634074 / temperature, 1e300), p.one, roots};      // (finite: the largest is 0 apart from itself)
 
     // end of what is kept: ranks of at least `cut`; where that is not known, keys above `cut_key`, and the first
     // `ties` tokens whose key it is
@@ -707,10 +757,23 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         const unsigned from = f.bin;
         if (f.before + f.inside <= kList) {
             for (int c = threadIdx.x; c < chunks; c += kDraw) parts[c] = 0;
-            each_token(row, v, [&](int i, float x) {
-                const u64 r = rank_of(x, i);
+            // of what is there already, the ones that the whole row's digit leaves; then the tokens not looked at
+            const int there = listed;
+            const bool ready = there <= kList;
+            u64 old[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (ready && (int)threadIdx.x + e * kDraw < there) old[e] = list[threadIdx.x + e * kDraw];
+            __syncthreads();
+            if (threadIdx.x == 0) listed = 0;
+            __syncthreads();
+            auto take = [&](u64 r) {
                 if (r >> 51 >= from) list[atomicAdd(&listed, 1)] = r;
-            });
+            };
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (ready && (int)threadIdx.x + e * kDraw < there) take(old[e]);
+            each_token(row, 0, ready ? head : v, [&](int i, float x) { take(rank_of(x, i)); });
             __syncthreads();
             keep_listed((int)(f.before + f.inside), (int)k, 0, part_of);
         }
@@ -723,24 +786,27 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     }
     if (done) {
     } else if (cut_p && !by_key) {
-        // The weights by their logarithm in equal steps, down to 2^-s of the largest: a step holds few tokens, in
-        // the logits' own bits hundreds (sorting those took 8 us of 50)
-        const double steps = (kCoarse - 1) / (double)(ilogb(p.one) + 2);
-        auto step_of = [&](double t) { return kCoarse - 1 + max((int)(t * steps), 1 - kCoarse); };
+        // The weights by their logarithm in 64ths, of which 2^-s of the largest has less than kCoarse: a step holds few
+        // tokens, in the logits' own bits hundreds (sorting those took 8 us of 50)
+        auto step_of = [&](const Weigher::Power& t) { return kCoarse - 1 + max(t.k, 1 - kCoarse); };
         for (int i = threadIdx.x; i < kCoarse; i += kDraw) coarse[i] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < v; i += 4 * kDraw) {           // (four at a time: one waits for its own products)
-            float x[4];
+        float x[4];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) x[n] = row[min(i + n * kDraw, v - 1)];
+        };
+        fetch(threadIdx.x);
+        for (int i = threadIdx.x; i - (int)threadIdx.x < v; i += 4 * kDraw) {           // (four at a time: one waits for its own products)
             u64 w[4];
             int at[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) x[n] = row[min(i + n * kDraw, v - 1)];
-#pragma unroll
             for (int n = 0; n < 4; ++n) {
-                const double t = weigh.power(x[n]);
+                const Weigher::Power t = weigh.power(x[n]);
                 w[n] = i + n * kDraw < v ? weigh.whole(weigh.real_of(t)) : 0;
                 at[n] = step_of(t);
             }
+            fetch(i + 4 * kDraw);                // (the last time the last token again)
 #pragma unroll
             for (int n = 0; n < 4; ++n)
                 if (w[n]) atomicAdd(&coarse[at[n]], w[n]);
@@ -748,24 +814,50 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         __syncthreads();
         u64 want = 0;
         const Found f = reach<kCoarse>(coarse, [&](u64 all) { return want = part_of(all); }, lds, &found);
+        // the logits from which on a token's step is at least `step`, as the first key, 64 keys at a time
+        auto first_of = [&](int step) {
+            u64 base = 0;
+            int c = 0;
+#pragma unroll
+            for (int shift = 26; shift >= -4; shift -= 6) {
+                const int by = max(shift, 0);
+                const u64 key = base + ((u64)lane << by);
+                const bool below = key < top_key && step_of(weigh.power(value_of((unsigned)key))) < step;
+                c = __popcll(__ballot(below));
+                base += (u64)(shift > 0 && c ? c - 1 : c) << by;
+            }
+            return max((unsigned)base, key_of(-__builtin_inff()));
+        };
+        const bool above = (int)f.bin < kCoarse - 1;
+        const float from_ending = value_of(first_of((int)f.bin)), from_kept = above ? value_of(first_of((int)f.bin + 1)) : 0.f;
         // The tokens of the step in which the beginning ends go to the list, if there is room; those of larger ones are
         // kept: a wave packs them together first, as most are not
         float* mine = (float*)coarse + wave * 512;
+        float next[8];
+        auto fetch_part = [&](int i0, int end) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) next[n] = row[min(i0 + 64 * n + lane, end - 1)];
+        };
+        if (wave < chunks) fetch_part(wave * chunk, min(v, (wave + 1) * chunk));
         for (int c = wave; c < chunks; c += kDraw / 64) {
             u64 sum = 0;
-            const int end = min(v, (c + 1) * chunk);
+            const int end = min(v, (c + 1) * chunk), after = c + kDraw / 64;
             for (int i0 = c * chunk; i0 < end; i0 += 512) {
                 float x[8];
-                int at[8], kept = 0, ending = 0;
 #pragma unroll
-                for (int n = 0; n < 8; ++n) x[n] = row[min(i0 + 64 * n + lane, end - 1)];
+                for (int n = 0; n < 8; ++n) x[n] = next[n];
+                if (i0 + 512 < end) fetch_part(i0 + 512, end);
+                else if (after < chunks) fetch_part(after * chunk, min(v, (after + 1) * chunk));
+                u64 ends[8];
+                int kept = 0, ending = 0;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    at[n] = i0 + 64 * n + lane < end ? step_of(weigh.power(x[n])) : -1;
-                    const u64 m = __ballot(at[n] > (int)f.bin);
-                    if (at[n] > (int)f.bin) mine[kept + __popcll(m & ((1ull << lane) - 1))] = x[n];
+                    const bool in = i0 + 64 * n + lane < end, keep = in && above && x[n] >= from_kept;
+                    const u64 m = __ballot(keep);
+                    if (keep) mine[kept + __popcll(m & ((1ull << lane) - 1))] = x[n];
                     kept += __popcll(m);
-                    ending += __popcll(__ballot(at[n] == (int)f.bin));
+                    ends[n] = __ballot(in && x[n] >= from_ending) & ~m;
+                    ending += __popcll(ends[n]);
                 }
                 __builtin_amdgcn_wave_barrier();
                 for (int j = lane; j < kept; j += 64) {
@@ -779,15 +871,12 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
                 to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const bool in = at[n] == (int)f.bin;
-                    const u64 m = __ballot(in);
-                    const int k = to + __popcll(m & ((1ull << lane) - 1));
-                    if (in && k < kList) list[k] = rank_of(x[n], i0 + 64 * n + lane);
-                    to += __popcll(m);
+                    const int k = to + __popcll(ends[n] & ((1ull << lane) - 1));
+                    if (ends[n] >> lane & 1 && k < kList) list[k] = rank_of(x[n], i0 + 64 * n + lane);
+                    to += __popcll(ends[n]);
                 }
             }
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+            sum = wave_sum(sum);
             if (lane == 0) parts[c] = sum;
         }
         __syncthreads();
@@ -836,11 +925,8 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
                     const double w = weigh.real(x);
                     sum += w >= min_p ? weigh.whole(w) : 0;
                 });
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                sum += __shfl_xor(sum, m);
-                tied += __shfl_xor(tied, m);
-            }
+            sum = wave_sum(sum);
+            tied = wave_sum(tied);
             if (lane == 0) parts[c] = sum, marks[c] = tied;
         }
     else
@@ -881,15 +967,10 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
             const u64 m = __ballot(tie);
             if (tie) in = tied + __popcll(m & ((1ull << lane) - 1)) < ties;
             tied += __popcll(m);
-            u64 run = in ? weigh.whole(w) : 0;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const u64 y = __shfl_up(run, d);
-                if (lane >= d) run += y;
-            }
+            const u64 run = wave_scan(in ? weigh.whole(w) : 0);
             const u64 past = __ballot(sum + run > target);
             if (past && token < 0) token = i1 + 64 * n + __builtin_ctzll(past);
-            sum += __shfl(run, 63);
+            sum += of_lane(run, 63);
         }
     }
     if (lane == 0) p.tokens[b] = token < 0 ? first : token;       // (one is always found: target < weight)
