@@ -413,39 +413,54 @@ __device__ __forceinline__ float value_of(unsigned key) {
 __device__ __forceinline__ u64 rank_of(float x, int i) { return (u64)key_of(x) << 32 | (unsigned)~i; }
 
 struct Weigher {
-    float top;
-    double by, one;       // log2(e) / temperature, 2^s
+    float least;          // smaller ones have no weight: -inf, NaN, and finite ones where the largest is infinite
+    float floor, high;    // for the arithmetic logits lie between: weights of about 2^-400 are nothing
+    double zero, by, one; // the largest logit, log2(e) / temperature, 2^s
     const double* roots;  // 2^(j/64)
-    // log2 of a weight in 64ths, and the rest: t = k / 64 + rest.  Rises with the logit, is 0 for the largest, and
-    // -64000 for what is far from it and for a NaN.
+    // log2 of a weight in 64ths, and the rest: t = k / 64 + rest.  Rises with the logit, is 0 for the largest.
     struct Power {
         int k;
         double rest;
     };
-    __device__ __forceinline__ Power power(float x) const {
-        double t;
-        if (top == __builtin_inff()) t = x == top ? 0.0 : -1000.0;
-        else t = fmax(((double)x - (double)top) * by, -1000.0);
-        const double shift = 105553116266496.0, u = t + shift;        // 1.5 * 2^46, whose last bit is 1/64 ...
-        return {(int)(unsigned)__double_as_longlong(u), t - (u - shift)};
+    __device__ __forceinline__ Weigher(float top, double rate, double one, const double* roots) : one(one), roots(roots) {
+        constexpr float far = 3.40282347e38f;
+        high = fminf(top, far), zero = high, least = top > far ? top : -far;
+        const float below = fmaxf(nextafterf(high, -__builtin_inff()), -far);
+        // (at the highest rate the next smaller logit has no weight; the floor's rounding moves t by 400 at most, and powers
+        // of two down to 2^-1022 can be told apart)
+        by = below < high ? fmin(rate, 400.0 / (zero - (double)below)) : 1.0;
+        floor = fminf(below, (float)fmax(zero - 400.0 / by, -(double)far));
     }
-    // 2^t: |rest| <= 1/128, a polynomial of degree 4 (own fit, relative error 5e-15) times a root times a power of two; no
-    // conversions, which take four times as long as a product
-    __device__ __forceinline__ double real_of(const Power& t) const {
-        const double f = t.rest;
+    __device__ __forceinline__ Power power(float x) const {
+        const double t = ((double)__builtin_amdgcn_fmed3f(x, floor, high) - zero) * by;
+        const double shift = 105553116266496.0, u = t + shift;            // 1.5 * 2^46, whose last bit is 1/64 ...
+        return {x >= least ? (int)(unsigned)__double_as_longlong(u) : -25600, t - (u - shift)};
+    }
+    // 2^rest: |rest| <= 1/128, a polynomial of degree 4 (own fit, relative error 5e-15).  No conversions to integers, which
+    // take four times as long as a product.
+    __device__ __forceinline__ static double part(double f) {
         double p = 0.009618138509201629;
         p = fma(p, f, 0.05550419004645178);
         p = fma(p, f, 0.24022650695902897);
         p = fma(p, f, 0.6931471805593244);
-        p = fma(p, f, 1.0);
-        const double root = roots[t.k & 63];
-        return p * __longlong_as_double(__double_as_longlong(root) + ((long long)(t.k >> 6) << 52));
+        return fma(p, f, 1.0);
     }
-    __device__ __forceinline__ double real(float x) const { return real_of(power(x)); }
-    // nearest whole number of w * 2^s <= 2^52: the low bits of its sum with 2^52
-    __device__ __forceinline__ u64 whole(double w) const {
-        const double x = fma(w, one, 4503599627370496.0);
+    __device__ __forceinline__ double whole_part(int k) const {
+        return __longlong_as_double(__double_as_longlong(roots[k & 63]) + ((long long)(k >> 6) << 52));
+    }
+    __device__ __forceinline__ double real(float x) const {
+        const Power t = power(x);
+        return part(t.rest) * whole_part(t.k);
+    }
+    // nearest whole number of 2^t * 2^s <= 2^52: the low bits of its sum with 2^52
+    __device__ __forceinline__ u64 whole_of(const Power& t) const {
+        const double x = fma(part(t.rest), whole_part(t.k) * one, 4503599627370496.0);
         return (u64)__double_as_longlong(x) - 0x4330000000000000ull;
+    }
+    __device__ __forceinline__ u64 whole(float x) const { return whole_of(power(x)); }
+    __device__ __forceinline__ u64 whole_from(float x, double min_p) const {      // 0 below min_p of the largest
+        const Power t = power(x);
+        return part(t.rest) * whole_part(t.k) >= min_p ? whole_of(t) : 0;
     }
 };
 
@@ -462,15 +477,14 @@ template <typename F> __device__ __forceinline__ void each_token(const float* ro
     for (; i < v; i += kDraw) f(i, row[i]);
 }
 
-// The same for one part of the row by one wave, from number `first` to `end`
+// f(logit) for one part of the row by one wave, from number `first` to `end`, with NaN for what the last turn has too much
 template <typename F> __device__ __forceinline__ void each_of_part(const float* row, int first, int end, F f) {
     for (int i0 = first + (threadIdx.x & 63); i0 < end; i0 += 512) {
         float x[8];
 #pragma unroll
         for (int n = 0; n < 8; ++n) x[n] = row[min(i0 + 64 * n, end - 1)];
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-            if (i0 + 64 * n < end) f(i0 + 64 * n, x[n]);
+        for (int n = 0; n < 8; ++n) f(i0 + 64 * n < end ? x[n] : __builtin_nanf(""));
     }
 }
 
@@ -496,6 +510,11 @@ template <typename F> __device__ __forceinline__ u64 of_wave(u64 x, F f) {
 }
 __device__ __forceinline__ u64 wave_sum(u64 x) {
     return of_wave(x, [](u64 a, u64 b) { return a + b; });
+}
+
+// Lanes before this one in a mask, and `more`
+__device__ __forceinline__ int lanes_before(u64 mask, int more) {
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, more));
 }
 
 // Sum over the wave's lanes up to this one
@@ -569,10 +588,10 @@ __device__ unsigned select(const float* row, int v, unsigned least, u64 ties, un
             const unsigned key = key_of(x);
             if (key < least || key == tie_key) continue;
             if (level && key >> (shift + bits) != prefix) continue;
-            atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], COUNT ? 1 : weigh.whole(weigh.real(x)));
+            atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], COUNT ? 1 : weigh.whole(x));
         }
         if (!COUNT && threadIdx.x == 0 && ties && (!level || tie_key >> (shift + bits) == prefix))
-            atomicAdd(&hist[tie_key >> shift & ((1u << bits) - 1)], ties * weigh.whole(weigh.real(value_of(tie_key))));
+            atomicAdd(&hist[tie_key >> shift & ((1u << bits) - 1)], ties * weigh.whole(value_of(tie_key)));
         __syncthreads();
         const u64 rest = want - before;
         const Found f = reach<kBins>(hist, [&](u64) { return rest; }, lds, found);
@@ -608,7 +627,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
     __shared__ Found found;
     __shared__ int listed, chunk_at;
     __shared__ u64 chunk_before, chunk_tied, cut_rank;
-    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float* row = p.logits + b * p.logits_stride;
     const int v = p.vocabulary;
     const double temperature = p.temperature ? p.temperature[b] : p.temperature_all;
@@ -698,7 +717,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
             if (me < n) {
                 rank[0] = list[me];
                 w[0] = weigh.real(value_of((unsigned)(rank[0] >> 32)));
-                weights[me] = x[0] = weigh.whole(w[0]);
+                weights[me] = x[0] = weigh.whole(value_of((unsigned)(rank[0] >> 32)));
             } else if (me < n + 8) {
                 list[me] = 0;                // (the loop below goes to a multiple of eight)
             }
@@ -727,7 +746,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
                 if (place + e < keep) {
                     rank[e] = list[place + e];
                     w[e] = weigh.real(value_of((unsigned)(rank[e] >> 32)));
-                    x[e] = weigh.whole(w[e]);
+                    x[e] = weigh.whole(value_of((unsigned)(rank[e] >> 32)));
                 }
             sum = scan(x[0] + x[1], lds, all);
         }
@@ -792,21 +811,26 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         for (int i = threadIdx.x; i < kCoarse; i += kDraw) coarse[i] = 0;
         __syncthreads();
         float x[4];
-        auto fetch = [&](int i) {
+        auto fetch = [&](int i0) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) x[n] = row[min(i + n * kDraw, v - 1)];
+            for (int n = 0; n < 4; ++n) {
+                const int first = i0 + n * kDraw;
+                if (first + kDraw <= v) x[n] = (row + first)[threadIdx.x];
+                else x[n] = row[min(first + (int)threadIdx.x, v - 1)];
+            }
         };
-        fetch(threadIdx.x);
-        for (int i = threadIdx.x; i - (int)threadIdx.x < v; i += 4 * kDraw) {           // (four at a time: one waits for its own products)
+        fetch(0);
+        for (int i0 = 0; i0 < v; i0 += 4 * kDraw) {           // (four at a time: one waits for its own products)
             u64 w[4];
             int at[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const Weigher::Power t = weigh.power(x[n]);
-                w[n] = i + n * kDraw < v ? weigh.whole(weigh.real_of(t)) : 0;
+                const u64 whole = weigh.whole_of(t);          // (ahead of the choice: a read of LDS inside it would be a branch)
+                w[n] = i0 + n * kDraw + (int)threadIdx.x < v ? whole : 0;
                 at[n] = step_of(t);
             }
-            fetch(i + 4 * kDraw);                // (the last time the last token again)
+            if (i0 + 4 * kDraw < v) fetch(i0 + 4 * kDraw);
 #pragma unroll
             for (int n = 0; n < 4; ++n)
                 if (w[n]) atomicAdd(&coarse[at[n]], w[n]);
@@ -829,14 +853,20 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
             return max((unsigned)base, key_of(-__builtin_inff()));
         };
         const bool above = (int)f.bin < kCoarse - 1;
-        const float from_ending = value_of(first_of((int)f.bin)), from_kept = above ? value_of(first_of((int)f.bin + 1)) : 0.f;
+        const float from_ending = value_of(first_of((int)f.bin)), from_kept = above ? value_of(first_of((int)f.bin + 1)) : __builtin_nanf("");
         // The tokens of the step in which the beginning ends go to the list, if there is room; those of larger ones are
         // kept: a wave packs them together first, as most are not
         float* mine = (float*)coarse + wave * 512;
         float next[8];
-        auto fetch_part = [&](int i0, int end) {
+        auto fetch_part = [&](int i0, int end) {         // (past the end NaN, which is neither)
+            const float* from = row + i0;
+            if (i0 + 512 <= end) {
 #pragma unroll
-            for (int n = 0; n < 8; ++n) next[n] = row[min(i0 + 64 * n + lane, end - 1)];
+                for (int n = 0; n < 8; ++n) next[n] = from[64 * n + lane];
+            } else {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) next[n] = i0 + 64 * n + lane < end ? from[64 * n + lane] : __builtin_nanf("");
+            }
         };
         if (wave < chunks) fetch_part(wave * chunk, min(v, (wave + 1) * chunk));
         for (int c = wave; c < chunks; c += kDraw / 64) {
@@ -852,17 +882,15 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
                 int kept = 0, ending = 0;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const bool in = i0 + 64 * n + lane < end, keep = in && above && x[n] >= from_kept;
-                    const u64 m = __ballot(keep);
-                    if (keep) mine[kept + __popcll(m & ((1ull << lane) - 1))] = x[n];
+                    const u64 m = __ballot(x[n] >= from_kept);
+                    if (x[n] >= from_kept) mine[lanes_before(m, kept)] = x[n];
                     kept += __popcll(m);
-                    ends[n] = __ballot(in && x[n] >= from_ending) & ~m;
+                    ends[n] = __ballot(x[n] >= from_ending) & ~m;
                     ending += __popcll(ends[n]);
                 }
                 __builtin_amdgcn_wave_barrier();
                 for (int j = lane; j < kept; j += 64) {
-                    const double w = weigh.real(mine[j]);
-                    if (w >= min_p) sum += weigh.whole(w);
+                    sum += weigh.whole_from(mine[j], min_p);
                 }
                 __builtin_amdgcn_wave_barrier();
                 if (!ending) continue;
@@ -871,7 +899,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
                 to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const int k = to + __popcll(ends[n] & ((1ull << lane) - 1));
+                    const int k = lanes_before(ends[n], to);
                     if (ends[n] >> lane & 1 && k < kList) list[k] = rank_of(x[n], i0 + 64 * n + lane);
                     to += __popcll(ends[n]);
                 }
@@ -886,7 +914,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
             keep_listed(n, n, f.before, [&](u64) { return want; });
         } else {
             cut_key = select<false>(row, v, 0, 0, no_key, want, weigh, coarse, lds, &found, before);
-            const u64 each = weigh.whole(weigh.real(value_of(cut_key)));
+            const u64 each = weigh.whole(value_of(cut_key));
             ties = each ? (want - before + each - 1) / each : 1;
             by_key = true;
         }
@@ -895,13 +923,13 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         u64 sum = 0, weight;
         for (int i = threadIdx.x; i < v; i += kDraw) {
             const float x = row[i];
-            if (key_of(x) > cut_key) sum += weigh.whole(weigh.real(x));
+            if (key_of(x) > cut_key) sum += weigh.whole(x);
         }
         scan(sum, lds, weight);
-        weight += ties * weigh.whole(weigh.real(value_of(cut_key)));
+        weight += ties * weigh.whole(value_of(cut_key));
         const u64 want = part_of(weight);
         const unsigned end = select<false>(row, v, cut_key, ties, cut_key, want, weigh, coarse, lds, &found, before);
-        const u64 each = weigh.whole(weigh.real(value_of(end)));
+        const u64 each = weigh.whole(value_of(end));
         u64 n = each ? (want - before + each - 1) / each : 1;
         if (end == cut_key && n > ties) n = ties;
         cut_key = end;
@@ -913,17 +941,15 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
             u64 sum = 0;
             unsigned tied = 0;
             if (by_key)
-                each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](int, float x) {
+                each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](float x) {
                     const unsigned key = key_of(x);
-                    const double w = weigh.real(x);
-                    if (key < cut_key || w < min_p) return;
-                    if (key == cut_key) ++tied;
-                    else sum += weigh.whole(w);
+                    if (key < cut_key) return;
+                    if (key > cut_key) sum += weigh.whole_from(x, min_p);
+                    else if (x == x && weigh.real(x) >= min_p) ++tied;
                 });
             else
-                each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](int, float x) {
-                    const double w = weigh.real(x);
-                    sum += w >= min_p ? weigh.whole(w) : 0;
+                each_of_part(row, c * chunk, min(v, (c + 1) * chunk), [&](float x) {
+                    sum += weigh.whole_from(x, min_p);
                 });
             sum = wave_sum(sum);
             tied = wave_sum(tied);
@@ -933,7 +959,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
         for (int c = threadIdx.x; c < chunks; c += kDraw) marks[c] = 0;
     __syncthreads();
     // the part and the token in which the draw falls
-    const u64 each = by_key ? weigh.whole(weigh.real(value_of(cut_key))) : 0;
+    const u64 each = by_key ? weigh.whole(value_of(cut_key)) : 0;
     const int c0 = 2 * threadIdx.x;
     const unsigned t0 = c0 < chunks ? marks[c0] : 0, t1 = c0 + 1 < chunks ? marks[c0 + 1] : 0;
     u64 every;
@@ -967,7 +993,7 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
             const u64 m = __ballot(tie);
             if (tie) in = tied + __popcll(m & ((1ull << lane) - 1)) < ties;
             tied += __popcll(m);
-            const u64 run = wave_scan(in ? weigh.whole(w) : 0);
+            const u64 run = wave_scan(in ? weigh.whole(x[n]) : 0);
             const u64 past = __ballot(sum + run > target);
             if (past && token < 0) token = i1 + 64 * n + __builtin_ctzll(past);
             sum += of_lane(run, 63);

@@ -429,6 +429,23 @@ def test_sample_with_parameters_at_their_ends(vocabulary):
         _draws(logits, u, temperature=temperature, top_k=5, top_p=0.5, min_p=0.9)
 
 
+@pytest.mark.parametrize("how", [dict(), dict(top_p=0.9), dict(top_k=3), dict(top_k=3, top_p=0.7, min_p=0.1)], ids=str)
+def test_sample_of_extreme_logits(how):
+    """What is not a number or -inf is never drawn, at no temperature; next to the ends of float32."""
+    rs = np.random.RandomState(4)
+    info, f = np.finfo(np.float32), np.float32
+    logits = np.tile(np.array([NAN, -INF, info.min, info.min, 0, NAN, -INF], f), (7, 100))
+    logits[1] = np.where(logits[1] == 0, np.nextafter(info.min, f(0)), logits[1])
+    logits[2] = np.where(logits[2] == 0, info.max, logits[2])
+    logits[3, 300:] = INF
+    logits[4, 4] = INF                                    # one, next to the largest finite ones
+    logits[4, 11] = info.max
+    logits[5] = np.where(logits[5] == 0, -INF, logits[5])
+    logits[6] = np.where(logits[6] == 0, info.tiny, logits[6])
+    for temperature in (1.0, 1e30, 1e-40, np.full(7, info.max), np.full(7, 1e20, f)):
+        _draws(logits, rs.rand(7), temperature=temperature, **how)
+
+
 def test_sample_from_the_device_generator():
     """The generator's lazy numbers are evaluated for the call; frequencies follow the weights: of 20000 draws
     each share is within five standard deviations."""
