@@ -226,75 +226,63 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Rot p, int lanes_log, 
     }
 }
 
-// Gradient with a norm.  A block owns up to HEADS heads and every `slots`-th run of tokens, its groups one token
-// each; a lane keeps the sums of its elements of dw, the groups meet in LDS, the blocks in `rotary_dw`.
-constexpr int kHeads = 2;
-
+// Gradient with a norm.  A block owns a head and every `slots`-th run of tokens, its groups one token each; a lane keeps
+// the sums of its elements of dw, the groups meet in LDS, the blocks in `rotary_dw`.  A group has one or a few
+// tokens, so it waits for memory more than it computes: one head for a block, whose registers leave room for four
+// waves on a SIMD (20 heads of 128, 3554 tokens: 22 us, 4.9 TB/s), not two, which share the angles but leave
+// room for two (30 us), and the loads ahead of the angles.
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_grad_kernel(Rot p, int lanes_log, int slots) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
     const int lanes = 1 << lanes_log, groups = kThreads >> lanes_log;
     const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
-    const int slot = blockIdx.x % slots, h0 = blockIdx.x / slots * kHeads;
+    const int slot = blockIdx.x % slots, h = blockIdx.x / slots;
     const int64_t tokens = (int64_t)p.batch * p.rows;
     double f[4];
     frequencies<T, WIDE>(p, lane, lanes, f);
-    Row<T, WIDE> w[kHeads];
-    T sums[kHeads][16];
+    Row<T, WIDE> w;
+    T sums[16];
+    w.load(p, (const T*)p.weight + h * p.weight_stride, lane, lanes, true);
 #pragma unroll
-    for (int k = 0; k < kHeads; ++k) {
-        w[k].load(p, (const T*)p.weight + (h0 + k) * p.weight_stride, lane, lanes, h0 + k < p.heads);
-#pragma unroll
-        for (int n = 0; n < 16; ++n) sums[k][n] = 0;
-    }
+    for (int n = 0; n < 16; ++n) sums[n] = 0;
     for (int64_t t0 = (int64_t)slot * groups; t0 < tokens; t0 += (int64_t)slots * groups) {
         const int64_t token = t0 + group;
         const bool live = token < tokens;
         const int b = live ? (int)(token / p.rows) : 0, l = live ? (int)(token % p.rows) : 0;
+        Row<T, WIDE> x, g;
+        x.load(p, (const T*)p.x + b * p.x_stride[0] + h * p.x_stride[1] + l * p.x_stride[2], lane, lanes, live);
+        g.load(p, (const T*)p.dy + b * p.dy_stride[0] + h * p.dy_stride[1] + l * p.dy_stride[2], lane, lanes, live);
         T c[4], s[4];
         angles<T>(p, position_of(p, b, l), f, c, s);
-#pragma unroll
-        for (int k = 0; k < kHeads; ++k) {
-            const int h = h0 + k;
-            const bool in = live && h < p.heads;
-            Row<T, WIDE> x, g;
-            x.load(p, (const T*)p.x + b * p.x_stride[0] + h * p.x_stride[1] + l * p.x_stride[2], lane, lanes, in);
-            g.load(p, (const T*)p.dy + b * p.dy_stride[0] + h * p.dy_stride[1] + l * p.dy_stride[2], lane, lanes, in);
-            g.turn(c, s);
-            T square = 0, dot = 0;
-            x.each([&](T& v, int n) {
-                square += v * v;
-                dot += v * g.at(n) * w[k].at(n);
-            });
-            square = group_sum(square, lanes);
-            dot = group_sum(dot, lanes);
-            const T r = T(1) / root(square / T(p.d) + T(p.eps));
-            const T mean = dot * r * r / T(p.d);            // mean(w g xhat) r
-            Row<T, WIDE> out;
-            out.each([&](T& v, int n) {
-                const T hat = x.at(n) * r;
-                sums[k][n] += in ? g.at(n) * hat : T(0);
-                v = r * g.at(n) * w[k].at(n) - x.at(n) * r * mean;
-            });
-            if (in) out.store(p, (T*)p.y + b * p.y_stride[0] + h * p.y_stride[1] + l * p.y_stride[2], lane, lanes);
-        }
+        g.turn(c, s);
+        T square = 0, dot = 0;
+        x.each([&](T& v, int n) {
+            square += v * v;
+            dot += v * g.at(n) * w.at(n);
+        });
+        square = group_sum(square, lanes);
+        dot = group_sum(dot, lanes);
+        const T r = T(1) / root(square / T(p.d) + T(p.eps));
+        const T mean = dot * r * r / T(p.d);            // mean(w g xhat) r
+        Row<T, WIDE> out;
+        out.each([&](T& v, int n) {
+            const T hat = x.at(n) * r;
+            sums[n] += live ? g.at(n) * hat : T(0);
+            v = r * g.at(n) * w.at(n) - x.at(n) * r * mean;
+        });
+        if (live) out.store(p, (T*)p.y + b * p.y_stride[0] + h * p.y_stride[1] + l * p.y_stride[2], lane, lanes);
     }
-    // [k][n][lane] summed over the groups in their order
+    // [n][lane] summed over the groups in their order
     T* lds = (T*)shared;
 #pragma unroll
-    for (int k = 0; k < kHeads; ++k) {
-        if (k) __syncthreads();
-#pragma unroll
-        for (int n = 0; n < 16; ++n) lds[n * kThreads + threadIdx.x] = sums[k][n];
-        __syncthreads();
-        if (h0 + k < p.heads)
-            for (int o = threadIdx.x; o < 16 << lanes_log; o += kThreads) {
-                const int n = o >> lanes_log, i = Row<T, WIDE>::element(p, o & (lanes - 1), lanes, n);
-                T total = 0;
+    for (int n = 0; n < 16; ++n) lds[n * kThreads + threadIdx.x] = sums[n];
+    __syncthreads();
+    for (int o = threadIdx.x; o < 16 << lanes_log; o += kThreads) {
+        const int n = o >> lanes_log, i = Row<T, WIDE>::element(p, o & (lanes - 1), lanes, n);
+        T total = 0;
 #pragma unroll 8
-                for (int j = 0; j < groups; ++j) total += lds[n * kThreads + j * lanes + (o & (lanes - 1))];
-                if (i >= 0) ((T*)p.work)[((int64_t)slot * p.heads + h0 + k) * p.d_pad + i] = total;
-            }
+        for (int j = 0; j < groups; ++j) total += lds[n * kThreads + j * lanes + (o & (lanes - 1))];
+        if (i >= 0) ((T*)p.work)[((int64_t)slot * p.heads + h) * p.d_pad + i] = total;
     }
 }
 
@@ -307,6 +295,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void rotary_dw(Rot 
     const int64_t count = shared_weight ? (int64_t)slots * p.heads : slots;
     double sum = 0.0;
     if (d < p.d)
+#pragma unroll 8
         for (int64_t n = part; n < count; n += 4)
             sum += (double)((const T*)p.work)[(shared_weight ? n : n * p.heads + head) * p.d_pad + d];
     lds[part][threadIdx.x & 63] = sum;
@@ -340,12 +329,12 @@ bool wide_of(const Rot& p) {
            quads(p.dy, p.dy_stride, 3, item) && quads(p.weight, &p.weight_stride, 1, item);
 }
 
-// Blocks for each pair of heads in the gradient: up to 2048 in all (8 for a compute unit), and two tokens
-// for each group, so that the parts of dw, a row for each block and head, stay below a thirtieth of dx
+// Blocks for each head in the gradient: up to 2048 in all (8 for a compute unit), and two tokens for each group:
+// with one the parts of dw, a row for each block, are twice as many and their sum takes twice as long (10 us for 5)
 int grad_slots(const Rot& p) {
-    const int64_t sets = p.heads ? (p.heads + kHeads - 1) / kHeads : 1, groups = kThreads >> lanes_log_of(p);
+    const int64_t groups = kThreads >> lanes_log_of(p);
     const int64_t runs = ((int64_t)p.batch * p.rows + groups - 1) / groups;
-    int64_t slots = 2048 / sets;
+    int64_t slots = 2048 / (p.heads ? p.heads : 1);
     if (slots > (runs + 1) / 2) slots = (runs + 1) / 2;
     return slots < 1 ? 1 : (int)slots;
 }
@@ -366,7 +355,7 @@ template <typename T> void launch_rotary(const Rot& p, hipStream_t s) {
 
 template <typename T> void launch_rotary_grad(const Rot& p, hipStream_t s) {
     const int log = lanes_log_of(p), slots = grad_slots(p);
-    const unsigned blocks = (unsigned)(((p.heads + kHeads - 1) / kHeads) * slots);
+    const unsigned blocks = (unsigned)(p.heads * slots);
     const unsigned lds = 16 * kThreads * sizeof(T);
     if (!blocks) {      // no heads: a weight for all of them has a gradient of zeros
     } else if (wide_of(p))
