@@ -672,41 +672,33 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
 // waves in turn, and its loads are the operands of v_mfma_f32_16x16x4f32 as they come (K: lane = key,
 // 16 bytes of its row; V: 16 neighbouring bytes of four rows each).  Key ranges of one sequence go to
 // `splits` blocks, whose results are joined by `attention_join`.
-template <int NB, int NQ, bool WIDE>
-__global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, float* part, float* part_lse) {
+template <int NB, bool WIDE>
+__global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, int sets, float* part, float* part_lse) {
     constexpr int KS = 4 * NB;                 // 16-byte steps of a key row for each quarter of the wave
     __shared__ __attribute__((aligned(16))) float merged[4][16][64 * NB + 4];
     __shared__ float stat[4][2][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, h = lane >> 4;
     const int heads = a.batch * a.hkv;
-    const int head = blockIdx.x % heads, split = blockIdx.x / heads;
+    int id = blockIdx.x;
+    const int head = id % heads;
+    id /= heads;
+    const int set = id % sets, split = id / sets;          // (sets of one range together: the others find its keys in L2)
     const int b = head / a.hkv, kh = head % a.hkv, group = a.hq / a.hkv;
     const Seq s = sequence(a, b);
     constexpr bool wide = WIDE;       // (apart, for the size of the code: short calls wait for it)
     const int rows = group * a.lq;
 
-    f32x4 own[NQ][KS];
-    int lim[NQ], pos[NQ], doc[NQ];
-    float slope2[NQ];
-    int top = 0, low = 0x7fffffff;
+    const int row = 16 * set + col;
+    const bool valid = row < rows;
+    const int g = valid ? row / a.lq : 0, i = valid ? row - g * a.lq : 0, qh = kh * group + g;
+    const int pos = s.start + i, lim = valid ? row_limit(a, s, pos) : 0;
+    const int doc = s.docs && lim > 0 ? s.docs[pos] : 0;
+    const float slope2 = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
+    const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
+    f32x4 own[KS];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int r = 16 * n + col;
-        const bool valid = r < rows;
-        const int g = valid ? r / a.lq : 0, i = valid ? r - g * a.lq : 0, qh = kh * group + g;
-        pos[n] = s.start + i;
-        lim[n] = valid ? row_limit(a, s, pos[n]) : 0;
-        doc[n] = s.docs && lim[n] > 0 ? s.docs[pos[n]] : 0;
-        slope2[n] = a.slopes ? a.slopes[qh] * kLog2e : 0.f;
-        const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
-#pragma unroll
-        for (int t = 0; t < KS; ++t) {
-            own[n][t] = load4(qrow, 16 * t + 4 * h, a.d, valid, wide);
-            own[n][t] *= a.scale;
-        }
-        top = max(top, lim[n]);
-        low = min(low, valid ? lim[n] : 0x7fffffff);
-    }
+    for (int t = 0; t < KS; ++t) own[t] = load4(qrow, 16 * t + 4 * h, a.d, valid, wide) * a.scale;
+    int top = lim, low = valid ? lim : 0x7fffffff;
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) {
         top = max(top, __shfl_xor(top, m));
@@ -716,16 +708,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
     const float* kbase = a.k + b * a.k_stride[0] + kh * a.k_stride[1];
     const float* vbase = a.v + b * a.v_stride[0] + kh * a.v_stride[1];
 
-    f32x4 acc[NQ][NB][4];
-    float most[NQ], total[NQ];
+    f32x4 acc[NB][4];
+    float most = -__builtin_inff(), total = 0.f;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        most[n] = -__builtin_inff(), total[n] = 0.f;
+    for (int e = 0; e < NB; ++e)
 #pragma unroll
-        for (int e = 0; e < NB; ++e)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[n][e][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+        for (int c = 0; c < 4; ++c) acc[e][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     f32x4 kx[KS], vx[4][NB];
     // Past the end of the range and of the row the last values are read again: such keys do not count, and such
     // elements meet zeros of q or are not stored.
@@ -771,53 +759,46 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
 #pragma unroll
                 for (int c = 0; c < 4; ++c) kx[t][c] = finite_(kx[t][c]) ? kx[t][c] : 0.f;
         }
-        f32x4 x[NQ];
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            x[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < KS; ++t)
 #pragma unroll
-            for (int t = 0; t < KS; ++t)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[t][c], own[n][t][c], x[n], 0, 0, 0);
-        }
+            for (int c = 0; c < 4; ++c) x = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[t][c], own[t][c], x, 0, 0, 0);
         if (j1 < end) fetch_keys(j1);         // (values follow when they are used up: each is a step ahead)
         const bool whole = j0 + 16 <= low && !s.docs && !kmask;
+        float peak = most;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            float peak = most[n];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int j = j0 + 4 * h + v;
-                float z = score(a, x[n][v], slope2[n], pos[n], j);
-                if (!whole) {
-                    if (kmask >> (4 * h + v) & 1) z = __builtin_nanf("");
-                    bool ok = j < lim[n] && j < end;
-                    if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc[n];
-                    z = ok ? z : -__builtin_inff();
-                }
-                x[n][v] = z;
-                peak = z > peak || z != z ? z : peak;
+        for (int v = 0; v < 4; ++v) {
+            const int j = j0 + 4 * h + v;
+            float z = score(a, x[v], slope2, pos, j);
+            if (!whole) {
+                if (kmask >> (4 * h + v) & 1) z = __builtin_nanf("");
+                bool ok = j < lim && j < end;
+                if (s.docs) ok = ok && s.docs[j < s.len ? j : 0] == doc;
+                z = ok ? z : -__builtin_inff();
             }
+            x[v] = z;
+            peak = z > peak || z != z ? z : peak;
+        }
 #pragma unroll
-            for (int m = 16; m < 64; m <<= 1) {
-                const float other = __shfl_xor(peak, m);
-                peak = other > peak || other != other ? other : peak;
-            }
-            const float ref = peak == -__builtin_inff() ? 0.f : peak;
-            const float shrink = exp2_(most[n] - ref);
-            if (__any(shrink != 1.f)) {
-                total[n] *= shrink;
+        for (int m = 16; m < 64; m <<= 1) {
+            const float other = __shfl_xor(peak, m);
+            peak = other > peak || other != other ? other : peak;
+        }
+        const float ref = peak == -__builtin_inff() ? 0.f : peak;
+        const float shrink = exp2_(most - ref);
+        if (__any(shrink != 1.f)) {
+            total *= shrink;
 #pragma unroll
-                for (int e = 0; e < NB; ++e)
+            for (int e = 0; e < NB; ++e)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[n][e][c] *= shrink;
-            }
-            most[n] = peak;
+                for (int c = 0; c < 4; ++c) acc[e][c] *= shrink;
+        }
+        most = peak;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                x[n][v] = exp2_(x[n][v] - ref);
-                total[n] += x[n][v];
-            }
+        for (int v = 0; v < 4; ++v) {
+            x[v] = exp2_(x[v] - ref);
+            total += x[v];
         }
         // values that are not finite become zeros here and are added by themselves below
         unsigned vbad = 0;
@@ -836,14 +817,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
             for (int m = 1; m < 64; m <<= 1) vbad |= __shfl_xor(vbad, m);
         }
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+        for (int e = 0; e < NB; ++e)
 #pragma unroll
-            for (int e = 0; e < NB; ++e)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        acc[n][e][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[v][e][c], x[n][v], acc[n][e][c], 0, 0, 0);
+                for (int v = 0; v < 4; ++v) acc[e][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[v][e][c], x[v], acc[e][c], 0, 0, 0);
         if (j1 < end) fetch_values(j1);
         for (unsigned m = vbad; m; m &= m - 1) {
             const int key = __builtin_ctz(m);
@@ -851,93 +829,83 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
             int hh = h;
             asm volatile("" : "+v"(hh));             // (nothing of this is computed ahead and kept)
             const float* vrow = vbase + (int64_t)(j0 + key) * a.v_stride[2];
+            float mine = 0.f;
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                float mine = 0.f;
+            for (int v = 0; v < 4; ++v) mine = v == (key & 3) ? x[v] : mine;
+            const float weight = __shfl(mine, col + 16 * (key >> 2));
 #pragma unroll
-                for (int v = 0; v < 4; ++v) mine = v == (key & 3) ? x[n][v] : mine;
-                const float weight = __shfl(mine, col + 16 * (key >> 2));
+            for (int e = 0; e < NB; ++e)
 #pragma unroll
-                for (int e = 0; e < NB; ++e)
+                for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            const int d = 64 * e + 4 * (4 * hh + v) + c;
-                            const float y = vrow[d < a.d ? d : 0], z = weight * y;
-                            acc[n][e][c][v] += !finite_(y) && d < a.d && weight != 0.f ? z : 0.f;
-                        }
-            }
+                    for (int v = 0; v < 4; ++v) {
+                        const int d = 64 * e + 4 * (4 * hh + v) + c;
+                        const float y = vrow[d < a.d ? d : 0], z = weight * y;
+                        acc[e][c][v] += !finite_(y) && d < a.d && weight != 0.f ? z : 0.f;
+                    }
         }
         j0 = j1;
     }
 
-    // the four waves' results, one group of 16 rows at a time
+    // the four waves' results
+    float sum = total;
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (h == 0) stat[wave][0][col] = most, stat[wave][1][col] = sum;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        float sum = total[n];
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        if (n) __syncthreads();
-        if (h == 0) stat[wave][0][col] = most[n], stat[wave][1][col] = sum;
+    for (int e = 0; e < NB; ++e)
 #pragma unroll
-        for (int e = 0; e < NB; ++e)
+        for (int v = 0; v < 4; ++v) {
+            f32x4 x;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                f32x4 x;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[c] = acc[n][e][c][v];
-                *(f32x4*)&merged[wave][col][64 * e + 4 * (4 * h + v)] = x;
-            }
-        __syncthreads();
-        const int q = threadIdx.x >> 4;             // 16 threads for each row
-        const int r = 16 * n + q;
-        if (r < rows) {
-            float peak = -__builtin_inff();
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float z = stat[w][0][q];
-                peak = z > peak || z != z ? z : peak;
-            }
-            const float ref = peak == -__builtin_inff() ? 0.f : peak;
-            float f[4], sum4 = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                f[w] = exp2_(stat[w][0][q] - ref);
-                sum4 += f[w] * stat[w][1][q];
-            }
-            const float by = sum4 > 0.f ? 1.f / sum4 : sum4 == 0.f ? 0.f : sum4;
-            const float lse = sum4 == 0.f ? -__builtin_inff() : (peak + __builtin_amdgcn_logf(sum4)) * kLn2;
-            const int g = r / a.lq, i = r - g * a.lq, qh = kh * group + g;
-            const int64_t prow = (((int64_t)split * a.batch + b) * a.hq + qh) * a.lq + i;
-            float* row = part ? part + prow * a.d : a.o + b * a.o_stride[0] + qh * a.o_stride[1] + i * a.o_stride[2];
-            const int at = threadIdx.x & 15;
-#pragma unroll
-            for (int e = 0; e < NB; ++e) {
-                const int d = 64 * e + 4 * at;
-                f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const f32x4 y = *(const f32x4*)&merged[w][q][d];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) x[c] += f[w] == 0.f ? 0.f : f[w] * y[c];
-                }
-                x *= by;
-                if (wide) {
-                    if (d < a.d) *(f32x4*)(row + d) = x;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (d + c < a.d) row[d + c] = x[c];
-                }
-            }
-            if (at == 0) {
-                if (part)
-                    part_lse[prow] = lse;
-                else if (a.lse)
-                    a.lse[((int64_t)b * a.hq + qh) * a.lq + i] = lse;
-            }
+            for (int c = 0; c < 4; ++c) x[c] = acc[e][c][v];
+            *(f32x4*)&merged[wave][col][64 * e + 4 * (4 * h + v)] = x;
         }
+    __syncthreads();
+    const int q = threadIdx.x >> 4, r = 16 * set + q;        // 16 threads for each row
+    if (r >= rows) return;
+    float peak = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float z = stat[w][0][q];
+        peak = z > peak || z != z ? z : peak;
+    }
+    const float ref = peak == -__builtin_inff() ? 0.f : peak;
+    float f[4], sum4 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = exp2_(stat[w][0][q] - ref);
+        sum4 += f[w] * stat[w][1][q];
+    }
+    const float by = sum4 > 0.f ? 1.f / sum4 : sum4 == 0.f ? 0.f : sum4;
+    const float lse = sum4 == 0.f ? -__builtin_inff() : (peak + __builtin_amdgcn_logf(sum4)) * kLn2;
+    const int og = r / a.lq, oi = r - og * a.lq, oh = kh * group + og, at = threadIdx.x & 15;
+    const int64_t prow = (((int64_t)split * a.batch + b) * a.hq + oh) * a.lq + oi;
+    float* to = part ? part + prow * a.d : a.o + b * a.o_stride[0] + oh * a.o_stride[1] + oi * a.o_stride[2];
+#pragma unroll
+    for (int e = 0; e < NB; ++e) {
+        const int d = 64 * e + 4 * at;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const f32x4 y = *(const f32x4*)&merged[w][q][d];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[c] += f[w] == 0.f ? 0.f : f[w] * y[c];
+        }
+        x *= by;
+        if (wide) {
+            if (d < a.d) *(f32x4*)(to + d) = x;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (d + c < a.d) to[d + c] = x[c];
+        }
+    }
+    if (at == 0) {
+        if (part)
+            part_lse[prow] = lse;
+        else if (a.lse)
+            a.lse[((int64_t)b * a.hq + oh) * a.lq + oi] = lse;
     }
 }
 
@@ -1418,6 +1386,9 @@ bool aligned(const void* p, const int64_t* stride) {
     return (uintptr_t)p % 16 == 0 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
 }
 
+// Sets of 16 rows of a key head (one without rows, for the sizes of workspaces)
+int few_sets(const Args& a) { return a.lq ? (int)(((int64_t)(a.hq / a.hkv) * a.lq + 15) / 16) : 1; }
+
 int row_tiles(const Args& a) { return (int)(((int64_t)(a.hq / a.hkv) * a.lq + kRows - 1) / kRows); }
 
 // Which forward kernel, and into how many key ranges.  Few rows: up to 32 rows of a key head, where the
@@ -1433,7 +1404,7 @@ Plan plan_forward(const Args& a) {
     const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
     p.few = rows <= 32;
     p.waves = heads * ((rows + 255) / 256) >= 256 ? 8 : 4;
-    const int64_t blocks = heads * (p.few ? 1 : (rows + 32 * p.waves - 1) / (32 * p.waves));
+    const int64_t blocks = heads * (p.few ? few_sets(a) : (rows + 32 * p.waves - 1) / (32 * p.waves));
     int64_t splits;
     if (p.few) {
         splits = (512 + blocks - 1) / blocks;
@@ -1537,12 +1508,12 @@ template <int NT> void launch_rows(const Args& a, const Plan& p, const Packed& i
 }
 
 template <bool WIDE> void launch_few(const Args& a, const Plan& p, float* part, float* part_lse, hipStream_t s) {
-    const dim3 grid((unsigned)(a.batch * a.hkv * p.splits));
-    const bool two = (int64_t)(a.hq / a.hkv) * a.lq > 16;
+    const int sets = few_sets(a);
+    const dim3 grid((unsigned)(a.batch * a.hkv * sets * p.splits));
     if (a.d <= 64)
-        two ? attention_few<1, 2, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<1, 1, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
+        attention_few<1, WIDE><<<grid, kThreads, 0, s>>>(a, p, sets, part, part_lse);
     else
-        two ? attention_few<2, 2, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse) : attention_few<2, 1, WIDE><<<grid, kThreads, 0, s>>>(a, p, part, part_lse);
+        attention_few<2, WIDE><<<grid, kThreads, 0, s>>>(a, p, sets, part, part_lse);
 }
 
 template <int NT> void launch_grad(const Args& a, const Plan& p, const Parts& parts, const Packed& in, float* part, hipStream_t s) {
