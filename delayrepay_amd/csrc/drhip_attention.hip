@@ -667,8 +667,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
 }
 
 // ---- forward, few rows ----------------------------------------------------------------------
-// At most 16 NQ rows against a long key range (single tokens, with all query heads of a key head
-// together): bound by reading keys and values once.  No LDS: a wave takes 16 keys at a time, the blocks'
+// Single tokens, with all query heads of a key head together, and small calls: 16 rows to a block, against a
+// long key range bound by reading keys and values once.  No LDS: a wave takes 16 keys at a time, the blocks'
 // waves in turn, and its loads are the operands of v_mfma_f32_16x16x4f32 as they come (K: lane = key,
 // 16 bytes of its row; V: 16 neighbouring bytes of four rows each).  Key ranges of one sequence go to
 // `splits` blocks, whose results are joined by `attention_join`.
@@ -1387,12 +1387,17 @@ bool aligned(const void* p, const int64_t* stride) {
 }
 
 // Sets of 16 rows of a key head (one without rows, for the sizes of workspaces)
+constexpr int64_t kSmall16 = 25000000;       // (sets of 16 rows) x keys x elements
+
 int few_sets(const Args& a) { return a.lq ? (int)(((int64_t)(a.hq / a.hkv) * a.lq + 15) / 16) : 1; }
 
 int row_tiles(const Args& a) { return (int)(((int64_t)(a.hq / a.hkv) * a.lq + kRows - 1) / kRows); }
 
-// Which forward kernel, and into how many key ranges.  Few rows: up to 32 rows of a key head, where the
-// blocks of the other kernel would be mostly empty.  Blocks of eight waves share each tile among 256 rows, of
+// Which forward kernel, and into how many key ranges.  Up to 64 rows of a key head, and few rows times keys in
+// all, go to the kernel for few rows, whose blocks are smaller and whose operands are not packed first: 32
+// sequences of 4096 keys, 8 key heads of 128, 64 rows: 621 us, in the other kernel 848; 96 rows: 927 and 857; 32 heads of 128
+// with 256 rows and keys 24 us and 36, 512 60 and 50; 16 with 64 of 777 and head size 80 35 and 40, 128 54 and
+// 43.  With documents only the other one passes over tiles.  Its blocks of eight waves share each tile among 256 rows, of
 // four where that leaves compute units without a block.  Ranges: enough for a block on each compute unit (two,
 // as causal blocks are of unequal length; not with documents, whose rows see a part of the keys alone: 60 us
 // against 85 for three sequences of 1111), none shorter than 256 keys, whose work pays for joining.  For few rows,
@@ -1402,7 +1407,7 @@ Plan plan_forward(const Args& a) {
     Plan p;
     p.wide = a.d % 4 == 0 && aligned(a.q, a.q_stride) && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride) && aligned(a.o, a.o_stride);
     const int64_t rows = (int64_t)(a.hq / a.hkv) * a.lq, heads = (int64_t)a.batch * a.hkv;
-    p.few = rows <= 32;
+    p.few = rows <= 64 || (!a.documents && heads * few_sets(a) * a.lk * a.d <= kSmall16);
     p.waves = heads * ((rows + 255) / 256) >= 256 ? 8 : 4;
     const int64_t blocks = heads * (p.few ? few_sets(a) : (rows + 32 * p.waves - 1) / (32 * p.waves));
     int64_t splits;

@@ -192,6 +192,44 @@ def test_strides_and_alignment(lq):
         assert np.all(x.get()[..., :1] == 7) and np.all(x.get()[..., 49:] == 7)
 
 
+# the same for calls that are not small: more than 64 rows of a key head, and many of them in all
+LARGE = [(2, 16, 8, 80, 1301, 128), (2, 16, 8, 80, 2100, 81), (2, 16, 8, 80, 5000, 33), (1, 30, 10, 131, 3100, 32)]
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("size", LARGE, ids=str)
+def test_attention_and_its_gradient_of_many_rows(size, mask):
+    b, hq, hkv, lq, lk, d = size
+    q, g, k, v = _normal(lq + lk, (b, hq, lq, d), (b, hq, lq, d), (b, hkv, lk, d), (b, hkv, lk, d))
+    _check(q, k, v, g, **_mask(mask, b, hq, lq, lk))
+
+
+def test_many_rows_and_keys_that_do_not_count():
+    """Behind the length, later than the row, in rows without keys: what is not finite stays where it is."""
+    b, hq, hkv, lq, lk, d = 2, 16, 8, 80, 1300, 128
+    q, g, k, v = _normal(23, (b, hq, lq, d), (b, hq, lq, d), (b, hkv, lk, d), (b, hkv, lk, d))
+    lengths = np.array([1250, 0], np.int32)
+    k[0, :, 1250:], v[0, :, 1250:] = INF, NAN
+    k[1], v[1], q[1], g[1] = NAN, -INF, INF, NAN
+    o, lse = _check(q, k, v, g, lengths=lengths, causal=True)
+    assert not o.get()[1].any() and np.all(lse.get()[1] == -np.inf)
+    clean = nn_oracle.attention(q, k, v, causal=True, lengths=lengths)
+    # a key that the last row alone sees, and a value that is infinite in one column
+    k[0, 1, 1249] = NAN
+    v[0, 2, 1249, 70] = -INF
+    dev = [_put(x) for x in (q, k, v)]
+    o, lse = nn.attention(*dev, causal=True, lengths=_put(lengths), with_lse=True)
+    got = o.get()
+    assert np.isnan(got[0, 2:4, -1]).all() and np.all(got[0, 4:6, -1, 70] == -INF)
+    keep = np.ones(got.shape, bool)
+    keep[0, 2:4, -1] = False
+    keep[0, 4:6, -1, 70] = False
+    _near(np.where(keep, got, 0), np.where(keep, clean["o"], 0), np.where(keep, clean["o_off"], 0), "o")
+    dq, dk, dv = (x.get() for x in nn.attention_grad(_put(g), *dev, o, lse, causal=True, lengths=_put(lengths)))
+    assert np.isfinite(dq[0, :, :-1]).all() and not dq[1].any() and not dk[1].any() and not dv[1].any()
+    assert np.isnan(dq[0, 2:4, -1]).any() and np.isfinite(dk[0, 3:]).all() and np.isfinite(dv[0, 3:]).all()
+
+
 def test_options_that_follow_each_other():
     """What is remembered of a call's geometry is told apart by every option of it."""
     q, k, v, g = _normal(21, (2, 2, 5, 16), (2, 2, 9, 16), (2, 2, 9, 16), (2, 2, 5, 16))
