@@ -1361,25 +1361,34 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad(Args a, Args same,
         grad_dq<NT, CAP>(same, plan, row_tiles, same_in, blockIdx.x - keys, shared);
 }
 
-// dK and dV from the parts of the query heads, in their order; one row of one of them for each wave
-__global__ __launch_bounds__(kThreads) void attention_add(Args a, int parts, const float* part) {
+// dK and dV from the parts of the query heads, in their order: half a wave for one row of one of them, four
+// elements to a lane and four parts on their way.  Bound by memory.
+__global__ __launch_bounds__(kThreads) void attention_add(Args a, int parts, int wide, const float* part) {
     const int64_t rows = (int64_t)a.batch * a.hkv * a.lk;
-    const int lane = threadIdx.x & 63;
-    int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int d = 4 * (threadIdx.x & 31);
+    int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
     if (row >= 2 * rows) return;
     const float* from = part + row * a.d;
-    float x0 = 0.f, x1 = 0.f;
-    for (int n = 0; n < parts; ++n, from += 2 * rows * a.d) {
-        if (lane < a.d) x0 += from[lane];
-        if (lane + 64 < a.d) x1 += from[lane + 64];
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int n0 = 0; n0 < parts; n0 += 4) {
+        f32x4 y[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) y[n] = load4(from + min(n0 + n, parts - 1) * 2 * rows * a.d, d, a.d, n0 + n < parts, wide);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) x += y[n];
     }
     const bool second = row >= rows;
     if (second) row -= rows;
     const int64_t* stride = second ? a.dv_stride : a.dk_stride;
     const int64_t bh = row / a.lk;
     float* to = (second ? a.dv : a.dk) + bh / a.hkv * stride[0] + bh % a.hkv * stride[1] + row % a.lk * stride[2];
-    if (lane < a.d) to[lane] = x0;
-    if (lane + 64 < a.d) to[lane + 64] = x1;
+    if (wide) {
+        if (d < a.d) *(f32x4*)(to + d) = x;
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (d + c < a.d) to[d + c] = x[c];
+    }
 }
 
 bool aligned(const void* p, const int64_t* stride) {
@@ -1537,7 +1546,7 @@ template <int NT> void launch_grad(const Args& a, const Plan& p, const Parts& pa
         attention_grad<NT, true><<<grid, kThreads, 0, s>>>(a, a, p, parts, in, in, tiles, dq_sets, sets, part);
     else
         attention_grad<NT, false><<<grid, kThreads, 0, s>>>(a, a, p, parts, in, in, tiles, dq_sets, sets, part);
-    if (a.lk && parts.count > 1) attention_add<<<dim3((unsigned)((2 * heads * a.lk + 3) / 4)), kThreads, 0, s>>>(a, parts.count, part);
+    if (a.lk && parts.count > 1) attention_add<<<dim3((unsigned)((2 * heads * a.lk + 7) / 8)), kThreads, 0, s>>>(a, parts.count, p.wide, part);
 }
 
 // Query heads of a key head go to blocks of their own where the keys alone give fewer than two blocks to a
