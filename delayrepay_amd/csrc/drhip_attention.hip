@@ -662,7 +662,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, 
     if (!valid) return;
     const float by = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;      // (a NaN stays one)
     const float lse = total == 0.f ? -__builtin_inff() : (most + __builtin_amdgcn_logf(total)) * kLn2;
-    if (part) {
+    if (split && lim <= plan.chunk) return;              // (the first range has all of the row's keys)
+    if (part && lim > plan.chunk) {
         const int64_t row = (((int64_t)split * a.batch + b) * a.hq + qh) * a.lq + i;
         if (total != 0.f) store_column<NT>(part + row * a.d, acc, by, a.d, wide, h);     // (the join reads no others)
         if (h == 0) part_lse[row] = lse;
@@ -917,13 +918,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
     }
 }
 
-// Results of `splits` key ranges into one, four elements to a lane.  Up to kNear ranges: half a wave for each row, all
-// loads at once (65536 rows of 128 in two ranges: 21 us, 4.8 TB/s; a wave for each row, which first finds the
-// largest sum, 42).  More: a block for each row, whose eight halves of waves take the ranges in turn (32 rows in
+// Results of key ranges into one (of many rows, those with keys in more than the first), four elements to a lane.  Up to kNear ranges: half a wave for each row, all
+// loads at once (65536 causal rows of 128 in two ranges, half of them with keys in both: 15 us; if all are joined
+// 21, 4.8 TB/s; a wave for each row, which first finds the largest sum, 42).  More: a block for each row, whose eight halves of waves take the ranges in turn (32 rows in
 // 40 ranges 4.7 us, with one wave 6.4).
 constexpr int kNear = 4;
 
-template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(Args a, int splits, int wide, const float* part, const float* part_lse) {
+template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(Args a, Plan plan, const float* part, const float* part_lse) {
     constexpr int HALVES = NEAR ? 1 : kThreads / 32, BATCH = NEAR ? kNear : 8;
     __shared__ f32x4 sums[HALVES][32];
     __shared__ float totals[HALVES];
@@ -931,6 +932,12 @@ template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(
     const int half = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
     const int64_t row = NEAR ? (int64_t)blockIdx.x * (kThreads / 32) + half : blockIdx.x;
     if (NEAR && row >= rows) return;
+    const int i = (int)(row % a.lq), splits = plan.splits, wide = plan.wide;
+    const int64_t bh = row / a.lq;
+    if (!plan.few) {
+        const Seq s = sequence(a, (int)(bh / a.hq));
+        if (row_limit(a, s, s.start + i) <= plan.chunk) return;      // (one range alone, and its result is where it belongs)
+    }
     const int first = NEAR ? 0 : half;
     float lse[BATCH], peak = -__builtin_inff(), sum = 0.f;
     f32x4 y[BATCH], x = {0.f, 0.f, 0.f, 0.f};
@@ -983,8 +990,6 @@ template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(
         }
     }
     const float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    const int i = (int)(row % a.lq);
-    const int64_t bh = row / a.lq;
     float* to = a.o + bh / a.hq * a.o_stride[0] + bh % a.hq * a.o_stride[1] + i * a.o_stride[2];
     if (wide) {
         if (d < a.d) *(f32x4*)(to + d) = x * by;
@@ -1605,9 +1610,9 @@ extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
     if (e != hipSuccess) return (int)e;
     if (p.splits > 1) {
         if (p.splits <= kNear)
-            attention_join<true><<<dim3((unsigned)((rows + 7) / 8)), kThreads, 0, s>>>(a, p.splits, p.wide, part, part_lse);
+            attention_join<true><<<dim3((unsigned)((rows + 7) / 8)), kThreads, 0, s>>>(a, p, part, part_lse);
         else
-            attention_join<false><<<dim3((unsigned)rows), kThreads, 0, s>>>(a, p.splits, p.wide, part, part_lse);
+            attention_join<false><<<dim3((unsigned)rows), kThreads, 0, s>>>(a, p, part, part_lse);
         e = hipGetLastError();
     }
     return (int)e;
