@@ -509,8 +509,8 @@ struct Active {
 // per column of its accumulators: S^T = K Q^T leaves the scores of a row in one lane pair, so the softmax
 // needs one exchange, and P^T in the layout that O^T += V^T P^T reads.
 // Keys and values come 32 at a time from the packed planes through LDS, two buffers, copied a tile ahead.
-// Bound by the matrix units: 32 heads, 4096 rows of 128, causal: 620 us, 222 TFLOP/s of float32 products (a large
-// product of f32 matrices reaches 155), 1.33 PFLOP/s of bfloat16 ones, of which the card holds 2.0 with nothing else to do.  Two waves on a SIMD fill each other's waits; four-wave blocks, two on a compute unit, read each tile twice as
+// Bound by the matrix units: 32 heads, 4096 rows of 128, causal: 640 us, 215 TFLOP/s of float32 products (a large
+// product of f32 matrices reaches 155), 1.29 PFLOP/s of bfloat16 ones, of which the card holds 2.0 with nothing else to do.  Two waves on a SIMD fill each other's waits; four-wave blocks, two on a compute unit, read each tile twice as
 // often from L2 (695 for 639 us).  With a cap a tanh for each pair comes on top (8 heads, 8192 rows: 720 us).
 template <int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, Packed in, float* part, float* part_lse) {
@@ -1006,7 +1006,7 @@ template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(
 // dQ (rows own their sums, keys pass by, as in the forward kernel) and dK, dV (keys own their sums, rows pass
 // by).  The scores are computed in both: seven products instead of five.  A wave holds two matrices of 32
 // columns in planes and its sums, more than 256 registers, so there is one for each SIMD, and what it does on
-// the vector unit stands between its matrix instructions.  Bound by the matrix units, which are busy for half
+// the vector unit stands between its matrix instructions.  Bound by the matrix units, which are busy for 54%
 // of the time: 2 sequences of 2048 rows, 16 heads of 128, causal: 702 us, 171 TFLOP/s of float32 products.
 template <int NT> struct GradLds {
     __attribute__((aligned(16))) char tile[2][2 * Planes<NT>::BYTES];

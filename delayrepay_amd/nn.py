@@ -21,7 +21,7 @@ from . import backend as be
 from .delayarray import DelayArray, NPArray
 
 _backend = be.backend
-_ops = _backend.operators
+_ops = getattr(_backend, "operators", None)
 _F32 = numpy.dtype(numpy.float32)
 _F64 = numpy.dtype(numpy.float64)
 _INTS = (numpy.dtype(numpy.int32), numpy.dtype(numpy.int64))
