@@ -452,6 +452,21 @@ def test_sample_with_parameters_for_each_row():
     assert nn.sample(dr.array(np.zeros((0, 5), f)), dr.array(np.zeros(0))).shape == (0,)
 
 
+@pytest.mark.parametrize("how", [dict(top_k=1), dict(top_k=50, top_p=0.9, temperature=0.8), dict(top_k=255), dict(top_k=257), dict(top_k=3000, min_p=0.01), dict(top_p=0.95), dict()], ids=str)
+@pytest.mark.parametrize("vocabulary", [65535, 70001, 131072])
+def test_sample_of_long_rows(vocabulary, how):
+    """Beginnings that the first part of the row says much about, little, and nothing."""
+    rs = np.random.RandomState(vocabulary)
+    logits = (rs.standard_normal((6, vocabulary)) * 2.5).astype(np.float32)
+    logits[1] = np.sort(logits[1])                         # the largest come last
+    logits[2] = np.sort(logits[2])[::-1]
+    logits[3] = np.round(logits[3])                        # many equal ones
+    logits[4, :20000] = NAN                                # fewer than k in the first part
+    logits[5] = -np.inf
+    logits[5, [5, 17000, vocabulary - 1]] = [1.0, 2.0, 2.0]
+    _draws(logits, rs.rand(6), **how)
+
+
 @pytest.mark.parametrize("vocabulary", [40, 5000])
 def test_sample_with_parameters_at_their_ends(vocabulary):
     """Out of range in an array: the nearest in it.  The smallest temperatures leave the largest logits."""
