@@ -11,8 +11,8 @@ _F32 = numpy.dtype(numpy.float32)
 
 
 def _dense(x):
-    """The array, copied if its last axis is not dense (or an index array not dense at all)."""
-    return x.copy() if x.shape[-1] > 1 and x._strides[-1] != 1 else x
+    """The array, copied if its last axis is not dense."""
+    return x if x._strides[-1] == 1 or x.shape[-1] <= 1 else x.copy()
 
 
 def _strides(x):
@@ -51,6 +51,13 @@ def _apart(x, others):
 def _places(outs, shapes, dtype, used, same=None):
     """Arrays to compute into: the ones asked for, or new ones where those are not dense
     in their last axis or share memory with an operand (`same`: one that may be exactly the output)."""
+    if len(outs) == 1 and outs[0] is not None and outs[0]._strides[-1] == 1:       # (the common call first)
+        a, n = outs[0].buf.ptr, outs[0].buf.nbytes
+        for y in used:
+            if y is not None and a < y.buf.ptr + y.buf.nbytes and y.buf.ptr < a + n:
+                break
+        else:
+            return [outs[0]]
     places = []
     for i, (out, shape) in enumerate(zip(outs, shapes)):
         if out is None:
@@ -112,6 +119,12 @@ def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
     def index(x):
         return _contiguous(x) if isinstance(x, ndarray) else None
     lengths, start, prefix = how.lengths, how.start, how.prefix
+    if how.plain and not grad:         # (the same with less to do: a short call is bound by this)
+        fields = (q.ptr, k.ptr, v.ptr, o.ptr, 0 if lse is None else lse.ptr, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        plain = (q.shape, q._strides, k.shape, k._strides, v._strides, o._strides, how.causal, "last" if start is None else start, how.scale, how.cap)
+        plan = _PLANS.get(plain)
+        if plan is not None:
+            return _run(func, hiprt.ATTENTION_HEAD, fields, plan, used, written)
     if isinstance(lengths, int):       # a number: the rows behind it do not exist
         k, v = k[:, :, :lengths], v[:, :, :lengths]
     documents = None if how.documents is None else _dense(how.documents)
@@ -133,14 +146,18 @@ def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
                 min(prefix, lk) if isinstance(prefix, int) else 0,
                 how.scale, how.cap or 0.0)
     plan = _plan(key, hiprt.ATTENTION_HEAD, hiprt.ATTENTION_TAIL, fields, make, lambda args: hiprt.attention_work(args, grad))
+    if how.plain and not grad:
+        _PLANS[plain] = plan
     _run(func, hiprt.ATTENTION_HEAD, fields, plan, used + [x for x in arrays if x is not None], written)
 
 
 def attention(q, k, v, how, outs):
     q, k, v = _dense(q), _dense(k), _dense(v)
-    masks = [how.documents, how.slopes] + [x for x in (how.lengths, how.start, how.prefix) if isinstance(x, ndarray)]
+    operands = [q, k, v]
+    if not how.plain:
+        operands += [how.documents, how.slopes] + [x for x in (how.lengths, how.start, how.prefix) if isinstance(x, ndarray)]
     shapes = [q.shape, q.shape[:3]][:len(outs)]
-    places = _places(outs, shapes, _F32, [q, k, v] + masks)
+    places = _places(outs, shapes, _F32, operands)
     if len(places) > 1 and not places[1].is_contiguous:
         places[1] = ndarray(shapes[1], _F32)
     _attention(hiprt.attention, False, q, k, v, places[0], places[1] if len(places) > 1 else None, None, (None, None, None), how, [q, k, v], places)

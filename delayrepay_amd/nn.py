@@ -94,6 +94,11 @@ def _targets(out, shapes, dtypes):
     """The arrays that `out` names, ready to be written to; Nones without it."""
     if out is None:
         return [None] * len(shapes)
+    if type(out) is NPArray and len(shapes) == 1:
+        arr = out.array
+        if arr.shape == shapes[0] and arr.dtype is dtypes[0] and 0 not in getattr(arr, "_strides", (0,)):
+            out._written()
+            return [arr]
     outs = [out] if not isinstance(out, (tuple, list)) else list(out)
     if len(outs) != len(shapes):
         raise ValueError(f"out names {len(shapes)} array{'s' if len(shapes) > 1 else ''}, not {len(outs)}")
@@ -134,19 +139,27 @@ def _results(out, arrays):
 class _Mask:
     """Checked arguments that say which pairs count and how their scores are made."""
 
-    __slots__ = ("scale", "causal", "start", "lengths", "prefix", "documents", "slopes", "cap")
+    __slots__ = ("scale", "causal", "start", "lengths", "prefix", "documents", "slopes", "cap", "plain")
 
     def __init__(self, q, k, scale, causal, start, lengths, prefix, documents, slopes, cap):
         batch, lk = k.shape[0], k.shape[2]
+        # a part of the key row's own or of the arguments an array: not a plain call
+        self.plain = lengths is None and prefix is None and documents is None and slopes is None and (start is None or type(start) is int)
         self.scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else _number(scale, "scale")
         if abs(self.scale) > _LARGE:
             raise ValueError(f"scale lies within 2**100 of 0, not at {self.scale:g}")
         if not isinstance(causal, (bool, numpy.bool_)):
             raise TypeError("causal is True or False")
         self.causal = bool(causal)
+        self.cap = None if cap is None else _number(cap, "cap", 0.0, above=True)
+        if cap is not None and not 1 / _LARGE <= self.cap <= _LARGE:
+            raise ValueError(f"cap lies between 2**-100 and 2**100, not at {self.cap:g}")
         self.start = _integers(start, "start", (batch,))
         if isinstance(self.start, int) and abs(self.start) > _FAR:
             raise ValueError(f"start lies within 2**30 of 0, not at {self.start}")
+        if self.plain:
+            self.lengths = self.prefix = self.documents = self.slopes = None
+            return
         self.lengths = _integers(lengths, "lengths", (batch,))
         if isinstance(self.lengths, int) and not 0 <= self.lengths <= lk:
             raise ValueError(f"lengths lies in [0, {lk}], the rows of k, not {self.lengths}")
@@ -157,9 +170,6 @@ class _Mask:
             raise ValueError(f"prefix is at least 0, not {self.prefix}")
         self.documents = _integers(documents, "documents", (batch, lk), number=False)
         self.slopes = None if slopes is None else _shaped(_floats(slopes, "slopes", 1), "slopes", (q.shape[1],))
-        self.cap = None if cap is None else _number(cap, "cap", 0.0, above=True)
-        if cap is not None and not 1 / _LARGE <= self.cap <= _LARGE:
-            raise ValueError(f"cap lies between 2**-100 and 2**100, not at {self.cap:g}")
 
 
 def _heads(q, k, v):
