@@ -7,7 +7,7 @@ import numpy
 from . import hip, hiprt
 from .devarray import Buffer, ndarray
 
-_F32 = numpy.dtype(numpy.float32)
+_F32, _I64 = numpy.dtype(numpy.float32), numpy.dtype(numpy.int64)
 
 
 def _dense(x):
@@ -90,15 +90,19 @@ _PLANS = {}
 _PLANS_MAX = 1024
 
 
+def _remember(key, plan):
+    if len(_PLANS) >= _PLANS_MAX:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
+
+
 def _plan(key, head, tail, fields, make, work_of):
     """The remembered plan, or a new one: `make()` gives the tail's fields, work_of(args) the workspace."""
     plan = _PLANS.get(key)
     if plan is None:
         packed = tail.pack(*make())
-        plan = packed, work_of(head.pack(*fields, 0, 0) + packed)
-        if len(_PLANS) >= _PLANS_MAX:
-            _PLANS.clear()
-        _PLANS[key] = plan
+        plan = _remember(key, (packed, work_of(head.pack(*fields, 0, 0) + packed)))
     return plan
 
 
@@ -147,7 +151,7 @@ def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
                 how.scale, how.cap or 0.0)
     plan = _plan(key, hiprt.ATTENTION_HEAD, hiprt.ATTENTION_TAIL, fields, make, lambda args: hiprt.attention_work(args, grad))
     if how.plain and not grad:
-        _PLANS[plain] = plan
+        _remember(plain, plan)
     _run(func, hiprt.ATTENTION_HEAD, fields, plan, used + [x for x in arrays if x is not None], written)
 
 
@@ -224,14 +228,21 @@ def rotary_grad(dy, x, how, outs):
 def sample(logits, uniforms, temperature, top_k, top_p, min_p, outs):
     logits, uniforms = _dense(logits), _contiguous(uniforms)
     batch, vocabulary = logits.shape
-
-    def either(x):
-        return (_contiguous(x), 0) if isinstance(x, ndarray) else (None, x)
-    (t, t_all), (k, k_all), (p, p_all), (m, m_all) = (either(x) for x in (temperature, top_k, top_p, min_p))
-    used = [x for x in (logits, uniforms, t, k, p, m) if x is not None]
-    places = _places(outs, [(batch,)], numpy.dtype(numpy.int64), used)
-    one = 2.0 ** min(52, 62 - max(1, (vocabulary - 1).bit_length()))      # (float64 holds it)
-    args = hiprt.SAMPLE_HEAD.pack(logits.ptr, uniforms.ptr, places[0].ptr, _ptr(t), _ptr(p), _ptr(m), _ptr(k)) \
-        + hiprt.SAMPLE_TAIL.pack(logits._strides[0], t_all, p_all, m_all, one, min(k_all, vocabulary), batch, vocabulary, int(uniforms.dtype.itemsize == 8))
+    used, places_of = [logits, uniforms], [0, 0, 0, 0]
+    numbers = (temperature, top_p, min_p, top_k)
+    if ndarray in (type(temperature), type(top_p), type(min_p), type(top_k)):
+        arrays = [_contiguous(x) if isinstance(x, ndarray) else None for x in numbers]
+        numbers = tuple(0 if isinstance(x, ndarray) else x for x in numbers)
+        places_of = [_ptr(x) for x in arrays]
+        used += [x for x in arrays if x is not None]
+    places = _places(outs, [(batch,)], _I64, used)
+    key = (logits._strides[0], batch, vocabulary, uniforms.dtype.itemsize, numbers)
+    tail = _PLANS.get(key)
+    if tail is None:
+        t, p, m, k = numbers
+        one = 2.0 ** min(52, 62 - max(1, (vocabulary - 1).bit_length()))      # (float64 holds it)
+        tail = hiprt.SAMPLE_TAIL.pack(logits._strides[0], t, p, m, one, min(k, vocabulary), batch, vocabulary, int(uniforms.dtype.itemsize == 8))
+        _remember(key, tail)
+    args = hiprt.SAMPLE_HEAD.pack(logits.ptr, uniforms.ptr, places[0].ptr, *places_of) + tail
     hip.issue_operator(hiprt.sample, args, used + places, places)
     return _give(outs, places)
