@@ -382,9 +382,9 @@ template <typename T> void launch_rotary_grad(const Rot& p, hipStream_t s) {
 // instead.  Weights are 64-bit whole numbers (the largest 2^s, s such that all fit, computed in float64), so that
 // sums do not depend on their order.
 //
-// 256 rows of 128000 with top-k 50: 43 us, half of it the first pass at memory's rate (131 MB).  One row of 32000
-// with top-p: 33 us on one compute unit, of which 9 are the weights of all tokens (float64, 13 products each), 7 the
-// kept ones' sums, 13 barriers and scans between the steps.
+// 256 rows of 128000 with top-k 50: 42 us, half of it the first pass at memory's rate (131 MB).  One row of 32000
+// with top-p: 31 us on one compute unit, of which 9 are the weights of all tokens (float64, 13 operations each), 7 the
+// kept ones' sums, 12 barriers and scans between the steps.
 
 typedef drhip_sample_t Smp;
 typedef unsigned long long u64;
@@ -948,18 +948,20 @@ __global__ __launch_bounds__(kDraw) void sample_kernel(Smp p) {
                     sum += weigh.whole_from(x, min_p);
                 });
             sum = wave_sum(sum);
-            tied = wave_sum(tied);
+            if (by_key) tied = wave_sum(tied);
             if (lane == 0) parts[c] = sum, marks[c] = tied;
         }
-    else
-        for (int c = threadIdx.x; c < chunks; c += kDraw) marks[c] = 0;
     __syncthreads();
     // the part and the token in which the draw falls
     const u64 each = by_key ? weigh.whole(value_of(cut_key)) : 0;
     const int c0 = 2 * threadIdx.x;
-    const unsigned t0 = c0 < chunks ? marks[c0] : 0, t1 = c0 + 1 < chunks ? marks[c0 + 1] : 0;
-    u64 every;
-    const u64 tied_before = scan(t0 + t1, lds, every);
+    unsigned t0 = 0, t1 = 0;
+    u64 every, tied_before = 0;
+    if (by_key) {
+        if (c0 < chunks) t0 = marks[c0];
+        if (c0 + 1 < chunks) t1 = marks[c0 + 1];
+        tied_before = scan(t0 + t1, lds, every);
+    }
     auto kept = [&](u64 from, u64 count) { return from >= ties ? 0 : (ties - from < count ? ties - from : count); };
     const u64 w0 = c0 < chunks ? parts[c0] + each * kept(tied_before, t0) : 0;
     const u64 w1 = c0 + 1 < chunks ? parts[c0 + 1] + each * kept(tied_before + t0, t1) : 0;
