@@ -513,7 +513,7 @@ struct Active {
 // product of f32 matrices reaches 155), 1.29 PFLOP/s of bfloat16 ones, of which the card holds 2.0 with nothing else to do.  Two waves on a SIMD fill each other's waits; four-wave blocks, two on a compute unit, read each tile twice as
 // often from L2 (695 for 639 us).  With a cap a tanh for each pair comes on top (8 heads, 8192 rows: 720 us).
 template <int NT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, Packed in, float* part, float* part_lse) {
+__global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, Packed in, float* part, float* part_lse) {
     using P = Planes<NT>;
     __shared__ __attribute__((aligned(16))) char lds[2][2 * P::BYTES];
     __shared__ int ends[WAVES], doc_range[2][WAVES];
