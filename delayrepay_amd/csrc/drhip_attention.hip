@@ -454,23 +454,31 @@ template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Arg
 // read of LDS, though that is one of the other buffer.  They have no result in registers; copies_done() and a
 // barrier stand before the first read of what they write.  (m0 is the compiler's own register, which these kernels
 // use for nothing else.)
-template <int WAVES> __device__ __forceinline__ void copy_to_lds(char* lds, const char* from, int bytes) {
+// The address is a base in scalar registers and 16 bytes for each lane, so that a copy costs no vector instructions
+// (the wait states are those between a vector instruction that writes a scalar register and a load that reads it).
+template <int WAVES, int BYTES> __device__ __forceinline__ void copy_to_lds(char* lds, const char* from) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    for (int at = wave * 1024; at < bytes; at += WAVES * 1024)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to + at)), "v"(from + at + lane * 16) : "memory");
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
+    const uint64_t base = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)from >> 32)) << 32 |
+                          (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)from);
+#pragma unroll
+    for (int n = 0; n < (BYTES / 1024 + WAVES - 1) / WAVES; ++n) {
+        const int at = (n * WAVES + wave) * 1024;
+        if (at < BYTES)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + at), "v"(lane * 16), "s"(base + at) : "memory");
+    }
 }
 
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// Whether the keys of a tile are of the lane's row's document, as bits in the order of the accumulator's registers
-__device__ __forceinline__ unsigned same_document(int key_docs, int doc, int h) {
+// Whether the tile's documents (one in each of 32 lanes, `range`: least and largest) are the lane's own, as bits in the
+// order of the accumulator's registers
+__device__ __forceinline__ unsigned same_document(int docs, int2 range, int doc, int h) {
+    if (range.x == range.y) return range.x == doc ? ~0u : 0u;
     unsigned m = 0;
+    asm volatile("" : "+v"(h));              // (no sixteen addresses computed ahead and kept)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-        const int lo = __builtin_amdgcn_readlane(key_docs, acc_row(v, 0)), hi = __builtin_amdgcn_readlane(key_docs, acc_row(v, 1));
-        m |= ((h ? hi : lo) == doc ? 1u : 0u) << v;
-    }
+    for (int v = 0; v < 16; ++v) m |= (__shfl(docs, acc_row(v, 0) + 4 * h) == doc ? 1u : 0u) << v;
     return m;
 }
 
@@ -487,19 +495,24 @@ struct Active {
     const int2* ranges;
     int count, lo, hi, group;
     unsigned long long mask;
+    int2 ours;
     __device__ __forceinline__ int next(int t) {
         while (t < count) {
             if (t >> 6 != group) {
                 group = t >> 6;
                 const int mine = (group << 6) + (threadIdx.x & 63);
-                const int2 r = ranges[mine < count ? mine : 0];
-                mask = __ballot(mine < count && r.x <= hi && r.y >= lo);
+                ours = ranges[mine < count ? mine : 0];
+                mask = __ballot(mine < count && ours.x <= hi && ours.y >= lo);
             }
             const unsigned long long left = mask >> (t & 63);
             if (left) return t + __builtin_ctzll(left);
             t = (group + 1) << 6;
         }
         return count;
+    }
+    // least and largest document of a tile that next() gave last
+    __device__ __forceinline__ int2 range(int t) const {
+        return make_int2(__builtin_amdgcn_readlane(ours.x, t & 63), __builtin_amdgcn_readlane(ours.y, t & 63));
     }
 };
 
@@ -576,10 +589,11 @@ __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_
     low = __builtin_amdgcn_readfirstlane(low);
 
     int docs_next = 0;
+    int2 range_next = {0, 0};
     // the first key of the next tile that any row of the block may see
     const int key_tiles = (a.lk + kTile - 1) / kTile;
     const int64_t place = (int64_t)head * key_tiles;
-    Active active{in.key_docs + place, (end + kTile - 1) / kTile, dlo, dhi, -1, 0};
+    Active active{in.key_docs + place, (end + kTile - 1) / kTile, dlo, dhi, -1, 0, {0, 0}};
     auto next = [&](int j0) {
         if (!s.docs) return j0;
         return __builtin_amdgcn_readfirstlane(active.next(j0 / kTile)) * kTile;
@@ -588,9 +602,9 @@ __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_
     auto copy = [&](int to, int j) {                  // (marks are read ahead of the copies: a wait for them would wait for these)
         marks_next[0] = in.key_marks[place + j / kTile];
         marks_next[1] = in.value_marks[place + j / kTile];
-        if (s.docs) docs_next = s.docs[min(j + (lane & 31), s.len - 1)];
-        copy_to_lds<WAVES>(lds[to], in.key + (place + j / kTile) * P::BYTES, P::BYTES);
-        copy_to_lds<WAVES>(lds[to] + P::BYTES, in.value + (place + j / kTile) * P::BYTES, P::BYTES);
+        if (s.docs) docs_next = s.docs[min(j + (lane & 31), s.len - 1)], range_next = active.range(j / kTile);
+        copy_to_lds<WAVES, P::BYTES>(lds[to], in.key + (place + j / kTile) * P::BYTES);
+        copy_to_lds<WAVES, P::BYTES>(lds[to] + P::BYTES, in.value + (place + j / kTile) * P::BYTES);
     };
 
     f32x16 acc[NT];
@@ -606,6 +620,7 @@ __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_
         copies_done();
         __syncthreads();                               // this tile is there, and everyone is done with the other buffer
         const int docs = docs_next;
+        const int2 range = range_next;
         const unsigned kbad = __builtin_amdgcn_readfirstlane(marks_next[0]), vbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
         const int j1 = next(j0 + kTile);
         if (j1 < end) copy(buf ^ 1, j1);
@@ -621,7 +636,7 @@ __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_
                 for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(p - j0 - 4 * h - acc_row(v, 0)));
             }
             if (j0 + kTile > low || s.docs || kbad) {
-                const unsigned same = s.docs ? same_document(docs, doc, h) : ~0u;
+                const unsigned same = s.docs ? same_document(docs, range, doc, h) : ~0u;
                 const unsigned nans = kbad >> 4 * h;
                 const int left = lim - j0 - 4 * h;
 #pragma unroll
@@ -1079,9 +1094,10 @@ __device__ __forceinline__ void grad_dq(const Args& a, const Plan& plan, int til
     low = __builtin_amdgcn_readfirstlane(low);
 
     int docs_next = 0;
+    int2 range_next = {0, 0};
     const int key_tiles = (a.lk + kTile - 1) / kTile;
     const int64_t place = (int64_t)head * key_tiles;
-    Active active{in.key_docs + place, (end + kTile - 1) / kTile, dlo, dhi, -1, 0};
+    Active active{in.key_docs + place, (end + kTile - 1) / kTile, dlo, dhi, -1, 0, {0, 0}};
     auto next = [&](int j0) {
         if (!s.docs) return j0;
         return __builtin_amdgcn_readfirstlane(active.next(j0 / kTile)) * kTile;
@@ -1090,9 +1106,9 @@ __device__ __forceinline__ void grad_dq(const Args& a, const Plan& plan, int til
     auto copy = [&](int to, int j) {                  // (marks are read ahead of the copies: a wait for them would wait for these)
         marks_next[0] = in.key_marks[place + j / kTile];
         marks_next[1] = in.value_marks[place + j / kTile];
-        if (s.docs) docs_next = s.docs[min(j + (lane & 31), s.len - 1)];
-        copy_to_lds<4>(lds[to], in.key + (place + j / kTile) * P::BYTES, P::BYTES);
-        copy_to_lds<4>(lds[to] + P::BYTES, in.value + (place + j / kTile) * P::BYTES, P::BYTES);
+        if (s.docs) docs_next = s.docs[min(j + (lane & 31), s.len - 1)], range_next = active.range(j / kTile);
+        copy_to_lds<4, P::BYTES>(lds[to], in.key + (place + j / kTile) * P::BYTES);
+        copy_to_lds<4, P::BYTES>(lds[to] + P::BYTES, in.value + (place + j / kTile) * P::BYTES);
     };
 
     f32x16 acc[NT];
@@ -1106,6 +1122,7 @@ __device__ __forceinline__ void grad_dq(const Args& a, const Plan& plan, int til
         copies_done();
         __syncthreads();
         const int docs = docs_next;
+        const int2 range = range_next;
         const unsigned kbad = __builtin_amdgcn_readfirstlane(marks_next[0]), vbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
         const int j1 = next(j0 + kTile);
         if (j1 < end) copy(buf ^ 1, j1);
@@ -1126,7 +1143,7 @@ __device__ __forceinline__ void grad_dq(const Args& a, const Plan& plan, int til
             }
             const bool whole = j0 + kTile <= low && !s.docs && !(kbad | vbad);
             if (!whole) {
-                const unsigned same = s.docs ? same_document(docs, doc, h) : ~0u;
+                const unsigned same = s.docs ? same_document(docs, range, doc, h) : ~0u;
                 const unsigned nans = kbad >> 4 * h;
                 const int left = lim - j0 - 4 * h;
 #pragma unroll
@@ -1224,8 +1241,9 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
     const int rows_end = min(a.lq, (slice % parts.ranges + 1) * parts.span);
     first = max(first, slice % parts.ranges * parts.span);
     int docs_next = 0;
+    int2 range_next = {0, 0};
     const int row_tiles = (a.lq + kTile - 1) / kTile;
-    Active active{in.query_docs + (int64_t)b * a.hq * row_tiles, (rows_end + kTile - 1) / kTile, dlo, dhi, -1, 0};      // (the same for every head)
+    Active active{in.query_docs + (int64_t)b * a.hq * row_tiles, (rows_end + kTile - 1) / kTile, dlo, dhi, -1, 0, {0, 0}};      // (the same for every head)
     auto next = [&](int& g, int& i0) {     // to a tile of rows that may see a key of the block
         for (; g < g1; ++g, i0 = first) {
             if (s.docs) i0 = __builtin_amdgcn_readfirstlane(active.next(i0 / kTile)) * kTile;
@@ -1242,6 +1260,7 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
         if (s.docs) {
             const int i = i0 + (lane & 31), p = s.start + i;
             docs_next = i < a.lq && p >= 0 && p < s.len ? s.docs[p] : 0;
+            range_next = active.range(i0 / kTile);
         }
         if (threadIdx.x < kTile) {
             const int i = i0 + threadIdx.x;
@@ -1249,8 +1268,8 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
             lse_next = i < a.lq ? a.lse[at] : -__builtin_inff();       // (used when it has come: a wait now would be for all copies)
             delta_next = i < a.lq ? in.delta[at] : 0.f;
         }
-        copy_to_lds<4>(lds[to], in.query + n * P::BYTES, P::BYTES);
-        copy_to_lds<4>(lds[to] + P::BYTES, in.grad + n * P::BYTES, P::BYTES);
+        copy_to_lds<4, P::BYTES>(lds[to], in.query + n * P::BYTES);
+        copy_to_lds<4, P::BYTES>(lds[to] + P::BYTES, in.grad + n * P::BYTES);
     };
     auto stage_stat = [&](int to) {           // weights of rows without pairs: exp2(x - inf) = 0
         if (threadIdx.x < kTile) {
@@ -1267,6 +1286,7 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
         stage_stat(buf);
         __syncthreads();                      // this tile is there, and everyone is done with the other buffer
         const int docs = docs_next;
+        const int2 range = range_next;
         const unsigned qbad = __builtin_amdgcn_readfirstlane(marks_next[0]), gbad = __builtin_amdgcn_readfirstlane(marks_next[1]);
         int ng = g, ni = i0 + kTile;
         next(ng, ni);
@@ -1290,7 +1310,7 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
             for (int v = 0; v < 16; ++v) x[v] -= slope2 * fabsf((float)(apart + acc_row(v, 0)));
         }
         if (i0 < all || s.docs || qbad) {
-            const unsigned same = s.docs ? same_document(docs, doc, h) : ~0u;
+            const unsigned same = s.docs ? same_document(docs, range, doc, h) : ~0u;
             const unsigned nans = qbad >> 4 * h;
             const int from = need - i0 - 4 * h;
 #pragma unroll
