@@ -32,6 +32,9 @@ template <typename T> __device__ __forceinline__ void store_quad(T* p, const T (
     *(Vec4<T>*)__builtin_assume_aligned(p, 16) = *(const Vec4<T>*)x;
 }
 
+__device__ __forceinline__ float fused(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return fma(a, b, c); }
+
 // A lane's share of a row: pairs (a[n], b[n]) with number idx[n], and elements behind `dims`
 template <typename T, bool WIDE> struct Row {
     T a[4], b[4], rest[8];
@@ -144,8 +147,8 @@ template <typename T, bool WIDE> struct Row {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const T x = a[n], y = b[n];
-            a[n] = x * c[n] - y * s[n];
-            b[n] = y * c[n] + x * s[n];
+            a[n] = fused(x, c[n], -y * s[n]);
+            b[n] = fused(y, c[n], x * s[n]);
         }
     }
 };
@@ -170,7 +173,8 @@ __device__ __forceinline__ void frequencies(const Rot& p, int lane, int lanes, d
     }
 }
 
-// cos and sin of position * f.  In float32 the angle is reduced to a part of a turn in 64 bits first.
+// cos and sin of position * f.  In float32 the angle is reduced to half turns between -1 and 1 in 64 bits first; what
+// rounding that takes away, up to 9e-8, is put back (cos(x + e) = cos x - e sin x).
 template <typename T>
 __device__ __forceinline__ void angles(const Rot& p, double position, const double (&f)[4], T (&c)[4], T (&s)[4]) {
 #pragma unroll
@@ -178,10 +182,12 @@ __device__ __forceinline__ void angles(const Rot& p, double position, const doub
         const double angle = position * f[n];
         double x, y;
         if constexpr (sizeof(T) == 4) {
-            const double turns = angle * 0.15915494309189533577;
+            const double turns = angle * 0.15915494309189533577, half = 2.0 * (turns - rint(turns));
+            const float near = (float)half, rest = (float)((half - (double)near) * 3.14159265358979323846);
             float u, v;
-            sincospif((float)(2.0 * (turns - rint(turns))), &u, &v);
-            c[n] = v * (float)p.magnitude, s[n] = u * (float)(p.sign * p.magnitude);
+            sincospif(near, &u, &v);
+            const float cosine = fmaf(-u, rest, v), sine = fmaf(v, rest, u);
+            c[n] = cosine * (float)p.magnitude, s[n] = sine * (float)(p.sign * p.magnitude);
         } else {
             sincos(angle, &x, &y);
             c[n] = y * p.magnitude, s[n] = x * p.sign * p.magnitude;
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Rot p, int lanes_log, 
         x.load(p, (const T*)p.x + b * p.x_stride[0] + h * p.x_stride[1] + l * p.x_stride[2], lane, lanes, live);
         if (p.weight) {
             T sum = 0;
-            x.each([&](T& v, int) { sum += v * v; });
+            x.each([&](T& v, int) { sum = fused(v, v, sum); });
             sum = group_sum(sum, lanes);
             const T r = T(1) / root(sum / T(p.d) + T(p.eps));
             Row<T, WIDE> w;
@@ -258,8 +264,8 @@ __global__ __launch_bounds__(kThreads) void rotary_grad_kernel(Rot p, int lanes_
         g.turn(c, s);
         T square = 0, dot = 0;
         x.each([&](T& v, int n) {
-            square += v * v;
-            dot += v * g.at(n) * w.at(n);
+            square = fused(v, v, square);
+            dot = fused(v, g.at(n) * w.at(n), dot);
         });
         square = group_sum(square, lanes);
         dot = group_sum(dot, lanes);
@@ -268,22 +274,22 @@ __global__ __launch_bounds__(kThreads) void rotary_grad_kernel(Rot p, int lanes_
         Row<T, WIDE> out;
         out.each([&](T& v, int n) {
             const T hat = x.at(n) * r;
-            sums[n] += live ? g.at(n) * hat : T(0);
-            v = r * g.at(n) * w.at(n) - x.at(n) * r * mean;
+            sums[n] = live ? fused(g.at(n), hat, sums[n]) : sums[n];
+            v = r * fused(-x.at(n), mean, g.at(n) * w.at(n));
         });
         if (live) out.store(p, (T*)p.y + b * p.y_stride[0] + h * p.y_stride[1] + l * p.y_stride[2], lane, lanes);
     }
-    // [n][lane] summed over the groups in their order
+    // [n][lane] summed over the groups in their order, in 64 bits (in 32 their roundings were half of dw's error)
     T* lds = (T*)shared;
 #pragma unroll
     for (int n = 0; n < 16; ++n) lds[n * kThreads + threadIdx.x] = sums[n];
     __syncthreads();
     for (int o = threadIdx.x; o < 16 << lanes_log; o += kThreads) {
         const int n = o >> lanes_log, i = Row<T, WIDE>::element(p, o & (lanes - 1), lanes, n);
-        T total = 0;
+        double total = 0.0;
 #pragma unroll 8
-        for (int j = 0; j < groups; ++j) total += lds[n * kThreads + j * lanes + (o & (lanes - 1))];
-        if (i >= 0) ((T*)p.work)[((int64_t)slot * p.heads + h) * p.d_pad + i] = total;
+        for (int j = 0; j < groups; ++j) total += (double)lds[n * kThreads + j * lanes + (o & (lanes - 1))];
+        if (i >= 0) ((T*)p.work)[((int64_t)slot * p.heads + h) * p.d_pad + i] = (T)total;
     }
 }
 
