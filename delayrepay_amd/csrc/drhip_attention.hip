@@ -524,7 +524,7 @@ struct Active {
 // Keys and values come 32 at a time from the packed planes through LDS, two buffers, copied a tile ahead.
 // Bound by the matrix units: 32 heads, 4096 rows of 128, causal: 605 us, 227 TFLOP/s of float32 products (a large
 // product of f32 matrices reaches 155), 1.36 PFLOP/s of bfloat16 ones, of which the card holds 2.0 with nothing else to do.  Two waves on a SIMD fill each other's waits; four-wave blocks, two on a compute unit, read each tile twice as
-// often from L2 (695 for 639 us).  With a cap a tanh for each pair comes on top (8 heads, 8192 rows: 720 us).
+// often from L2 (695 for 639 us).  With a cap a tanh for each pair comes on top (8 heads, 8192 rows: 690 us).
 template <int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, Packed in, float* part, float* part_lse) {
     using P = Planes<NT>;

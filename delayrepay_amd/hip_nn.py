@@ -194,13 +194,14 @@ def _rotary(x, how, outs, sign, dy=None):
     frequencies = None if how.frequencies is None else _contiguous(how.frequencies)
     used = [a for a in (x, dy, weight, positions, frequencies) if a is not None]
     grad = dy is not None and x is not None
-    shapes = [rows.shape] + ([weight.shape] if grad else [])
+    shapes = [rows.shape, weight.shape] if grad else [rows.shape]
     # a row is read whole before it is written: the result may take an operand's place
     places = _places(outs, shapes, rows.dtype, used, same=dy if grad else rows)
     if grad and not places[1].is_contiguous:
         places[1] = ndarray(shapes[1], rows.dtype)
-    fields = (rows.ptr, places[0].ptr, _ptr(weight), dy.ptr if grad else 0, places[1].ptr if grad else 0, _ptr(positions), _ptr(frequencies))
-    key = (grad, sign, rows.shape, rows._strides, places[0]._strides, _steps(dy), rows.dtype.itemsize, per_head and weight._strides,
+    fields = (rows.ptr, places[0].ptr, 0 if weight is None else weight.ptr, dy.ptr if grad else 0, places[1].ptr if grad else 0,
+              0 if positions is None else positions.ptr, 0 if frequencies is None else frequencies.ptr)
+    key = (grad, sign, rows.shape, rows._strides, places[0]._strides, dy._strides if grad else None, rows.dtype.itemsize, per_head and weight._strides,
            None if positions is None else (positions.shape, positions._strides, positions.dtype.itemsize),
            how.first, how.base, how.dims, how.stretch, how.magnitude, how.eps, how.interleaved)
 

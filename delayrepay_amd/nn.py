@@ -197,13 +197,14 @@ def attention(q, k, v, *, scale=None, causal=False, start=None, lengths=None, pr
     sequence if `start` is not given.  A key counts for a row if j < `lengths` (all key rows
     without it), with `causal` if also j <= position of the row or j < `prefix`, and with
     `documents` (batch, key rows) if its document is the one at the row's position (rows outside the
-    sequence have none).  A row without keys gives zeros.  Keys that do not count may hold anything, also what is not finite; a pair that counts
-    gives NaN if its q or k is not finite.
+    sequence have none).  A row without keys gives zeros.  Keys that do not count may hold anything, also
+    what is not finite; a pair that counts gives NaN if its q or k is not finite.  `start` lies within 2**30
+    of 0, `scale` within 2**100 of 0 and `cap` between 2**-100 and 2**100.
 
     `with_lse` returns (output, lse): lse (batch, heads, rows), the logarithm of the sum of the
     exponentials of the scores (-inf for a row without keys), which `attention_grad` needs.
 
-    One row and many, long caches and short: a few rows are split over the key range.
+    One row and many, long caches and short: where the rows are few, blocks take ranges of the keys.
     """
     q, k, v = _heads(q, k, v)
     how = _Mask(q, k, scale, causal, start, lengths, prefix, documents, slopes, cap)
@@ -239,12 +240,15 @@ class _Turn:
         batch, heads, rows, size = x.shape
         if not 1 <= size <= MAX_ROTARY_HEAD:
             raise ValueError(f"head sizes from 1 to {MAX_ROTARY_HEAD} are supported, not {size}")
-        self.dims = size - size % 2 if dims is None else dims
-        if not isinstance(self.dims, (int, numpy.integer)) or isinstance(self.dims, bool) or self.dims % 2 or not 0 <= self.dims <= size:
+        if dims is None:
+            dims = size - size % 2
+        elif not isinstance(dims, (int, numpy.integer)) or isinstance(dims, bool) or dims % 2 or not 0 <= dims <= size:
             raise ValueError(f"dims is an even number of a head's {size} elements, not {dims!r}")
-        self.dims = int(self.dims)
+        self.dims = int(dims)
         self.positions, self.first = None, 0
-        if type(positions) is not NPArray and isinstance(positions, (numbers.Integral, numpy.integer)) and not isinstance(positions, (bool, numpy.bool_)):
+        if type(positions) is int and -(1 << 52) < positions < 1 << 52:
+            self.first = positions
+        elif type(positions) is not NPArray and isinstance(positions, (numbers.Integral, numpy.integer)) and not isinstance(positions, (bool, numpy.bool_)):
             self.first = int(positions)
             if abs(self.first) >= 1 << 52:
                 raise ValueError("positions lie below 2**52")
@@ -255,7 +259,7 @@ class _Turn:
             if tuple(p.shape) not in ((rows,), (batch, rows)):
                 raise ValueError(f"positions has the shape {(rows,)} or {(batch, rows)}, not {tuple(p.shape)}")
             self.positions = p
-        self.base = _number(base, "base", 0.0, above=True)
+        self.base = base if type(base) is float and 0.0 < base < math.inf else _number(base, "base", 0.0, above=True)
         self.frequencies = None
         if frequencies is not None:
             f = _array(frequencies, "frequencies")
@@ -265,9 +269,9 @@ class _Turn:
         if not isinstance(interleaved, (bool, numpy.bool_)):
             raise TypeError("interleaved is True or False")
         self.interleaved = bool(interleaved)
-        self.stretch = _number(stretch, "stretch", 0.0, above=True)
-        self.magnitude = _number(magnitude, "magnitude")
-        self.eps = _number(eps, "eps", 0.0)
+        self.stretch = stretch if type(stretch) is float and 0.0 < stretch < math.inf else _number(stretch, "stretch", 0.0, above=True)
+        self.magnitude = magnitude if type(magnitude) is float and abs(magnitude) < math.inf else _number(magnitude, "magnitude")
+        self.eps = eps if type(eps) is float and 0.0 <= eps < math.inf else _number(eps, "eps", 0.0)
         self.weight = None
         if weight is not None:
             w = _array(weight, "weight")
@@ -287,7 +291,7 @@ def rotary(x, positions, *, base=10000.0, frequencies=None, dims=None, interleav
     `interleaved`.  Frequencies are base ** (-2 i / dims), or a float64 array (dims/2,); `stretch`
     scales positions for contexts longer than those trained on, `magnitude` multiplies the turned
     elements.  `positions` is an integer array (rows,) or (batch, rows), or the first row's position.
-    Angles are computed in 64 bits.
+    Angles are computed in 64 bits (positions of an int64 array beyond 2**53 are rounded).
 
     With `weight`, (size,) or (heads, size), each row is first divided by the root of (the mean of its
     squares + eps) and multiplied by the weight: the norm of queries and keys in the same pass.
@@ -321,7 +325,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     numbers), `top_p` of these the first whose weights reach that part of their sum, `min_p` of these the
     ones of at least that part of the largest.  The token is the first one, by number, at which the
     kept weights summed up exceed uniforms[row] (in [0, 1): `random.device().random(batch)`) of their sum.
-    A temperature of 0 takes the largest.  Each of the four is a number or an array (batch,), float32 or
+    A temperature of 0 takes the largest; numbers go up to 1e30.  Each of the four is a number or an array (batch,), float32 or
     (top_k) integers, in which a top_k below 1 stands for all and numbers out of range for the nearest in it.
     A logit that is NaN or -inf is never drawn; a row without another gives -1.
 

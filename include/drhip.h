@@ -128,7 +128,8 @@ int drhip_cumsum(int kind, const void* in_dev, void* out_dev, size_t n);
  * j < prefix, with `documents` if documents[j] = documents[position] (none at
  * positions outside the sequence).
  * Scores: scale q.k, with cap > 0 cap tanh(scale q.k / cap), with slopes less
- * slopes[head] |position - j|.  o = softmax(scores) v, lse (may be NULL) the
+ * slopes[head] |position - j|; |scale| and cap within 2^100, cap > 2^-100 if
+ * positive.  o = softmax(scores) v, lse (may be NULL) the
  * logarithm of the sum of their exponentials; a row without keys gives zeros
  * and -inf.  drhip_attention_grad: dq, dk, dv from dout and the forward call's
  * o and lse. */
