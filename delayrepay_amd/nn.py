@@ -325,7 +325,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     numbers), `top_p` of these the first whose weights reach that part of their sum, `min_p` of these the
     ones of at least that part of the largest.  The token is the first one, by number, at which the
     kept weights summed up exceed uniforms[row] (in [0, 1): `random.device().random(batch)`) of their sum.
-    A temperature of 0 takes the largest; numbers go up to 1e30.  Each of the four is a number or an array (batch,), float32 or
+    A temperature of 0 takes the largest; they go up to float32's largest.  Each of the four is a number or an array (batch,), float32 or
     (top_k) integers, in which a top_k below 1 stands for all and numbers out of range for the nearest in it.
     A logit that is NaN or -inf is never drawn; a row without another gives -1.
 
@@ -348,7 +348,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, min_p=N
                 raise ValueError(f"{name} lies in {'(' if above else '['}{low:g}, {high:g}], not at {x:g}")
             return x
         return _shaped(_floats(x, name, 1), name, (batch,))
-    temperature = part(temperature, "temperature", 1.0, 0.0, 1e30, False)
+    temperature = part(temperature, "temperature", 1.0, 0.0, 3.4028234663852886e38, False)
     top_p = part(top_p, "top_p", 1.0, 0.0, 1.0, True)
     min_p = part(min_p, "min_p", 0.0, 0.0, 1.0, False)
     top_k = _integers(top_k, "top_k", (batch,))

@@ -495,7 +495,7 @@ def test_sample_of_extreme_logits(how):
     logits[4, 11] = info.max
     logits[5] = np.where(logits[5] == 0, -INF, logits[5])
     logits[6] = np.where(logits[6] == 0, info.tiny, logits[6])
-    for temperature in (1.0, 1e30, 1e-40, np.full(7, info.max), np.full(7, 1e20, f)):
+    for temperature in (1.0, 1e30, 1e-40, float(info.max), np.full(7, info.max), np.full(7, 1e20, f)):
         _draws(logits, rs.rand(7), temperature=temperature, **how)
 
 
