@@ -467,6 +467,27 @@ def test_sample_of_long_rows(vocabulary, how):
     _draws(logits, rs.rand(6), **how)
 
 
+def test_sample_of_rows_in_large_parts():
+    """Rows so long that their parts are no multiple of what a wave reads at a time; against running sums in 64 bits,
+    whose roundings (2e6 of 2^-53) a draw meets with a probability of 1e-9."""
+    rs = np.random.RandomState(6)
+    n = 2200003
+    logits = (rs.standard_normal((2, n)) * 2.5).astype(np.float32)
+    u = np.array([0.37, 0.81])
+    dev, draw = dr.array(logits), dr.array(u)
+    for how in (dict(), dict(top_p=0.6), dict(top_k=200), dict(top_k=5000, top_p=0.9), dict(min_p=0.01)):
+        got = nn.sample(dev, draw, **how).get()
+        for row, x, token in zip(logits.astype(np.float64), u, got):
+            w = np.exp(row - row.max())
+            order = np.argsort(-row, kind="stable")
+            w[order[how.get("top_k", n):]] = 0.0
+            run = np.cumsum(w[order])
+            w[order[1:][run[:-1] >= how.get("top_p", 2.0) * run[-1]]] = 0.0
+            w[w < how.get("min_p", 0.0)] = 0.0
+            run = np.cumsum(w)
+            assert token == np.searchsorted(run, x * run[-1], side="right"), how
+
+
 @pytest.mark.parametrize("vocabulary", [40, 5000])
 def test_sample_with_parameters_at_their_ends(vocabulary):
     """Out of range in an array: the nearest in it.  The smallest temperatures leave the largest logits."""
