@@ -124,7 +124,10 @@ def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
         return _contiguous(x) if isinstance(x, ndarray) else None
     lengths, start, prefix = how.lengths, how.start, how.prefix
     if how.plain and not grad:         # (the same with less to do: a short call is bound by this)
-        fields = (q.ptr, k.ptr, v.ptr, o.ptr, 0 if lse is None else lse.ptr, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        if lengths is not None:
+            lengths = _contiguous(lengths)
+            used = used + [lengths]
+        fields = (q.ptr, k.ptr, v.ptr, o.ptr, 0 if lse is None else lse.ptr, 0, 0, 0, 0, 0 if lengths is None else lengths.ptr, 0, 0, 0, 0)
         plain = (q.shape, q._strides, k.shape, k._strides, v._strides, o._strides, how.causal, "last" if start is None else start, how.scale, how.cap)
         plan = _PLANS.get(plain)
         if plan is not None:
@@ -158,7 +161,9 @@ def _attention(func, grad, q, k, v, o, lse, dout, grads, how, used, written):
 def attention(q, k, v, how, outs):
     q, k, v = _dense(q), _dense(k), _dense(v)
     operands = [q, k, v]
-    if not how.plain:
+    if how.plain:
+        operands.append(how.lengths)
+    else:
         operands += [how.documents, how.slopes] + [x for x in (how.lengths, how.start, how.prefix) if isinstance(x, ndarray)]
     shapes = [q.shape, q.shape[:3]][:len(outs)]
     places = _places(outs, shapes, _F32, operands)

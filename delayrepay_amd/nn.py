@@ -143,8 +143,8 @@ class _Mask:
 
     def __init__(self, q, k, scale, causal, start, lengths, prefix, documents, slopes, cap):
         batch, lk = k.shape[0], k.shape[2]
-        # a part of the key row's own or of the arguments an array: not a plain call
-        self.plain = lengths is None and prefix is None and documents is None and slopes is None and (start is None or type(start) is int)
+        # the common calls: no arguments but these, of them only `lengths` an array
+        self.plain = prefix is None and documents is None and slopes is None and (start is None or type(start) is int) and type(lengths) is not int
         self.scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else _number(scale, "scale")
         if abs(self.scale) > _LARGE:
             raise ValueError(f"scale lies within 2**100 of 0, not at {self.scale:g}")
@@ -157,10 +157,12 @@ class _Mask:
         self.start = _integers(start, "start", (batch,))
         if isinstance(self.start, int) and abs(self.start) > _FAR:
             raise ValueError(f"start lies within 2**30 of 0, not at {self.start}")
-        if self.plain:
-            self.lengths = self.prefix = self.documents = self.slopes = None
-            return
         self.lengths = _integers(lengths, "lengths", (batch,))
+        if self.plain:
+            self.plain = not isinstance(self.lengths, int)
+        if self.plain:
+            self.prefix = self.documents = self.slopes = None
+            return
         if isinstance(self.lengths, int) and not 0 <= self.lengths <= lk:
             raise ValueError(f"lengths lies in [0, {lk}], the rows of k, not {self.lengths}")
         self.prefix = _integers(prefix, "prefix", (batch,))
