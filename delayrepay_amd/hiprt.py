@@ -224,11 +224,10 @@ def cumsum(kind, src, dst, n):
 # The argument structs of the operators are packed as bytes (native alignment), in the order of
 # include/drhip.h; `work` and `work_bytes` are the last pointer and the word behind it.
 ATTENTION = struct.Struct("@15PQ25q10i2f")
-ROTARY = struct.Struct("@8PQ12q5d9i")
-SAMPLE = struct.Struct("@7Pq4d4i")
+ROTARY = struct.Struct("@8PQ12q5d9i0q")      # (0q: filled up to whole words, as the C struct is)
 # the same in two pieces: addresses, and what depends on geometry and options alone
 ATTENTION_HEAD, ATTENTION_TAIL = struct.Struct("@15PQ"), struct.Struct("@25q10i2f")
-ROTARY_HEAD, ROTARY_TAIL = struct.Struct("@8PQ"), struct.Struct("@12q5d9i")
+ROTARY_HEAD, ROTARY_TAIL = struct.Struct("@8PQ"), struct.Struct("@12q5d9i0q")
 SAMPLE_HEAD, SAMPLE_TAIL = struct.Struct("@7P"), struct.Struct("@q4d4i")
 
 

@@ -233,3 +233,14 @@ def test_the_library_refuses_what_its_launches_cannot_hold():
     assert attention(batch=1 << 21, grad=0) == 0          # (fewer matrices to pack)
     for bad in (dict(d=513, pad=516), dict(dims=7), dict(dims=10), dict(pad=6), dict(rows=-1), dict(batch=1 << 20, rows=1 << 20)):
         assert rotary(**bad) == 20002, bad
+
+
+def test_argument_structs_have_the_size_of_the_header(tmp_path):
+    """The packed bytes are read as C structs: none shorter than its struct, fillings at the end included."""
+    from delayrepay_amd import hiprt
+    source, program = tmp_path / "sizes.c", tmp_path / "sizes"
+    source.write_text('#include <stdio.h>\n#include "drhip.h"\nint main(void) { printf("%zu %zu %zu", sizeof(drhip_attention_t), sizeof(drhip_rotary_t), sizeof(drhip_sample_t)); return 0; }\n')
+    subprocess.run(["cc", "-I", os.path.join(ROOT, "include"), "-o", str(program), str(source)], check=True)
+    sizes = [int(x) for x in subprocess.run([str(program)], capture_output=True, text=True, check=True).stdout.split()]
+    assert sizes == [a.size + b.size for a, b in ((hiprt.ATTENTION_HEAD, hiprt.ATTENTION_TAIL), (hiprt.ROTARY_HEAD, hiprt.ROTARY_TAIL), (hiprt.SAMPLE_HEAD, hiprt.SAMPLE_TAIL))]
+    assert sizes[:2] == [hiprt.ATTENTION.size, hiprt.ROTARY.size]
