@@ -2,6 +2,9 @@
 import numpy as np
 
 
+def narrowed(x, low, high):
+    return np.clip(x, low, high).astype(np.int32)
+
 
 def _out(outs, values, dtype):
     """Results in the arrays asked for, or as new ones."""
@@ -23,7 +26,7 @@ def _sequence(q, k, how, b):
     """(rows in use, positions of the rows, which pairs count) of one sequence."""
     lq, lk = q.shape[2], k.shape[2]
     n = lk if how.lengths is None else min(max(_of(how.lengths, b), 0), lk)
-    start = n - lq if how.start is None else _of(how.start, b)
+    start = n - lq if how.start is None else min(max(_of(how.start, b), -1 << 30), 1 << 30)
     p, j = start + np.arange(lq), np.arange(n)
     ok = np.ones((lq, n), bool)
     if how.causal:

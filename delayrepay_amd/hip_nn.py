@@ -10,6 +10,11 @@ from .devarray import Buffer, ndarray
 _F32, _I64 = numpy.dtype(numpy.float32), numpy.dtype(numpy.int64)
 
 
+def narrowed(x, low, high):
+    """The int64 array in int32, with its numbers clamped to [low, high]."""
+    return hip.materialise(x, numpy.int32, within=(low, high))
+
+
 def _dense(x):
     """The array, copied if its last axis is not dense."""
     return x if x._strides[-1] == 1 or x.shape[-1] <= 1 else x.copy()

@@ -29,6 +29,7 @@ _INTS = (numpy.dtype(numpy.int32), numpy.dtype(numpy.int64))
 MAX_HEAD = 128           # elements of an attention head
 MAX_ROTARY_HEAD = 512
 _FAR = 1 << 30            # positions of rows are nearer to 0
+_COUNTS = (-1, (1 << 31) - 1)
 _LARGE = 2.0 ** 100       # scales and caps are smaller, and caps larger than its inverse: their products fit float32
 
 
@@ -61,8 +62,8 @@ def _shaped(x, name, shape):
     return x
 
 
-def _integers(x, name, shape, number=True):
-    """None, a whole number, or an int32 array of `shape` (int64 arrays are converted)."""
+def _integers(x, name, shape, number=True, within=_COUNTS):
+    """None, a whole number, or an int32 array of `shape` (numbers of int64 arrays outside `within` are clamped to it)."""
     if x is None:
         return None
     if type(x) is NPArray and x.dtype == _INTS[0] and x.shape == shape:
@@ -75,7 +76,7 @@ def _integers(x, name, shape, number=True):
     if x.dtype not in _INTS:
         raise TypeError(f"{name} holds int32 or int64, not {x.dtype}")
     _shaped(x, name, shape)
-    return x if x.dtype == _INTS[0] else x.astype(_INTS[0])
+    return x if x.dtype == _INTS[0] else x.astype(_INTS[0]) if within is None else _ops.narrowed(x, *within)
 
 
 def _number(x, name, low=-math.inf, above=False):
@@ -154,7 +155,7 @@ class _Mask:
         self.cap = None if cap is None else _number(cap, "cap", 0.0, above=True)
         if cap is not None and not 1 / _LARGE <= self.cap <= _LARGE:
             raise ValueError(f"cap lies between 2**-100 and 2**100, not at {self.cap:g}")
-        self.start = _integers(start, "start", (batch,))
+        self.start = _integers(start, "start", (batch,), within=(-_FAR, _FAR))
         if isinstance(self.start, int) and abs(self.start) > _FAR:
             raise ValueError(f"start lies within 2**30 of 0, not at {self.start}")
         self.lengths = _integers(lengths, "lengths", (batch,))
@@ -170,7 +171,7 @@ class _Mask:
             raise ValueError("prefix belongs to causal attention: without causal=True every row sees every key")
         if isinstance(self.prefix, int) and self.prefix < 0:
             raise ValueError(f"prefix is at least 0, not {self.prefix}")
-        self.documents = _integers(documents, "documents", (batch, lk), number=False)
+        self.documents = _integers(documents, "documents", (batch, lk), number=False, within=None)
         self.slopes = None if slopes is None else _shaped(_floats(slopes, "slopes", 1), "slopes", (q.shape[1],))
 
 
