@@ -6,6 +6,10 @@ def narrowed(x, low, high):
     return np.clip(x, low, high).astype(np.int32)
 
 
+def renumbered(x):
+    return x            # (compared in 64 bits here)
+
+
 def _out(outs, values, dtype):
     """Results in the arrays asked for, or as new ones."""
     done = []

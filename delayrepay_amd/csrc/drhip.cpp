@@ -33,6 +33,7 @@ extern "C" int drhip_k_cumsum(int kind, void* temp, size_t* temp_bytes, const vo
 extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad);
 extern "C" int drhip_k_attention(const drhip_attention_t* a, hipStream_t s);
 extern "C" int drhip_k_attention_grad(const drhip_attention_t* a, hipStream_t s);
+extern "C" int drhip_k_renumber(const drhip_renumber_t* a, int log, hipStream_t s);
 extern "C" uint64_t drhip_k_rotary_work(const drhip_rotary_t* p);
 extern "C" int drhip_k_rotary(const drhip_rotary_t* p, hipStream_t s);
 extern "C" int drhip_k_sample(const drhip_sample_t* p, hipStream_t s);
@@ -377,6 +378,18 @@ int drhip_attention_grad(const drhip_attention_t* a) {
     const uint64_t need = drhip_k_attention_work(a, 1);
     if (need && (!a->work || a->work_bytes < need)) return fail(DRHIP_EINVAL, "drhip_attention_grad", "workspace too small");
     if (int rc = drhip_k_attention_grad(a, g_stream)) return fail(rc, "drhip_attention_grad", hipGetErrorString((hipError_t)rc));
+    g_cnt.n_launches++;
+    return 0;
+}
+
+int drhip_renumber(const drhip_renumber_t* a) {
+    if (!a) return fail(DRHIP_EINVAL, "drhip_renumber", "null argument");
+    if (a->batch < 0 || a->n < 0 || a->n >= 1 << 28 || (int64_t)a->batch * (a->n / 256 + 1) >= kMostBlocks) return fail(DRHIP_EINVAL, "drhip_renumber", "bad size");
+    if (a->slots < 2 || a->slots & (a->slots - 1) || a->slots / 2 < a->n) return fail(DRHIP_EINVAL, "drhip_renumber", "slots is not a power of two of at least 2 n");
+    NEED_INIT();
+    if (!a->batch || !a->n) return 0;
+    if (!a->x || !a->y || !a->table) return fail(DRHIP_EINVAL, "drhip_renumber", "null operand");
+    if (int rc = drhip_k_renumber(a, __builtin_ctz((unsigned)a->slots), g_stream)) return fail(rc, "drhip_renumber", hipGetErrorString((hipError_t)rc));
     g_cnt.n_launches++;
     return 0;
 }

@@ -1425,6 +1425,49 @@ __global__ __launch_bounds__(kThreads) void attention_add(Args a, int parts, int
     }
 }
 
+// ---- document numbers of 64 bits ---------------------------------------------------------------
+// Documents are told apart by equality alone, so a number may become the place where it first stands in its
+// sequence.  A table of at least twice as many slots as there are numbers holds for each of them that place: the first of each
+// run of equal numbers looks for its slot from the number's hash on (multiplicative, upwards), then every number reads
+// its place.  What it gives does not depend on timing.  Bound by its three launches.
+constexpr int kFree = 0x7fffffff;
+
+__device__ __forceinline__ unsigned slot_of(int64_t x, int log) { return (unsigned)((uint64_t)x * 0x9e3779b97f4a7c15ull >> (64 - log)); }
+
+__global__ __launch_bounds__(kThreads) void renumber_clear(int32_t* table, int64_t count) {
+    for (int64_t n = (int64_t)blockIdx.x * kThreads + threadIdx.x; n < count; n += (int64_t)gridDim.x * kThreads) table[n] = kFree;
+}
+
+__global__ __launch_bounds__(kThreads) void renumber_enter(drhip_renumber_t a, int log, int blocks) {
+    const int b = blockIdx.x / blocks, j = blockIdx.x % blocks * kThreads + threadIdx.x;
+    if (j >= a.n) return;
+    const int64_t* row = a.x + b * a.x_stride;
+    const int64_t x = row[j];
+    if (j && row[j - 1] == x) return;
+    int32_t* table = a.table + ((int64_t)b << log);
+    for (unsigned at = slot_of(x, log);; at = (at + 1) & ((1u << log) - 1)) {      // (half of the slots stay free)
+        const int i = atomicCAS(&table[at], kFree, j);
+        if (i != kFree && row[i] != x) continue;
+        if (i != kFree) atomicMin(&table[at], j);
+        return;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void renumber_read(drhip_renumber_t a, int log, int blocks) {
+    const int b = blockIdx.x / blocks, j = blockIdx.x % blocks * kThreads + threadIdx.x;
+    if (j >= a.n) return;
+    const int64_t* row = a.x + b * a.x_stride;
+    const int64_t x = row[j];
+    const int32_t* table = a.table + ((int64_t)b << log);
+    unsigned at = slot_of(x, log);
+    int i = table[at];
+    while (i != kFree && row[i] != x) {
+        at = (at + 1) & ((1u << log) - 1);
+        i = table[at];
+    }
+    a.y[(int64_t)b * a.n + j] = i;
+}
+
 bool aligned(const void* p, const int64_t* stride) {
     return (uintptr_t)p % 16 == 0 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
 }
@@ -1655,5 +1698,14 @@ extern "C" int drhip_k_attention_grad(const drhip_attention_t* args, hipStream_t
         case 3: launch_grad<3>(a, p, parts, in, part, s); break;
         default: launch_grad<4>(a, p, parts, in, part, s); break;
     }
+    return (int)hipGetLastError();
+}
+
+extern "C" int drhip_k_renumber(const drhip_renumber_t* a, int log, hipStream_t s) {
+    const int64_t count = (int64_t)a->batch << log;
+    const int blocks = (a->n + kThreads - 1) / kThreads;
+    renumber_clear<<<dim3((unsigned)(count < 2048 * kThreads ? (count + kThreads - 1) / kThreads : 2048)), kThreads, 0, s>>>(a->table, count);
+    renumber_enter<<<dim3((unsigned)(a->batch * blocks)), kThreads, 0, s>>>(*a, log, blocks);
+    renumber_read<<<dim3((unsigned)(a->batch * blocks)), kThreads, 0, s>>>(*a, log, blocks);
     return (int)hipGetLastError();
 }

@@ -20,6 +20,18 @@ def _dense(x):
     return x if x._strides[-1] == 1 or x.shape[-1] <= 1 else x.copy()
 
 
+def renumbered(x):
+    """An int32 array of numbers that are equal within a row where those of the int64 array are."""
+    x = _dense(x)
+    batch, n = x.shape
+    out = ndarray(x.shape, numpy.int32)
+    if x.size:
+        slots = 1 << (2 * n - 1).bit_length()
+        table = Buffer(batch * slots * 4)
+        hip.issue_operator(hiprt.renumber, hiprt.RENUMBER.pack(x.ptr, out.ptr, table.ptr, x._strides[0], batch, n, slots), [x, out, table], [out])
+    return out
+
+
 def _strides(x):
     return x._strides[:3]
 

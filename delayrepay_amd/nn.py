@@ -63,7 +63,8 @@ def _shaped(x, name, shape):
 
 
 def _integers(x, name, shape, number=True, within=_COUNTS):
-    """None, a whole number, or an int32 array of `shape` (numbers of int64 arrays outside `within` are clamped to it)."""
+    """None, a whole number, or an int32 array of `shape`: numbers of int64 arrays outside `within` are clamped to it,
+    or without it all become others that are equal where they are."""
     if x is None:
         return None
     if type(x) is NPArray and x.dtype == _INTS[0] and x.shape == shape:
@@ -76,7 +77,7 @@ def _integers(x, name, shape, number=True, within=_COUNTS):
     if x.dtype not in _INTS:
         raise TypeError(f"{name} holds int32 or int64, not {x.dtype}")
     _shaped(x, name, shape)
-    return x if x.dtype == _INTS[0] else x.astype(_INTS[0]) if within is None else _ops.narrowed(x, *within)
+    return x if x.dtype == _INTS[0] else _ops.renumbered(x) if within is None else _ops.narrowed(x, *within)
 
 
 def _number(x, name, low=-math.inf, above=False):
@@ -171,8 +172,8 @@ class _Mask:
             raise ValueError("prefix belongs to causal attention: without causal=True every row sees every key")
         if isinstance(self.prefix, int) and self.prefix < 0:
             raise ValueError(f"prefix is at least 0, not {self.prefix}")
-        self.documents = _integers(documents, "documents", (batch, lk), number=False, within=None)
         self.slopes = None if slopes is None else _shaped(_floats(slopes, "slopes", 1), "slopes", (q.shape[1],))
+        self.documents = _integers(documents, "documents", (batch, lk), number=False, within=None)
 
 
 def _heads(q, k, v):

@@ -156,6 +156,18 @@ int drhip_attention_work(const drhip_attention_t* a, int grad, uint64_t* bytes);
 int drhip_attention(const drhip_attention_t* a);
 int drhip_attention_grad(const drhip_attention_t* a);
 
+/* Numbers of 64 bits as numbers of 32 that are equal where they are: y[batch][n] is
+ * the place at which x[batch][n] first stands in its row (of documents for
+ * attention).  `table`: device memory of batch rows of `slots` words, a power of
+ * two of at least 2 n. */
+typedef struct drhip_renumber_t {
+    const int64_t* x;
+    int32_t *y, *table;
+    int64_t x_stride;             /* of rows                                   */
+    int32_t batch, n, slots;
+} drhip_renumber_t;
+int drhip_renumber(const drhip_renumber_t* a);
+
 /* Rotary positions of x[batch][heads][rows][d] (d <= 512), float or double: the
  * pair of elements number i < dims/2 turns by sign * position * frequency_i *
  * squeeze, frequency_i = 2^(i * step) or from the table, and is multiplied by

@@ -50,3 +50,46 @@ def test_numbers_of_64_bits_are_clamped(lq):
     rs = np.random.RandomState(0)
     logits, u = dr.array(rs.standard_normal((4, 500)).astype(np.float32)), dr.array(rs.rand(4))
     assert nn.sample(logits, u, top_k=dr.array(wide)).get().tolist() == nn.sample(logits, u).get().tolist()
+
+@pytest.mark.parametrize("size", [(2, 3, 90), (2, 40, 90), (1, 90, 700), (1, 2, 5000)], ids=str)
+def test_documents_of_64_bits(size):
+    """Numbers that agree in their low 32 bits, or in the high ones, are different documents."""
+    b, lq, lk = size
+    rs = np.random.RandomState(lk)
+    names = np.array([1, 1 + (1 << 32), 1 - (1 << 32), -1, 0, 2 ** 63 - 1, -2 ** 63, 1 << 32, 7, 8])
+    order = np.repeat(rs.randint(0, len(names), lk), rs.randint(1, max(2, lk // 9), lk))[:b * lk].reshape(b, lk)      # (they come back)
+    q, g, k, v = _normal(lk, (b, 4, lq, 32), (b, 4, lq, 32), (b, 2, lk, 32), (b, 2, lk, 32))
+    for how in (dict(), dict(causal=True, lengths=rs.randint(lk // 2, lk + 1, b).astype(np.int32))):
+        _same_bits(_all(q, k, v, g, documents=names[order], **how), _all(q, k, v, g, documents=order.astype(np.int32), **how))
+    dev = [dr.array(x) for x in (q, k, v)]
+    wide = dr.array(np.stack([names[order], names[order] * 0], 2))[:, :, 0]              # every other number
+    want = nn.attention(*dev, documents=dr.array(order.astype(np.int32))).get()
+    _same_bits([nn.attention(*dev, documents=wide).get()], [want])
+
+
+def test_documents_of_64_bits_all_alike_and_all_apart():
+    rs = np.random.RandomState(3)
+    lk = 3000
+    q, g, k, v = _normal(lk, (2, 2, 70, 16), (2, 2, 70, 16), (2, 1, lk, 16), (2, 1, lk, 16))
+    apart = rs.permutation(lk).astype(np.int64) << 40
+    ids = np.stack([np.full(lk, -5 << 33), apart])
+    _same_bits(_all(q, k, v, g, documents=ids), _all(q, k, v, g, documents=np.stack([np.zeros(lk), apart >> 40]).astype(np.int32)))
+
+
+def test_recorded_documents_of_64_bits():
+    """A recording and its graph renumber what the array holds when they are replayed."""
+    from delayrepay_amd import hip
+    rs = np.random.RandomState(4)
+    q, k, v = (dr.array(x) for x in _normal(4, (2, 2, 5, 32), (2, 2, 60, 32), (2, 2, 60, 32)))
+    ids = dr.array(np.zeros((2, 60), np.int64))
+    with hip.record() as plan:
+        out = nn.attention(q, k, v, documents=ids)
+    plan.as_graph()
+    for turn in range(4):
+        now = rs.randint(0, 3, (2, 60)) * (1 << 32)
+        ids[...] = dr.array(now)
+        plan()
+        want = nn.attention(q, k, v, documents=dr.array((now >> 32).astype(np.int32))).get()
+        _same_bits([out.get()], [want])
+
+

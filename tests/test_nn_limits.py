@@ -32,3 +32,31 @@ def test_numbers_of_64_bits_are_clamped():
         logits, u = dnp.array(rs.standard_normal((4, 50)).astype(np.float32)), dnp.array(rs.rand(4))
         assert dnp.nn.sample(logits, u, top_k=wide).get().tolist() == dnp.nn.sample(logits, u).get().tolist()
     """, DELAY_CPU="1")
+
+
+def test_documents_of_64_bits():
+    """Numbers that agree in their low 32 bits are different documents."""
+    _child("""
+        import numpy as np
+        import delayrepay as dnp
+        rs = np.random.RandomState(2)
+        q, k, v = (dnp.array(rs.standard_normal(s).astype(np.float32)) for s in ((2, 2, 5, 8), (2, 2, 9, 8), (2, 2, 9, 8)))
+        order = rs.randint(0, 3, (2, 9))
+        ids = np.array([1, 1 + 2 ** 32, -2 ** 63 + 1])[order]
+        got, want = (dnp.nn.attention(q, k, v, documents=x).get() for x in (ids, order.astype(np.int32)))
+        assert np.array_equal(got, want)
+    """, DELAY_CPU="1")
+
+
+def test_the_library_checks_the_table_of_renumbered_documents():
+    from delayrepay_amd import hiprt
+    for batch, n, slots in ((-1, 3, 8), (1, -1, 8), (1, 3, 4), (1, 3, 7), (1, 0, 1), (1, 1 << 28, 1 << 29), (1 << 23, 3, 8), (1, 3, -8)):
+        assert hiprt.lib().drhip_renumber(hiprt.RENUMBER.pack(16, 16, 16, n, batch, n, slots)) == 20002, (batch, n, slots)
+
+
+def test_argument_structs_have_the_size_of_the_header(tmp_path):
+    from delayrepay_amd import hiprt
+    source, program = tmp_path / "sizes.c", tmp_path / "sizes"
+    source.write_text('#include <stdio.h>\n#include "drhip.h"\nint main(void) { printf("%zu", sizeof(drhip_renumber_t)); return 0; }\n')
+    subprocess.run(["cc", "-I", os.path.join(ROOT, "include"), "-o", str(program), str(source)], check=True)
+    assert int(subprocess.run([str(program)], capture_output=True, text=True, check=True).stdout) == hiprt.RENUMBER.size
