@@ -31,6 +31,7 @@ extern "C" int drhip_k_cumsum(int kind, void* temp, size_t* temp_bytes, const vo
                               size_t n, hipStream_t s);
 
 extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad);
+extern "C" int drhip_k_attention_packs(const drhip_attention_t* a);
 extern "C" int drhip_k_attention(const drhip_attention_t* a, hipStream_t s);
 extern "C" int drhip_k_attention_grad(const drhip_attention_t* a, hipStream_t s);
 extern "C" int drhip_k_renumber(const drhip_renumber_t* a, int log, hipStream_t s);
@@ -336,9 +337,10 @@ static const char* attention_fault(const drhip_attention_t* a, int grad) {
     if (a->d < 1 || a->d > 128) return "head size outside 1..128";
     if (a->lq >= 1 << 28 || a->lk >= 1 << 28) return "more than 2^28 rows";
     const int64_t heads = (int64_t)a->batch * a->hq;
-    // (one launch packs keys and values, in the gradient q and dout as well)
+    // (one launch packs keys and values, in the gradient q and dout as well; few rows against a long cache pack nothing)
     const int64_t most = grad ? kMostBlocks / 2 : kMostBlocks;
-    if (heads >= most || heads * (a->lq / 32 + 1) >= most || heads * (a->lk / 32 + 1) >= most)
+    if (heads >= most || heads * (a->lq / 32 + 1) >= most ||
+        ((int64_t)a->batch * a->hkv * (a->lk / 32 + 1) >= most && heads && (grad || drhip_k_attention_packs(a))))
         return "more blocks than one launch holds";
     if (a->prefix_value < 0) return "negative prefix";
     if (!(a->scale >= -0x1p100f && a->scale <= 0x1p100f) || !(a->cap <= 0.f || (a->cap >= 0x1p-100f && a->cap <= 0x1p100f))) return "scale or cap outside 2^100";

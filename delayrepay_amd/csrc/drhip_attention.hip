@@ -1650,6 +1650,9 @@ extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad)
     return grad ? room_grad(*a, plan_parts(*a)).all : room_forward(*a, plan_forward(*a)).all;
 }
 
+// Whether the forward call packs its keys and values
+extern "C" int drhip_k_attention_packs(const drhip_attention_t* a) { return !plan_forward(*a).few; }
+
 extern "C" int drhip_k_attention(const drhip_attention_t* args, hipStream_t s) {
     const Args& a = *args;
     const Plan p = plan_forward(a);

@@ -209,6 +209,8 @@ def attention(q, k, v, *, scale=None, causal=False, start=None, lengths=None, pr
     exponentials of the scores (-inf for a row without keys), which `attention_grad` needs.
 
     One row and many, long caches and short: where the rows are few, blocks take ranges of the keys.
+    batch * heads * (rows + 32) is below 2**28, and for more than 64 rows of a key head batch * key heads *
+    (key rows + 32) as well (in the gradient both below 2**27).
     """
     q, k, v = _heads(q, k, v)
     how = _Mask(q, k, scale, causal, start, lengths, prefix, documents, slopes, cap)

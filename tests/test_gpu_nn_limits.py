@@ -93,3 +93,17 @@ def test_recorded_documents_of_64_bits():
         _same_bits([out.get()], [want])
 
 
+
+
+def test_caches_of_many_sequences():
+    """One token for each of 64 sequences of up to 65536 keys, 64 heads on 8 (17 GB if the sequences did not share their keys here)."""
+    b, hq, hkv, lk, d = 64, 64, 8, 65536, 64
+    q, k, v = _normal(5, (b, hq, 1, d), (1, hkv, lk, d), (1, hkv, lk, d))
+    lengths = (lk - 977 * np.arange(b)).astype(np.int32)
+    dev = [dr.array(q)] + [dr.broadcast_to(dr.array(x), (b, hkv, lk, d)) for x in (k, v)]
+    o, lse = (x.get() for x in nn.attention(*dev, causal=True, lengths=dr.array(lengths), with_lse=True))
+    for s, h in ((0, 0), (17, 63), (63, 20)):
+        n = int(lengths[s])
+        p = np.array([n - 1])
+        want = nn_oracle.head(q[s, h], k[0, h // 8, :n], v[0, h // 8, :n], p, np.ones((1, n), bool), d ** -0.5)
+        assert np.all(np.abs(o[s, h] - want["o"]) <= 2 * want["o_off"]) and np.all(np.abs(lse[s, h] - want["lse"]) <= 2 * want["lse_off"])

@@ -60,3 +60,21 @@ def test_argument_structs_have_the_size_of_the_header(tmp_path):
     source.write_text('#include <stdio.h>\n#include "drhip.h"\nint main(void) { printf("%zu", sizeof(drhip_renumber_t)); return 0; }\n')
     subprocess.run(["cc", "-I", os.path.join(ROOT, "include"), "-o", str(program), str(source)], check=True)
     assert int(subprocess.run([str(program)], capture_output=True, text=True, check=True).stdout) == hiprt.RENUMBER.size
+
+
+def test_caches_that_fit_the_device_are_not_refused():
+    """Blocks are counted by key heads, and only where keys are packed."""
+    import ctypes
+    from delayrepay_amd import hiprt
+
+    def work(batch, hq, hkv, lq, lk, d=128, grad=0):
+        args = hiprt.ATTENTION.pack(*[0] * 15, 0, *[0] * 25, batch, hq, hkv, lq, lk, d, 1, 0, 0, 0, 1.0, 0.0)
+        n = ctypes.c_uint64()
+        return hiprt.lib().drhip_attention_work(args, grad, ctypes.byref(n)), n.value
+    for batch, hq, hkv, lk in ((64, 64, 8, 65536), (64, 32, 8, 131072), (32, 64, 8, 131072), (256, 32, 8, 131072), (1 << 20, 2, 1, 3000), (1, 1, 1, (1 << 28) - 1)):
+        rc, n = work(batch, hq, hkv, 1, lk)
+        assert rc == 0 and n < 1 << 30, (batch, hq, hkv, lk)
+    assert work(64, 64, 8, 128, 65536)[0] == 0 and work(16, 64, 8, 128, 65536, grad=1)[0] == 0        # (bounds by heads of q refused both)
+    # what does not fit one launch still is
+    for bad in (dict(batch=64, hq=64, hkv=64, lq=128, lk=65536), dict(batch=64, hq=64, hkv=32, lq=1, lk=65536, grad=1), dict(batch=1 << 13, hq=64, hkv=1, lq=512, lk=8)):
+        assert work(**bad)[0] == 20002, bad
