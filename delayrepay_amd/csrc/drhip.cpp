@@ -36,6 +36,7 @@ extern "C" int drhip_k_attention(const drhip_attention_t* a, hipStream_t s);
 extern "C" int drhip_k_attention_grad(const drhip_attention_t* a, hipStream_t s);
 extern "C" int drhip_k_renumber(const drhip_renumber_t* a, int log, hipStream_t s);
 extern "C" uint64_t drhip_k_rotary_work(const drhip_rotary_t* p);
+extern "C" int64_t drhip_k_rotary_blocks(const drhip_rotary_t* p);
 extern "C" int drhip_k_rotary(const drhip_rotary_t* p, hipStream_t s);
 extern "C" int drhip_k_sample(const drhip_sample_t* p, hipStream_t s);
 
@@ -329,7 +330,7 @@ int drhip_cumsum(int kind, const void* in, void* out, size_t n) {
 // ---- operators of language models -----------------------------------------------
 
 // The launches count blocks in one dimension, of at most 2^32 threads
-static const int64_t kMostRows = int64_t(1) << 28, kMostBlocks = int64_t(1) << 23;
+static const int64_t kMostBlocks = int64_t(1) << 23;
 
 static const char* attention_fault(const drhip_attention_t* a, int grad) {
     if (a->batch < 0 || a->hq < 0 || a->hkv < 0 || a->lq < 0 || a->lk < 0) return "negative size";
@@ -401,7 +402,7 @@ static const char* rotary_fault(const drhip_rotary_t* p) {
     if (p->d < 1 || p->d > 512) return "head size outside 1..512";
     if (p->dims < 0 || p->dims > p->d || p->dims % 2) return "dims is not an even number of elements of a head";
     if (p->d_pad < p->d || p->d_pad % 4) return "bad d_pad";
-    if ((int64_t)p->batch * p->rows >= kMostRows || (int64_t)p->batch * p->rows * (p->heads / 8 + 1) >= 4 * kMostBlocks || p->heads >= 1 << 20)
+    if ((int64_t)p->batch * p->rows >= int64_t(1) << 32 || p->heads >= 1 << 20 || (!p->dweight && drhip_k_rotary_blocks(p) >= 2 * kMostBlocks))
         return "more rows than one launch holds";
     return nullptr;
 }

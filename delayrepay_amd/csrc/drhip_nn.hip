@@ -347,14 +347,21 @@ int grad_slots(const Rot& p) {
     return slots < 1 ? 1 : (int)slots;
 }
 
-template <typename T> void launch_rotary(const Rot& p, hipStream_t s) {
-    const int log = lanes_log_of(p);
+// Groups for each token's heads.  Two heads share the angles (4 x 4096 tokens of 40 heads of 128: 124 us; four heads
+// 129, eight 137), one where the rows would not fill the device
+int rotary_slots(const Rot& p) {
     const int64_t tokens = (int64_t)p.batch * p.rows;
-    // Two heads share the angles (4 x 4096 tokens of 40 heads of 128: 124 us; four heads 129, eight 137), one where
-    // the rows would not fill the device
-    const int slots = tokens * ((p.heads + 1) / 2) << log < 256 * 2048 ? p.heads : (p.heads + 1) / 2;
-    const int64_t groups = tokens * slots;
-    const unsigned blocks = (unsigned)(((groups << log) + kThreads - 1) / kThreads);
+    return tokens * ((p.heads + 1) / 2) << lanes_log_of(p) < 256 * 2048 ? p.heads : (p.heads + 1) / 2;
+}
+
+int64_t rotary_blocks(const Rot& p) {
+    return (((int64_t)p.batch * p.rows * rotary_slots(p) << lanes_log_of(p)) + kThreads - 1) / kThreads;
+}
+
+template <typename T> void launch_rotary(const Rot& p, hipStream_t s) {
+    const int log = lanes_log_of(p), slots = rotary_slots(p);
+    const int64_t groups = (int64_t)p.batch * p.rows * slots;
+    const unsigned blocks = (unsigned)rotary_blocks(p);
     if (wide_of(p))
         rotary_kernel<T, true><<<blocks, kThreads, 0, s>>>(p, log, slots, groups);
     else
@@ -1040,6 +1047,8 @@ extern "C" uint64_t drhip_k_rotary_work(const drhip_rotary_t* p) {
     if (!p->dweight) return 0;
     return (uint64_t)grad_slots(*p) * p->heads * p->d_pad * (p->is_double ? 8 : 4);
 }
+
+extern "C" int64_t drhip_k_rotary_blocks(const drhip_rotary_t* p) { return rotary_blocks(*p); }
 
 extern "C" int drhip_k_rotary(const drhip_rotary_t* p, hipStream_t s) {
     if (p->dweight)

@@ -78,3 +78,19 @@ def test_caches_that_fit_the_device_are_not_refused():
     # what does not fit one launch still is
     for bad in (dict(batch=64, hq=64, hkv=64, lq=128, lk=65536), dict(batch=64, hq=64, hkv=32, lq=1, lk=65536, grad=1), dict(batch=1 << 13, hq=64, hkv=1, lq=512, lk=8)):
         assert work(**bad)[0] == 20002, bad
+
+
+def test_rotary_counts_the_threads_of_its_launch():
+    """2^32 threads and more are refused by the library itself, fewer are not."""
+    import ctypes
+    from delayrepay_amd import hiprt
+
+    def work(batch, heads, rows, d):
+        args = hiprt.ROTARY.pack(*[0] * 8, 0, *[0] * 12, 0.0, 1.0, 1.0, 1.0, 0.0, batch, heads, rows, d, d, d, 0, 0, 0)
+        n = ctypes.c_uint64()
+        return hiprt.lib().drhip_rotary_work(args, ctypes.byref(n))
+    # heads of 264 take 64 lanes, for two heads where there are many: 2^27 of them are 2^32 threads
+    assert work(1, 8, 1 << 24, 264) == 20002 and work(1, 8, (1 << 24) - 4, 264) == 0
+    assert work(1, 1, 1 << 26, 264) == 20002 and work(1, 1, (1 << 26) - 4, 264) == 0
+    assert work(4, 1, 1 << 26, 8) == 0 and work(1 << 20, 1 << 19, 1 << 20, 8) == 20002
+    assert work(1 << 16, 1, 1 << 16, 8) == 20002
