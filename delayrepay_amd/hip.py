@@ -1323,6 +1323,21 @@ def _same_view(a, b):
             and a.dtype == b.dtype)
 
 
+def _reads_what_it_overwrites(a, dst):
+    """Whether writing `dst` changes what a kernel still has to read of the leaf `a`."""
+    if a.buf is dst.buf:
+        if _same_view(a, dst):
+            return False
+        at = to = 0
+    elif type(a.buf) is Borrowed and type(dst.buf) is Borrowed:       # two views of one memory may be taken over apart
+        at, to = a.buf.ptr, dst.buf.ptr
+    else:
+        return False
+    (lo, hi), (d_lo, d_hi) = _extent(a), _extent(dst)
+    size, d_size = a.dtype.itemsize, dst.dtype.itemsize
+    return at + lo * size < to + d_hi * d_size and to + d_lo * d_size < at + hi * size
+
+
 def _plan_write(tracer, root, dst):
     """Plan for launching traced `root` into the existing view `dst`; decides
     whether the kernel would read what it overwrites."""
@@ -1333,14 +1348,7 @@ def _plan_write(tracer, root, dst):
         if tuple(numpy.broadcast_shapes(gen, shape)) != tuple(shape):
             raise ValueError(f"could not broadcast input array from shape {tuple(gen)} "
                              f"into shape {tuple(shape)}")
-    hazard = False
-    d_lo, d_hi = _extent(dst)
-    for a in tracer.leaves:
-        if a.buf is dst.buf and not _same_view(a, dst):
-            a_lo, a_hi = _extent(a)
-            it = dst.dtype.itemsize
-            if a_lo * a.dtype.itemsize < d_hi * it and d_lo * it < a_hi * a.dtype.itemsize:
-                hazard = True
+    hazard = any(_reads_what_it_overwrites(a, dst) for a in tracer.leaves)
     if hazard:
         # the kernel will write a different allocation: lower it as not-in-place
         stand_in = ndarray(dst.shape, dst.dtype, _Elsewhere(dst.buf.nbytes), dst.offset,

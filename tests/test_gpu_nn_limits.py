@@ -107,3 +107,44 @@ def test_caches_of_many_sequences():
         p = np.array([n - 1])
         want = nn_oracle.head(q[s, h], k[0, h // 8, :n], v[0, h // 8, :n], p, np.ones((1, n), bool), d ** -0.5)
         assert np.all(np.abs(o[s, h] - want["o"]) <= 2 * want["o_off"]) and np.all(np.abs(lse[s, h] - want["lse"]) <= 2 * want["lse_off"])
+
+
+def _in_a_program_with_torch(script):
+    """A child process that imports torch first, as programs that use both do."""
+    r = subprocess.run([sys.executable, "-u", "-c", textwrap.dedent(script)], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "done" in r.stdout, r.stdout[-1500:] + r.stderr[-3000:]
+
+
+def test_writes_over_views_of_one_memory_taken_over_apart():
+    """They read everything before they write, as those of one view do."""
+    _in_a_program_with_torch("""
+        import torch
+        import numpy as np
+        torch.zeros(1, device="cuda")
+        import delayrepay_amd as dr
+        n = 3000000
+        for step in (1, 7, 100003):
+            for up in (True, False):
+                x = torch.arange(n, device="cuda", dtype=torch.float64)
+                head, tail = dr.from_dlpack(x[:n - step]), dr.from_dlpack(x[step:])
+                to, of = (tail, head) if up else (head, tail)
+                want = np.arange(n, dtype=np.float64)
+                for turn in range(3):
+                    to[...] = of * 0.5 + 1.0
+                    want[step if up else 0:n if up else n - step] = want[0 if up else step:n - step if up else n] * 0.5 + 1.0
+                dr.synchronize()
+                assert np.array_equal(x.cpu().numpy(), want), (step, up)
+        x = torch.arange(40.0, device="cuda").view(4, 10)
+        a, b = dr.from_dlpack(x[:, ::2]), dr.from_dlpack(x[:, 1::2])
+        a[:, 1:] = a[:, :-1] + 100.0            # (its memory has elements of b in between)
+        b[1:] = b[:-1] * -1.0
+        c = dr.from_dlpack(x.t())
+        c[...] = dr.from_dlpack(x).reshape((10, 4)) * 1.0
+        want = np.arange(40.0, dtype=np.float32).reshape(4, 10)
+        want[:, 2::2] = want[:, 0:-2:2] + 100
+        want[1:, 1::2] = -want[:-1, 1::2]
+        want.T[...] = want.reshape(10, 4).copy()
+        dr.synchronize()
+        assert np.array_equal(x.cpu().numpy(), want)
+        print("done")
+    """)
