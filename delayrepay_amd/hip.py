@@ -1363,16 +1363,19 @@ def _plan_write(tracer, root, dst):
 
 class _Elsewhere(Buffer):
     """Stands for "an allocation other than the source buffer, same layout" while
-    lowering a ping-pong write; owns no memory."""
+    lowering a ping-pong write, or for such an allocation's memory; owns none."""
 
     __slots__ = ()
 
-    def __init__(self, nbytes):
+    def __init__(self, nbytes, ptr=0):
         self.nbytes = nbytes
-        self.ptr = 0
+        self.ptr = ptr
         self.version = 0
         self.shadow = None
         self.shadow_region = None
+
+    def __del__(self):
+        pass
 
 
 def _write(plan, dst):
@@ -1395,13 +1398,17 @@ def _write(plan, dst):
         if borrowed and _RECORDING is not None:
             raise RuntimeError("hip.record(): an update that reads what it overwrites cannot be recorded "
                                "for an array taken over from another library")
-        if buf.shadow_region != plan.region:
-            hiprt.memcpy_d2d(buf.shadow, buf.ptr, buf.nbytes)
-        _fire(plan, [buf.shadow + off])
         if borrowed:
-            hiprt.memcpy_d2d(buf.ptr, buf.shadow, buf.nbytes)
-            buf.touch()
+            # the elements between those of the view are the other library's: neither read nor written
+            _fire(plan, [buf.shadow + off])
+            mirror = _Elsewhere(buf.nbytes, buf.shadow)
+            tracer = Tracer()
+            root = tracer.leaf(ndarray(dst.shape, dst.dtype, mirror, dst.offset, dst._strides))
+            _write(_plan_write(tracer, root, dst), dst)
         else:
+            if buf.shadow_region != plan.region:
+                hiprt.memcpy_d2d(buf.shadow, buf.ptr, buf.nbytes)
+            _fire(plan, [buf.shadow + off])
             buf.ptr, buf.shadow = buf.shadow, buf.ptr
             buf.shadow_region = plan.region
             buf.version += 1

@@ -35,3 +35,20 @@ def test_types_and_pitches_of_overlapping_views():
     assert _plan(_taken(base, 10, strides=(3,)), _taken(base + 108, 10)).hazard
     assert not _plan(_taken(base, 10, strides=(3,)), _taken(base + 112, 10)).hazard
     assert not _plan(hip.placeholder((100,), np.float32), _taken(base, 100)).hazard
+
+
+def test_only_the_view_is_copied_back(monkeypatch):
+    """What stands between the elements of a view belongs to the other library: no copy passes over it."""
+    fired, base, shadow = [], 1 << 33, 1 << 34
+    monkeypatch.setattr(hip, "_fire", lambda plan, outs: fired.append((plan, outs)))
+    monkeypatch.setattr(hip.hiprt, "malloc", lambda nbytes: shadow)
+    monkeypatch.setattr(hip.hiprt, "memcpy_d2d", lambda *args: pytest.fail("a copy of the whole span"))
+    whole = _taken(base, 10, strides=(3,))
+    dst, src = whole[1:], whole[:-1]
+    hip._write(_plan(dst, src), dst)
+    whole.buf.shadow = None
+    (first, to_shadow), (second, to_memory) = fired
+    assert first.hazard and to_shadow == [shadow + 12] and [a.ptr for a in first.leaves] == [base]
+    assert not second.hazard and to_memory == [base + 12]
+    assert [(a.ptr, a.shape, a._strides) for a in second.leaves] == [(shadow + 12, (9,), (3,))]
+    assert whole.buf.ptr == base and whole.buf.version > 0
