@@ -627,11 +627,15 @@ class NumpyEx(DelayArray, metaclass=Memoiser):
         d.pop("_plan", None)
         d.pop("_multi", None)
         d.pop("_gen", None)
-        key = d.get("_key")
-        if key is not None and Memoiser._cache.get(key) is self:
-            Memoiser._cache.pop(key)
+        self._unlist()
         self.children = []
         self._depth = 0
+
+    def _unlist(self):
+        """Building the same expression again makes a new node from now on."""
+        key = self.__dict__.get("_key")
+        if key is not None and Memoiser._cache.get(key) is self:
+            Memoiser._cache.pop(key)
 
     @classmethod
     def _memo_key(cls, func, *children):

@@ -70,8 +70,10 @@ class Borrowed(Buffer):
     that read what they overwrite copy back instead of swapping allocations (hip._write)."""
 
     __slots__ = ("owner",)
+    taken = False      # whether there ever was one
 
     def __init__(self, nbytes, ptr, owner):
+        Borrowed.taken = True
         self.owner = None
         super().__init__(nbytes, ptr)
         self.owner = owner
@@ -462,9 +464,10 @@ _DL_KINDS = {0: "int", 1: "uint", 2: "float", 6: "bool"}
 def from_dlpack(x):
     """Array over the memory of another library's device array, without a copy (host arrays
     are uploaded).  Work queued there before the call is waited for on the device; later
-    work, in either direction, is for the caller to order (`synchronize()`).  Take each array
-    over once and keep it: two arrays over one memory do not see each other's writes as
-    changes of a cached result."""
+    work, in either direction, is for the caller to order (`synchronize()`).  What was computed
+    from the array keeps its value when the other library writes to the memory; the same
+    expression built again is computed again.  Take each array over once and keep it: two
+    arrays over one memory do not see each other's writes as changes of a cached result."""
     device_type, device = x.__dlpack_device__()
     if device_type in _DL_HOST:
         return ndarray.from_host(np.from_dlpack(x))

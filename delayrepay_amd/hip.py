@@ -1208,6 +1208,17 @@ def _run_unfused(ex, evaluated):
     return out
 
 
+def _computed(ex, deps, generation):
+    """Note what the result of `ex` was computed from.  Writes of another library to its memory are not
+    seen here, so a result of such memory is not found again when the same expression is built again."""
+    d = ex.__dict__
+    d["_deps"], d["_gen"] = deps, generation
+    if Borrowed.taken and any(type(dep[0]) is Borrowed for dep in deps):
+        unlist = getattr(ex, "_unlist", None)
+        if unlist is not None:
+            unlist()
+
+
 def run(ex):
     """Evaluate one DAG root; returns a new device array owned by the caller
     (cf. cuda.py:91-96)."""
@@ -1249,8 +1260,7 @@ def run(ex):
     out = _launch_fresh(plan)[0]
     if out.shape != tuple(ex.shape) and _kind(ex) == "ReduceEx":
         out = out.reshape(tuple(ex.shape))      # the reduced axes kept, or a row kernel's column
-    d["_deps"] = plan.deps()
-    d["_gen"] = plan.generation()
+    _computed(ex, plan.deps(), plan.generation())
     return out
 
 
@@ -1300,8 +1310,7 @@ def run_multi(exs):
             if out.shape != shape:   # every leaf of this root was a broadcast scalar
                 out = materialise(out, shape=shape)
             results[i] = out
-            exs[i].__dict__["_deps"] = deps
-            exs[i].__dict__["_gen"] = gen
+            _computed(exs[i], deps, gen)
     return results
 
 

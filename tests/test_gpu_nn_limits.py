@@ -148,3 +148,39 @@ def test_writes_over_views_of_one_memory_taken_over_apart():
         assert np.array_equal(x.cpu().numpy(), want)
         print("done")
     """)
+
+
+def test_what_is_computed_of_another_librarys_array_follows_its_writes():
+    """An expression that is built again after the other library wrote is computed again."""
+    _in_a_program_with_torch("""
+        import torch
+        import numpy as np
+        torch.zeros(1, device="cuda")
+        import delayrepay_amd as dr
+        from delayrepay_amd import nn
+        t = torch.arange(6.0, device="cuda").view(2, 3)
+        a = dr.from_dlpack(t)
+        held = a + 1.0
+        first = held.get()
+        kept = dr.array(np.ones((2, 3), np.float32))
+        for turn in range(1, 4):
+            before = [(a + 1.0).get(), (a * 2.0 + 3.0).sum(axis=1).get(), dr.sum(a).get(), (kept * a).get()]
+            t += 10.0
+            torch.cuda.synchronize()
+            x = np.arange(6.0, dtype=np.float32).reshape(2, 3) + 10 * turn
+            got = [(a + 1.0).get(), (a * 2.0 + 3.0).sum(axis=1).get(), dr.sum(a).get(), (kept * a).get(), ((a + 1.0) * 2.0).get()]
+            for y, want in zip(got, (x + 1, (x * 2 + 3).sum(1), x.sum(), x, (x + 1) * 2)):
+                assert np.allclose(y, want), (turn, y, want)
+        x = torch.randn(1, 2, 40, 32, device="cuda")
+        q = dr.from_dlpack(x)
+        for _ in range(3):
+            x.normal_()
+            torch.cuda.synchronize()
+            o = nn.attention(q * 2.0, q, q).get()
+            s = torch.softmax(2 * x @ x.transpose(2, 3) / 32 ** 0.5, -1) @ x
+            assert np.abs(o - s.cpu().numpy()).max() < 1e-5
+        # this library's own writes are followed by what is held, as ever
+        a[...] = 0.0
+        assert np.array_equal(held.get(), np.ones((2, 3)))
+        print("done")
+    """)
