@@ -139,17 +139,19 @@ struct Three {
     bf16x8 p[3];
 };
 
-__device__ __forceinline__ void split2(f32x2 x, int at, Three& out) {
+// (numbers past bfloat16's largest would round to infinity)
+__device__ __forceinline__ float in_range(float x) { return __builtin_amdgcn_fmed3f(x, -3.3895313892515355e38f, 3.3895313892515355e38f); }
+
+// With FULL x may be any finite number (one past bfloat16's largest is that and the rest); a NaN or an infinity has a NaN
+// among its parts
+template <bool FULL = false> __device__ __forceinline__ void split2(f32x2 x, int at, Three& out) {
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
-        const bf16x2 y = __builtin_convertvector(x, bf16x2);
+        const bf16x2 y = __builtin_convertvector(FULL && n == 0 ? f32x2{in_range(x[0]), in_range(x[1])} : x, bf16x2);
         out.p[n][at] = y[0], out.p[n][at + 1] = y[1];
         if (n < 2) x = x - __builtin_convertvector(y, f32x2);
     }
 }
-
-// (numbers past bfloat16's largest would round to infinity)
-__device__ __forceinline__ float in_range(float x) { return __builtin_amdgcn_fmed3f(x, -3.3895313892515355e38f, 3.3895313892515355e38f); }
 
 __device__ __forceinline__ f32x16 mac6(const Three& a, const Three& b, f32x16 c) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
@@ -405,7 +407,7 @@ template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Arg
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             fine = fine && finite_(x[c]);
-            lds[row][d + c] = finite_(x[c]) ? in_range(x[c]) : 0.f;
+            lds[row][d + c] = finite_(x[c]) ? x[c] : 0.f;
         }
         if (!fine) atomicOr(&bad, 1u << row);
     }
@@ -429,7 +431,7 @@ template <int NT> __global__ __launch_bounds__(kThreads) void attention_pack(Arg
         Three x;
         const int row = at & 31, chunk = at >> 5;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) split2(f32x2{lds[row][8 * chunk + e], lds[row][8 * chunk + e + 1]}, e, x);
+        for (int e = 0; e < 8; e += 2) split2<true>(f32x2{lds[row][8 * chunk + e], lds[row][8 * chunk + e + 1]}, e, x);
 #pragma unroll
         for (int k = 0; k < 3; ++k) *(bf16x8*)(to + k * Planes<NT>::PLANE + Planes<NT>::place(row, chunk)) = x.p[k];
     }
@@ -560,8 +562,8 @@ __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
             const f32x4 x = load4(qrow, 16 * t + 8 * h + e, a.d, valid, wide) * scale;
-            split2(f32x2{x[0], x[1]}, e, own[t]);
-            split2(f32x2{x[2], x[3]}, e + 2, own[t]);
+            split2<true>(f32x2{x[0], x[1]}, e, own[t]);
+            split2<true>(f32x2{x[2], x[3]}, e + 2, own[t]);
         }
     }
 
@@ -1064,11 +1066,11 @@ __device__ __forceinline__ void grad_dq(const Args& a, const Plan& plan, int til
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
             const f32x4 x = load4(qrow, 16 * t + 8 * h + e, a.d, lim > 0, wide) * scale;
-            split2(f32x2{x[0], x[1]}, e, own[t]);
-            split2(f32x2{x[2], x[3]}, e + 2, own[t]);
+            split2<true>(f32x2{x[0], x[1]}, e, own[t]);
+            split2<true>(f32x2{x[2], x[3]}, e + 2, own[t]);
             const f32x4 y = load4(grow, 16 * t + 8 * h + e, a.d, lim > 0, wide);
-            split2(f32x2{y[0], y[1]}, e, dout[t]);
-            split2(f32x2{y[2], y[3]}, e + 2, dout[t]);
+            split2<true>(f32x2{y[0], y[1]}, e, dout[t]);
+            split2<true>(f32x2{y[2], y[3]}, e + 2, dout[t]);
         }
     }
 
@@ -1206,11 +1208,11 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
             const f32x4 x = load4(krow, 16 * t + 8 * h + e, a.d, counts, wide) * scale;
-            split2(f32x2{x[0], x[1]}, e, key[t]);
-            split2(f32x2{x[2], x[3]}, e + 2, key[t]);
+            split2<true>(f32x2{x[0], x[1]}, e, key[t]);
+            split2<true>(f32x2{x[2], x[3]}, e + 2, key[t]);
             const f32x4 y = load4(vrow, 16 * t + 8 * h + e, a.d, counts, wide);
-            split2(f32x2{y[0], y[1]}, e, val[t]);
-            split2(f32x2{y[2], y[3]}, e + 2, val[t]);
+            split2<true>(f32x2{y[0], y[1]}, e, val[t]);
+            split2<true>(f32x2{y[2], y[3]}, e + 2, val[t]);
         }
     }
     f32x16 dk[NT], dv[NT];

@@ -203,7 +203,8 @@ def attention(q, k, v, *, scale=None, causal=False, start=None, lengths=None, pr
     `documents` (batch, key rows) if its document is the one at the row's position (rows outside the
     sequence have none).  A row without keys gives zeros.  Keys that do not count may hold anything, also
     what is not finite; a pair that counts gives NaN if its q or k is not finite.  `start` lies within 2**30
-    of 0, `scale` within 2**100 of 0 and `cap` between 2**-100 and 2**100.
+    of 0, `scale` within 2**100 of 0 and `cap` between 2**-100 and 2**100.  Sums are float32 and divided last: scores,
+    and values times the number of keys, lie below 2**127; past that results are infinite or NaN.
 
     `with_lse` returns (output, lse): lse (batch, heads, rows), the logarithm of the sum of the
     exponentials of the scores (-inf for a row without keys), which `attention_grad` needs.
@@ -224,7 +225,8 @@ def attention_grad(dout, q, k, v, o, lse, *, scale=None, causal=False, start=Non
     """(dq, dk, dv) of `attention` from the gradient of its output, its operands, output and lse.
 
     A key head's gradients are summed over the heads of q that share it.  The sums do not depend on
-    timing: equal calls give equal bits.  `slopes` are constants.
+    timing: equal calls give equal bits.  `slopes` are constants.  What of the operands is not finite, or
+    passes float32 in a sum, makes the gradients that it enters infinite or NaN.
     """
     q, k, v = _heads(q, k, v)
     dout = _shaped(_floats(dout, "dout", 4), "dout", q.shape)

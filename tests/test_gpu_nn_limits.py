@@ -109,6 +109,44 @@ def test_caches_of_many_sequences():
         assert np.all(np.abs(o[s, h] - want["o"]) <= 2 * want["o_off"]) and np.all(np.abs(lse[s, h] - want["lse"]) <= 2 * want["lse_off"])
 
 
+def _near(got, want, names):
+    """Within twice the oracle's bounds.  These count relative roundings; what lies below the smallest normal number, 2^-126,
+    may become zero besides: of each sum at most 6 products (the parts of a float32 one) of 200 pairs, 2^-115 in all."""
+    for x, name in zip(got, names):
+        off = 2 * want[name + "_off"] + 2.0 ** -115
+        fine = bool(np.all((x == want[name]) | (np.abs(x.astype(np.float64) - want[name]) <= off)))
+        assert fine, (name, np.abs(x - want[name]).max(), off.max())
+
+
+@pytest.mark.parametrize("lq", [5, 90])
+def test_operands_next_to_the_largest(lq):
+    """Finite numbers above bfloat16's largest, 3.39e38, are what they are, in packed operands and others.  What meets
+    them is small and has one bit, so that the products are exact."""
+    big = np.float32(3.395e38)
+    one = np.float32(2.0 ** -126)
+    names = ("o", "lse", "dq", "dk", "dv")
+    shapes = (2, 2, lq, 64), (2, 2, lq, 64), (2, 1, 130, 64), (2, 1, 130, 64)
+    docs = np.zeros((2, 130), np.int32)
+    # (a cap: without one the scale of q takes in log2 e, and its products with k would have more bits)
+    how = dict(scale=1.0, cap=50.0, documents=docs)
+    q, g, k, v = _normal(6, *shapes)
+    q, k, g = q * np.float32(0.1), k * np.float32(0.1), g * np.float32(1e-3)
+    q[..., 3] = np.where(np.arange(lq) % 3, 0, one)
+    k[:, :, :, 3] = np.where(np.arange(130) % 5, 0, big)
+    _near(_all(q, k, v, g, **how), nn_oracle.attention(q, k, v, dout=g, **how), names)
+    q, g, k, v = _normal(7, *shapes)
+    q, k, g = q * np.float32(0.1), k * np.float32(0.1), g * np.float32(1e-3)
+    k[..., 3] = np.where(np.arange(130) % 3, 0, one)
+    q[:, :, :, 3] = np.where(np.arange(lq) % 4, 0, big)
+    _near(_all(q, k, v, g, **how)[:3], nn_oracle.attention(q, k, v, dout=g, **how), names[:3])
+    q, g, k, v = _normal(8, *shapes)
+    v[:, :, 77, 5], g[..., 5] = -big, 0
+    _near(_all(q, k, v, g, documents=docs), nn_oracle.attention(q, k, v, dout=g, documents=docs), names)
+    q, g, k, v = _normal(9, *shapes)
+    g[:, 0, 2, 5], v[..., 5] = big, np.float32(2.0 ** -100)
+    _near(_all(q, k, v, g, documents=docs), nn_oracle.attention(q, k, v, dout=g, documents=docs), names)
+
+
 def _in_a_program_with_torch(script):
     """A child process that imports torch first, as programs that use both do."""
     r = subprocess.run([sys.executable, "-u", "-c", textwrap.dedent(script)], cwd=ROOT, capture_output=True, text=True, timeout=100)
