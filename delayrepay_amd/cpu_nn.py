@@ -48,6 +48,8 @@ def _scores(q, k, p, ok, slope, how):
     """Scores of one head, and tanh of the capped ones."""
     with np.errstate(invalid="ignore"):
         s, t = q @ k.T * how.scale, None
+    s[~np.isfinite(q).all(1)] = np.nan
+    s[:, ~np.isfinite(k).all(1)] = np.nan
     if how.cap is not None:
         t = np.tanh(s / how.cap)
         s = how.cap * t

@@ -723,7 +723,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
     const float* qrow = a.q + b * a.q_stride[0] + qh * a.q_stride[1] + i * a.q_stride[2];
     f32x4 own[KS];
 #pragma unroll
-    for (int t = 0; t < KS; ++t) own[t] = load4(qrow, 16 * t + 4 * h, a.d, valid, wide) * a.scale;
+    for (int t = 0; t < KS; ++t) {
+        own[t] = load4(qrow, 16 * t + 4 * h, a.d, valid, wide) * a.scale;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) own[t][c] = finite_(own[t][c]) ? own[t][c] : __builtin_nanf("");      // (an infinity could give -inf, a pair without weight)
+    }
     int top = lim, low = valid ? lim : 0x7fffffff;
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) {

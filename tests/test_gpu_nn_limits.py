@@ -147,6 +147,26 @@ def test_operands_next_to_the_largest(lq):
     _near(_all(q, k, v, g, documents=docs), nn_oracle.attention(q, k, v, dout=g, documents=docs), names)
 
 
+@pytest.mark.parametrize("lq", [5, 90])
+@pytest.mark.parametrize("what", [INF, -INF, NAN])
+def test_rows_that_are_not_finite(lq, what):
+    """A pair that counts gives NaN if its q or k is not finite, whatever sign their product has; rows beside it keep their values."""
+    q, g, k, v = _normal(10, (2, 2, lq, 64), (2, 2, lq, 64), (2, 1, 130, 64), (2, 1, 130, 64))
+    k = np.abs(k)
+    docs = np.zeros((2, 130), np.int32)
+    clean = nn_oracle.attention(q, k, v, documents=docs)
+    q[0, 1, 3, 7] = what
+    q[1, 0, 2] = what
+    o, lse, dq, dk, dv = _all(q, k, v, g, documents=docs)
+    bad = np.zeros((2, 2, lq), bool)
+    bad[0, 1, 3] = bad[1, 0, 2] = True
+    assert np.isnan(o[bad]).all() and np.isnan(lse[bad]).all() and np.isnan(dq[bad]).all()
+    assert np.all(np.abs(o - clean["o"])[~bad] <= 2 * clean["o_off"][~bad]) and np.isfinite(lse[~bad]).all() and np.isfinite(dq[~bad]).all()
+    # a row without keys does not look at what it holds
+    o, lse, dq, dk, dv = _all(q, k, v, g, documents=docs, lengths=0)
+    assert not (o.any() or dq.any() or dk.any() or dv.any()) and np.all(lse == -INF)
+
+
 def _in_a_program_with_torch(script):
     """A child process that imports torch first, as programs that use both do."""
     r = subprocess.run([sys.executable, "-u", "-c", textwrap.dedent(script)], cwd=ROOT, capture_output=True, text=True, timeout=100)

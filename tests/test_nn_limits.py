@@ -94,3 +94,34 @@ def test_rotary_counts_the_threads_of_its_launch():
     assert work(1, 1, 1 << 26, 264) == 20002 and work(1, 1, (1 << 26) - 4, 264) == 0
     assert work(4, 1, 1 << 26, 8) == 0 and work(1 << 20, 1 << 19, 1 << 20, 8) == 20002
     assert work(1 << 16, 1, 1 << 16, 8) == 20002
+
+
+def test_pairs_that_are_not_finite():
+    """A pair that counts gives NaN if its q or k is not finite, whatever sign their product has."""
+    _child("""
+        import numpy as np
+        import delayrepay as dnp
+        rs = np.random.RandomState(3)
+        q, k, v, g = (rs.standard_normal(s).astype(np.float32) for s in ((1, 1, 4, 8), (1, 1, 6, 8), (1, 1, 6, 8), (1, 1, 4, 8)))
+        k = np.abs(k)
+
+        def run(q, k):
+            dev = [dnp.array(x) for x in (q, k, v, g)]
+            o, lse = dnp.nn.attention(*dev[:3], causal=True, start=0, with_lse=True)
+            return [x.get()[0, 0] for x in (o, lse, *dnp.nn.attention_grad(dev[3], *dev[:3], o, lse, causal=True, start=0))]
+        clean = run(q, k)
+        for what in (np.inf, -np.inf, np.nan):
+            bad = q.copy()
+            bad[0, 0, 1, 3] = what
+            o, lse, dq, dk, dv = run(bad, k)
+            assert np.isnan(o[1]).all() and np.isnan(lse[1]) and np.isnan(dq[1]).all()
+            for x, y in zip((o, lse, dq), clean):
+                assert np.array_equal(np.delete(x, 1, 0), np.delete(y, 1, 0))
+            assert np.isnan(dk[:2]).any()
+            for x, y in zip((dk, dv), clean[3:]):          # (sums in 64 bits in another order, rounded to 32)
+                assert np.allclose(x[2:], y[2:], rtol=2.0 ** -23, atol=1e-12)
+            bad = k.copy()
+            bad[0, 0, 2, 5] = what
+            o, lse, dq, dk, dv = run(q, bad)
+            assert np.isnan(o[2:]).all() and np.array_equal(o[:2], clean[0][:2]) and np.array_equal(dq[:2], clean[2][:2])
+    """, DELAY_CPU="1")
