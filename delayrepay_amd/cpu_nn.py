@@ -97,7 +97,7 @@ def attention_grad(dout, q, k, v, o, lse, how, outs):
             row = np.isfinite(lse[b, h])[:, None] | np.isnan(lse[b, h])[:, None]
             qq, g = (np.where(row, x[b, h], 0.0).astype(np.float64) for x in (q, dout))
             s, t = _scores(qq, kk, p, ok & row, slope, how)
-            w = np.exp(s - np.where(row, lse[b, h][:, None], 0.0))
+            w = np.where(ok & row, np.exp(s - np.where(row, lse[b, h][:, None], 0.0)), 0.0)      # (a row's lse may be NaN)
             with np.errstate(invalid="ignore"):
                 d = g @ vv.T - (g * np.where(row, o[b, h], 0.0)).sum(1, keepdims=True)
                 ds = np.where(ok & row, w * d * (how.scale if t is None else how.scale * (1.0 - t * t)), 0.0)
