@@ -1200,8 +1200,10 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
     const int key0 = tile * kRows, j = key0 + wave * 32 + (lane & 31);
     const bool valid = j < a.lk, counts = j < s.len;
     const int doc = s.docs && counts ? s.docs[j] : 0;
-    // the first row that sees the key
-    const int need = !counts ? 0x7fffffff : a.causal && j >= s.prefix ? max(j - s.start, 0) : 0;
+    // the first row that may see the key, and how many: with documents rows inside the sequence alone.  (The rest of the
+    // last tile is no row: a key that is not finite would make its pairs NaN.)
+    const int need = max(max(a.causal && j >= s.prefix ? j - s.start : 0, s.docs ? -s.start : 0), 0);
+    const unsigned sees = counts ? max((s.docs ? min(a.lq, s.len - s.start) : a.lq) - need, 0) : 0;
 
     const float scale = CAP ? a.scale : a.scale * kLog2e;
     Three key[2 * NT], val[2 * NT];
@@ -1225,7 +1227,7 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
 #pragma unroll
         for (int v = 0; v < 16; ++v) dk[c][v] = 0.f, dv[c][v] = 0.f;
 
-    int dlo = counts ? doc : 0x7fffffff, dhi = counts ? doc : -0x7fffffff - 1, all = need;
+    int dlo = counts ? doc : 0x7fffffff, dhi = counts ? doc : -0x7fffffff - 1, all = counts ? need : 0x7fffffff;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
         dlo = min(dlo, __shfl_xor(dlo, m));
@@ -1321,7 +1323,7 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
             const int from = need - i0 - 4 * h;
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                const bool ok = acc_row(v, 0) >= from && counts && (same >> v & 1);
+                const bool ok = (unsigned)(acc_row(v, 0) - from) < sees && (same >> v & 1);
                 x[v] = nans >> acc_row(v, 0) & 1 ? __builtin_nanf("") : x[v];
                 x[v] = ok ? x[v] : -__builtin_inff();
             }

@@ -167,6 +167,33 @@ def test_rows_that_are_not_finite(lq, what):
     assert not (o.any() or dq.any() or dk.any() or dv.any()) and np.all(lse == -INF)
 
 
+def test_rows_outside_the_sequence_belong_to_no_document():
+    """Not to document 0 either: a key of document 0 that no row sees may hold anything, and its gradient is zero."""
+    q, g, k, v = _normal(11, (1, 2, 60, 64), (1, 2, 60, 64), (1, 1, 100, 64), (1, 1, 100, 64))
+    docs = np.ones((1, 100), np.int32)
+    docs[0, 10:14], docs[0, 98:] = 0, 2
+    how = dict(documents=docs, start=70)                  # rows at 70 to 129: 100 and 101 are outside, in a tile with documents 1 and 2
+    want = nn_oracle.attention(q, k, v, dout=g, **how)
+    k[0, 0, 10:14], v[0, 0, 12] = [[NAN], [INF], [-INF], [1.0]], NAN
+    got = _all(q, k, v, g, **how)
+    _near(got, want, ("o", "lse", "dq", "dk", "dv"))
+    assert not got[3][0, 0, 10:14].any() and not got[4][0, 0, 10:14].any()
+
+
+@pytest.mark.parametrize("lq", [1, 10, 33, 64, 200])
+def test_keys_that_no_row_sees_have_no_gradient(lq):
+    """Behind the last row, in front of the first one's document, behind the length: they may hold anything."""
+    q, g, k, v = _normal(12, (2, 4, lq, 64), (2, 4, lq, 64), (2, 2, 300, 64), (2, 2, 300, 64))
+    for how in (dict(causal=True, start=0), dict(causal=True, start=np.array([3, 50], np.int32)), dict(causal=True, start=2, cap=5.0, slopes=np.ones(4, np.float32))):
+        want = nn_oracle.attention(q, k, v, dout=g, **how)
+        hidden = k.copy(), v.copy()
+        for b in range(2):
+            last = lq + (how["start"] if np.ndim(how["start"]) == 0 else how["start"][b])
+            hidden[0][b, :, last::2], hidden[0][b, :, last + 1::4], hidden[1][b, :, last:, 3] = NAN, INF, -INF
+        got = _all(q, *hidden, g, **how)
+        _near(got, want, ("o", "lse", "dq", "dk", "dv"))
+
+
 def _in_a_program_with_torch(script):
     """A child process that imports torch first, as programs that use both do."""
     r = subprocess.run([sys.executable, "-u", "-c", textwrap.dedent(script)], cwd=ROOT, capture_output=True, text=True, timeout=100)
