@@ -156,7 +156,8 @@ def sample(logits, uniforms, temperature, top_k, top_p, min_p, outs):
     batch, vocabulary = logits.shape
     tokens = np.full(batch, -1, np.int64)
     for b in range(batch):
-        t, k, p, m = (x if isinstance(x, (int, float)) else x[b].item() for x in (temperature, top_k, top_p, min_p))
+        t, k, p, m, u = (x if isinstance(x, (int, float)) else x[b].item() for x in (temperature, top_k, top_p, min_p, uniforms))
+        t, p, m, u = (0.0 if x != x else min(x, 3.4028234663852886e38) for x in (t, p, m, u))
         row = np.where(np.isnan(logits[b]), -np.inf, logits[b].astype(np.float64))
         order = np.argsort(-row, kind="stable")
         top = row[order[0]]
@@ -174,10 +175,10 @@ def sample(logits, uniforms, temperature, top_k, top_p, min_p, outs):
             keep = before < p * w.sum()
             keep[0] = True
             w[~keep] = 0.0
-        w[w < min(max(m, 0.0) if m == m else 0.0, 1.0)] = 0.0
+        w[w < min(max(m, 0.0), 1.0)] = 0.0
         by_number = np.zeros(vocabulary)
         by_number[order] = w
         run = np.cumsum(by_number)
-        hit = np.flatnonzero((run > float(uniforms[b]) * run[-1]) & (by_number > 0))
+        hit = np.flatnonzero((run > u * run[-1]) & (by_number > 0))
         tokens[b] = hit[0] if len(hit) else np.flatnonzero(by_number)[-1]
     return _out(outs, [tokens], np.int64)

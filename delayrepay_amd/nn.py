@@ -334,7 +334,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     ones of at least that part of the largest.  The token is the first one, by number, at which the
     kept weights summed up exceed uniforms[row] (in [0, 1): `random.device().random(batch)`) of their sum.
     A temperature of 0 takes the largest; they go up to float32's largest.  Each of the four is a number or an array (batch,), float32 or
-    (top_k) integers, in which a top_k below 1 stands for all and numbers out of range for the nearest in it.
+    (top_k) integers, in which a top_k below 1 stands for all, numbers out of range for the nearest in it and NaN for 0.
     A logit that is NaN or -inf is never drawn; a row without another gives -1.
 
     Sums are whole numbers of 62 bits: the token depends on no order of summation.

@@ -194,6 +194,20 @@ def test_keys_that_no_row_sees_have_no_gradient(lq):
         _near(got, want, ("o", "lse", "dq", "dk", "dv"))
 
 
+def test_parameters_of_sampling_that_are_not_numbers():
+    """NaN in an array of parameters, or as a uniform number, counts as 0."""
+    rs = np.random.RandomState(12)
+    logits = (rs.standard_normal((3, 700)) * 2).astype(np.float32)
+    logits[:, ::2] = -INF
+    nan, zero = dr.array(np.full(3, NAN)), dr.array(np.zeros(3, np.float32))
+    dev, u = dr.array(logits), dr.array(np.array([0.1, 0.5, 0.99]))
+    for name in ("temperature", "top_p", "min_p"):
+        assert nn.sample(dev, u, **{name: nan}).get().tolist() == nn.sample(dev, u, **{name: zero}).get().tolist(), name
+    assert nn.sample(dev, nan).get().tolist() == nn.sample(dev, zero).get().tolist()
+    got = nn.sample(dev, u, temperature=dr.array(np.full(3, INF))).get()
+    assert got.tolist() == [nn_oracle.sample(r, x, temperature=1e300) for r, x in zip(logits, (0.1, 0.5, 0.99))]
+
+
 def _in_a_program_with_torch(script):
     """A child process that imports torch first, as programs that use both do."""
     r = subprocess.run([sys.executable, "-u", "-c", textwrap.dedent(script)], cwd=ROOT, capture_output=True, text=True, timeout=100)

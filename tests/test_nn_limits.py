@@ -125,3 +125,23 @@ def test_pairs_that_are_not_finite():
             o, lse, dq, dk, dv = run(q, bad)
             assert np.isnan(o[2:]).all() and np.array_equal(o[:2], clean[0][:2]) and np.array_equal(dq[:2], clean[2][:2])
     """, DELAY_CPU="1")
+
+
+def test_parameters_of_sampling_that_are_not_numbers():
+    """NaN counts as 0, an infinite temperature as the largest: neither draws what has no weight."""
+    _child("""
+        import numpy as np
+        import delayrepay as dnp
+        from oracle import nn_oracle
+        rs = np.random.RandomState(4)
+        logits = (rs.standard_normal((3, 70)) * 2).astype(np.float32)
+        logits[:, ::2], logits[1, 1] = -np.inf, np.nan
+        f = lambda x: dnp.array(np.full(3, x, np.float32))
+        u = dnp.array(np.array([0.1, 0.5, 0.99]))
+        for name in ("temperature", "top_p", "min_p"):
+            got, want = (dnp.nn.sample(dnp.array(logits), u, **{name: f(x)}).get().tolist() for x in (np.nan, 0.0))
+            assert got == want, name
+        assert dnp.nn.sample(dnp.array(logits), f(np.nan)).get().tolist() == dnp.nn.sample(dnp.array(logits), f(0.0)).get().tolist()
+        got = dnp.nn.sample(dnp.array(logits), u, temperature=f(np.inf)).get()
+        assert got.tolist() == [nn_oracle.sample(r, x, temperature=1e300) for r, x in zip(logits, (0.1, 0.5, 0.99))]
+    """, DELAY_CPU="1")
