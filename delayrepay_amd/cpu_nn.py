@@ -60,10 +60,15 @@ def _scores(q, k, p, ok, slope, how):
 
 def _weighted(w, x):
     """w @ x in which a weight of zero takes nothing, whatever x holds."""
-    if np.isfinite(x).all():
+    fine = np.isfinite(x)
+    if fine.all():
         return w @ x
     with np.errstate(invalid="ignore"):
-        return np.where(w[:, :, None] != 0, w[:, :, None] * x[None], 0.0).sum(1)
+        y = w @ np.where(fine, x, 0.0)
+        for j in np.flatnonzero(~fine.all(1)):
+            rows = np.flatnonzero(w[:, j])
+            y[rows] += w[rows, j, None] * np.where(fine[j], 0.0, x[j])
+    return y
 
 
 def attention(q, k, v, how, outs):

@@ -145,3 +145,31 @@ def test_parameters_of_sampling_that_are_not_numbers():
         got = dnp.nn.sample(dnp.array(logits), u, temperature=f(np.inf)).get()
         assert got.tolist() == [nn_oracle.sample(r, x, temperature=1e300) for r, x in zip(logits, (0.1, 0.5, 0.99))]
     """, DELAY_CPU="1")
+
+
+def test_keys_that_do_not_count_take_no_memory():
+    """What is not finite is added row by row: 1500 rows and keys of 64 would otherwise take 1.1 GB for each product."""
+    _child("""
+        import resource
+        import numpy as np
+        import delayrepay as dnp
+        rs = np.random.RandomState(5)
+        q, k, v, g = (rs.standard_normal((1, 1, 1500, 64)).astype(np.float32) for _ in range(4))
+        args = dict(causal=True, start=-700)
+        dev = [dnp.array(x) for x in (q, k, v, g)]
+        dnp.nn.attention(*dev[:3], **args)
+        before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+        clean = dnp.nn.attention(*dev[:3], with_lse=True, **args)
+        clean = [*clean, *dnp.nn.attention_grad(dev[3], *dev[:3], *clean, **args)]
+        k[:, :, 800:], v[:, :, 800:] = np.nan, np.inf
+        dev = [dnp.array(x) for x in (q, k, v, g)]
+        got = dnp.nn.attention(*dev[:3], with_lse=True, **args)
+        got = [*got, *dnp.nn.attention_grad(dev[3], *dev[:3], *got, **args)]
+        for x, y in zip(got, clean):
+            assert np.allclose(x.get(), y.get(), rtol=2.0 ** -23, atol=1e-12)
+        assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 500 << 10
+        v[0, 0, 5, 3], v[0, 0, 6, 3], v[0, 0, 9, 4] = np.inf, -np.inf, np.nan
+        o = dnp.nn.attention(*dev[:2], dnp.array(v), **args).get()[0, 0]
+        assert np.isfinite(o[:705]).all() and np.all(o[705, 3] == np.inf) and np.isnan(o[706:, 3]).all() and np.isnan(o[709:, 4]).all()
+        assert np.isfinite(o[:709, 4]).all() and np.isfinite(np.delete(o, [3, 4], 1)).all()
+    """, DELAY_CPU="1")
