@@ -173,3 +173,16 @@ def test_keys_that_do_not_count_take_no_memory():
         assert np.isfinite(o[:705]).all() and np.all(o[705, 3] == np.inf) and np.isnan(o[706:, 3]).all() and np.isnan(o[709:, 4]).all()
         assert np.isfinite(o[:709, 4]).all() and np.isfinite(np.delete(o, [3, 4], 1)).all()
     """, DELAY_CPU="1")
+
+
+def test_a_lost_part_of_the_products_would_be_noticed():
+    """What the GPU test of attention's precision allows lies between products of three bfloat16 parts and those of two."""
+    import numpy as np
+    from tests import nn_precision as p
+    for size in p.SIZES:
+        x = p.inputs(*size)
+        want = p.attention(*x, p.plain_product, np.float64)
+        plain, three, two = ({n: p.error(y, want[n]) for n, y in p.attention(*x, product).items()}
+                             for product in (p.plain_product, p.split_product(3), p.split_product(2)))
+        for n in want:
+            assert three[n] <= 1.5 * plain[n] and two[n] >= 3 * p.WORST * plain[n], (size, n, plain[n], three[n], two[n])
