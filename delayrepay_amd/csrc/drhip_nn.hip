@@ -393,7 +393,7 @@ template <typename T> void launch_rotary_grad(const Rot& p, hipStream_t s) {
 // of the digit or step where a beginning ends, or the few kept ones themselves, go to LDS and are ordered there.
 // Where more share a step than LDS holds (many equal logits) the end is found digit by digit over the whole row
 // instead.  Weights are 64-bit whole numbers (the largest 2^s, s such that all fit, computed in float64), so that
-// sums do not depend on their order.
+// sums do not depend on their order; what is below 2^-(s + 1) of the largest is none (s = 45 for 128000 tokens).
 //
 // 256 rows of 128000 with top-k 50: 40 us, more than half of it the first pass at memory's rate (131 MB).  One row of 32000
 // with top-p: 31 us on one compute unit, of which 9 are the weights of all tokens (float64, 13 operations each), 7 the

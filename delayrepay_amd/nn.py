@@ -337,7 +337,9 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     (top_k) integers, in which a top_k below 1 stands for all, numbers out of range for the nearest in it and NaN for 0.
     A logit that is NaN or -inf is never drawn; a row without another gives -1.
 
-    Sums are whole numbers of 62 bits: the token depends on no order of summation.
+    Sums are whole numbers of 62 bits: the token depends on no order of summation.  A weight is a multiple of 2**-s of
+    the largest, s = 62 - (bits of the vocabulary) but at most 52 (45 for 128000 tokens); what is smaller than
+    half of that is none, vocabulary * 2**-(s + 1) of the largest at most in all (2**-29, and 2**-7 for 2**28 tokens).
     """
     logits = _floats(logits, "logits", 2)
     batch, vocabulary = logits.shape

@@ -208,6 +208,24 @@ def test_parameters_of_sampling_that_are_not_numbers():
     assert got.tolist() == [nn_oracle.sample(r, x, temperature=1e300) for r, x in zip(logits, (0.1, 0.5, 0.99))]
 
 
+def test_sample_of_the_longest_rows():
+    """2^25 tokens: each weight is a multiple of 2^-37 of the largest.  Equal ones share the range of the uniform
+    numbers evenly; of two levels e^-3 apart the lower one's weight is off by less than 2^-33 of itself."""
+    n = 1 << 25
+    logits = np.zeros((1, n), np.float32)
+    dev = dr.array(logits)
+    for u in (0.0, 0.3, 0.75, 1 - 2.0 ** -26):
+        assert nn.sample(dev, dr.array(np.array([u]))).get()[0] == int(u * n), u
+    logits[0, :n // 2] = -3.0
+    low = np.exp(-3.0)
+    dev = dr.array(logits)
+    for u in (0.02, 0.04, 0.3, 0.9):
+        at = u * (n // 2) * (1 + low)
+        want = at / low if at < n // 2 * low else n // 2 + at - n // 2 * low
+        for got in (nn.sample(dev, dr.array(np.array([u]))).get()[0], nn.sample(dev, dr.array(np.array([u])), min_p=0.01).get()[0]):
+            assert abs(got - want) <= 1 + n * 2.0 ** -32, (u, got, want)
+
+
 def _in_a_program_with_torch(script):
     """A child process that imports torch first, as programs that use both do."""
     r = subprocess.run([sys.executable, "-u", "-c", textwrap.dedent(script)], cwd=ROOT, capture_output=True, text=True, timeout=100)
