@@ -34,6 +34,7 @@ extern "C" uint64_t drhip_k_attention_work(const drhip_attention_t* a, int grad)
 extern "C" int drhip_k_attention_packs(const drhip_attention_t* a);
 extern "C" int drhip_k_attention(const drhip_attention_t* a, hipStream_t s);
 extern "C" int drhip_k_attention_grad(const drhip_attention_t* a, hipStream_t s);
+extern "C" int drhip_k_clamp(const drhip_clamp_t* a, hipStream_t s);
 extern "C" int drhip_k_renumber(const drhip_renumber_t* a, int log, hipStream_t s);
 extern "C" uint64_t drhip_k_rotary_work(const drhip_rotary_t* p);
 extern "C" int64_t drhip_k_rotary_blocks(const drhip_rotary_t* p);
@@ -393,6 +394,17 @@ int drhip_renumber(const drhip_renumber_t* a) {
     if (!a->batch || !a->n) return 0;
     if (!a->x || !a->y || !a->table) return fail(DRHIP_EINVAL, "drhip_renumber", "null operand");
     if (int rc = drhip_k_renumber(a, __builtin_ctz((unsigned)a->slots), g_stream)) return fail(rc, "drhip_renumber", hipGetErrorString((hipError_t)rc));
+    g_cnt.n_launches++;
+    return 0;
+}
+
+int drhip_clamp(const drhip_clamp_t* a) {
+    if (!a) return fail(DRHIP_EINVAL, "drhip_clamp", "null argument");
+    if (a->n < 0 || a->n >= 1 << 28 || a->low > a->high) return fail(DRHIP_EINVAL, "drhip_clamp", "bad size");
+    NEED_INIT();
+    if (!a->n) return 0;
+    if (!a->x || !a->y) return fail(DRHIP_EINVAL, "drhip_clamp", "null operand");
+    if (int rc = drhip_k_clamp(a, g_stream)) return fail(rc, "drhip_clamp", hipGetErrorString((hipError_t)rc));
     g_cnt.n_launches++;
     return 0;
 }

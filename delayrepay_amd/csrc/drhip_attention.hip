@@ -1433,8 +1433,16 @@ __global__ __launch_bounds__(kThreads) void attention_add(Args a, int parts, int
     }
 }
 
-// ---- document numbers of 64 bits ---------------------------------------------------------------
-// Documents are told apart by equality alone, so a number may become the place where it first stands in its
+// ---- arguments of 64 bits -----------------------------------------------------------------------
+
+__global__ __launch_bounds__(kThreads) void clamp_numbers(drhip_clamp_t a) {
+    const int n = blockIdx.x * kThreads + threadIdx.x;
+    if (n >= a.n) return;
+    const int64_t x = a.x[n * a.x_stride];
+    a.y[n] = (int32_t)(x < a.low ? a.low : x > a.high ? a.high : x);
+}
+
+// Document numbers are told apart by equality alone, so a number may become the place where it first stands in its
 // sequence.  A table of at least twice as many slots as there are numbers holds for each of them that place: the first of each
 // run of equal numbers looks for its slot from the number's hash on (multiplicative, upwards), then every number reads
 // its place.  What it gives does not depend on timing.  Bound by its three launches.
@@ -1718,5 +1726,10 @@ extern "C" int drhip_k_renumber(const drhip_renumber_t* a, int log, hipStream_t 
     renumber_clear<<<dim3((unsigned)(count < 2048 * kThreads ? (count + kThreads - 1) / kThreads : 2048)), kThreads, 0, s>>>(a->table, count);
     renumber_enter<<<dim3((unsigned)(a->batch * blocks)), kThreads, 0, s>>>(*a, log, blocks);
     renumber_read<<<dim3((unsigned)(a->batch * blocks)), kThreads, 0, s>>>(*a, log, blocks);
+    return (int)hipGetLastError();
+}
+
+extern "C" int drhip_k_clamp(const drhip_clamp_t* a, hipStream_t s) {
+    clamp_numbers<<<dim3((unsigned)((a->n + kThreads - 1) / kThreads)), kThreads, 0, s>>>(*a);
     return (int)hipGetLastError();
 }

@@ -1469,12 +1469,10 @@ def assign(dst, value):
     _write(_plan_write(tracer, root, dst), dst)
 
 
-def materialise(arr, dtype=None, shape=None, within=None):
-    """Contiguous copy of a device array, optionally clamped to `within`, converted / broadcast."""
+def materialise(arr, dtype=None, shape=None):
+    """Contiguous copy of a device array, optionally converted / broadcast."""
     tracer = Tracer()
     root = tracer.leaf(arr)
-    for name, bound in zip(("maximum", "minimum"), within or ()):
-        root = tracer.op(name, root[1], root[1], [root[0], tracer.scalar(bound, root[1])[0]])
     if dtype is not None and numpy.dtype(dtype) != arr.dtype:
         code = dtype_code(dtype)
         root = tracer.op("cast", code, code, [root[0]])

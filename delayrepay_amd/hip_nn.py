@@ -11,8 +11,11 @@ _F32, _I64 = numpy.dtype(numpy.float32), numpy.dtype(numpy.int64)
 
 
 def narrowed(x, low, high):
-    """The int64 array in int32, with its numbers clamped to [low, high]."""
-    return hip.materialise(x, numpy.int32, within=(low, high))
+    """The int64 array (one dimension) in int32, with its numbers clamped to [low, high]."""
+    out = ndarray(x.shape, numpy.int32)
+    if x.size:
+        hip.issue_operator(hiprt.clamp, hiprt.CLAMP.pack(x.ptr, out.ptr, x._strides[0], x.size, low, high), [x, out], [out])
+    return out
 
 
 def _dense(x):

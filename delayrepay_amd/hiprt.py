@@ -79,6 +79,7 @@ _SIGNATURES = {
     "drhip_attention_work": (C.c_int, [C.c_char_p, C.c_int, C.POINTER(C.c_uint64)]),
     "drhip_attention": (C.c_int, [C.c_char_p]),
     "drhip_attention_grad": (C.c_int, [C.c_char_p]),
+    "drhip_clamp": (C.c_int, [C.c_char_p]),
     "drhip_renumber": (C.c_int, [C.c_char_p]),
     "drhip_rotary_work": (C.c_int, [C.c_char_p, C.POINTER(C.c_uint64)]),
     "drhip_rotary": (C.c_int, [C.c_char_p]),
@@ -229,7 +230,7 @@ ROTARY = struct.Struct("@8PQ12q5d9i0q")      # (0q: filled up to whole words, as
 # the same in two pieces: addresses, and what depends on geometry and options alone
 ATTENTION_HEAD, ATTENTION_TAIL = struct.Struct("@15PQ"), struct.Struct("@25q10i2f")
 ROTARY_HEAD, ROTARY_TAIL = struct.Struct("@8PQ"), struct.Struct("@12q5d9i0q")
-RENUMBER = struct.Struct("@3Pq3i0q")
+CLAMP, RENUMBER = struct.Struct("@2Pq3i0q"), struct.Struct("@3Pq3i0q")
 SAMPLE_HEAD, SAMPLE_TAIL = struct.Struct("@7P"), struct.Struct("@q4d4i")
 
 
@@ -249,6 +250,10 @@ def attention_grad(args):
     rc = _lib.drhip_attention_grad(args)
     if rc:
         _check(rc)
+
+
+def clamp(args):
+    _check(_lib.drhip_clamp(args))
 
 
 def renumber(args):

@@ -302,7 +302,8 @@ def rotary(x, positions, *, base=10000.0, frequencies=None, dims=None, interleav
     Angles are computed in 64 bits (positions of an int64 array beyond 2**53 are rounded).
 
     With `weight`, (size,) or (heads, size), each row is first divided by the root of (the mean of its
-    squares + eps) and multiplied by the weight: the norm of queries and keys in the same pass.
+    squares + eps) and multiplied by the weight: the norm of queries and keys in the same pass.  Squares, eps and
+    magnitude are numbers of the rows' type: elements of float32 rows lie below 2**59, of float64 ones below 2**507.
     """
     x = _floats(x, "x", 4, (_F32, _F64))
     how = _Turn(x, positions, base, frequencies, dims, interleaved, stretch, magnitude, weight, eps)

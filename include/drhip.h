@@ -168,6 +168,16 @@ typedef struct drhip_renumber_t {
 } drhip_renumber_t;
 int drhip_renumber(const drhip_renumber_t* a);
 
+/* y[n] = x[n] clamped to [low, high], numbers of 64 bits to 32 (of lengths and
+ * their like). */
+typedef struct drhip_clamp_t {
+    const int64_t* x;
+    int32_t* y;
+    int64_t x_stride;
+    int32_t n, low, high;
+} drhip_clamp_t;
+int drhip_clamp(const drhip_clamp_t* a);
+
 /* Rotary positions of x[batch][heads][rows][d] (d <= 512), float or double: the
  * pair of elements number i < dims/2 turns by sign * position * frequency_i *
  * squeeze, frequency_i = 2^(i * step) or from the table, and is multiplied by

@@ -54,12 +54,19 @@ def test_the_library_checks_the_table_of_renumbered_documents():
         assert hiprt.lib().drhip_renumber(hiprt.RENUMBER.pack(16, 16, 16, n, batch, n, slots)) == 20002, (batch, n, slots)
 
 
+def test_the_library_checks_what_it_clamps():
+    from delayrepay_amd import hiprt
+    for n, low, high in ((-1, 0, 1), (1 << 28, 0, 1), (3, 2, 1)):
+        assert hiprt.lib().drhip_clamp(hiprt.CLAMP.pack(16, 16, 1, n, low, high)) == 20002, (n, low, high)
+
+
 def test_argument_structs_have_the_size_of_the_header(tmp_path):
     from delayrepay_amd import hiprt
     source, program = tmp_path / "sizes.c", tmp_path / "sizes"
-    source.write_text('#include <stdio.h>\n#include "drhip.h"\nint main(void) { printf("%zu", sizeof(drhip_renumber_t)); return 0; }\n')
+    source.write_text('#include <stdio.h>\n#include "drhip.h"\nint main(void) { printf("%zu %zu", sizeof(drhip_renumber_t), sizeof(drhip_clamp_t)); return 0; }\n')
     subprocess.run(["cc", "-I", os.path.join(ROOT, "include"), "-o", str(program), str(source)], check=True)
-    assert int(subprocess.run([str(program)], capture_output=True, text=True, check=True).stdout) == hiprt.RENUMBER.size
+    sizes = subprocess.run([str(program)], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(x) for x in sizes] == [hiprt.RENUMBER.size, hiprt.CLAMP.size]
 
 
 def test_caches_that_fit_the_device_are_not_refused():
