@@ -524,9 +524,11 @@ struct Active {
 // per column of its accumulators: S^T = K Q^T leaves the scores of a row in one lane pair, so the softmax
 // needs one exchange, and P^T in the layout that O^T += V^T P^T reads.
 // Keys and values come 32 at a time from the packed planes through LDS, two buffers, copied a tile ahead.
-// Bound by the matrix units: 32 heads, 4096 rows of 128, causal: 605 us, 227 TFLOP/s of float32 products (a large
-// product of f32 matrices reaches 155), 1.36 PFLOP/s of bfloat16 ones, of which the card holds 2.0 with nothing else to do.  Two waves on a SIMD fill each other's waits; four-wave blocks, two on a compute unit, read each tile twice as
-// often from L2 (695 for 639 us).  With a cap a tanh for each pair comes on top (8 heads, 8192 rows: 690 us).
+// Bound by the matrix units: 32 heads, 4096 rows of 128, causal: 651 us at best and 690 at the median under the profiler,
+// 199 TFLOP/s of float32 products (a large product of f32 matrices reaches 155), 1.2 PFLOP/s of bfloat16 ones, of which a
+// loop of nothing else reaches 2.1 to 2.25.  Two waves on a SIMD fill each other's waits; four-wave blocks, two on a
+// compute unit, read each tile twice as often from L2 (695 for 639 us).  With a cap a tanh for each pair comes on top (8
+// heads, 8192 rows: 695 and 711 us).
 template <int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_rows(Args a, Plan plan, int tiles, Packed in, float* part, float* part_lse) {
     using P = Planes<NT>;
@@ -696,7 +698,7 @@ __global__ __launch_bounds__(64 * WAVES, NT < 4 ? 2 : WAVES / 4) void attention_
 // waves in turn, and its loads are the operands of v_mfma_f32_16x16x4f32 as they come (K: lane = key,
 // 16 bytes of its row; V: 16 neighbouring bytes of four rows each).  Key ranges of one sequence go to
 // `splits` blocks, whose results are joined by `attention_join`.  64 sequences of up to 8192 keys, 8 key heads of
-// 128: 452 us, 5.8 TB/s.  One sequence of 5000: 18 us, a third of it the blocks' start, a quarter the first
+// 128: 451 us, 5.8 TB/s.  One sequence of 5000: 17 us, a third of it the blocks' start, a quarter the first
 // load's way.
 template <int NB, bool WIDE>
 __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, int sets, float* part, float* part_lse) {
@@ -942,7 +944,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few(Args a, Plan plan, 
 // Results of key ranges into one (of many rows, those with keys in more than the first), four elements to a lane.  Up to kNear ranges: half a wave for each row, all
 // loads at once (65536 causal rows of 128 in two ranges, half of them with keys in both: 15 us; if all are joined
 // 21, 4.8 TB/s; a wave for each row, which first finds the largest sum, 42).  More: a block for each row, whose eight halves of waves take the ranges in turn (32 rows in
-// 40 ranges 4.7 us, with one wave 6.4).
+// 40 ranges 4 us, with one wave 6.4).
 constexpr int kNear = 4;
 
 template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(Args a, Plan plan, const float* part, const float* part_lse) {
@@ -1028,7 +1030,8 @@ template <bool NEAR> __global__ __launch_bounds__(kThreads) void attention_join(
 // by).  The scores are computed in both: seven products instead of five.  A wave holds two matrices of 32
 // columns in planes and its sums, more than 256 registers, so there is one for each SIMD, and what it does on
 // the vector unit stands between its matrix instructions.  Bound by the matrix units, which are busy for 54%
-// of the time: 2 sequences of 2048 rows, 16 heads of 128, causal: 702 us, 171 TFLOP/s of float32 products.
+// of the time: 2 sequences of 2048 rows, 16 heads of 128, causal: 640 us at best and 669 at the median under the
+// profiler, 180 TFLOP/s of float32 products.
 template <int NT> struct GradLds {
     __attribute__((aligned(16))) char tile[2][2 * Planes<NT>::BYTES];
     __attribute__((aligned(16))) float stat[2][2][kTile];
@@ -1389,7 +1392,7 @@ __device__ __forceinline__ void grad_dkv(const Args& a, const Plan& plan, const 
 }
 
 // Both in one launch, the longer dK, dV blocks first: neither waits for the other's last blocks (3 sequences of
-// 517 rows, 6 heads of 64: 43 us, in two launches 68; 2 of 2048 rows, 16 heads of 128: 702 and 710).  The two take their
+// 517 rows, 6 heads of 64: 40 us, in two launches 25 more; 2 of 2048 rows, 16 heads of 128: 8 more).  The two take their
 // arguments from copies: of one the compiler would read all values ahead of the choice and keep them, a hundred
 // scalar registers more than there are.  Mixing the two kinds block by block costs 5%: an XCD's L2 then holds
 // neither's matrices.
@@ -1445,7 +1448,8 @@ __global__ __launch_bounds__(kThreads) void clamp_numbers(drhip_clamp_t a) {
 // Document numbers are told apart by equality alone, so a number may become the place where it first stands in its
 // sequence.  A table of at least twice as many slots as there are numbers holds for each of them that place: the first of each
 // run of equal numbers looks for its slot from the number's hash on (multiplicative, upwards), then every number reads
-// its place.  What it gives does not depend on timing.  Bound by its three launches.
+// its place.  What it gives does not depend on timing.  Bound by its three launches (3 sequences of
+// 1111: 4, 2.3 and 2.8 us, 6 us more for a call than with numbers of 32 bits).
 constexpr int kFree = 0x7fffffff;
 
 __device__ __forceinline__ unsigned slot_of(int64_t x, int log) { return (unsigned)((uint64_t)x * 0x9e3779b97f4a7c15ull >> (64 - log)); }

@@ -16,8 +16,8 @@ constexpr int kThreads = 256;
 //   (i, i + dims/2) or (2i, 2i + 1); elements from `dims` on are left as they are
 //   gradient: g = R^T dy,  dx = r (w g - xhat mean(w g xhat)),  dw = sum over rows of g xhat,  xhat = r x
 //
-// Bound by memory: a row is read and written once (4 sequences of 4096, 40 heads of 128: 671 MB in 122 us,
-// 5.5 TB/s).  A row belongs to a group of 2^k lanes, eight elements
+// Bound by memory: a row is read and written once (4 sequences of 4096, 40 heads of 128: 671 MB in 123 us,
+// 5.5 TB/s; in float64 1342 MB in 244).  A row belongs to a group of 2^k lanes, eight elements
 // each (the halves of four pairs); a group takes two heads of one token, so that the angles, which need 64 bits
 // (positions of a million turn by a million radians), are computed once for them.
 
@@ -236,8 +236,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Rot p, int lanes_log, 
 // Gradient with a norm.  A block owns a head and every `slots`-th run of tokens, its groups one token each; a lane keeps
 // the sums of its elements of dw, the groups meet in LDS, the blocks in `rotary_dw`.  A group has one or a few
 // tokens, so it waits for memory more than it computes: one head for a block, whose registers leave room for four
-// waves on a SIMD (20 heads of 128, 3554 tokens: 22 us, 4.9 TB/s), not two, which share the angles but leave
-// room for two (30 us), and the loads ahead of the angles.
+// waves on a SIMD (20 heads of 128, 3554 tokens: 25 us, 4.4 TB/s; in float64 39, 5.6), not two, which share the angles
+// but leave room for two (8 us more), and the loads ahead of the angles.
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_grad_kernel(Rot p, int lanes_log, int slots) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
@@ -395,8 +395,8 @@ template <typename T> void launch_rotary_grad(const Rot& p, hipStream_t s) {
 // instead.  Weights are 64-bit whole numbers (the largest 2^s, s such that all fit, computed in float64), so that
 // sums do not depend on their order; what is below 2^-(s + 1) of the largest is none (s = 45 for 128000 tokens).
 //
-// 256 rows of 128000 with top-k 50: 40 us, more than half of it the first pass at memory's rate (131 MB).  One row of 32000
-// with top-p: 31 us on one compute unit, of which 9 are the weights of all tokens (float64, 13 operations each), 7 the
+// 256 rows of 128000 with top-k 50: 39 us, more than half of it the first pass at memory's rate (131 MB).  One row of 32000
+// with top-p: 33 us on one compute unit, of which 9 are the weights of all tokens (float64, 13 operations each), 7 the
 // kept ones' sums, 12 barriers and scans between the steps.
 
 typedef drhip_sample_t Smp;
