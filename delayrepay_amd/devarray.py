@@ -66,7 +66,8 @@ _LEAVING = []     # (event, owner) of borrowed memory whose last view is gone
 class Borrowed(Buffer):
     """Device memory of another library, as `from_dlpack` takes it over.  `owner` is kept until
     the work queued here when the last view went has run: the other library may hand the
-    memory out again as soon as its object is released.  The address never changes: updates
+    memory out again as soon as its object is released.  (Calls that look whether it has: a
+    takeover, the end of another such array, `synchronize()`.)  The address never changes: updates
     that read what they overwrite copy back instead of swapping allocations (hip._write)."""
 
     __slots__ = ("owner",)

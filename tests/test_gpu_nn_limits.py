@@ -93,6 +93,39 @@ def test_recorded_documents_of_64_bits():
         _same_bits([out.get()], [want])
 
 
+def test_recorded_lengths_of_64_bits_and_gradients_of_a_part():
+    """What a replay clamps and clears is what the arrays hold then."""
+    from delayrepay_amd import hip
+    q, g, k, v = (dr.array(x) for x in _normal(14, (2, 2, 40, 32), (2, 2, 40, 32), (2, 2, 60, 32), (2, 2, 60, 32)))
+    lengths = dr.array(np.array([60, 60]))
+    grads = [dr.array(np.full(x.shape, 7, np.float32)) for x in (q, k, v)]
+    with hip.record() as plan:
+        o, lse = nn.attention(q, k, v, lengths=lengths, with_lse=True)
+        part = nn.attention(q, k, v, lengths=50, with_lse=True)
+        nn.attention_grad(g, q, k, v, *part, lengths=50, out=grads)
+    plan.as_graph()
+    want = [x.get() for x in nn.attention_grad(g, q, k, v, *part, lengths=50)]
+    for now in ([2 ** 40, 3], [0, -(2 ** 50)], [17, 2 ** 31]):
+        lengths[...] = dr.array(np.array(now))
+        for x in grads:
+            x[...] = 7.0
+        plan()
+        small = dr.array(np.clip(now, 0, 60).astype(np.int32))
+        _same_bits([x.get() for x in (o, lse)], [x.get() for x in nn.attention(q, k, v, lengths=small, with_lse=True)])
+        _same_bits([x.get() for x in grads], want)
+        assert not want[1][:, :, 50:].any()
+
+
+def test_nothing_at_all_in_64_bits():
+    """No sequences, no keys, no rows: results of their shapes."""
+    for b, lq, lk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        q, k = (dr.array(np.ones((b, 2, n, 8), np.float32)) for n in (lq, lk))
+        how = dict(lengths=dr.array(np.zeros(b, np.int64)), documents=dr.array(np.zeros((b, lk), np.int64)), start=dr.array(np.zeros(b, np.int64)))
+        o, lse = nn.attention(q, k, k, with_lse=True, **how)
+        dq, dk, dv = nn.attention_grad(q, q, k, k, o, lse, **how)
+        assert o.shape == dq.shape == (b, 2, lq, 8) and dk.shape == dv.shape == (b, 2, lk, 8) and lse.shape == (b, 2, lq)
+        assert not any(x.get().any() for x in (o, dq, dk, dv)) and np.all(lse.get() == -INF)
+    assert nn.sample(dr.array(np.zeros((0, 5), np.float32)), dr.array(np.zeros(0)), top_k=dr.array(np.zeros(0, np.int64))).shape == (0,)
 
 
 def test_caches_of_many_sequences():
