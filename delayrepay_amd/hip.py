@@ -1403,24 +1403,22 @@ def _write(plan, dst):
         if buf.shadow is None:
             buf.shadow = hiprt.malloc(max(buf.nbytes, 1))
             buf.shadow_region = None
-        borrowed = type(buf) is Borrowed       # its address is another library's too
-        if borrowed and _RECORDING is not None:
-            raise RuntimeError("hip.record(): an update that reads what it overwrites cannot be recorded "
-                               "for an array taken over from another library")
-        if borrowed:
-            # the elements between those of the view are the other library's: neither read nor written
+        if type(buf) is Borrowed:
+            # Its address is another library's too, and so are the elements between those of the view: the view alone
+            # is copied back
             _fire(plan, [buf.shadow + off])
+            if _RECORDING is not None:
+                _RECORDING.keep += plan.leaves
             mirror = _Elsewhere(buf.nbytes, buf.shadow)
             tracer = Tracer()
             root = tracer.leaf(ndarray(dst.shape, dst.dtype, mirror, dst.offset, dst._strides))
-            _write(_plan_write(tracer, root, dst), dst)
-        else:
-            if buf.shadow_region != plan.region:
-                hiprt.memcpy_d2d(buf.shadow, buf.ptr, buf.nbytes)
-            _fire(plan, [buf.shadow + off])
-            buf.ptr, buf.shadow = buf.shadow, buf.ptr
-            buf.shadow_region = plan.region
-            buf.version += 1
+            return _write(_plan_write(tracer, root, dst), dst)
+        if buf.shadow_region != plan.region:
+            hiprt.memcpy_d2d(buf.shadow, buf.ptr, buf.nbytes)
+        _fire(plan, [buf.shadow + off])
+        buf.ptr, buf.shadow = buf.shadow, buf.ptr
+        buf.shadow_region = plan.region
+        buf.version += 1
     if _RECORDING is not None:
         _RECORDING.keep += [dst] + plan.leaves
         _RECORDING.written.append((buf, plan.hazard))

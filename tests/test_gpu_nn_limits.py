@@ -334,3 +334,37 @@ def test_what_is_computed_of_another_librarys_array_follows_its_writes():
         assert np.array_equal(held.get(), np.ones((2, 3)))
         print("done")
     """)
+
+
+def test_recorded_writes_over_views_of_one_memory():
+    """Views taken over apart, disjoint columns among them: a replay does what the writes did."""
+    _in_a_program_with_torch("""
+        import torch
+        import numpy as np
+        torch.zeros(1, device="cuda")
+        import delayrepay_amd as dr
+        from delayrepay_amd import hip
+        x = torch.arange(4000.0, device="cuda").view(40, 100)
+        even, odd = dr.from_dlpack(x[:, ::2]), dr.from_dlpack(x[:, 1::2])
+        with hip.record() as plan:
+            even[...] = odd * 0.5
+            odd[1:] = odd[:-1] + even[1:]
+        dr.synchronize()
+        want = np.arange(4000.0, dtype=np.float32).reshape(40, 100)
+
+        def step():
+            want[:, ::2] = want[:, 1::2] * np.float32(0.5)
+            want[1:, 1::2] = want[:-1, 1::2] + want[1:, ::2]
+        step()
+        assert np.array_equal(x.cpu().numpy(), want)
+        plan.as_graph()
+        for turn in range(3):
+            x += 1.0
+            want += 1.0
+            torch.cuda.synchronize()
+            plan()
+            dr.synchronize()
+            step()
+            assert np.array_equal(x.cpu().numpy(), want), turn
+        print("done")
+    """)
